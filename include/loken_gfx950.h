@@ -763,6 +763,84 @@ void loken_stable_sort_u32(const uint32_t* keys, uint32_t* sorted, uint32_t* ord
 /* The decode-size form (cuda/moe/gate_topk.cu:453-477; src/inference/moe_cuda/dense/gate.rs:185):
  * same result for m keys; the reference serves m <= 32, this m <= 256, nothing is launched above. */
 void loken_argsort_small_u32(const uint32_t* in, uint32_t* sorted_out, uint32_t* index_out, int m, void* stream);
+/* ---------------------------------------------------------------------------------------
+ * Between the linears of a served step: a paged key / value cache in 8 bits, attention over it, and the next
+ * token from the logits. No counterparts in the reference (it keeps its own caches and kernels for these).
+ *
+ * The cache is `pages` pages of `page_tokens` (16, 32, 64, 128 or 256) consecutive positions of one sequence, each with
+ * `kv_heads` heads of `head_dim` (64, 128 or 256) values; a value is code (int8, -127 .. 127) * scale, the scale
+ * one for a page, head and side:
+ *   k_codes   int8 [pages][kv_heads][page_tokens][head_dim], 16-byte aligned
+ *   v_codes   int8 [pages][kv_heads][page_tokens / 16][head_dim][16], 16-byte aligned: sixteen tokens of a column together
+ *   k_scales, v_scales   f32 [pages][kv_heads]
+ * Slot s is page s / page_tokens, token s % page_tokens. A slot or page number below zero or past the cache is absent: nothing
+ * is read from or written to it. Table: row i of `table` (int32, `table_stride` entries apart, `table_cols` of them used) holds
+ * the pages of sequence i in the order of its positions.
+ * ------------------------------------------------------------------------------------- */
+#define LK_KV_PLAN_SEQS 8192   /* sequences of one plan */
+
+/* Pages and slots of a batch from its request lengths. Sequence i has past[i] tokens in the cache and brings fresh[i]
+ * (below zero: none). It gets ceil((past + fresh) / page_tokens) - ceil(past / page_tokens) pages, the next ones of
+ * free_pages[n_free] behind the first *taken (nullable: 0), sequences in their order; they are stored behind the entries that
+ * its table row has (-1 where the list is out; columns from table_cols on are not stored).
+ *   lens[seqs]         past + fresh
+ *   starts[seqs + 1]   the first row of each sequence in the batch, and their number
+ *   slots[rows], positions[rows]   of each row: -1 and the position where its page is absent; -1 and 0 behind the last sequence
+ *   *taken_out         *taken + the pages asked for (above n_free: that many more are wanted); not the address of `taken`
+ * Rows past `rows` are left out of slots and positions. Sums past 2^31 - 1 stay there. More than LK_KV_PLAN_SEQS sequences: LK_ERR_SIZE. */
+int lk_kv_plan(const int32_t* past, const int32_t* fresh, int seqs, int page_tokens, const int32_t* free_pages, int n_free,
+               const int32_t* taken, int32_t* table, int64_t table_stride, int table_cols, int32_t* lens, int32_t* starts,
+               int64_t* slots, int32_t* positions, int rows, int32_t* taken_out, void* stream);
+
+/* New rows of keys and values (`type` LK_TYPE_F32 | F16 | BF16, [tokens][kv_heads][head_dim], k_stride / v_stride elements from
+ * token to token) into the slots that `slots` (8-byte aligned) names; a slot below zero or past the cache: the row is skipped.
+ * The rows of one page stand together, as lk_kv_plan gives them, or with skipped rows between them (of a slot named twice the last row
+ * stays); where rows of other pages stand between them, or two sequences write one page, what that page holds is not defined. Per page, head and side:
+ *   s_old = the page's scale; 0 if the page's first token is among the new rows, which starts the page anew
+ *   s = max(s_old, max |x| / 127) over the new finite x (0 below 2^-126)
+ *   codes that were there become round(c * s_old / s), new ones round(x / s): exact quotients, halves away from zero
+ * An infinite x is stored as +-127 s, one that is not a number as 0. */
+int lk_kv_write_q8(const void* k, const void* v, int type, int64_t k_stride, int64_t v_stride, const int64_t* slots, int tokens,
+                   int kv_heads, int head_dim, int page_tokens, int pages, void* k_codes, void* v_codes, float* k_scales,
+                   float* v_scales, void* stream);
+
+/* Rows of the cache as values: k_out, v_out [tokens][kv_heads][head_dim] of `type`, zeros where a slot is absent. */
+int lk_kv_read_q8(const int64_t* slots, int tokens, int kv_heads, int head_dim, int page_tokens, int pages, const void* k_codes,
+                  const void* v_codes, const float* k_scales, const float* v_scales, void* k_out, void* v_out, int type,
+                  void* stream);
+
+/* Attention of the batch's rows over the cache. Rows starts[i] .. starts[i + 1] - 1 of q ([rows][heads][head_dim] of `type`,
+ * q_stride elements from row to row) are the last positions of sequence i, whose lens[i] tokens are in the cache: row r stands at
+ * p = lens[i] - (starts[i + 1] - starts[i]) + r - starts[i]. Head h reads key / value head h / (heads / kv_heads):
+ *   out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j   over p - window < j <= p (window 0: all j <= p)
+ * leaving out positions whose page is absent. A row that sees none gives zeros, one whose q holds a value that is not finite gives
+ * values that are not numbers. Rows behind the last sequence are left as they were. `out` has q's type, out_stride elements from row
+ * to row; it does not overlap q. max_fresh and max_len: the most rows and the most tokens of a sequence as the caller knows
+ * them; they choose launch shapes only, a sequence with more is served too.
+ * Scores, softmax and sums are held in f32 (sums of products of codes in int32 as long as they are exact). Partial results of a
+ * context that is split over workgroups go through scratch of the stream (LK_ERR_NOMEM where there is none; while a
+ * graph is recorded, where no call outside a recording has needed as much). */
+int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, void* out, int64_t out_stride, const void* k_codes,
+                       const void* v_codes, const float* k_scales, const float* v_scales, int pages, int page_tokens,
+                       const int32_t* table, int64_t table_stride, int table_cols, const int32_t* lens, const int32_t* starts,
+                       int seqs, int rows, int max_fresh, int max_len, int heads, int kv_heads, int head_dim, float scale,
+                       int window, void* stream);
+
+/* The next token of each row of logits (`type` LK_TYPE_F32 | F16 | BF16, [rows][vocab], `stride` elements from row to row). With
+ * M the row's largest logit and w = exp((logit - M) / temperature[r]), the words are ordered by logit, the largest first, equal
+ * ones by their number; words whose logit is -inf or not a number are none. Of that order
+ *   top_k[r] > 0: the first top_k words (n1 of them; else all),
+ *   top_p[r] < 1: the fewest first words of these whose weights reach top_p of the weight of all of these,
+ *   and of those the words with w >= min_p[r]; the first word always stays.
+ * The token is the first word of the kept ones at which the running sum of weights exceeds uniform[r] (0 <= uniform < 1) of their
+ * sum; tokens[r] its number, probs[r] (nullable) its weight over that sum. temperature <= 0 (or not a number): the first word of the order,
+ * probability 1. A row without words: -1 and 0. Arrays top_k, top_p, min_p may be null (no such rule).
+ * Weights are summed as integers of 2^-42, so results do not depend on the order of execution; a word whose weight
+ * rounds to none is not drawn. vocab up to LK_SAMPLE_VOCAB, else LK_ERR_SIZE. */
+#define LK_SAMPLE_VOCAB (1 << 20)
+int lk_sample(const void* logits, int type, int64_t stride, int rows, int vocab, const float* uniform, const float* temperature,
+              const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, float* probs, void* stream);
+
 /* Frees what the expert launchers, the expert block, the router and the f16 tiles hold on the current device, for
  * every stream and every recorded graph: none recorded over them may be replayed after. The host linears' workspaces
  * stay (lkh_release_workspaces). Synchronizes the device (cuda/moe/moe_gguf.cu:104-118). */

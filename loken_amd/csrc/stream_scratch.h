@@ -24,6 +24,8 @@ enum LkScratchUse {
     LK_SCRATCH_LINEAR,     // host linear: quantized rows
     LK_SCRATCH_FIXUP,      // tiled matmul: partial products of a cut K
     LK_SCRATCH_TOKENS,     // f16 tiles: token operands
+    LK_SCRATCH_SAMPLE,     // sampling: a row's largest words and histogram
+    LK_SCRATCH_ATTENTION,  // attention: partial results of a split context
     LK_SCRATCH_USES
 };
 

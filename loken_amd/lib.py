@@ -164,6 +164,11 @@ SIGNATURES.update({
     "loken_rms_quantize_q8_1_bf16": (None, [_vp, _vp, _vp, _i, _f, _vp]),
     "lk_moe_fold": (_i, [_vp, _vp, _vp, _i, _vp, _i64, _i, _i, _i, _vp]),
     "loken_moe_mmq_fold": (None, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _vp]),
+    "lk_kv_plan": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp]),
+    "lk_kv_write_q8": (_i, [_vp, _vp, _i, _i64, _i64, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "lk_kv_read_q8": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "lk_kv_attention_q8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _vp, _i64, _i, _vp, _vp] + [_i] * 7 + [_f, _i, _vp]),
+    "lk_sample": (_i, [_vp, _i, _i64, _i, _i] + [_vp] * 8),
 })
 
 _lib = None
