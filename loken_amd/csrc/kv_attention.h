@@ -1,0 +1,73 @@
+// What the kernels of lk_kv_attention_q8 share: the call, which rows and positions a workgroup has, and partial results.
+#pragma once
+#include <math.h>
+
+#include "kv_cache.h"
+
+constexpr int KV_TILE = 64;   // positions of a step
+
+struct Attend {
+    const void* q;
+    void* out;
+    int64_t q_stride, out_stride;
+    KvPool pool;
+    const int32_t *table, *lens, *starts;
+    int64_t table_stride;
+    int table_cols, seqs, rows, heads, group, window;
+    float scale;
+    // A context is cut into at most `splits` parts of at least `least_tiles` steps. With more than one the parts meet through
+    // part_o [rows][heads][splits][head_dim] (sums relative to the part's maximum) and part_ml [rows][heads][splits] (that
+    // maximum in powers of two, and the sum of weights); rows are those of the batch, or part_seq for each sequence (one
+    // that has more is not cut).
+    int splits, least_tiles, part_seq;
+    float* part_o;
+    float2* part_ml;
+    // The few-rows kernel takes the sequences of up to so many rows (token, head of the group), the other kernel the rest.
+    int few_rows;
+    __device__ __forceinline__ int64_t part_row(int seq, const struct KvSeq& s, int row) const;
+};
+
+// The rows of a sequence, as far as the batch holds them.
+struct KvSeq {
+    int first, end;        // rows [first, end)
+    int64_t pos_of_0;      // position of row r is pos_of_0 + r
+    int64_t limit;         // positions that the table has columns for
+    __device__ __forceinline__ KvSeq(const Attend& a, int seq) {
+        const int s = a.starts[seq], e = a.starts[seq + 1];
+        first = max(s, 0);
+        end = min(e, a.rows);
+        pos_of_0 = (int64_t)a.lens[seq] - e;
+        limit = (int64_t)a.table_cols << a.pool.page_shift;
+    }
+    __device__ __forceinline__ int tokens() const { return max(end - first, 0); }
+};
+
+__device__ __forceinline__ int64_t Attend::part_row(int seq, const KvSeq& s, int row) const {
+    return part_seq ? (int64_t)seq * part_seq + (row - s.first) : row;
+}
+
+// Steps [0, tiles) from position `lo` on cover what rows ra .. rb see.
+struct KvSpan {
+    int lo, hi, tiles;     // positions lo (a multiple of the step) .. hi - 1
+    int per_part, parts;   // steps of a part, and how many parts
+    __device__ __forceinline__ KvSpan(const Attend& a, const KvSeq& s, int ra, int rb) {
+        const int64_t pa = s.pos_of_0 + ra, pb = s.pos_of_0 + rb;
+        hi = (int)max((int64_t)0, min(pb + 1, s.limit));
+        lo = a.window > 0 ? (int)max((int64_t)0, pa - a.window + 1) & ~(KV_TILE - 1) : 0;
+        tiles = hi > lo ? (hi - lo + KV_TILE - 1) / KV_TILE : 0;
+        const bool whole = a.splits == 1 || (a.part_seq && s.tokens() > a.part_seq);
+        per_part = whole ? max(tiles, 1) : max(a.least_tiles, (tiles + a.splits - 1) / a.splits);
+        parts = max(1, (tiles + per_part - 1) / per_part);
+    }
+};
+
+// Rows of a workgroup of the two kernels. The few-rows one takes two operands' rows in one pass over the keys where there are
+// that many and the registers hold them (256 columns: not).
+constexpr int KV_MANY_ROWS = 128;
+constexpr int kv_few_rows(bool f32, int head_dim, int max_rows) {
+    const int one = f32 ? 4 : 8;
+    return head_dim < 256 && max_rows > one ? 2 * one : one;
+}
+
+int kv_attention_few(const Attend& a, int type, int head_dim, int max_rows, hipStream_t stream);
+int kv_attention_many(const Attend& a, int type, int head_dim, int max_rows, hipStream_t stream);

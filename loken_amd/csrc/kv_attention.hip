@@ -1,82 +1,69 @@
-// Attention over the paged 8-bit cache (lk_kv_attention_q8).
+// Attention over the paged 8-bit cache (lk_kv_attention_q8): which kernel takes a sequence, how contexts are cut into parts,
+// and the launch that joins the parts.
 
-#include <math.h>
-
-#include "kv_cache.h"
+#include "kv_attention.h"
+#include "stream_scratch.h"
 
 namespace {
 
-struct Attend {
-    const void* q;
-    void* out;
-    int64_t q_stride, out_stride;
-    KvPool pool;
-    const int32_t *table, *lens, *starts;
-    int64_t table_stride;
-    int table_cols, rows, heads, group, window;
-    float scale;
-};
-
-// One wave to a row and head: sixty-four positions at a time, a lane to a position for the scores, a lane to
-// a column for the sums.
+// The parts of a row's context: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A wave to a row and head, rows of a workgroup of the
+// launch before (`per` of them) having the same parts.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void kv_attention_row_kernel(Attend a, int seqs) {
+__global__ __launch_bounds__(256) void kv_join_kernel(Attend a, int per, bool few, int tokens) {
     constexpr int PER = D / 64;
-    __shared__ float q_lds[D], p_lds[64];
-    const int lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y, kv = head / a.group;
-    int seq = -1;
-    for (int i = lane; i < seqs; i += 64)
-        if (a.starts[i] <= row && row < a.starts[i + 1]) seq = i;
-    for (int o = 32; o; o >>= 1) seq = max(seq, __shfl_xor(seq, o));
-    if (seq < 0) return;
-    const int shift = a.pool.page_shift, P = 1 << shift;
-    const int64_t pos = (int64_t)a.lens[seq] - (a.starts[seq + 1] - row);
-    const int64_t last = min(pos, ((int64_t)a.table_cols << shift) - 1);
-    const int64_t first = a.window > 0 ? max((int64_t)0, pos - a.window + 1) : 0;
-    for (int i = 0; i < PER; ++i) q_lds[lane + 64 * i] = to_f32(((const T*)a.q)[row * a.q_stride + head * D + lane + 64 * i]) * a.scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, acc[PER] = {};
-    for (int64_t j0 = first & ~(int64_t)63; j0 <= last; j0 += 64) {
-        const int64_t j = j0 + lane;
-        const int64_t page = j >= first && j <= last ? a.table[seq * a.table_stride + (j >> shift)] : -1;
-        const bool seen = page >= 0 && page < a.pool.pages;
-        const int64_t at = (seen ? page : 0) * a.pool.heads + kv;
-        float s = -INFINITY;
-        if (seen) {
-            const int8_t* k = a.pool.k + ((at << shift) + (j & (P - 1))) * D;
-            float dot = 0.f;
-            for (int d = 0; d < D; ++d) dot += q_lds[d] * (float)k[d];
-            s = dot * a.pool.k_scales[at];
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t seq = item / ((int64_t)tokens * a.heads);
+    if (seq >= a.seqs) return;
+    const int head = (int)(item % a.heads);
+    const KvSeq s(a, (int)seq);
+    const int64_t all_rows = (int64_t)s.tokens() * a.group;
+    if ((all_rows <= a.few_rows) != few) return;
+    for (int tok = (int)(item / a.heads % tokens); tok < s.tokens(); tok += tokens) {
+        const int64_t r0 = ((int64_t)tok * a.group + head % a.group) / per * per, r1 = min(r0 + per, all_rows) - 1;
+        const KvSpan span(a, s, s.first + (int)(r0 / a.group), s.first + (int)(r1 / a.group));
+        const int parts = span.parts;
+        if (parts == 1) continue;
+        const int64_t from = (a.part_row((int)seq, s, s.first + tok) * a.heads + head) * a.splits;
+        float m = -INFINITY;
+        for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.part_ml[from + p].x);
+        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        float l = 0.f, acc[PER] = {};
+        for (int p = 0; p < parts; ++p) {
+            const float2 ml = a.part_ml[from + p];
+            // (a part whose scores are no numbers has no maximum and a sum that is none)
+            const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
+            l += ml.x == -INFINITY ? ml.y : ml.y * f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) acc[i] += f == 0.f ? 0.f : a.part_o[(from + p) * D + lane + 64 * i] * f;
         }
-        float top = s;
-        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const float m_new = fmaxf(m, top), keep = m_new == -INFINITY ? 1.f : expf(m - m_new);
-        const float p = seen ? expf(s - m_new) : 0.f;
-        l = l * keep + wave_sum(p);
-        m = m_new;
-        for (int i = 0; i < PER; ++i) acc[i] *= keep;
-        p_lds[lane] = seen ? p * a.pool.v_scales[at] : 0.f;
-        __syncthreads();
-        for (int b = 0; b < 4; ++b) {
-            const int64_t jb = min(j0 + 16 * b, last);
-            int64_t vp = a.table[seq * a.table_stride + (jb >> shift)];
-            if (vp < 0 || vp >= a.pool.pages) vp = 0;
-            const int8_t* v = a.pool.v + ((vp * a.pool.heads + kv) << shift) * D + ((jb & (P - 1)) >> 4) * D * 16;
-            for (int t = 0; t < 16; ++t)
-                for (int i = 0; i < PER; ++i) acc[i] += p_lds[16 * b + t] * (float)v[(lane + 64 * i) * 16 + t];
-        }
-        __syncthreads();
+        T* out = (T*)a.out + (int64_t)(s.first + tok) * a.out_stride + (int64_t)head * D + lane;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) out[64 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
     }
-    for (int i = 0; i < PER; ++i)
-        ((T*)a.out)[row * a.out_stride + head * D + lane + 64 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
 }
 
 template <typename T>
-static void launch(const Attend& a, int seqs, int head_dim, hipStream_t s) {
-    const dim3 grid(a.rows, a.heads);
-    if (head_dim == 64) hipLaunchKernelGGL((kv_attention_row_kernel<T, 64>), grid, dim3(64), 0, s, a, seqs);
-    else if (head_dim == 128) hipLaunchKernelGGL((kv_attention_row_kernel<T, 128>), grid, dim3(64), 0, s, a, seqs);
-    else hipLaunchKernelGGL((kv_attention_row_kernel<T, 256>), grid, dim3(64), 0, s, a, seqs);
+static int join(const Attend& a, int head_dim, int per, bool few, int tokens, hipStream_t s) {
+    const int64_t blocks = ((int64_t)a.seqs * tokens * a.heads + 3) / 4;
+    if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
+    const dim3 grid((unsigned)blocks);
+    if (head_dim == 64) hipLaunchKernelGGL((kv_join_kernel<T, 64>), grid, dim3(256), 0, s, a, per, few, tokens);
+    else if (head_dim == 128) hipLaunchKernelGGL((kv_join_kernel<T, 128>), grid, dim3(256), 0, s, a, per, few, tokens);
+    else hipLaunchKernelGGL((kv_join_kernel<T, 256>), grid, dim3(256), 0, s, a, per, few, tokens);
+    return lk_launch_status();
+}
+
+// Sequences of up to this many rows (token, head of a group) are the few-rows kernel's.
+constexpr int FEW_ROWS = 16;
+
+// Parts of a context of `tiles` steps for `groups` workgroups of one part each: until there are `want` workgroups, of at
+// least `least` steps.
+static void cut(Attend& a, int64_t groups, int tiles, int want, int least) {
+    int64_t parts = (want + groups - 1) / groups;
+    parts = parts < (tiles + least - 1) / least ? parts : (tiles + least - 1) / least;
+    a.splits = parts < 1 ? 1 : (int)parts;
+    a.least_tiles = tiles > a.splits ? (tiles + a.splits - 1) / a.splits : 1;
 }
 
 }  // namespace
@@ -97,10 +84,54 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     if (!q || !out || !lens || !starts || (table_cols > 0 && !table) || (((uintptr_t)q | (uintptr_t)out) & (size - 1)) || q_stride < row ||
         out_stride < row)
         return LK_ERR_ARG;
+    if ((int64_t)table_cols * page_tokens > 0x7FFFFF00) return LK_ERR_SIZE;   // positions and what is added to them fit 32 bits
+    hipStream_t s = (hipStream_t)stream;
+    const int group = heads / kv_heads;
     const Attend a{q, out, q_stride, out_stride, {(int8_t*)k_codes, (int8_t*)v_codes, (float*)k_scales, (float*)v_scales, pages, kv_heads, kv_log2(page_tokens)},
-                   table, lens, starts, table_stride, table_cols, rows, heads, heads / kv_heads, window, scale};
-    if (type == LK_TYPE_F32) launch<float>(a, seqs, head_dim, (hipStream_t)stream);
-    else if (type == LK_TYPE_F16) launch<__half>(a, seqs, head_dim, (hipStream_t)stream);
-    else launch<__hip_bfloat16>(a, seqs, head_dim, (hipStream_t)stream);
-    return lk_launch_status();
+                   table, lens, starts, table_stride, table_cols, seqs, rows, heads, group, window, scale, 1, 1, 0, nullptr, nullptr, 0};
+    // What the caller says of the sizes chooses launches; whatever the sequences are, one of the kernels takes each.
+    const int tokens = max_fresh < 1 ? 1 : max_fresh < rows ? max_fresh : rows;
+    const int64_t most_rows = (int64_t)tokens * group;
+    const int max_rows = most_rows < 0x7FFFFFFF ? (int)most_rows : 0x7FFFFFFF;
+    const bool many = max_rows > FEW_ROWS, few = group <= FEW_ROWS && (!many || seqs > 1);
+    const int64_t table_tokens = (int64_t)table_cols * page_tokens;
+    const int64_t seen = window > 0 && window < max_len ? (int64_t)window + tokens : max_len;
+    const int tiles = (int)((min(seen, table_tokens) + KV_TILE - 1) / KV_TILE);
+    Attend af = a, am = a;
+    const int few_max = many ? FEW_ROWS : max_rows, few_per = kv_few_rows(type == LK_TYPE_F32, head_dim, few_max);
+    const int cus = lk_device().cus;
+    size_t rows_f = 0, rows_m = 0;   // whose parts are kept
+    if (few) {
+        af.few_rows = many ? FEW_ROWS : 0x7FFFFFFF;
+        cut(af, (int64_t)seqs * kv_heads * ((few_max + few_per - 1) / few_per), tiles, 4 * cus, 16);
+        af.part_seq = many ? FEW_ROWS / group : tokens;
+        if (af.splits > 1) rows_f = (size_t)seqs * af.part_seq;
+    }
+    if (many) {
+        am.few_rows = few ? FEW_ROWS : 0;
+        cut(am, ((int64_t)rows * group + KV_MANY_ROWS - 1) / KV_MANY_ROWS * kv_heads, tiles, 2 * cus, 16);
+        if (am.splits > 1) rows_m = rows;
+    }
+    LkScratch scratch(s);
+    const size_t floats_f = rows_f * heads * af.splits * (head_dim + 2), floats_m = rows_m * heads * am.splits * (head_dim + 2);
+    if (floats_f + floats_m) {
+        float* mem = (float*)scratch.get(LK_SCRATCH_ATTENTION, (floats_f + floats_m) * 4);
+        if (!mem) return LK_ERR_NOMEM;
+        af.part_ml = (float2*)mem;
+        af.part_o = mem + rows_f * heads * af.splits * 2;
+        mem += floats_f;
+        am.part_ml = (float2*)mem;
+        am.part_o = mem + rows_m * heads * am.splits * 2;
+    }
+    auto join_parts = [&](const Attend& x, int per, bool is_few, int toks) {
+        if (type == LK_TYPE_F32) return join<float>(x, head_dim, per, is_few, toks, s);
+        if (type == LK_TYPE_F16) return join<__half>(x, head_dim, per, is_few, toks, s);
+        return join<__hip_bfloat16>(x, head_dim, per, is_few, toks, s);
+    };
+    int status = LK_OK;
+    if (many) status = kv_attention_many(am, type, head_dim, max_rows, s);
+    if (status == LK_OK && few) status = kv_attention_few(af, type, head_dim, few_max, s);
+    if (status == LK_OK && many && am.splits > 1) status = join_parts(am, KV_MANY_ROWS, false, tokens);
+    if (status == LK_OK && few && af.splits > 1) status = join_parts(af, few_per, true, af.part_seq);
+    return status;
 }

@@ -143,12 +143,12 @@ def test_lengths_past_the_end_of_the_table(fresh, dtype):
 def test_starts_past_the_batch_are_cut():
     """A plan of more rows than the batch holds: those that it holds are computed, nothing is written behind it."""
     b = Batch([40, 60], [10, 20], 2, 1, 64, 16, "f32", seed=12)
-    full = b.check()
-    short = torch.full((25, 2, 64), 7.0, device="cuda")
     guard = torch.full((40, 2, 64), 9.0, device="cuda")
-    out = guard[:17]
-    kv.kv_attention(b.q[:17].cuda().contiguous(), b.cache(), i32(b.table), i32(b.lens), i32(b.starts), max_fresh=20, max_len=60, out=out)
-    assert torch.equal(out, full[:17]) and (guard[17:] == 9).all() and (short == 7).all()
+    kv.kv_attention(b.q[:17].cuda().contiguous(), b.cache(), i32(b.table), i32(b.lens), i32(b.starts), max_fresh=20, max_len=60, out=guard[:17])
+    assert (guard[17:] == 9).all()
+    # the seven rows that are left of the second sequence are few enough for another kernel: held to the definition, not to its bits
+    b.q, b.rows = b.q[:17], 17
+    assert torch.equal(b.check(max_fresh=20, max_len=60), guard[:17])
 
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
