@@ -6,51 +6,79 @@
 
 namespace {
 
-// The parts of a row's context: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A wave to a row and head, rows of a workgroup of the
-// launch before (`per` of them) having the same parts.
+constexpr int MOST_PARTS = 1024, JOIN_WAVES = 4;
+
+// The parts of a row's context: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A workgroup to a row and head (rows of a workgroup of
+// the launch before, `per` of them, have the same parts), its waves taking parts in turn, eight parts' loads in flight: with one after
+// the other 128 parts of one row took 88 us.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(Attend a, int per, bool few, int tokens) {
-    constexpr int PER = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t seq = item / ((int64_t)tokens * a.heads);
-    if (seq >= a.seqs) return;
-    const int head = (int)(item % a.heads);
-    const KvSeq s(a, (int)seq);
+__global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_kernel(Attend a, int per, bool few, int tokens) {
+    constexpr int PER = D / 64, AHEAD = 8;
+    __shared__ float share[MOST_PARTS], sums[JOIN_WAVES][D], meet[JOIN_WAVES][2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int head = blockIdx.x % a.heads, seq = blockIdx.x / a.heads / tokens;
+    const KvSeq s(a, seq);
     const int64_t all_rows = (int64_t)s.tokens() * a.group;
     if ((all_rows <= a.few_rows) != few) return;
-    for (int tok = (int)(item / a.heads % tokens); tok < s.tokens(); tok += tokens) {
+    for (int tok = blockIdx.x / a.heads % tokens; tok < s.tokens(); tok += tokens) {
         const int64_t r0 = ((int64_t)tok * a.group + head % a.group) / per * per, r1 = min(r0 + per, all_rows) - 1;
         const KvSpan span(a, s, s.first + (int)(r0 / a.group), s.first + (int)(r1 / a.group));
-        const int parts = span.parts;
+        const int parts = span.parts;   // at most a.splits
         if (parts == 1) continue;
-        const int64_t from = (a.part_row((int)seq, s, s.first + tok) * a.heads + head) * a.splits;
+        const int64_t from = (a.part_row(seq, s, s.first + tok) * a.heads + head) * a.splits;
         float m = -INFINITY;
-        for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.part_ml[from + p].x);
+        for (int p = threadIdx.x; p < parts; p += 64 * JOIN_WAVES) m = fmaxf(m, a.part_ml[from + p].x);
         for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        float l = 0.f, acc[PER] = {};
-        for (int p = 0; p < parts; ++p) {
+        if (lane == 0) meet[wave][0] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(meet[0][0], meet[1][0]), fmaxf(meet[2][0], meet[3][0]));
+        float l = 0.f;
+        for (int p = threadIdx.x; p < parts; p += 64 * JOIN_WAVES) {
             const float2 ml = a.part_ml[from + p];
             // (a part whose scores are no numbers has no maximum and a sum that is none)
             const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
             l += ml.x == -INFINITY ? ml.y : ml.y * f;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) acc[i] += f == 0.f ? 0.f : a.part_o[(from + p) * D + lane + 64 * i] * f;
+            share[p] = f;
         }
-        T* out = (T*)a.out + (int64_t)(s.first + tok) * a.out_stride + (int64_t)head * D + lane;
+        l = wave_sum(l);
+        if (lane == 0) meet[wave][1] = l;
+        __syncthreads();
+        l = (meet[0][1] + meet[1][1]) + (meet[2][1] + meet[3][1]);
+        float acc[PER] = {};
+        for (int p0 = wave; p0 < parts; p0 += AHEAD * JOIN_WAVES) {
+            float x[AHEAD][PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) out[64 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
+            for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                for (int i = 0; i < PER; ++i) x[j][i] = a.part_o[(from + min(p0 + j * JOIN_WAVES, parts - 1)) * D + lane + 64 * i];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+                if (p0 + j * JOIN_WAVES < parts) {
+                    const float f = share[p0 + j * JOIN_WAVES];
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) acc[i] = fmaf(x[j][i], f, acc[i]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sums[wave][lane + 64 * i] = acc[i];
+        __syncthreads();
+        T* out = (T*)a.out + (int64_t)(s.first + tok) * a.out_stride + (int64_t)head * D;
+        for (int d = threadIdx.x; d < D; d += 64 * JOIN_WAVES) {
+            const float total = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
+            out[d] = from_f32<T>(l == 0.f ? 0.f : total / l);
+        }
+        __syncthreads();
     }
 }
 
 template <typename T>
 static int join(const Attend& a, int head_dim, int per, bool few, int tokens, hipStream_t s) {
-    const int64_t blocks = ((int64_t)a.seqs * tokens * a.heads + 3) / 4;
+    const int64_t blocks = (int64_t)a.seqs * tokens * a.heads;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
     const dim3 grid((unsigned)blocks);
-    if (head_dim == 64) hipLaunchKernelGGL((kv_join_kernel<T, 64>), grid, dim3(256), 0, s, a, per, few, tokens);
-    else if (head_dim == 128) hipLaunchKernelGGL((kv_join_kernel<T, 128>), grid, dim3(256), 0, s, a, per, few, tokens);
-    else hipLaunchKernelGGL((kv_join_kernel<T, 256>), grid, dim3(256), 0, s, a, per, few, tokens);
+    if (head_dim == 64) hipLaunchKernelGGL((kv_join_kernel<T, 64>), grid, dim3(64 * JOIN_WAVES), 0, s, a, per, few, tokens);
+    else if (head_dim == 128) hipLaunchKernelGGL((kv_join_kernel<T, 128>), grid, dim3(64 * JOIN_WAVES), 0, s, a, per, few, tokens);
+    else hipLaunchKernelGGL((kv_join_kernel<T, 256>), grid, dim3(64 * JOIN_WAVES), 0, s, a, per, few, tokens);
     return lk_launch_status();
 }
 
@@ -62,7 +90,7 @@ constexpr int FEW_ROWS = 16;
 static void cut(Attend& a, int64_t groups, int tiles, int want, int least) {
     int64_t parts = (want + groups - 1) / groups;
     parts = parts < (tiles + least - 1) / least ? parts : (tiles + least - 1) / least;
-    a.splits = parts < 1 ? 1 : (int)parts;
+    a.splits = parts < 1 ? 1 : parts < MOST_PARTS ? (int)parts : MOST_PARTS;
     a.least_tiles = tiles > a.splits ? (tiles + a.splits - 1) / a.splits : 1;
 }
 

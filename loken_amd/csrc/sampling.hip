@@ -2,13 +2,18 @@
 //
 // All three rules keep a prefix of the words in falling order of their logits, so a row needs no sorted vocabulary:
 // the kept words' weight is S = min(S_k, S_p, S_m) of the three rules' prefixes, and the token is the first word
-// whose running sum reaches floor(u S) + 1. Each of S_k, S_p and the token is one search in the running sums, by number or by
-// weight: first in a histogram of the row over 2048 steps of the logit, then among the words of one step, which are gathered and
-// sorted in LDS.
+// whose running sum reaches floor(u S) + 1. Three launches, each over pieces of rows:
+//   peak     the row's largest word, and its smallest
+//   steps    a histogram of the row over 2048 steps of the logit: numbers of words, their weights, or both
+//   choose   from the running sums over the steps: in which steps S_k, S_p and the token lie. Their words are gathered (a few
+//            hundred of a vocabulary), and the last workgroup of the row sorts them and makes the choice.
+// Where those steps hold more words than are sorted at once (thousands of equal logits), that workgroup searches the row
+// itself, in steps of steps.
 //
 // Weights 2^x, x = (logit - M) log2(e) / T, decide between neighbours whose shares differ by one part in a million and
-// less, so they are made to 1e-10 and summed exactly, as integers of 2^-42 (2^20 words of weight 1 fit 64 bits). Sums of
-// integers do not depend on the order in which the LDS and global adds land.
+// less: were the sums off by 1e-10, one draw in 1e5 from a vocabulary of 1.5e5 words would give the next word. They are made to
+// 2e-13 and summed exactly, as integers of 2^-42 (2^20 words of weight 1 fit 64 bits). Sums of integers do not depend on the order
+// in which the LDS and global adds land.
 
 #include <math.h>
 
@@ -34,20 +39,29 @@ static __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key ^ ((int)key < 0 ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// Calls f(value, index) for the words begin + thread, begin + thread + threads, .. below `end` of a row.
-template <typename T, class F>
+// Calls f(value, index) for the words begin .. end - 1 of a row, sixteen bytes a load, the loads of AHEAD out before the first is used.
+template <int AHEAD, typename T, class F>
 static __device__ __forceinline__ void each_word(const T* __restrict__ row, int begin, int end, F f) {
-    constexpr int AHEAD = 8;
-    const int step = blockDim.x;
-    int i = begin + threadIdx.x;
-    for (; i + (AHEAD - 1) * step < end; i += AHEAD * step) {
-        T raw[AHEAD];
+    constexpr int VEC = 16 / sizeof(T);
+    struct __attribute__((aligned(sizeof(T)))) Load { T v[VEC]; };   // rows start on any word
+    const int step = SAMPLE_WG * VEC;
+    int i = begin + (int)threadIdx.x * VEC;
+    for (; i + (AHEAD - 1) * step + VEC <= end; i += AHEAD * step) {
+        Load raw[AHEAD];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) raw[j] = row[i + j * step];
+        for (int j = 0; j < AHEAD; ++j) raw[j] = *(const Load*)(row + i + j * step);
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) f(to_f32(raw[j]), i + j * step);
+        for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f(to_f32(raw[j].v[e]), i + j * step + e);
     }
-    for (; i < end; i += step) f(to_f32(row[i]), i);
+    for (; i + VEC <= end; i += step) {
+        const Load raw = *(const Load*)(row + i);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f(to_f32(raw.v[e]), i + e);
+    }
+    const int rest = end - (end - begin) % VEC + (int)threadIdx.x;
+    if (rest < end) f(to_f32(row[rest]), rest);
 }
 
 struct Peak {
@@ -74,10 +88,12 @@ struct Sampling {
     int32_t* tokens;
     float* probs;
     Peak* peaks;          // [rows][chunks]
-    uint64_t* mass;       // [rows][BINS], where a row has several chunks
+    uint64_t* mass;       // [rows][BINS]
     uint32_t* count;      // [rows][BINS]
     uint64_t* floor_mass; // [rows]: what min-p keeps
-    uint32_t* arrived;    // [rows]
+    uint64_t* list;       // [rows][LIST]: gathered words
+    uint32_t* listed;     // [rows]: how many there are
+    uint32_t* arrived;    // [rows]: workgroups that have gathered
 };
 
 // The largest and the smallest word of a piece of a row; clears the row's histogram on the way.
@@ -85,22 +101,20 @@ template <typename T>
 __global__ __launch_bounds__(SAMPLE_WG) void sample_peak_kernel(Sampling a) {
     __shared__ Peak meet[SAMPLE_WAVES];
     const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
-    Peak p{0, 0xFFFFFFFFu, 0};
-    each_word((const T*)a.logits + row * a.stride, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](float v, int i) {
-        if (v > -INFINITY) {
-            const uint32_t key = key_of(v);
-            const uint64_t word = (uint64_t)key << 32 | (uint32_t)~i;
-            p.best = word > p.best ? word : p.best;
-            p.lowest = key < p.lowest ? key : p.lowest;
-        }
+    float best = -INFINITY, lowest = INFINITY;
+    int at = 0x7FFFFFFF;
+    each_word<4>((const T*)a.logits + row * a.stride, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](float v, int i) {
+        const bool more = v > best;   // a thread meets the words in rising order
+        best = more ? v : best;
+        at = more ? i : at;
+        lowest = v > -INFINITY ? fminf(lowest, v) : lowest;   // (fminf passes over what is not a number)
     });
-    if (a.chunks > 1) {
-        for (int i = c * SAMPLE_WG + t; i < BINS; i += a.chunks * SAMPLE_WG) {
-            a.mass[(int64_t)row * BINS + i] = 0;
-            a.count[(int64_t)row * BINS + i] = 0;
-        }
-        if (c == 0 && t == 0) { a.floor_mass[row] = 0; a.arrived[row] = 0; }
+    for (int i = c * SAMPLE_WG + t; i < BINS; i += a.chunks * SAMPLE_WG) {
+        a.mass[(int64_t)row * BINS + i] = 0;
+        a.count[(int64_t)row * BINS + i] = 0;
     }
+    if (c == 0 && t == 0) { a.floor_mass[row] = 0; a.listed[row] = 0; a.arrived[row] = 0; }
+    Peak p{best > -INFINITY ? (uint64_t)key_of(best) << 32 | (uint32_t)~at : 0, key_of(lowest), 0};
     wave_peak(p);
     if ((t & 63) == 0) meet[t >> 6] = p;
     __syncthreads();
@@ -110,42 +124,88 @@ __global__ __launch_bounds__(SAMPLE_WG) void sample_peak_kernel(Sampling a) {
     if (t == 0) a.peaks[(int64_t)row * a.chunks + c] = p;
 }
 
+// 2^x, -43 <= x <= 0, as an integer of 2^-42. x = n + r, |r| <= 1/2; of the series of e^(r ln 2) the terms up to the fifth in 64
+// bits, the sixth to the tenth, which are below 2.4e-6 of it, in 32; what is left out is below 2.2e-13.
+static __device__ __forceinline__ uint64_t weight_of(double x) {
+    const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
+    const double y = x + magic;
+    const int n = (int)(uint32_t)__double_as_longlong(y);
+    const double r = (x - (y - magic)) * 0.6931471805599453;
+    const float s = (float)r;
+    const float high = fmaf(s, fmaf(s, fmaf(s, fmaf(s, 1.0f / 3628800.0f, 1.0f / 362880.0f), 1.0f / 40320.0f), 1.0f / 5040.0f), 1.0f / 720.0f);
+    double p = fma(r, (double)high, 1.0 / 120.0);
+    p = fma(r, p, 1.0 / 24.0);
+    p = fma(r, p, 1.0 / 6.0);
+    p = fma(r, p, 0.5);
+    p = fma(r, p, 1.0);
+    p = fma(r, p, 1.0);
+    // times 2^n in the exponent; 1024 more, and the last place is 2^-42: what the sum rounds to is the integer
+    const uint64_t scaled = (uint64_t)__double_as_longlong(p) + ((uint64_t)(uint32_t)(n << 20) << 32);
+    return (uint64_t)__double_as_longlong(__longlong_as_double((long long)scaled) + 1024.0) - 0x4090000000000000ull;
+}
+
 // What a row's weights and steps go by.
 struct Scale {
-    float top;        // M
+    float top;        // M; where it is infinite the words that are too count as 0, all others as none
     double rate;      // log2(e) / T
+    double top_rate;  // M times that
     float reach;      // words further below the top weigh nothing
     float steps;      // steps of the histogram per unit of the logit
     double least;     // log2(min_p)
-    __device__ __forceinline__ bool live(float v) const { return v > -INFINITY && (v == top || top - v <= reach); }
-    __device__ __forceinline__ int bin(float v) const {
-        const float at = (top - v) * steps;
-        return v == top ? 0 : at < (float)(BINS - 1) ? (int)at : BINS - 1;
+    bool infinite;
+
+    // From the row's peaks; false where there is nothing to weigh (no words, or the first of them is the choice).
+    __device__ __forceinline__ bool init(const Peak& peak, float temperature, float min_p) {
+        if (peak.best == 0 || !(temperature > 0.0f)) return false;
+        top = value_of((uint32_t)(peak.best >> 32));
+        infinite = top == INFINITY;
+        float lowest = value_of(peak.lowest);
+        if (infinite) top = lowest = 0.0f;
+        rate = 1.4426950408889634 / (double)temperature;
+        top_rate = (double)top * rate;
+        reach = fminf((float)(LIVE / rate), 3.402823466e38f);
+        const float range = fminf(reach, top - lowest);
+        steps = range > 0.0f ? (float)(BINS - 1) / range : 0.0f;
+        if (!(steps <= 3.402823466e38f)) steps = 3.402823466e38f;
+        least = min_p > 0.0f ? log2((double)min_p) : -1e300;
+        return true;
     }
-    __device__ __forceinline__ double power(float v) const { return v == top ? 0.0 : ((double)v - (double)top) * rate; }
+    // How far a word is below the top (not at all a number: for one that is none).
+    __device__ __forceinline__ float below(float v) const { return infinite ? (v == INFINITY ? 0.0f : NAN) : top - v; }
+    __device__ __forceinline__ bool live(float d) const { return d <= reach; }
+    // The step of a live word, as a number that has not been cut to an integer.
+    __device__ __forceinline__ float step(float d) const { return fminf(d * steps, (float)(BINS - 1)); }
+    __device__ __forceinline__ double power(float v) const { return infinite ? 0.0 : ((double)v - (double)top) * rate; }
 };
 
-// 2^x, -43 <= x <= 0, as an integer of 2^-42: x = n + i / 256 + r, 2^(i / 256) from a table in LDS, 2^r by three terms
-// (the fourth is below 2e-13) in 32 bits, whose error is 1e-10 of the result.
-static __device__ __forceinline__ uint64_t weight_of(double x, const double* table) {
-    const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
-    const double y = x * 256.0 + magic;
-    const int k = (int)(uint32_t)__double_as_longlong(y);
-    const float r = (float)fma(y - magic, -1.0 / 256.0, x);
-    const float p = r * fmaf(r, fmaf(r, 0.05550411f, 0.2402265f), 0.6931472f);
-    const double base = table[k & 255];
-    const uint64_t bits = (uint64_t)__double_as_longlong(fma(base, (double)p, base));   // just below 1 where r is below 0 at i = 0
-    const uint64_t m = (bits & 0xFFFFFFFFFFFFFull) | 0x10000000000000ull;
-    const int shift = 52 - ONE_BITS - (k >> 8) + 1023 - (int)(bits >> 52);
-    return (m + (1ull << (shift - 1))) >> shift;
+static __device__ __forceinline__ Peak peak_of_row(const Sampling& a, int row) {
+    Peak peak{0, 0xFFFFFFFFu, 0};
+    for (int i = threadIdx.x & 63; i < a.chunks; i += 64) {
+        const Peak p = a.peaks[(int64_t)row * a.chunks + i];
+        peak.best = p.best > peak.best ? p.best : peak.best;
+        peak.lowest = p.lowest < peak.lowest ? p.lowest : peak.lowest;
+    }
+    wave_peak(peak);
+    return peak;
 }
+
+// Whether a row's histogram counts words, and whether it weighs them. The top-k words, where they are few, are all
+// gathered: then their weights are taken from the list.
+struct Wants {
+    bool count, mass, above;
+    __device__ __forceinline__ Wants(const Sampling& a, int row) {
+        const int k = a.top_k ? a.top_k[row] : 0;
+        count = k > 0 && k < a.vocab;
+        mass = !(count && k <= LIST / 2);
+        above = mass && a.min_p && a.min_p[row] > 0.0f;
+    }
+};
 
 static_assert(BINS <= LIST, "the finer histogram stands where the list does");
 struct Shared {
     uint64_t mass[BINS];      // running sums once scanned
     uint32_t count[BINS];
     uint64_t list[LIST], sums[LIST];   // also a finer histogram, while there is no list
-    double table[256];
     uint64_t meet[SAMPLE_WAVES][2];
     uint64_t found;
     uint32_t low, high;
@@ -197,6 +257,47 @@ static __device__ __forceinline__ int first_reaching(const V* sums, int n, uint6
     return lo;
 }
 
+// Sorts the n <= LIST words of the list, the largest first, and gives their running sums of weights. A word's number is part of
+// what is compared, so the order the words came in does not show.
+static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale& sc) {
+    const int t = threadIdx.x;
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + t; i < size; i += SAMPLE_WG) sh.list[i] = 0;
+    __syncthreads();
+    for (int run = 2; run <= size; run <<= 1)
+        for (int gap = run >> 1; gap > 0; gap >>= 1) {
+            for (int j = t; j < size / 2; j += SAMPLE_WG) {
+                const int lo = 2 * j - (j & (gap - 1)), hi = lo + gap;
+                const uint64_t x = sh.list[lo], y = sh.list[hi];
+                if ((x < y) == ((lo & run) == 0)) { sh.list[lo] = y; sh.list[hi] = x; }
+            }
+            __syncthreads();
+        }
+    constexpr int PER = LIST / SAMPLE_WG;
+    uint64_t m[PER], ms = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = t * PER + i;
+        if (at < n) ms += weight_of(sc.power(value_of((uint32_t)(sh.list[at] >> 32))));
+        m[i] = ms;
+    }
+    const uint64_t before = sum_before(ms, sh.meet, 0);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (t * PER + i < n) sh.sums[t * PER + i] = before + m[i];
+    __syncthreads();
+}
+
+// floor(share * whole) + 1, at most `whole`, and ceil(share * whole), at least 1: the sums that the draw and top-p look for.
+static __device__ __forceinline__ uint64_t drawn_sum(float u, uint64_t whole) {
+    return min((uint64_t)floor((double)(u > 0.0f ? fminf(u, 1.0f) : 0.0f) * (double)whole) + 1, whole);
+}
+static __device__ __forceinline__ uint64_t nucleus_sum(float top_p, uint64_t whole) {
+    const double wanted = ceil((double)fmaxf(top_p, 0.0f) * (double)whole);
+    return wanted > 1.0 ? min((uint64_t)wanted, whole) : 1;
+}
+
 // A place in the row's order: the word, its weight, and the sum up to and with it.
 struct Place {
     int token;
@@ -222,43 +323,18 @@ struct Searcher {
         __syncthreads();
         if (t == 0) sh.n = 0;
         __syncthreads();
-        each_word(row, 0, vocab, [&](float v, int i) {
-            const int b = sc.bin(v);
+        each_word<2>(row, 0, vocab, [&](float v, int i) {
+            const float d = sc.below(v);
+            const int b = (int)sc.step(d);
             const uint32_t key = key_of(v);
-            if (sc.live(v) && b >= from && b <= to && key >= low && key <= high) {
+            if (sc.live(d) && b >= from && b <= to && key >= low && key <= high) {
                 const int at = atomicAdd(&sh.n, 1);
                 if (at < LIST) sh.list[at] = (uint64_t)key << 32 | (uint32_t)~i;
             }
         });
         __syncthreads();
         n = min(sh.n, LIST);
-        int size = 2;
-        while (size < n) size <<= 1;
-        for (int i = n + t; i < size; i += SAMPLE_WG) sh.list[i] = 0;
-        __syncthreads();
-        // sorted downwards; a word's number is part of what is compared, so the order the words came in does not show
-        for (int run = 2; run <= size; run <<= 1)
-            for (int gap = run >> 1; gap > 0; gap >>= 1) {
-                for (int j = t; j < size / 2; j += SAMPLE_WG) {
-                    const int lo = 2 * j - (j & (gap - 1)), hi = lo + gap;
-                    const uint64_t x = sh.list[lo], y = sh.list[hi];
-                    if ((x < y) == ((lo & run) == 0)) { sh.list[lo] = y; sh.list[hi] = x; }
-                }
-                __syncthreads();
-            }
-        constexpr int PER = LIST / SAMPLE_WG;
-        uint64_t m[PER], ms = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int at = t * PER + i;
-            if (at < n) ms += weight_of(sc.power(value_of((uint32_t)(sh.list[at] >> 32))), sh.table);
-            m[i] = ms;
-        }
-        const uint64_t before = sum_before(ms, sh.meet, 0);
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (t * PER + i < n) sh.sums[t * PER + i] = before + m[i];
-        __syncthreads();
+        sort_list(sh, n, sc);
     }
 
     // The word at which the running number (by_mass: the running weight) reaches `target` >= 1, which some word does.
@@ -286,9 +362,10 @@ struct Searcher {
                     for (int i = t; i < BINS; i += SAMPLE_WG) { sub_mass[i] = 0; sub_count[i] = 0; }
                     __syncthreads();
                     uint32_t lo = 0xFFFFFFFFu, hi = 0;
-                    each_word(row, 0, vocab, [&](float v, int) {
+                    each_word<2>(row, 0, vocab, [&](float v, int) {
                         const uint32_t key = key_of(v);
-                        const bool in = sc.live(v) && sc.bin(v) == b && key >= low && key <= high;
+                        const float d = sc.below(v);
+                        const bool in = sc.live(d) && (int)sc.step(d) == b && key >= low && key <= high;
                         lo = in ? min(lo, key) : lo;
                         hi = in ? max(hi, key) : hi;
                     });
@@ -300,11 +377,12 @@ struct Searcher {
                     if (low >= high) return equal(sh, high, by_mass, target);
                     int shift = 0;
                     while (((high - low) >> shift) >= BINS) ++shift;
-                    each_word(row, 0, vocab, [&](float v, int) {
+                    each_word<2>(row, 0, vocab, [&](float v, int) {
                         const uint32_t key = key_of(v);
-                        if (sc.live(v) && sc.bin(v) == b && key >= low && key <= high) {
+                        const float d = sc.below(v);
+                        if (sc.live(d) && (int)sc.step(d) == b && key >= low && key <= high) {
                             const uint32_t at = (high - key) >> shift;   // below BINS
-                            atomicAdd((unsigned long long*)&sub_mass[at], (unsigned long long)weight_of(sc.power(v), sh.table));
+                            atomicAdd((unsigned long long*)&sub_mass[at], (unsigned long long)weight_of(sc.power(v)));
                             atomicAdd(&sub_count[at], 1u);
                         }
                     });
@@ -331,7 +409,7 @@ struct Searcher {
     // More equal words than the list takes: the one whose turn it is, counted in the order of their numbers.
     __device__ __forceinline__ Place equal(Shared& sh, uint32_t key, bool by_mass, uint64_t target) {
         const int t = threadIdx.x;
-        const uint64_t w = weight_of(sc.power(value_of(key)), sh.table);
+        const uint64_t w = weight_of(sc.power(value_of(key)));
         const uint32_t turn = (uint32_t)(by_mass ? (target - base_mass + w - 1) / w : target - base_count);
         uint32_t passed = 0;
         b0 = b1 = -1;
@@ -358,80 +436,67 @@ struct Searcher {
     }
 };
 
+// The histogram of a piece of a row, into LDS arrays that are clear; the weight of what min-p keeps, of the thread's words.
 template <typename T>
-__global__ __launch_bounds__(SAMPLE_WG) void sample_kernel(Sampling a) {
-    __shared__ Shared sh;
-    __shared__ int is_last;
-    const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
-    const T* x = (const T*)a.logits + row * a.stride;
-    Peak peak{0, 0xFFFFFFFFu, 0};
-    for (int i = t & 63; i < a.chunks; i += 64) {
-        const Peak p = a.peaks[(int64_t)row * a.chunks + i];
-        peak.best = p.best > peak.best ? p.best : peak.best;
-        peak.lowest = p.lowest < peak.lowest ? p.lowest : peak.lowest;
-    }
-    wave_peak(peak);
-    const float temperature = a.temperature[row];
-    if (peak.best == 0 || !(temperature > 0.0f)) {   // no words, or the first of them
-        if (c == 0 && t == 0) {
-            a.tokens[row] = peak.best ? (int)~(uint32_t)peak.best : -1;
-            if (a.probs) a.probs[row] = peak.best ? 1.0f : 0.0f;
+static __device__ __forceinline__ uint64_t weigh(const T* x, int begin, int end, const Scale& sc, const Wants& wants, uint64_t* mass, uint32_t* count) {
+    uint64_t above = 0;
+    each_word<2>(x, begin, end, [&](float v, int) {
+        const float d = sc.below(v);
+        if (!sc.live(d)) return;
+        const int b = (int)sc.step(d);
+        if (wants.count) atomicAdd(&count[b], 1u);
+        if (wants.mass) {
+            const double power = sc.power(v);
+            const uint64_t w = weight_of(power);
+            atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w);
+            if (wants.above) above += power >= sc.least ? w : 0;
         }
-        return;
-    }
+    });
+    return above;
+}
+
+template <typename T>
+__global__ __launch_bounds__(SAMPLE_WG) void sample_steps_kernel(Sampling a) {
+    __shared__ uint64_t mass[BINS];
+    __shared__ uint32_t count[BINS];
+    const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     Scale sc;
-    sc.top = value_of((uint32_t)(peak.best >> 32));
-    sc.rate = 1.4426950408889634 / (double)temperature;
-    sc.reach = sc.top < INFINITY ? (float)(LIVE / sc.rate) : -1.0f;   // (beside an infinite word there is no other)
-    const float range = fminf(sc.reach, sc.top - value_of(peak.lowest));
-    sc.steps = range > 0.0f && range <= 3.402823466e38f ? (float)(BINS - 1) / range : 0.0f;
-    const float min_p = a.min_p ? a.min_p[row] : 0.0f;
-    sc.least = min_p > 0.0f ? log2((double)min_p) : -1e300;
-    if (t < 256) sh.table[t] = exp2((double)t / 256.0);
+    if (!sc.init(peak_of_row(a, row), a.temperature[row], a.min_p ? a.min_p[row] : 0.0f)) return;
+    const Wants wants(a, row);
+    for (int i = t; i < BINS; i += SAMPLE_WG) { mass[i] = 0; count[i] = 0; }
+    __syncthreads();
+    uint64_t above = weigh((const T*)a.logits + row * a.stride, c * a.chunk, min((c + 1) * a.chunk, a.vocab), sc, wants, mass, count);
+    if (wants.above) {
+        for (int o = 32; o; o >>= 1) above += __shfl_xor((unsigned long long)above, o);
+        if ((t & 63) == 0 && above) atomicAdd((unsigned long long*)&a.floor_mass[row], (unsigned long long)above);
+    }
+    __syncthreads();
+    for (int i = t; i < BINS; i += SAMPLE_WG) {
+        if (mass[i]) atomicAdd((unsigned long long*)&a.mass[(int64_t)row * BINS + i], (unsigned long long)mass[i]);
+        if (count[i]) atomicAdd(&a.count[(int64_t)row * BINS + i], count[i]);
+    }
+}
+
+// The choice by one workgroup alone, from the row itself: where the steps in question hold more words than are sorted at once.
+template <typename T>
+static __device__ __forceinline__ void choose_alone(const Sampling& a, int row, const Scale& sc, Shared& sh) {
+    const int t = threadIdx.x;
+    const T* x = (const T*)a.logits + row * a.stride;
+    __syncthreads();
     for (int i = t; i < BINS; i += SAMPLE_WG) { sh.mass[i] = 0; sh.count[i] = 0; }
     if (t == 0) sh.found = 0;
     __syncthreads();
-    uint64_t above = 0;   // what min-p keeps
-    each_word(x, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](float v, int) {
-        if (!sc.live(v)) return;
-        const double power = sc.power(v);
-        const uint64_t w = weight_of(power, sh.table);
-        const int b = sc.bin(v);
-        atomicAdd((unsigned long long*)&sh.mass[b], (unsigned long long)w);
-        atomicAdd(&sh.count[b], 1u);
-        above += power >= sc.least ? w : 0;
-    });
+    Wants wants(a, row);
+    wants.count = wants.mass = wants.above = true;
+    uint64_t above = weigh(x, 0, a.vocab, sc, wants, sh.mass, sh.count);
     for (int o = 32; o; o >>= 1) above += __shfl_xor((unsigned long long)above, o);
     if ((t & 63) == 0) atomicAdd((unsigned long long*)&sh.found, (unsigned long long)above);
     __syncthreads();
-    if (a.chunks > 1) {
-        uint64_t* mass = a.mass + (int64_t)row * BINS;
-        uint32_t* count = a.count + (int64_t)row * BINS;
-        for (int i = t; i < BINS; i += SAMPLE_WG)
-            if (sh.count[i]) {
-                atomicAdd((unsigned long long*)&mass[i], (unsigned long long)sh.mass[i]);
-                atomicAdd(&count[i], sh.count[i]);
-            }
-        if (t == 0) atomicAdd((unsigned long long*)&a.floor_mass[row], (unsigned long long)sh.found);
-        // this workgroup's adds are done before it is counted; the last one to be counted goes on with the row
-        __threadfence();
-        __syncthreads();
-        if (t == 0) is_last = atomicAdd(&a.arrived[row], 1u) == (uint32_t)a.chunks - 1;
-        __syncthreads();
-        if (!is_last) return;
-        __threadfence();
-        for (int i = t; i < BINS; i += SAMPLE_WG) {
-            sh.mass[i] = __hip_atomic_load(&mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            sh.count[i] = __hip_atomic_load(&count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        if (t == 0) sh.found = __hip_atomic_load(&a.floor_mass[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-    }
     const uint64_t one = 1ull << ONE_BITS, kept_m = sh.found > one ? sh.found : one;
     scan_bins(sh.mass, sh.count, sh.meet);
     Searcher<T> at{x, a.vocab, sc};
     const uint64_t words = sh.count[BINS - 1], k = a.top_k && a.top_k[row] > 0 ? (uint64_t)a.top_k[row] : words;
-    const float top_p = a.top_p ? a.top_p[row] : 1.0f, u = a.uniform[row];
+    const float top_p = a.top_p ? a.top_p[row] : 1.0f;
     uint64_t kept = sh.mass[BINS - 1];
 #pragma unroll 1
     for (int step = 0; step < 3; ++step) {   // top-k, top-p, the draw
@@ -439,12 +504,11 @@ __global__ __launch_bounds__(SAMPLE_WG) void sample_kernel(Sampling a) {
         if (step == 0 && k >= words) continue;
         if (step == 1) {
             if (!(top_p < 1.0f)) continue;
-            const double wanted = ceil((double)fmaxf(top_p, 0.0f) * (double)kept);
-            target = wanted > 1.0 ? min((uint64_t)wanted, kept) : 1;
+            target = nucleus_sum(top_p, kept);
         }
         if (step == 2) {
             kept = min(kept, kept_m);
-            target = min((uint64_t)floor((double)(u > 0.0f ? fminf(u, 1.0f) : 0.0f) * (double)kept) + 1, kept);
+            target = drawn_sum(a.uniform[row], kept);
         }
         const Place p = at.search(sh, step > 0, target);
         if (step < 2) {
@@ -457,10 +521,143 @@ __global__ __launch_bounds__(SAMPLE_WG) void sample_kernel(Sampling a) {
 }
 
 template <typename T>
+__global__ __launch_bounds__(SAMPLE_WG) void sample_choose_kernel(Sampling a) {
+    __shared__ Shared sh;
+    const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
+    const T* x = (const T*)a.logits + row * a.stride;
+    const Peak peak = peak_of_row(a, row);
+    Scale sc;
+    if (!sc.init(peak, a.temperature[row], a.min_p ? a.min_p[row] : 0.0f)) {   // no words, or the first of them
+        if (c == 0 && t == 0) {
+            a.tokens[row] = peak.best ? (int)~(uint32_t)peak.best : -1;
+            if (a.probs) a.probs[row] = peak.best ? 1.0f : 0.0f;
+        }
+        return;
+    }
+    const Wants wants(a, row);
+    for (int i = t; i < BINS; i += SAMPLE_WG) {
+        sh.mass[i] = wants.mass ? a.mass[(int64_t)row * BINS + i] : 0;
+        sh.count[i] = wants.count ? a.count[(int64_t)row * BINS + i] : 0;
+    }
+    __syncthreads();
+    scan_bins(sh.mass, sh.count, sh.meet);
+    const uint64_t one = 1ull << ONE_BITS, kept_m = wants.above ? max((uint64_t)a.floor_mass[row], one) : ~0ull;
+    const float top_p = a.top_p ? a.top_p[row] : 1.0f, u = a.uniform[row];
+    const int k = wants.count ? a.top_k[row] : 0;
+    const bool cut_k = wants.count && (uint32_t)k < sh.count[BINS - 1];
+    // The steps that are gathered: up to three ranges, the last one nearest to the top.
+    int from[3], to[3], ranges = 0;
+    if (!wants.mass) {   // the top-k words and the rest of their last step
+        from[0] = 0;
+        to[0] = first_reaching(sh.count, BINS, k);
+        ranges = 1;
+    } else {
+        auto take = [&](int lo, int hi) {   // each search's steps lie in front of those of the one before it, or touch them
+            if (ranges && hi >= from[ranges - 1] - 1) { from[ranges - 1] = min(from[ranges - 1], lo); to[ranges - 1] = max(to[ranges - 1], hi); }
+            else { from[ranges] = lo; to[ranges] = hi; ++ranges; }
+        };
+        auto before = [&](int b) { return b > 0 ? sh.mass[b - 1] : 0; };
+        uint64_t least = sh.mass[BINS - 1], most = least;   // bounds of what is kept so far
+        if (cut_k) {
+            const int b = first_reaching(sh.count, BINS, k);
+            take(b, b);
+            least = before(b) + 1;
+            most = sh.mass[b];
+        }
+        if (top_p < 1.0f) {
+            const int lo = first_reaching(sh.mass, BINS, nucleus_sum(top_p, least)), hi = first_reaching(sh.mass, BINS, nucleus_sum(top_p, most));
+            take(lo, hi);
+            least = before(lo) + 1;
+            most = sh.mass[hi];
+        }
+        least = min(least, kept_m);
+        most = min(most, kept_m);
+        take(first_reaching(sh.mass, BINS, drawn_sum(u, least)), first_reaching(sh.mass, BINS, drawn_sum(u, most)));
+    }
+    const float f0 = (float)from[0], t0 = (float)(to[0] + 1);
+    const float f1 = ranges > 1 ? (float)from[1] : 1e9f, t1 = ranges > 1 ? (float)(to[1] + 1) : 0.0f;
+    const float f2 = ranges > 2 ? (float)from[2] : 1e9f, t2 = ranges > 2 ? (float)(to[2] + 1) : 0.0f;
+    uint64_t* list = a.list + (int64_t)row * LIST;
+    bool full = false;
+    each_word<4>(x, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](float v, int i) {
+        const float d = sc.below(v), s = sc.step(d);
+        if (!full && sc.live(d) && ((s >= f0 && s < t0) || (s >= f1 && s < t1) || (s >= f2 && s < t2))) {
+            const uint32_t at = atomicAdd(&a.listed[row], 1u);
+            full = at >= LIST;
+            if (!full) __hip_atomic_store(&list[at], (uint64_t)key_of(sc.infinite ? 0.0f : v) << 32 | (uint32_t)~i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    });
+    // this workgroup's words are stored before it is counted; the last one to be counted goes on with the row
+    if (a.chunks > 1) {
+        __threadfence();
+        __syncthreads();
+        if (t == 0) sh.at = atomicAdd(&a.arrived[row], 1u) == (uint32_t)a.chunks - 1;
+        __syncthreads();
+        if (!sh.at) return;
+        __threadfence();
+    } else {
+        __threadfence();
+        __syncthreads();
+    }
+    const uint32_t listed = __hip_atomic_load(&a.listed[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (listed > LIST || listed == 0) {
+        choose_alone<T>(a, row, sc, sh);
+        return;
+    }
+    const int n = (int)listed;
+    for (int i = t; i < n; i += SAMPLE_WG) sh.list[i] = __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    sort_list(sh, n, sc);
+    // The list's running sums as the row's: each range starts at the weight of what lies in front of it.
+    int first_of_k = 0;
+    uint64_t shift[3] = {0, 0, 0};
+    int starts[3] = {0, 0, 0};
+    for (int r = ranges - 1, place = 0; r >= 0; --r) {   // from the top of the list on
+        // the range's first word: the first whose step is not below it
+        int lo = place, hi = n;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            const float s = sc.step(sc.infinite ? 0.0f : sc.top - value_of((uint32_t)(sh.list[mid] >> 32)));
+            if (s >= (float)from[r]) hi = mid;
+            else lo = mid + 1;
+        }
+        starts[r] = place = lo;
+        shift[r] = (wants.mass && from[r] > 0 ? sh.mass[from[r] - 1] : 0) - (lo > 0 ? sh.sums[max(lo - 1, 0)] : 0);
+        if (r == 0) first_of_k = lo;
+    }
+    __syncthreads();
+    for (int i = t; i < n; i += SAMPLE_WG) {
+        const uint64_t add = ranges > 2 && i < starts[1] ? shift[2] : ranges > 1 && i < starts[0] ? shift[1] : shift[0];
+        sh.sums[i] += add;
+    }
+    __syncthreads();
+    uint64_t kept = wants.mass ? sh.mass[BINS - 1] : sh.sums[n - 1];
+    if (cut_k) kept = sh.sums[min(first_of_k + k - 1 - (int)(from[0] > 0 ? sh.count[from[0] - 1] : 0), n - 1)];
+    if (top_p < 1.0f) kept = sh.sums[first_reaching(sh.sums, n, nucleus_sum(top_p, kept))];
+    uint64_t above = kept_m;
+    if (!wants.mass && a.min_p && a.min_p[row] > 0.0f) {   // what min-p keeps of the list, which is a prefix
+        int lo = 1, hi = n;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (sc.power(value_of((uint32_t)(sh.list[mid] >> 32))) >= sc.least) lo = mid + 1;
+            else hi = mid;
+        }
+        above = sh.sums[lo - 1];
+    }
+    kept = min(kept, above);
+    const int at = first_reaching(sh.sums, n, drawn_sum(u, kept));
+    if (t == 0) {
+        a.tokens[row] = (int)~(uint32_t)sh.list[at];
+        if (a.probs) a.probs[row] = (float)((double)weight_of(sc.power(value_of((uint32_t)(sh.list[at] >> 32)))) / (double)kept);
+    }
+}
+
+template <typename T>
 static void launch(const Sampling& a, int rows, hipStream_t s) {
     const dim3 grid(a.chunks, rows);
     hipLaunchKernelGGL((sample_peak_kernel<T>), grid, dim3(SAMPLE_WG), 0, s, a);
-    hipLaunchKernelGGL((sample_kernel<T>), grid, dim3(SAMPLE_WG), 0, s, a);
+    hipLaunchKernelGGL((sample_steps_kernel<T>), grid, dim3(SAMPLE_WG), 0, s, a);
+    hipLaunchKernelGGL((sample_choose_kernel<T>), grid, dim3(SAMPLE_WG), 0, s, a);
 }
 
 }  // namespace
@@ -473,23 +670,24 @@ extern "C" int lk_sample(const void* logits, int type, int64_t stride, int rows,
     if (vocab > LK_SAMPLE_VOCAB) return LK_ERR_SIZE;
     if (rows == 0) return LK_OK;
     if (!logits || !uniform || !temperature || !tokens || ((uintptr_t)logits & (size - 1))) return LK_ERR_ARG;
-    // pieces of a row: enough workgroups for two to a CU, at least 2048 words each
+    // pieces of a row: enough workgroups for two to a CU, of at least 4096 words
+    const int vec = SAMPLE_WG * 16 / size;
     int chunks = (2 * lk_device().cus + rows - 1) / rows;
-    if (chunks > (vocab + 2047) / 2048) chunks = (vocab + 2047) / 2048;
-    Sampling a{logits, stride, vocab, (vocab + chunks - 1) / chunks, 0, uniform, temperature, top_p, min_p, top_k, tokens, probs, nullptr, nullptr, nullptr, nullptr, nullptr};
+    if (chunks > (vocab + 4095) / 4096) chunks = (vocab + 4095) / 4096;
+    Sampling a{logits, stride, vocab, 0, 0, uniform, temperature, top_p, min_p, top_k, tokens, probs, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+    a.chunk = ((vocab + chunks - 1) / chunks + vec - 1) / vec * vec;
     a.chunks = (vocab + a.chunk - 1) / a.chunk;
-    const size_t of_row = (a.chunks > 1 ? (size_t)BINS * 12 + 16 : 0) + (size_t)a.chunks * sizeof(Peak);
+    const size_t of_row = (size_t)BINS * 12 + (size_t)LIST * 8 + 16 + (size_t)a.chunks * sizeof(Peak);
     LkScratch scratch((hipStream_t)stream);
     uint8_t* mem = (uint8_t*)scratch.get(LK_SCRATCH_SAMPLE, (size_t)rows * of_row);
     if (!mem) return LK_ERR_NOMEM;
     a.peaks = (Peak*)mem;
-    mem += (size_t)rows * a.chunks * sizeof(Peak);
-    if (a.chunks > 1) {
-        a.mass = (uint64_t*)mem;
-        a.floor_mass = a.mass + (size_t)rows * BINS;
-        a.count = (uint32_t*)(a.floor_mass + rows);
-        a.arrived = a.count + (size_t)rows * BINS;
-    }
+    a.mass = (uint64_t*)(a.peaks + (size_t)rows * a.chunks);
+    a.list = a.mass + (size_t)rows * BINS;
+    a.floor_mass = a.list + (size_t)rows * LIST;
+    a.count = (uint32_t*)(a.floor_mass + rows);
+    a.listed = a.count + (size_t)rows * BINS;
+    a.arrived = a.listed + rows;
     if (type == LK_TYPE_F32) launch<float>(a, rows, (hipStream_t)stream);
     else if (type == LK_TYPE_F16) launch<__half>(a, rows, (hipStream_t)stream);
     else launch<__hip_bfloat16>(a, rows, (hipStream_t)stream);
