@@ -71,15 +71,77 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_kernel(Attend a, int 
     }
 }
 
+// The same for a few parts: a wave to a row and head. `few`: items are (sequence, one of `tokens`, head); else (row of the batch, head).
+template <typename T, int D>
+__global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_few_parts_kernel(Attend a, int per, bool few, int tokens, int64_t items) {
+    constexpr int PER = D / 64, AHEAD = 8;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * JOIN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (item >= items) return;
+    const int head = (int)(item % a.heads);
+    int seq = (int)(item / a.heads / tokens), tok = (int)(item / a.heads % tokens);
+    if (!few) {   // the last sequence that starts at or before the row
+        const int row = (int)(item / a.heads);
+        int lo = 0, hi = a.seqs - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (a.starts[mid] <= row) lo = mid;
+            else hi = mid - 1;
+        }
+        seq = lo;
+        tok = row - max(a.starts[seq], 0);
+    }
+    const KvSeq s(a, seq);
+    const int64_t all_rows = (int64_t)s.tokens() * a.group;
+    if ((all_rows <= a.few_rows) != few || tok < 0) return;
+    for (; tok < s.tokens(); tok += few ? tokens : 0x40000000) {
+        const int64_t r0 = ((int64_t)tok * a.group + head % a.group) / per * per, r1 = min(r0 + per, all_rows) - 1;
+        const KvSpan span(a, s, s.first + (int)(r0 / a.group), s.first + (int)(r1 / a.group));
+        const int parts = span.parts;
+        if (parts > 1) {
+            const int64_t from = (a.part_row(seq, s, s.first + tok) * a.heads + head) * a.splits;
+            float m = -INFINITY, l = 0.f, acc[PER] = {};
+            for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[from + p].x);
+            for (int p0 = 0; p0 < parts; p0 += AHEAD) {
+                float x[AHEAD][PER];
+                float2 ml[AHEAD];
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    ml[j] = a.part_ml[from + min(p0 + j, parts - 1)];
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) x[j][i] = a.part_o[(from + min(p0 + j, parts - 1)) * D + lane + 64 * i];
+                }
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j)
+                    if (p0 + j < parts) {
+                        const float f = ml[j].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[j].x - m);
+                        l += ml[j].x == -INFINITY ? ml[j].y : ml[j].y * f;
+#pragma unroll
+                        for (int i = 0; i < PER; ++i) acc[i] = fmaf(x[j][i], f, acc[i]);
+                    }
+            }
+            T* out = (T*)a.out + (int64_t)(s.first + tok) * a.out_stride + (int64_t)head * D + lane;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) out[64 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
+        }
+    }
+}
+
+template <typename T, int D>
+static int join_of(const Attend& a, int per, bool few, int tokens, hipStream_t s) {
+    const int64_t items = few ? (int64_t)a.seqs * tokens * a.heads : (int64_t)a.rows * a.heads;
+    const bool wide = few && a.splits > 8;   // four waves to a row from nine parts on
+    const int64_t blocks = wide ? items : (items + JOIN_WAVES - 1) / JOIN_WAVES;
+    if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
+    const dim3 grid((unsigned)blocks), threads(64 * JOIN_WAVES);
+    if (wide) hipLaunchKernelGGL((kv_join_kernel<T, D>), grid, threads, 0, s, a, per, few, tokens);
+    else hipLaunchKernelGGL((kv_join_few_parts_kernel<T, D>), grid, threads, 0, s, a, per, few, tokens, items);
+    return lk_launch_status();
+}
+
 template <typename T>
 static int join(const Attend& a, int head_dim, int per, bool few, int tokens, hipStream_t s) {
-    const int64_t blocks = (int64_t)a.seqs * tokens * a.heads;
-    if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
-    const dim3 grid((unsigned)blocks);
-    if (head_dim == 64) hipLaunchKernelGGL((kv_join_kernel<T, 64>), grid, dim3(64 * JOIN_WAVES), 0, s, a, per, few, tokens);
-    else if (head_dim == 128) hipLaunchKernelGGL((kv_join_kernel<T, 128>), grid, dim3(64 * JOIN_WAVES), 0, s, a, per, few, tokens);
-    else hipLaunchKernelGGL((kv_join_kernel<T, 256>), grid, dim3(64 * JOIN_WAVES), 0, s, a, per, few, tokens);
-    return lk_launch_status();
+    return head_dim == 64 ? join_of<T, 64>(a, per, few, tokens, s) : head_dim == 128 ? join_of<T, 128>(a, per, few, tokens, s) : join_of<T, 256>(a, per, few, tokens, s);
 }
 
 // Sequences of up to this many rows (token, head of a group) are the few-rows kernel's.
@@ -131,13 +193,13 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     size_t rows_f = 0, rows_m = 0;   // whose parts are kept
     if (few) {
         af.few_rows = many ? FEW_ROWS : 0x7FFFFFFF;
-        cut(af, (int64_t)seqs * kv_heads * ((few_max + few_per - 1) / few_per), tiles, 4 * cus, 16);
+        cut(af, (int64_t)seqs * kv_heads * ((few_max + few_per - 1) / few_per), tiles, (getenv("KVW") ? atoi(getenv("KVW")) : 4) * cus, getenv("KVL") ? atoi(getenv("KVL")) : 16);
         af.part_seq = many ? FEW_ROWS / group : tokens;
         if (af.splits > 1) rows_f = (size_t)seqs * af.part_seq;
     }
     if (many) {
         am.few_rows = few ? FEW_ROWS : 0;
-        cut(am, ((int64_t)rows * group + KV_MANY_ROWS - 1) / KV_MANY_ROWS * kv_heads, tiles, 2 * cus, 16);
+        cut(am, ((int64_t)rows * group + KV_MANY_ROWS - 1) / KV_MANY_ROWS * kv_heads, tiles, (getenv("KVM") ? atoi(getenv("KVM")) : 2) * cus, 16);
         if (am.splits > 1) rows_m = rows;
     }
     LkScratch scratch(s);

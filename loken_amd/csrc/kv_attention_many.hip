@@ -10,9 +10,13 @@
 // so the running maximum, its corrections and the sum of weights are the lane's own, with one exchange between the two halves.
 //
 // Queries come in f16 scaled by a power of two of their row (bf16 fits with its 8 bits, f16 as it is); f32 ones as a high and a
-// low half, two products each, as are its weights: 22 bits. A page's key scale goes onto the scores, its value scale onto
-// the weights, relative to the largest value scale so far, so that no scale is too small for f16; weights stand 2^14 above 1 for
-// the same reason.
+// low half, two products each, as are its weights: 22 bits. A page's key scale goes onto the scores. Its value scale goes onto the
+// weights, relative to the largest value scale so far, so that no scale is too small for f16: as its logarithm, in the exponent that
+// the weight is made from (off by 5e-7 of the weight at most, a last place of the logarithm), and back out of the sum of
+// weights run by run.
+//
+// The sums are put to a new maximum only where that lies 2^8 above the one they go by: weights up to 2^8 then, which stand
+// LIFT = 2^7 above one and stay below 2^15, f16's largest; a weight of 2^-21 still has all its bits, one of 2^-31 some.
 
 #include "kv_attention.h"
 
@@ -20,9 +24,10 @@ namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES, RUNS = KV_TILE / 16;
-constexpr float LIFT = 16384.f;   // a weight of one
+constexpr float LIFT = 7.f, SLACK = 8.f;   // powers of two
 
 // Sixteen codes as f16, as they lie: 0x6400 + (code + 128) is the f16 number 1152 + code.
 static __device__ __forceinline__ void to_halves(uint4 w, uint4* out) {
@@ -50,22 +55,41 @@ struct Many {
     static constexpr int K_BYTES = KV_TILE * K_PITCH, V_BYTES = D * V_PITCH;
     static constexpr int BUFFERS = D < 256 ? 2 : 1;
     static constexpr int CHUNKS = KV_TILE * D / 16 / THREADS;   // of sixteen codes, a thread and side
-    static constexpr int LDS = BUFFERS * (K_BYTES + V_BYTES + 2 * RUNS * 4);
+    static constexpr int LDS = BUFFERS * (K_BYTES + V_BYTES);
+};
+
+// What a step's pages have for everybody.
+struct Step {
+    float ks[RUNS];     // key scales; -1: the page is absent
+    float bias[RUNS];   // log2 of the value scale over `ref`, and LIFT; of a page whose values are all zero LIFT alone
+    float back[RUNS];   // 2^-bias
+    uint32_t live[RUNS];   // all bits, or none where the values are zero
+    float shrink;       // what `ref` before this step is of it now
+    float ref;          // the largest value scale so far
+    int absent;         // whether a page is
+    int pad;
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_kernel(Attend a, int row_tiles) {
+__global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_kernel(Attend a, int row_tiles, int cus) {
     using M = Many<T, D>;
     extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ Step steps[2];
+    __shared__ int pages[2][RUNS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
+    // Workgroups in rounds of one to a CU, every other round backwards: row tiles that see the most come first, and where two rounds are
+    // all there is a CU with much of one has little of the other.
     unsigned at = blockIdx.x;
+    {
+        const unsigned round = at / cus, first = round * cus, size = min((unsigned)cus, gridDim.x - first);
+        if (round & 1) at = first + (size - 1 - (at - first));
+    }
     const int part = at % a.splits;
     at /= a.splits;
-    // the last row tiles see the most: they start first
-    const int tile0 = row_tiles - 1 - (int)(at % row_tiles);
-    at /= row_tiles;
-    const int kv = at % a.pool.heads, seq = at / a.pool.heads;
+    const int kv = at % a.pool.heads;
+    at /= a.pool.heads;
+    const int seq = at % a.seqs, tile0 = row_tiles - 1 - (int)(at / a.seqs);
     const KvSeq s(a, seq);
     const int64_t all_rows = (int64_t)s.tokens() * a.group;
     if (all_rows <= a.few_rows) return;
@@ -73,8 +97,6 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
     const int32_t* entries = a.table + seq * a.table_stride;
     auto k_lds = [&](int buffer) { return lds + buffer * (M::K_BYTES + M::V_BYTES); };
     auto v_lds = [&](int buffer) { return lds + buffer * (M::K_BYTES + M::V_BYTES) + M::K_BYTES; };
-    // scales of the step's four runs; a run that is absent: both -1
-    auto scales = [&](int buffer) { return (float*)(lds + M::BUFFERS * (M::K_BYTES + M::V_BYTES)) + buffer * 2 * RUNS; };
 
     for (int64_t r_tile = (int64_t)tile0 * KV_MANY_ROWS; r_tile < all_rows; r_tile += (int64_t)row_tiles * KV_MANY_ROWS) {
         const int64_t r_end = min(r_tile + KV_MANY_ROWS, all_rows);
@@ -122,34 +144,36 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[b][e] = 0.f;
         float m = -INFINITY, l = 0.f;
-        float vs_most = 0.f;   // the largest value scale so far; the same in every lane
 
-        // a step's codes: thread tid has chunk tid, tid + 256, .. of sixteen
+        // A step's codes: thread tid has chunk tid, tid + 256, .. of sixteen. Its pages have been in LDS since the step before.
         uint4 kc[M::CHUNKS], vc[M::CHUNKS];
-        float my_scale = -1.f;
+        auto entry = [&](int t) {   // of run tid, in the first lanes
+            const int p0 = span.lo + t * KV_TILE + 16 * (tid & (RUNS - 1));
+            const int page = t < t_end && p0 < span.hi ? entries[p0 >> shift] : -1;
+            return (unsigned)page < (unsigned)a.pool.pages ? page : -1;
+        };
+        float ks = -1.f, vs = 0.f, ref = 0.f;
         auto fetch = [&](int t) {
+            const int* page = pages[t & 1];
 #pragma unroll
             for (int c = 0; c < M::CHUNKS; ++c) {
                 const int n = tid + c * THREADS;
                 const int token = n / (D / 16), run_v = n / D;
-                auto page_at = [&](int run) {
-                    const int p0 = span.lo + t * KV_TILE + 16 * run;
-                    const int page = p0 < span.hi ? entries[p0 >> shift] : -1;
-                    return (unsigned)page < (unsigned)a.pool.pages ? page : 0;
-                };
                 const int off_k = (span.lo + t * KV_TILE + token) & ((1 << shift) - 1);
-                kc[c] = *(const uint4*)(a.pool.k + ((((int64_t)page_at(token >> 4) * a.pool.heads + kv) << shift) + off_k) * D + (n % (D / 16)) * 16);
+                kc[c] = *(const uint4*)(a.pool.k + ((((int64_t)max(page[token >> 4], 0) * a.pool.heads + kv) << shift) + off_k) * D + (n % (D / 16)) * 16);
                 const int off_v = (span.lo + t * KV_TILE + 16 * run_v) & ((1 << shift) - 1);
-                vc[c] = *(const uint4*)(a.pool.v + ((((int64_t)page_at(run_v) * a.pool.heads + kv) << shift) + off_v) * D + (n % D) * 16);
+                vc[c] = *(const uint4*)(a.pool.v + ((((int64_t)max(page[run_v], 0) * a.pool.heads + kv) << shift) + off_v) * D + (n % D) * 16);
             }
-            if (tid < 2 * RUNS) {
-                const int p0 = span.lo + t * KV_TILE + 16 * (tid % RUNS);
-                const int page = p0 < span.hi ? entries[p0 >> shift] : -1;
-                my_scale = -1.f;
-                if ((unsigned)page < (unsigned)a.pool.pages) my_scale = (tid < RUNS ? a.pool.k_scales : a.pool.v_scales)[(int64_t)page * a.pool.heads + kv];
+            if (tid < RUNS) {
+                const int p = page[tid];
+                const int64_t at_scale = (int64_t)max(p, 0) * a.pool.heads + kv;
+                ks = a.pool.k_scales[at_scale];
+                vs = a.pool.v_scales[at_scale];
+                if (p < 0) { ks = -1.f; vs = 0.f; }
             }
         };
-        auto store = [&](int buffer) {
+        auto store = [&](int t) {
+            const int buffer = M::BUFFERS == 2 ? t & 1 : 0;
 #pragma unroll
             for (int c = 0; c < M::CHUNKS; ++c) {
                 const int n = tid + c * THREADS;
@@ -163,21 +187,51 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
                 to[0] = w[0];
                 to[1] = w[1];
             }
-            if (tid < 2 * RUNS) scales(buffer)[tid] = my_scale;
+            if (tid < RUNS) {
+                Step& st = steps[t & 1];
+                float most = vs, least = ks;
+                for (int o = 1; o < RUNS; o <<= 1) { most = fmaxf(most, __shfl_xor(most, o)); least = fminf(least, __shfl_xor(least, o)); }
+                const float now = fmaxf(ref, most);
+                st.ks[tid] = ks;
+                const float bias = vs > 0.f ? __builtin_amdgcn_logf(vs / now) + LIFT : LIFT;
+                st.bias[tid] = bias;
+                st.back[tid] = __builtin_amdgcn_exp2f(-bias);
+                st.live[tid] = vs > 0.f ? 0xFFFFFFFFu : 0u;
+                if (tid == 0) {
+                    st.shrink = ref > 0.f ? ref / now : 1.f;   // (up to then the sums are zeros)
+                    st.ref = now;
+                    st.absent = least < 0.f;
+                }
+                ref = now;
+            }
         };
 
         __syncthreads();   // the last row tile's reads of LDS
-        if (t_begin < t_end) {
-            fetch(t_begin);
-            store(0);
+        int next = -1;
+        if (tid < RUNS) {
+            pages[t_begin & 1][tid] = entry(t_begin);
+            next = entry(t_begin + 1);
         }
         __syncthreads();
+        if (t_begin < t_end) {
+            fetch(t_begin);
+            store(t_begin);
+        }
+        if (tid < RUNS) pages[(t_begin + 1) & 1][tid] = next;
+        __syncthreads();
+        float ref_of_sums = 0.f;
         for (int t = t_begin; t < t_end; ++t) {
-            const int buffer = M::BUFFERS == 2 ? (t - t_begin) & 1 : 0;
+            const int buffer = M::BUFFERS == 2 ? t & 1 : 0;
             if (t + 1 < t_end) fetch(t + 1);
+            if (tid < RUNS) next = entry(t + 2);
             const int base = span.lo + t * KV_TILE;
-            const float* sc = scales(buffer);
-            const float vs_new = fmaxf(fmaxf(vs_most, fmaxf(sc[RUNS], sc[RUNS + 1])), fmaxf(sc[RUNS + 2], sc[RUNS + 3]));
+            const Step& st = steps[t & 1];
+            ref_of_sums = st.ref;
+            if (st.shrink < 1.f) {
+                const float f = st.shrink;
+#pragma unroll
+                for (int b = 0; b < M::NB; ++b) o[b] *= f;
+            }
             // a wave whose rows see nothing of the step leaves it
             if (base <= pos_most && (a.window == 0 || base + KV_TILE - 1 > pos_least - a.window)) {
                 const uint8_t *kl = k_lds(buffer), *vl = v_lds(buffer);
@@ -197,18 +251,17 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
                     }
                 }
                 // scores in powers of two; element e of x[u]: position base + 32 u + 16 (e / 8) + 8 half + e % 8
-                const bool absent = fminf(fminf(sc[0], sc[1]), fminf(sc[2], sc[3])) < 0.f;
-                const bool whole = base + KV_TILE - 1 <= pos_least && (a.window == 0 || base > pos_most - a.window) && !absent;
+                const bool whole = base + KV_TILE - 1 <= pos_least && (a.window == 0 || base > pos_most - a.window) && !st.absent;
                 float by[RUNS], top = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < RUNS; ++n) by[n] = sc[n] * unit;
+                for (int n = 0; n < RUNS; ++n) by[n] = st.ks[n] * unit;
                 if (!whole) {
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const int p = base + 32 * u + 16 * (e / 8) + 8 * half + e % 8, n = 2 * u + e / 8;
-                            const bool seen = p <= pos && (a.window == 0 || p > pos - a.window) && sc[n] >= 0.f;
+                            const bool seen = p <= pos && (a.window == 0 || p > pos - a.window) && st.ks[n] >= 0.f;
                             x[u][e] = seen ? x[u][e] * by[n] : -INFINITY;
                         }
 #pragma unroll
@@ -225,31 +278,41 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
                     const auto r2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                     top = fmaxf(__uint_as_float(r2[0]), __uint_as_float(r2[1]));
                 }
-                if (__ballot(top > m) != 0 || vs_new > vs_most) {
+                if (__ballot(top > m + SLACK || (m == -INFINITY && top > m)) != 0) {
                     const float m_new = fmaxf(m, top);
                     const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
                     l *= keep;
-                    const float keep_o = vs_most > 0.f ? keep * (vs_most / vs_new) : 0.f;
 #pragma unroll
-                    for (int b = 0; b < M::NB; ++b) o[b] *= keep_o;
+                    for (int b = 0; b < M::NB; ++b) o[b] *= keep;
                     m = m_new;
-                    vs_most = vs_new;
                 }
                 const float m_base = m == -INFINITY ? 0.f : m;
-                float cut[RUNS];
-#pragma unroll
-                for (int n = 0; n < RUNS; ++n) cut[n] = vs_most > 0.f && sc[RUNS + n] > 0.f ? sc[RUNS + n] / vs_most * LIFT : 0.f;
-                float sum = 0.f;
 #pragma unroll
                 for (int n = 0; n < RUNS; ++n) {
                     h8 w[M::PARTS];
+                    const float add = st.bias[n] - m_base;
+                    float sum = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float p = __builtin_amdgcn_exp2f(fmaf(x[n / 2][8 * (n % 2) + e], by[n], -m_base));
-                        sum += p;
-                        const float y = p * cut[n];
-                        w[0][e] = (_Float16)y;
-                        if (M::FINE) w[M::PARTS - 1][e] = (_Float16)(y - (float)w[0][e]);
+                    for (int e = 0; e < 8; e += 2) {
+                        const f2 y = {__builtin_amdgcn_exp2f(fmaf(x[n / 2][8 * (n % 2) + e], by[n], add)),
+                                      __builtin_amdgcn_exp2f(fmaf(x[n / 2][8 * (n % 2) + e + 1], by[n], add))};
+                        sum += y[0];
+                        sum += y[1];
+                        const h2 hi = __builtin_convertvector(y, h2);
+                        w[0][e] = hi[0];
+                        w[0][e + 1] = hi[1];
+                        if (M::FINE) {
+                            const f2 left = {y[0] - (float)hi[0], y[1] - (float)hi[1]};
+                            const h2 lo = __builtin_convertvector(left, h2);
+                            w[M::PARTS - 1][e] = lo[0];
+                            w[M::PARTS - 1][e + 1] = lo[1];
+                        }
+                    }
+                    l = fmaf(sum, st.back[n], l);
+#pragma unroll
+                    for (int p = 0; p < M::PARTS; ++p) {   // values of a page whose scale is zero: zeros, whatever its codes are
+                        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+                        w[p] = __builtin_bit_cast(h8, __builtin_bit_cast(u4, w[p]) & st.live[n]);
                     }
 #pragma unroll
                     for (int b = 0; b < M::NB; ++b) {
@@ -258,14 +321,14 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
                         for (int p = 0; p < M::PARTS; ++p) o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, w[p], o[b], 0, 0, 0);
                     }
                 }
-                l += sum;
             }
             if (M::BUFFERS == 1) __syncthreads();
-            if (t + 1 < t_end) store(M::BUFFERS == 2 ? buffer ^ 1 : 0);
+            if (t + 1 < t_end) store(t + 1);
+            if (tid < RUNS) pages[t & 1][tid] = next;   // of step t + 2; those of t have been read
             __syncthreads();
         }
         l += __shfl_xor(l, 32);
-        const float back = vs_most / LIFT;
+        const float back = ref_of_sums * 0.0078125f;   // 2^-LIFT
         if (!row_is) continue;
         // element e of o[b]: column 32 b + 8 (e / 4) + 4 half + e % 4
         if (parts == 1) {
@@ -294,12 +357,12 @@ static int launch(const Attend& a, int max_rows, hipStream_t s) {
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
     constexpr int bytes = Many<T, D>::LDS;
     // a kernel gets 64 KB of LDS unless the runtime is told otherwise
-    if (bytes > 64 * 1024 &&
+    if (bytes > 60 * 1024 &&
         hipFuncSetAttribute((const void*)kv_attention_many_kernel<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) {
         (void)hipGetLastError();
         return LK_ERR_LAUNCH;
     }
-    hipLaunchKernelGGL((kv_attention_many_kernel<T, D>), dim3((unsigned)blocks), dim3(THREADS), bytes, s, a, row_tiles);
+    hipLaunchKernelGGL((kv_attention_many_kernel<T, D>), dim3((unsigned)blocks), dim3(THREADS), bytes, s, a, row_tiles, lk_device().cus);
     return lk_launch_status();
 }
 

@@ -91,9 +91,9 @@ struct Sampling {
     uint64_t* mass;       // [rows][BINS]
     uint32_t* count;      // [rows][BINS]
     uint64_t* floor_mass; // [rows]: what min-p keeps
-    uint64_t* list;       // [rows][LIST]: gathered words
-    uint32_t* listed;     // [rows]: how many there are
-    uint32_t* arrived;    // [rows]: workgroups that have gathered
+    uint64_t* list;       // [rows][chunks][LIST]: gathered words, where a row has several pieces
+    uint32_t* listed;     // [rows][chunks]: how many each piece has
+    uint32_t* arrived;    // [rows]: pieces that have been gathered
 };
 
 // The largest and the smallest word of a piece of a row; clears the row's histogram on the way.
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(SAMPLE_WG) void sample_peak_kernel(Sampling a) {
         a.mass[(int64_t)row * BINS + i] = 0;
         a.count[(int64_t)row * BINS + i] = 0;
     }
-    if (c == 0 && t == 0) { a.floor_mass[row] = 0; a.listed[row] = 0; a.arrived[row] = 0; }
+    if (c == 0 && t == 0) { a.floor_mass[row] = 0; a.arrived[row] = 0; }
     Peak p{best > -INFINITY ? (uint64_t)key_of(best) << 32 | (uint32_t)~at : 0, key_of(lowest), 0};
     wave_peak(p);
     if ((t & 63) == 0) meet[t >> 6] = p;
@@ -545,94 +545,105 @@ __global__ __launch_bounds__(SAMPLE_WG) void sample_choose_kernel(Sampling a) {
     const float top_p = a.top_p ? a.top_p[row] : 1.0f, u = a.uniform[row];
     const int k = wants.count ? a.top_k[row] : 0;
     const bool cut_k = wants.count && (uint32_t)k < sh.count[BINS - 1];
-    // The steps that are gathered: up to three ranges, the last one nearest to the top.
-    int from[3], to[3], ranges = 0;
+    // The steps that are gathered: up to three ranges, [a0, a1] around the end of the top-k words, [b0, b1] around that of top-p's, which
+    // is nearer to the top or touches it, [c0, c1] around the draw, nearer still. A range that touches the next one is part of it.
+    int a0 = BINS, a1 = -1, b0 = BINS, b1 = -1, c0 = BINS, c1 = -1;
     if (!wants.mass) {   // the top-k words and the rest of their last step
-        from[0] = 0;
-        to[0] = first_reaching(sh.count, BINS, k);
-        ranges = 1;
+        a0 = 0;
+        a1 = first_reaching(sh.count, BINS, k);
     } else {
-        auto take = [&](int lo, int hi) {   // each search's steps lie in front of those of the one before it, or touch them
-            if (ranges && hi >= from[ranges - 1] - 1) { from[ranges - 1] = min(from[ranges - 1], lo); to[ranges - 1] = max(to[ranges - 1], hi); }
-            else { from[ranges] = lo; to[ranges] = hi; ++ranges; }
-        };
-        auto before = [&](int b) { return b > 0 ? sh.mass[b - 1] : 0; };
+        auto before = [&](int b) { return b > 0 ? sh.mass[max(b - 1, 0)] : 0; };
         uint64_t least = sh.mass[BINS - 1], most = least;   // bounds of what is kept so far
         if (cut_k) {
-            const int b = first_reaching(sh.count, BINS, k);
-            take(b, b);
-            least = before(b) + 1;
-            most = sh.mass[b];
+            a0 = a1 = first_reaching(sh.count, BINS, k);
+            least = before(a0) + 1;
+            most = sh.mass[a0];
         }
         if (top_p < 1.0f) {
-            const int lo = first_reaching(sh.mass, BINS, nucleus_sum(top_p, least)), hi = first_reaching(sh.mass, BINS, nucleus_sum(top_p, most));
-            take(lo, hi);
-            least = before(lo) + 1;
-            most = sh.mass[hi];
+            b0 = first_reaching(sh.mass, BINS, nucleus_sum(top_p, least));
+            b1 = first_reaching(sh.mass, BINS, nucleus_sum(top_p, most));
+            least = before(b0) + 1;
+            most = sh.mass[b1];
+            if (b1 >= a0 - 1) { a0 = min(a0, b0); b0 = BINS; b1 = -1; }
         }
         least = min(least, kept_m);
         most = min(most, kept_m);
-        take(first_reaching(sh.mass, BINS, drawn_sum(u, least)), first_reaching(sh.mass, BINS, drawn_sum(u, most)));
+        c0 = first_reaching(sh.mass, BINS, drawn_sum(u, least));
+        c1 = first_reaching(sh.mass, BINS, drawn_sum(u, most));
+        if (b1 >= 0 && c1 >= b0 - 1) { b0 = min(b0, c0); c0 = BINS; c1 = -1; }
+        else if (b1 < 0 && c1 >= a0 - 1) { a0 = min(a0, c0); c0 = BINS; c1 = -1; }
     }
-    const float f0 = (float)from[0], t0 = (float)(to[0] + 1);
-    const float f1 = ranges > 1 ? (float)from[1] : 1e9f, t1 = ranges > 1 ? (float)(to[1] + 1) : 0.0f;
-    const float f2 = ranges > 2 ? (float)from[2] : 1e9f, t2 = ranges > 2 ? (float)(to[2] + 1) : 0.0f;
-    uint64_t* list = a.list + (int64_t)row * LIST;
-    bool full = false;
+    const float fa = (float)a0, ta = (float)(a1 + 1), fb = (float)b0, tb = (float)(b1 + 1), fc = (float)c0, tc = (float)(c1 + 1);
+    if (t == 0) sh.n = 0;
+    __syncthreads();
     each_word<4>(x, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](float v, int i) {
         const float d = sc.below(v), s = sc.step(d);
-        if (!full && sc.live(d) && ((s >= f0 && s < t0) || (s >= f1 && s < t1) || (s >= f2 && s < t2))) {
-            const uint32_t at = atomicAdd(&a.listed[row], 1u);
-            full = at >= LIST;
-            if (!full) __hip_atomic_store(&list[at], (uint64_t)key_of(sc.infinite ? 0.0f : v) << 32 | (uint32_t)~i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (sc.live(d) && ((s >= fa && s < ta) || (s >= fb && s < tb) || (s >= fc && s < tc))) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < LIST) sh.list[at] = (uint64_t)key_of(sc.infinite ? 0.0f : v) << 32 | (uint32_t)~i;
         }
     });
-    // this workgroup's words are stored before it is counted; the last one to be counted goes on with the row
+    __syncthreads();
+    int n = sh.n;
     if (a.chunks > 1) {
-        __threadfence();
+        uint64_t* list = a.list + ((int64_t)row * a.chunks + c) * LIST;
+        uint32_t* listed = a.listed + (int64_t)row * a.chunks;
+        for (int i = t; i < min(n, LIST); i += SAMPLE_WG) __hip_atomic_store(&list[i], sh.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (t == 0) __hip_atomic_store(&listed[c], (uint32_t)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // Stores of agent scope go through the XCD's cache to where every XCD reads: once each wave has waited for its own, the
+        // workgroup is counted, and the last one to be counted goes on with the row. (A fence writes the whole cache back, once a
+        // wave: 64 rows took 150 us with two of them.)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (t == 0) sh.at = atomicAdd(&a.arrived[row], 1u) == (uint32_t)a.chunks - 1;
         __syncthreads();
         if (!sh.at) return;
-        __threadfence();
-    } else {
-        __threadfence();
-        __syncthreads();
+        list = a.list + (int64_t)row * a.chunks * LIST;
+        // each wave takes pieces in turn; where a piece's words go is what the pieces before it hold
+        const int lane = t & 63, wave = t >> 6;
+        uint32_t all = 0;
+        for (int p0 = 0; p0 < a.chunks; p0 += 64) {
+            const uint32_t mine = p0 + lane < a.chunks ? __hip_atomic_load(&listed[p0 + lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+            uint32_t up_to = mine;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t v = __shfl_up(up_to, o);
+                if (lane >= o) up_to += v;
+            }
+            for (int j = wave; j < min(64, a.chunks - p0); j += SAMPLE_WAVES) {
+                const uint32_t count = __shfl(mine, j), to = all + __shfl(up_to, j) - count;
+                for (uint32_t i = lane; i < min(count, (uint32_t)LIST); i += 64)
+                    if (to + i < LIST) sh.list[to + i] = __hip_atomic_load(&list[(int64_t)(p0 + j) * LIST + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            all += __shfl(up_to, 63);   // at most 2^20 words
+        }
+        n = (int)all;
     }
-    const uint32_t listed = __hip_atomic_load(&a.listed[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (listed > LIST || listed == 0) {
+    if (n > LIST || n == 0) {
         choose_alone<T>(a, row, sc, sh);
         return;
     }
-    const int n = (int)listed;
-    for (int i = t; i < n; i += SAMPLE_WG) sh.list[i] = __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     sort_list(sh, n, sc);
     // The list's running sums as the row's: each range starts at the weight of what lies in front of it.
-    int first_of_k = 0;
-    uint64_t shift[3] = {0, 0, 0};
-    int starts[3] = {0, 0, 0};
-    for (int r = ranges - 1, place = 0; r >= 0; --r) {   // from the top of the list on
-        // the range's first word: the first whose step is not below it
-        int lo = place, hi = n;
+    auto first_at = [&](int step) {   // the first word of the list whose step is not in front of `step`
+        int lo = 0, hi = n;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            const float s = sc.step(sc.infinite ? 0.0f : sc.top - value_of((uint32_t)(sh.list[mid] >> 32)));
-            if (s >= (float)from[r]) hi = mid;
+            if (sc.step(sc.infinite ? 0.0f : sc.top - value_of((uint32_t)(sh.list[mid] >> 32))) >= (float)step) hi = mid;
             else lo = mid + 1;
         }
-        starts[r] = place = lo;
-        shift[r] = (wants.mass && from[r] > 0 ? sh.mass[from[r] - 1] : 0) - (lo > 0 ? sh.sums[max(lo - 1, 0)] : 0);
-        if (r == 0) first_of_k = lo;
-    }
+        return lo;
+    };
+    auto shift_of = [&](int step, int first) {
+        return (wants.mass && step > 0 && step < BINS ? sh.mass[min(max(step - 1, 0), BINS - 1)] : 0) - (first > 0 ? sh.sums[max(first - 1, 0)] : 0);
+    };
+    const int in_a = a1 >= 0 ? first_at(a0) : n, in_b = b1 >= 0 ? first_at(b0) : in_a;
+    const uint64_t shift_a = shift_of(a0, in_a), shift_b = shift_of(b0, in_b), shift_c = shift_of(c0, 0);
     __syncthreads();
-    for (int i = t; i < n; i += SAMPLE_WG) {
-        const uint64_t add = ranges > 2 && i < starts[1] ? shift[2] : ranges > 1 && i < starts[0] ? shift[1] : shift[0];
-        sh.sums[i] += add;
-    }
+    for (int i = t; i < n; i += SAMPLE_WG) sh.sums[i] += i >= in_a ? shift_a : i >= in_b ? shift_b : shift_c;
     __syncthreads();
     uint64_t kept = wants.mass ? sh.mass[BINS - 1] : sh.sums[n - 1];
-    if (cut_k) kept = sh.sums[min(first_of_k + k - 1 - (int)(from[0] > 0 ? sh.count[from[0] - 1] : 0), n - 1)];
+    if (cut_k) kept = sh.sums[min(in_a + k - 1 - (int)(a0 > 0 ? sh.count[max(a0 - 1, 0)] : 0), n - 1)];
     if (top_p < 1.0f) kept = sh.sums[first_reaching(sh.sums, n, nucleus_sum(top_p, kept))];
     uint64_t above = kept_m;
     if (!wants.mass && a.min_p && a.min_p[row] > 0.0f) {   // what min-p keeps of the list, which is a prefix
@@ -677,17 +688,17 @@ extern "C" int lk_sample(const void* logits, int type, int64_t stride, int rows,
     Sampling a{logits, stride, vocab, 0, 0, uniform, temperature, top_p, min_p, top_k, tokens, probs, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     a.chunk = ((vocab + chunks - 1) / chunks + vec - 1) / vec * vec;
     a.chunks = (vocab + a.chunk - 1) / a.chunk;
-    const size_t of_row = (size_t)BINS * 12 + (size_t)LIST * 8 + 16 + (size_t)a.chunks * sizeof(Peak);
+    const size_t of_row = (size_t)BINS * 12 + 12 + a.chunks * (sizeof(Peak) + 4 + (a.chunks > 1 ? (size_t)LIST * 8 : 0));
     LkScratch scratch((hipStream_t)stream);
     uint8_t* mem = (uint8_t*)scratch.get(LK_SCRATCH_SAMPLE, (size_t)rows * of_row);
     if (!mem) return LK_ERR_NOMEM;
     a.peaks = (Peak*)mem;
     a.mass = (uint64_t*)(a.peaks + (size_t)rows * a.chunks);
     a.list = a.mass + (size_t)rows * BINS;
-    a.floor_mass = a.list + (size_t)rows * LIST;
+    a.floor_mass = a.list + (a.chunks > 1 ? (size_t)rows * a.chunks * LIST : 0);
     a.count = (uint32_t*)(a.floor_mass + rows);
     a.listed = a.count + (size_t)rows * BINS;
-    a.arrived = a.listed + rows;
+    a.arrived = a.listed + (size_t)rows * a.chunks;
     if (type == LK_TYPE_F32) launch<float>(a, rows, (hipStream_t)stream);
     else if (type == LK_TYPE_F16) launch<__half>(a, rows, (hipStream_t)stream);
     else launch<__hip_bfloat16>(a, rows, (hipStream_t)stream);
