@@ -8,6 +8,35 @@ namespace {
 
 constexpr int MOST_PARTS = 1024, JOIN_WAVES = 4;
 
+// Where the parts of a row and head are.
+struct PartsOf {
+    int parts;
+    int64_t base, step, first;
+    __device__ __forceinline__ PartsOf(const Attend& a, const KvSeq& s, int seq, int tok, int head, int per) {
+        const int64_t all_rows = (int64_t)s.tokens() * a.group, r = (int64_t)tok * a.group + head % a.group;
+        if (a.chunks) {
+            parts = 1;
+            base = step = first = 0;
+            if (all_rows > per) return;
+            const KvPieces pieces(a, per);
+            const int at = KvPieces::first_of(a, per, seq), steps = kv_steps_of(a, seq, per);
+            const int c0 = at / pieces.length, c1 = (at + steps - 1) / pieces.length;
+            parts = c1 - c0 + 1;
+            // the piece that the sequence starts in has it second, the others first
+            base = ((int64_t)(head / a.group) * a.chunks + c0) * 2 * per + r;
+            step = 2 * per;
+            first = per;
+            return;
+        }
+        const int64_t r0 = r / per * per, r1 = min(r0 + per, all_rows) - 1;
+        parts = KvSpan(a, s, s.first + (int)(r0 / a.group), s.first + (int)(r1 / a.group)).parts;
+        base = (a.part_row(seq, s, s.first + tok) * a.heads + head) * a.splits;
+        step = 1;
+        first = 0;
+    }
+    __device__ __forceinline__ int64_t at(int p) const { return base + p * step + (p == 0 ? first : 0); }
+};
+
 // The parts of a row's context: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A workgroup to a row and head (rows of a workgroup of
 // the launch before, `per` of them, have the same parts), its waves taking parts in turn, eight parts' loads in flight: with one after
 // the other 128 parts of one row took 88 us.
@@ -21,20 +50,18 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_kernel(Attend a, int 
     const int64_t all_rows = (int64_t)s.tokens() * a.group;
     if ((all_rows <= a.few_rows) != few) return;
     for (int tok = blockIdx.x / a.heads % tokens; tok < s.tokens(); tok += tokens) {
-        const int64_t r0 = ((int64_t)tok * a.group + head % a.group) / per * per, r1 = min(r0 + per, all_rows) - 1;
-        const KvSpan span(a, s, s.first + (int)(r0 / a.group), s.first + (int)(r1 / a.group));
-        const int parts = span.parts;   // at most a.splits
+        const PartsOf of(a, s, seq, tok, head, per);
+        const int parts = of.parts;   // at most MOST_PARTS
         if (parts == 1) continue;
-        const int64_t from = (a.part_row(seq, s, s.first + tok) * a.heads + head) * a.splits;
         float m = -INFINITY;
-        for (int p = threadIdx.x; p < parts; p += 64 * JOIN_WAVES) m = fmaxf(m, a.part_ml[from + p].x);
+        for (int p = threadIdx.x; p < parts; p += 64 * JOIN_WAVES) m = fmaxf(m, a.part_ml[of.at(p)].x);
         for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
         if (lane == 0) meet[wave][0] = m;
         __syncthreads();
         m = fmaxf(fmaxf(meet[0][0], meet[1][0]), fmaxf(meet[2][0], meet[3][0]));
         float l = 0.f;
         for (int p = threadIdx.x; p < parts; p += 64 * JOIN_WAVES) {
-            const float2 ml = a.part_ml[from + p];
+            const float2 ml = a.part_ml[of.at(p)];
             // (a part whose scores are no numbers has no maximum and a sum that is none)
             const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
             l += ml.x == -INFINITY ? ml.y : ml.y * f;
@@ -50,7 +77,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_kernel(Attend a, int 
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
-                for (int i = 0; i < PER; ++i) x[j][i] = a.part_o[(from + min(p0 + j * JOIN_WAVES, parts - 1)) * D + lane + 64 * i];
+                for (int i = 0; i < PER; ++i) x[j][i] = a.part_o[of.at(min(p0 + j * JOIN_WAVES, parts - 1)) * D + lane + 64 * i];
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
                 if (p0 + j * JOIN_WAVES < parts) {
@@ -95,21 +122,20 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_few_parts_kernel(Atte
     const int64_t all_rows = (int64_t)s.tokens() * a.group;
     if ((all_rows <= a.few_rows) != few || tok < 0) return;
     for (; tok < s.tokens(); tok += few ? tokens : 0x40000000) {
-        const int64_t r0 = ((int64_t)tok * a.group + head % a.group) / per * per, r1 = min(r0 + per, all_rows) - 1;
-        const KvSpan span(a, s, s.first + (int)(r0 / a.group), s.first + (int)(r1 / a.group));
-        const int parts = span.parts;
+        const PartsOf of(a, s, seq, tok, head, per);
+        const int parts = of.parts;
         if (parts > 1) {
-            const int64_t from = (a.part_row(seq, s, s.first + tok) * a.heads + head) * a.splits;
             float m = -INFINITY, l = 0.f, acc[PER] = {};
-            for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[from + p].x);
+            for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[of.at(p)].x);
             for (int p0 = 0; p0 < parts; p0 += AHEAD) {
                 float x[AHEAD][PER];
                 float2 ml[AHEAD];
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) {
-                    ml[j] = a.part_ml[from + min(p0 + j, parts - 1)];
+                    const int64_t from = of.at(min(p0 + j, parts - 1));
+                    ml[j] = a.part_ml[from];
 #pragma unroll
-                    for (int i = 0; i < PER; ++i) x[j][i] = a.part_o[(from + min(p0 + j, parts - 1)) * D + lane + 64 * i];
+                    for (int i = 0; i < PER; ++i) x[j][i] = a.part_o[from * D + lane + 64 * i];
                 }
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j)
@@ -130,7 +156,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_few_parts_kernel(Atte
 template <typename T, int D>
 static int join_of(const Attend& a, int per, bool few, int tokens, hipStream_t s) {
     const int64_t items = few ? (int64_t)a.seqs * tokens * a.heads : (int64_t)a.rows * a.heads;
-    const bool wide = few && a.splits > 8;   // four waves to a row from nine parts on
+    const bool wide = few && (a.chunks ? a.chunks > 8 * a.seqs : a.splits > 8);   // four waves to a row from nine parts on
     const int64_t blocks = wide ? items : (items + JOIN_WAVES - 1) / JOIN_WAVES;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
     const dim3 grid((unsigned)blocks), threads(64 * JOIN_WAVES);
@@ -178,7 +204,7 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     hipStream_t s = (hipStream_t)stream;
     const int group = heads / kv_heads;
     const Attend a{q, out, q_stride, out_stride, {(int8_t*)k_codes, (int8_t*)v_codes, (float*)k_scales, (float*)v_scales, pages, kv_heads, kv_log2(page_tokens)},
-                   table, lens, starts, table_stride, table_cols, seqs, rows, heads, group, window, scale, 1, 1, 0, nullptr, nullptr, 0};
+                   table, lens, starts, table_stride, table_cols, seqs, rows, heads, group, window, scale, (((uintptr_t)q | (uintptr_t)(q_stride * size)) & 15) == 0, 1, 1, 0, nullptr, nullptr, 0, 0};
     // What the caller says of the sizes chooses launches; whatever the sequences are, one of the kernels takes each.
     const int tokens = max_fresh < 1 ? 1 : max_fresh < rows ? max_fresh : rows;
     const int64_t most_rows = (int64_t)tokens * group;
@@ -190,28 +216,41 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     Attend af = a, am = a;
     const int few_max = many ? FEW_ROWS : max_rows, few_per = kv_few_rows(type == LK_TYPE_F32, head_dim, few_max);
     const int cus = lk_device().cus;
-    size_t rows_f = 0, rows_m = 0;   // whose parts are kept
     if (few) {
         af.few_rows = many ? FEW_ROWS : 0x7FFFFFFF;
-        cut(af, (int64_t)seqs * kv_heads * ((few_max + few_per - 1) / few_per), tiles, (getenv("KVW") ? atoi(getenv("KVW")) : 4) * cus, getenv("KVL") ? atoi(getenv("KVL")) : 16);
-        af.part_seq = many ? FEW_ROWS / group : tokens;
-        if (af.splits > 1) rows_f = (size_t)seqs * af.part_seq;
+        const int64_t groups = (int64_t)seqs * kv_heads * ((few_max + few_per - 1) / few_per);
+        // Long contexts of several sequences whose rows fit a workgroup each: pieces of equal length, two to a CU (as many as run at
+        // once). 64 sequences of 1 to 8010 tokens, 32 heads over 8 of 128 f32 values: 116 us against 139 with parts per sequence; all of
+        // 4096 104 against 107. With more than four heads and sequences to a CU parts per sequence balance by themselves (256 of 1024
+        // tokens: 108 us, 121 in pieces, whose every sequence costs a start of 3 us).
+        const int64_t most_steps = (int64_t)seqs * ((table_tokens + KV_TILE - 1) / KV_TILE + 1);
+        if (seqs > 1 && few_max <= few_per && groups <= 4 * cus && groups * tiles > 16 * cus && most_steps < 0x7FFFFFFF) {
+            af.chunks = (2 * cus + kv_heads - 1) / kv_heads;
+            af.least_tiles = 4;
+        } else {
+            // A context of up to 1024 positions stays in one launch; a longer one in parts of at least a step for each wave. One sequence
+            // of 1024 / 2048 / 8192 tokens: 12.1 / 13.6 / 13.9 us a call, with parts of 16 steps 12.0 / 16.7 / 17.9, of 4 steps from
+            // the start 13.8 / 13.6 / 13.9.
+            cut(af, groups, tiles, 2 * cus, tiles <= 16 ? 16 : 4);
+            af.part_seq = many ? FEW_ROWS / group : tokens;
+        }
     }
+    const int64_t part_rows_f = !few ? 0 : af.chunks ? (int64_t)kv_heads * af.chunks * 2 * few_per : af.splits > 1 ? (int64_t)seqs * af.part_seq * heads * af.splits : 0;
+    int64_t part_rows_m = 0;
     if (many) {
         am.few_rows = few ? FEW_ROWS : 0;
-        cut(am, ((int64_t)rows * group + KV_MANY_ROWS - 1) / KV_MANY_ROWS * kv_heads, tiles, (getenv("KVM") ? atoi(getenv("KVM")) : 2) * cus, 16);
-        if (am.splits > 1) rows_m = rows;
+        cut(am, ((int64_t)rows * group + KV_MANY_ROWS - 1) / KV_MANY_ROWS * kv_heads, tiles, 2 * cus, 16);
+        if (am.splits > 1) part_rows_m = (int64_t)rows * heads * am.splits;
     }
     LkScratch scratch(s);
-    const size_t floats_f = rows_f * heads * af.splits * (head_dim + 2), floats_m = rows_m * heads * am.splits * (head_dim + 2);
-    if (floats_f + floats_m) {
-        float* mem = (float*)scratch.get(LK_SCRATCH_ATTENTION, (floats_f + floats_m) * 4);
+    if (part_rows_f + part_rows_m) {
+        const size_t floats = (size_t)(part_rows_f + part_rows_m) * (head_dim + 2);
+        float* mem = (float*)scratch.get(LK_SCRATCH_ATTENTION, floats * 4);
         if (!mem) return LK_ERR_NOMEM;
         af.part_ml = (float2*)mem;
-        af.part_o = mem + rows_f * heads * af.splits * 2;
-        mem += floats_f;
-        am.part_ml = (float2*)mem;
-        am.part_o = mem + rows_m * heads * am.splits * 2;
+        am.part_ml = af.part_ml + part_rows_f;
+        af.part_o = mem + 2 * (part_rows_f + part_rows_m);
+        am.part_o = af.part_o + part_rows_f * head_dim;
     }
     auto join_parts = [&](const Attend& x, int per, bool is_few, int toks) {
         if (type == LK_TYPE_F32) return join<float>(x, head_dim, per, is_few, toks, s);
@@ -221,7 +260,7 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     int status = LK_OK;
     if (many) status = kv_attention_many(am, type, head_dim, max_rows, s);
     if (status == LK_OK && few) status = kv_attention_few(af, type, head_dim, few_max, s);
-    if (status == LK_OK && many && am.splits > 1) status = join_parts(am, KV_MANY_ROWS, false, tokens);
-    if (status == LK_OK && few && af.splits > 1) status = join_parts(af, few_per, true, af.part_seq);
+    if (status == LK_OK && part_rows_m) status = join_parts(am, KV_MANY_ROWS, false, tokens);
+    if (status == LK_OK && part_rows_f) status = join_parts(af, few_per, true, many ? FEW_ROWS / group : tokens);
     return status;
 }

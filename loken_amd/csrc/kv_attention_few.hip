@@ -56,34 +56,108 @@ static __device__ __forceinline__ uint32_t four_digits(int t0, int t1, int t2, i
 }
 
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_few_kernel(Attend a, int row_tiles) {
+__global__ __launch_bounds__(64 * WAVES, D < 256 && !(D == 128 && NT == 2) ? 2 : 1) void kv_attention_few_kernel(Attend a, int row_tiles) {
     using F = Few<T, D, NT>;
     __shared__ float sums[WAVES][F::ROWS][D];
     __shared__ float tops[WAVES][F::ROWS], weights[WAVES][F::ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
-    // the workgroup's place: part fastest, then row tile, head, sequence
-    unsigned at = blockIdx.x;
-    const int part = at % a.splits;
-    at /= a.splits;
-    const int tile0 = at % row_tiles;
-    at /= row_tiles;
-    const int kv = at % a.pool.heads, seq = at / a.pool.heads;
-    const KvSeq s(a, seq);
-    const int all_rows = s.tokens() * a.group;
-    if (all_rows > a.few_rows) return;
     const int shift = a.pool.page_shift, runs = shift - 4;   // log2 of the runs of a page
     const int slot = i % F::SLOTS;
     const float digit = slot >= F::DIGITS ? 0.f : slot == F::DIGITS - 1 ? 1.f : slot == F::DIGITS - 2 ? 256.f : 65536.f;
     // v_perm selector of the slot's byte out of two words, zeros above; the slot without a digit takes zeros
     const uint32_t byte = F::DIGITS - 1 - slot, pick = slot < F::DIGITS ? 0x0C0C0000u | byte | (byte + 4) << 8 : 0x0C0C0C0Cu;
-    for (int tile = tile0; tile * F::ROWS < all_rows; tile += row_tiles) {
+    // The workgroup's place: (part, row tile, head, sequence), the part fastest; or (head, piece), a piece being of one or
+    // several sequences.
+    int kv, seq, seq_end, tile0 = 0, part = 0;
+    int first_step = 0, at_step = 0, end_step = 0, length = 1;   // the first step of `seq`, the piece's steps, and how many a piece has
+    if (a.chunks) {
+        kv = blockIdx.x % a.pool.heads;
+        part = blockIdx.x / a.pool.heads;
+        const KvPieces pieces(a, F::ROWS);
+        length = pieces.length;
+        if ((int64_t)part * length >= pieces.total) return;
+        at_step = part * length;
+        end_step = (int)min((int64_t)at_step + length, (int64_t)pieces.total);
+        seq = __builtin_amdgcn_readfirstlane(KvPieces::sequence_at(a, F::ROWS, at_step, first_step));
+        first_step = __builtin_amdgcn_readfirstlane(first_step);
+        seq_end = a.seqs;
+        row_tiles = 1;
+    } else {
+        unsigned at = blockIdx.x;
+        part = at % a.splits;
+        at /= a.splits;
+        tile0 = at % row_tiles;
+        at /= row_tiles;
+        kv = at % a.pool.heads;
+        seq = at / a.pool.heads;
+        seq_end = seq + 1;
+    }
+    for (int steps = 0; seq < seq_end && (a.chunks == 0 || first_step < end_step); ++seq, first_step += steps) {
+      const KvSeq s(a, seq);
+      const int64_t rows_of_all = (int64_t)s.tokens() * a.group;
+      steps = 0;
+      if (rows_of_all == 0 || rows_of_all > a.few_rows) continue;
+      const int all_rows = (int)rows_of_all;
+      for (int tile = tile0; tile * F::ROWS < all_rows; tile += row_tiles) {
         const int r0 = tile * F::ROWS, r1 = min(r0 + F::ROWS, all_rows) - 1;
         const KvSpan span(a, s, s.first + r0 / a.group, s.first + r1 / a.group);
-        const int per_part = span.per_part, parts = span.parts;
-        if (part >= parts) continue;
-        const int t_end = min(span.tiles, (part + 1) * per_part);
+        int t_begin = 0, t_end = span.tiles;
+        int64_t to = -1;   // the first row of the sums' place among the parts; -1: they are not a part
+        if (a.chunks) {
+            steps = all_rows > F::ROWS ? 1 : max(1, span.tiles);   // as kv_steps_of
+            if (all_rows <= F::ROWS) {
+                t_begin = max(at_step - first_step, 0);
+                t_end = min(end_step - first_step, span.tiles);
+                if (first_step < at_step || first_step + steps > end_step)
+                    to = (((int64_t)kv * a.chunks + part) * 2 + (first_step / length == part ? 1 : 0)) * F::ROWS;
+            }
+        } else {
+            if (part >= span.parts) continue;
+            t_begin = part * span.per_part;
+            t_end = min(span.tiles, t_begin + span.per_part);
+            if (span.parts > 1) to = 0;
+        }
 
+        // The first step's keys and values are on their way while the rows' digits are made.
+        // A step's page of the lane's run: of run i / 4 as the keys' operand has it, of run g for everything else
+        const int32_t* entries = a.table + seq * a.table_stride;
+        auto page_of = [&](int t, int run) {
+            const int p0 = span.lo + t * KV_TILE + 16 * run;
+            const int page = t < t_end && p0 < span.hi ? entries[p0 >> shift] : -1;
+            return (unsigned)page < (unsigned)a.pool.pages ? page : -1;
+        };
+        uint4 k[4 * F::KK], v[F::NB];
+        float ks = 0.f, vs = 0.f;
+        auto load_keys = [&](int t, int kp) {
+            const int64_t page = (int64_t)max(kp, 0) * a.pool.heads + kv;
+            const int run = ((span.lo >> 4) + 4 * t + (i >> 2)) & ((1 << runs) - 1);
+            const int8_t* from = a.pool.k + ((page << shift) + 16 * run + (i & 3)) * D + 16 * g;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int kk = 0; kk < F::KK; ++kk) k[b * F::KK + kk] = *(const uint4*)(from + 4 * b * D + 64 * kk);
+        };
+        auto load_values = [&](int t, int vp) {
+            const int64_t page = (int64_t)max(vp, 0) * a.pool.heads + kv;
+            const int run = ((span.lo >> 4) + 4 * t + g) & ((1 << runs) - 1);
+            const int8_t* from = a.pool.v + (page << shift) * D + (run * D + i) * 16;
+#pragma unroll
+            for (int b = 0; b < F::NB; ++b) v[b] = *(const uint4*)(from + 256 * b);
+        };
+        auto load_scales = [&](int vp) {
+            const int64_t page = (int64_t)max(vp, 0) * a.pool.heads + kv;
+            ks = a.pool.k_scales[page];
+            vs = vp >= 0 ? a.pool.v_scales[page] : 0.f;
+        };
+        int t = t_begin + wave;
+        int kp = page_of(t, i >> 2), vp = page_of(t, g);
+        if (t < t_end) {
+            load_keys(t, kp);
+            load_scales(vp);
+            load_values(t, vp);
+        }
+        int kp_next = page_of(t + WAVES, i >> 2), vp_next = page_of(t + WAVES, g);
         // the rows' digits, and what a unit of the scores is in powers of two
         uint4 q[NT][F::KK];
         float unit[NT];
@@ -96,9 +170,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_few_kernel(Attend 
             const T* row = (const T*)a.q + tok * a.q_stride + (int64_t)head * D + 16 * g;
             float x[F::KK][16];
 #pragma unroll
-            for (int kk = 0; kk < F::KK; ++kk)
+            for (int kk = 0; kk < F::KK; ++kk) {
+                if (a.q_aligned) {
+                    T raw[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[kk][e] = to_f32(row[64 * kk + e]);
+                    for (int e = 0; e < (int)sizeof(T); ++e) ((uint4*)raw)[e] = ((const uint4*)(row + 64 * kk))[e];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[kk][e] = to_f32(raw[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[kk][e] = to_f32(row[64 * kk + e]);
+                }
+            }
             uint32_t most = 0;   // as bits, where what is not a number is the largest
 #pragma unroll
             for (int kk = 0; kk < F::KK; ++kk)
@@ -148,44 +231,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_few_kernel(Attend 
                 for (int b = 0; b < F::NB; ++b) acc[n][p][b] = 0.f;
         }
 
-        // a step's page of the lane's run: of run i / 4 as the keys' operand has it, of run g for everything else
-        const int32_t* entries = a.table + seq * a.table_stride;
-        auto page_of = [&](int t, int run) {
-            const int p0 = span.lo + t * KV_TILE + 16 * run;
-            const int page = t < t_end && p0 < span.hi ? entries[p0 >> shift] : -1;
-            return (unsigned)page < (unsigned)a.pool.pages ? page : -1;
-        };
-        uint4 k[4 * F::KK], v[F::NB];
-        float ks = 0.f, vs = 0.f;
-        auto load_keys = [&](int t, int kp) {
-            const int64_t page = (int64_t)max(kp, 0) * a.pool.heads + kv;
-            const int run = ((span.lo >> 4) + 4 * t + (i >> 2)) & ((1 << runs) - 1);
-            const int8_t* from = a.pool.k + ((page << shift) + 16 * run + (i & 3)) * D + 16 * g;
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int kk = 0; kk < F::KK; ++kk) k[b * F::KK + kk] = *(const uint4*)(from + 4 * b * D + 64 * kk);
-        };
-        auto load_values = [&](int t, int vp) {
-            const int64_t page = (int64_t)max(vp, 0) * a.pool.heads + kv;
-            const int run = ((span.lo >> 4) + 4 * t + g) & ((1 << runs) - 1);
-            const int8_t* from = a.pool.v + (page << shift) * D + (run * D + i) * 16;
-#pragma unroll
-            for (int b = 0; b < F::NB; ++b) v[b] = *(const uint4*)(from + 256 * b);
-        };
-        auto load_scales = [&](int vp) {
-            const int64_t page = (int64_t)max(vp, 0) * a.pool.heads + kv;
-            ks = a.pool.k_scales[page];
-            vs = vp >= 0 ? a.pool.v_scales[page] : 0.f;
-        };
-        int t = part * per_part + wave;
-        int kp = page_of(t, i >> 2), vp = page_of(t, g);
-        if (t < t_end) {
-            load_keys(t, kp);
-            load_scales(vp);
-            load_values(t, vp);
-        }
-        int kp_next = page_of(t + WAVES, i >> 2), vp_next = page_of(t + WAVES, g);
         for (; t < t_end; t += WAVES) {
             const int p0 = span.lo + t * KV_TILE + 16 * g;   // the lane's first position
             // whether every row sees every position of the step
@@ -318,15 +363,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_few_kernel(Attend 
             }
             const int64_t row = s.first + (r0 + r) / a.group;
             const int head = kv * a.group + (r0 + r) % a.group;
-            if (parts == 1) {
+            if (to < 0) {
                 ((T*)a.out)[row * a.out_stride + (int64_t)head * D + d] = from_f32<T>(lw == 0.f ? 0.f : total / lw);
             } else {
-                const int64_t to = (a.part_row(seq, s, (int)row) * a.heads + head) * a.splits + part;
-                a.part_o[to * D + d] = total;
-                if (d == 0) a.part_ml[to] = make_float2(top, lw);
+                const int64_t place = a.chunks ? to + r : (a.part_row(seq, s, (int)row) * a.heads + head) * a.splits + part;
+                a.part_o[place * D + d] = total;
+                if (d == 0) a.part_ml[place] = make_float2(top, lw);
             }
         }
         __syncthreads();
+      }
     }
 }
 
@@ -334,7 +380,7 @@ template <typename T, int D>
 static int launch(const Attend& a, int max_rows, hipStream_t s) {
     const int per = kv_few_rows(sizeof(T) == 4, D, max_rows), row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / per + 1;
     const bool two = per > Few<T, D, 1>::RPT;
-    const int64_t blocks = (int64_t)a.seqs * a.pool.heads * row_tiles * a.splits;
+    const int64_t blocks = a.chunks ? (int64_t)a.chunks * a.pool.heads : (int64_t)a.seqs * a.pool.heads * row_tiles * a.splits;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
     if (two) hipLaunchKernelGGL((kv_attention_few_kernel<T, D, (D < 256 ? 2 : 1)>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a, row_tiles);
     else hipLaunchKernelGGL((kv_attention_few_kernel<T, D, 1>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a, row_tiles);

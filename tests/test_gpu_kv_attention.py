@@ -241,3 +241,22 @@ def test_a_row_does_not_depend_on_its_companions():
         one = kv.kv_attention(b.q[i:i + 1].cuda(), b.cache(), i32(b.table[i:i + 1]), i32(b.lens[i:i + 1]), i32([0, 1]), max_fresh=1, max_len=900)
         assert (one[0] - whole[i]).abs().max() <= 2e-5 * whole[i].abs().max()   # split over other workgroups: the parts join in another order
     assert torch.equal(whole, b.check(max_len=900))
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("what", ["ragged", "one long", "window", "more rows than said", "beside a prompt"])
+def test_many_contexts_are_cut_into_equal_pieces(what, dtype):
+    """Enough sequences for pieces that hold several of them, ends of them, and sequences without rows or tokens."""
+    g = np.random.default_rng(40)
+    lens = [0, 1, 64, 65, 0] + [int(v) for v in g.integers(1, 5000, 36)] + [0, 3]
+    fresh = [0] + [1] * 42
+    fresh[4], fresh[11], fresh[20], fresh[42] = 1, 0, 2, 0
+    if what == "one long":
+        lens = [100] * 42 + [40000]
+    if what == "more rows than said":
+        fresh[7], fresh[30] = 9, 40
+    if what == "beside a prompt":
+        fresh[9] = 70
+    b = Batch(lens, fresh, 2, 1, 64, 16, dtype, seed=41, pad=3)
+    out = b.check(window=700 if what == "window" else 0, max_fresh=2 if what != "beside a prompt" else 70, max_len=9000)
+    assert (out[-3:] == 7).all()
