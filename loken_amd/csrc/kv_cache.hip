@@ -116,14 +116,21 @@ __global__ __launch_bounds__(PLAN_WG) void kv_plan_kernel(const int32_t* __restr
 }
 
 // ---------------------------------------------------------------------------------------------
-// New rows into the cache. The rows of a call that belong to one page, with no row of another between them, are a run; the wave that
-// finds a run's first row writes the run. With s_old the page's scale (0 where the run holds the page's first
-// token, which starts the page anew):
+// New rows into the cache. The rows of a call that belong to one page, with no row of another between them, are a run; the workgroup that
+// finds a run's first row writes the run: a workgroup for its keys, one for its values, of as many waves as hold a page. With s_old the page's scale (0 where the run
+// holds the page's first token, which starts the page anew):
 //     s = max(s_old, max |x| / 127),   old codes c -> round(c s_old / s),   new codes round(x / s)
 // quotients exact, halves away from zero. A product with 1 / s gives the quotient's whole part q or its neighbour; the
 // remainder x - q s is exact in one fused multiply-add (for q > 0 both are multiples of s's last place, and what is left is
 // below 2 s), and at least half of s where the code is one more.
+//
+// What it costs is latency: slots, then rows and scale, then (where a scale grows) the page. A lane holds four columns of eight
+// consecutive rows, whose loads are all in flight together: four codes of a key row are one store, eight of a value column another.
+// 64 single tokens of 8 heads of 128 in f32: 6 us; 4400 rows in bf16: 10 us. (Slots looked up row by row, with a fence before the new
+// codes: 12 and 51 us.)
 // ---------------------------------------------------------------------------------------------
+constexpr int ROWS_HELD = 8, WRITE_WAVES = 8;
+
 static __device__ __forceinline__ float wave_most(float v) {
     for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
     return v;
@@ -145,139 +152,229 @@ static __device__ __forceinline__ int rescaled(int c, float ratio, double s_old,
     return c < 0 ? -q : q;
 }
 
+static __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+    return (uint32_t)(a & 0xFF) | (uint32_t)(b & 0xFF) << 8 | (uint32_t)(c & 0xFF) << 16 | (uint32_t)(d & 0xFF) << 24;
+}
+
 template <typename T, int D>
-__global__ __launch_bounds__(128) void kv_write_kernel(const T* __restrict__ k, const T* __restrict__ v, int64_t k_stride, int64_t v_stride,
-                                                       const int64_t* __restrict__ slots, int tokens, KvPool pool, int window) {
-    constexpr int PER = D / 64;
-    const int lane = threadIdx.x & 63, head = blockIdx.y;
-    const bool values = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) != 0;   // wave 0: keys, wave 1: values
+__global__ __launch_bounds__(64 * WRITE_WAVES) void kv_write_kernel(const T* __restrict__ k, const T* __restrict__ v, int64_t k_stride, int64_t v_stride,
+                                                       bool aligned, const int64_t* __restrict__ slots, int tokens, KvPool pool, int window) {
+    constexpr int LANES = D / 4;                       // of a row
+    constexpr int OF_WAVE = ROWS_HELD * (64 / LANES);  // rows that a wave holds
+    __shared__ uint32_t tables[64];
+    __shared__ float meet[WRITE_WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int head = blockIdx.y, side = blockIdx.z;    // keys, values
+    const int batch = OF_WAVE * waves, d0 = 4 * (lane % LANES), row0 = OF_WAVE * wave + ROWS_HELD * (lane / LANES);
     const int P = 1 << pool.page_shift, shift = pool.page_shift;
-    auto page_at = [&](int t) -> int64_t {
-        if (t < 0 || t >= tokens) return -1;
-        const int64_t s = slots[t];
-        return s < 0 || (s >> shift) >= pool.pages ? -1 : s >> shift;
-    };
-    const T* rows = (values ? v : k) + (int64_t)head * D + lane;
-    const int64_t stride = values ? v_stride : k_stride;
-    const int first = blockIdx.x * window;
-    const int64_t mine = lane < window ? page_at(first + lane) : -1;
-    uint64_t leaders = __ballot(mine >= 0 && mine != page_at(first + lane - 1));
+    auto page_of = [&](int64_t slot) -> int64_t { return slot < 0 || (slot >> shift) >= pool.pages ? -1 : slot >> shift; };
+    auto slot_at = [&](int t) -> int64_t { return t < 0 || t >= tokens ? -1 : slots[t]; };
+    const T* rows = (side ? v : k) + (int64_t)head * D + d0;
+    const int64_t stride = side ? v_stride : k_stride;
+    // the window's rows, the one before them and what fits behind
+    const int first = blockIdx.x * window, base = first - 1;
+    const int64_t my_slot = slot_at(base + lane), my_page = page_of(my_slot);
+    const int64_t page_before = __shfl_up((long long)my_page, 1);   // (by all lanes: one that is left out has nothing to give)
+    uint64_t leaders = __ballot(my_page >= 0 && my_page != page_before) & ((1ull << window) - 1) << 1;
     while (leaders) {
-        const int t0 = first + __ffsll((unsigned long long)leaders) - 1;
+        const int at = __ffsll((unsigned long long)leaders) - 1, t0 = base + at;
         leaders &= leaders - 1;
-        const int64_t page = page_at(t0);
+        const int64_t page = __shfl((long long)my_page, at), slot0 = __shfl((long long)my_slot, at);
         // absent rows do not end a run: the last row before them may be of the same page
         bool inside = false;
-        for (int t = t0; t > 0; t -= 64) {
-            const int64_t before = page_at(t - 1 - lane);
-            const uint64_t there = __ballot(before >= 0);
-            if (!there) continue;
-            inside = (__ballot(before == page) >> (__ffsll((unsigned long long)there) - 1)) & 1;
-            break;
-        }
-        if (inside) continue;
-        // the run's length, and whether it holds the page's first token
-        int n = 0;
-        bool anew = false;
-        for (;;) {
-            const int t = t0 + n + lane;
-            const int64_t here = page_at(t);
-            const uint64_t ends = __ballot(t >= tokens || (here >= 0 && here != page));
-            const uint64_t zero = __ballot(here == page && (slots[t] & (P - 1)) == 0);
-            const int more = ends ? __ffsll((unsigned long long)ends) - 1 : 64;
-            anew = anew || (zero & (more == 64 ? ~0ull : (1ull << more) - 1)) != 0;
-            n += more;
-            if (more < 64) break;
-        }
-        float most = 0.0f;
-        for (int j = 0; j < n; ++j) {
-            if (page_at(t0 + j) != page) continue;   // an absent row
-            const T* row = rows + (int64_t)(t0 + j) * stride;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const float a = fabsf(to_f32(row[64 * i]));
-                most = fmaxf(most, a <= 3.402823466e38f ? a : 0.0f);   // the scale is that of the finite values
+        if (t0 > 0 && __shfl((long long)my_page, at - 1) < 0)
+            for (int t = t0; t > 0; t -= 64) {
+                const int64_t before = page_of(slot_at(t - 1 - lane));
+                const uint64_t there = __ballot(before >= 0);
+                if (!there) continue;
+                inside = (__ballot(before == page) >> (__ffsll((unsigned long long)there) - 1)) & 1;
+                break;
             }
+        if (inside) continue;
+        // The run's length; whether it holds the page's first token; whether its rows are the page's tokens in their order.
+        int n = 0;
+        bool anew = false, straight = true;
+        for (int skip = at;; skip = 0) {
+            const int t = n == 0 ? base + lane : t0 + n + lane;
+            const int64_t slot = n == 0 ? my_slot : slot_at(t), here = page_of(slot);
+            const uint64_t from = ~0ull << skip;
+            const uint64_t ends = __ballot(t >= tokens || (here >= 0 && here != page)) & from;
+            const int stop = ends ? __ffsll((unsigned long long)ends) - 1 : 64;
+            const uint64_t in = from & (stop == 64 ? ~0ull : (1ull << stop) - 1);
+            anew = anew || (__ballot(here == page && (slot & (P - 1)) == 0) & in) != 0;
+            straight = straight && (__ballot(slot != slot0 + (t - t0)) & in) == 0;
+            n += stop - skip;
+            if (stop < 64) break;
+        }
+        const bool whole = straight && n == P;   // (then it starts with the first)
+        float x[ROWS_HELD][4];
+        int64_t off[ROWS_HELD];   // the token's place in the page; -1: not the page's
+        auto load = [&](int j0) {
+#pragma unroll
+            for (int i = 0; i < ROWS_HELD; ++i) {
+                const int j = j0 + row0 + i;
+                off[i] = -1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
+                if (j < n) {
+                    const T* row = rows + (int64_t)(t0 + j) * stride;
+                    if (aligned) {
+                        const float4 f = Load4<T>::at(row);
+                        x[i][0] = f.x; x[i][1] = f.y; x[i][2] = f.z; x[i][3] = f.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[i][e] = to_f32(row[e]);
+                    }
+                    const int64_t slot = straight ? slot0 + j : slots[t0 + j];
+                    off[i] = page_of(slot) == page ? slot & (P - 1) : -1;
+                }
+            }
+        };
+        float* scale_at = (side ? pool.v_scales : pool.k_scales) + page * pool.heads + head;
+        const float stored = *scale_at;
+        float most = 0.0f;
+        for (int j0 = 0; j0 < n; j0 += batch) {
+            load(j0);
+#pragma unroll
+            for (int i = 0; i < ROWS_HELD; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = fabsf(x[i][e]);
+                    most = fmaxf(most, off[i] >= 0 && a <= 3.402823466e38f ? a : 0.0f);   // the scale is that of the finite values
+                }
         }
         most = wave_most(most);
-        float* scale_at = (values ? pool.v_scales : pool.k_scales) + page * pool.heads + head;
-        const float stored = *scale_at;
+        if (waves > 1) {
+            __syncthreads();   // the last run's reads
+            if (lane == 0) meet[wave] = most;
+            __syncthreads();
+            for (int w = 0; w < waves; ++w) most = fmaxf(most, meet[w]);
+        }
         const float s_old = !anew && stored <= 3.402823466e38f && stored > 0.0f ? stored : 0.0f;
         float s = fmaxf(s_old, most / 127.0f);
         if (s < 1.17549435e-38f) s = 0.0f;   // a scale with no normal 1 / s: the page holds zeros
-        int8_t* codes = (values ? pool.v : pool.k) + ((page * pool.heads + head) << shift) * D;
-        if (anew || s != s_old) {
+        int8_t* codes = (side ? pool.v : pool.k) + ((page * pool.heads + head) << shift) * D;
+        if ((anew || s != s_old) && threadIdx.x == 0) *scale_at = s;
+        if ((anew && !whole) || (!anew && s != s_old)) {
             const float ratio = s > 0.0f ? s_old / s : 0.0f;
-            for (int at = lane * 16; at < (D << shift); at += 64 * 16) {
+            // what each byte becomes: four of them a lane
+            uint8_t* table = (uint8_t*)tables;
+            if (s_old > 0.0f) {
+                if (wave == 0) tables[lane] = pack4(rescaled((int8_t)(4 * lane), ratio, s_old, s), rescaled((int8_t)(4 * lane + 1), ratio, s_old, s),
+                                           rescaled((int8_t)(4 * lane + 2), ratio, s_old, s), rescaled((int8_t)(4 * lane + 3), ratio, s_old, s));
+                __syncthreads();
+            }
+            for (int p = threadIdx.x * 16; p < (D << shift); p += blockDim.x * 16) {
                 uint4 w = make_uint4(0, 0, 0, 0);
                 if (s_old > 0.0f) {
-                    w = *(const uint4*)(codes + at);
+                    w = *(const uint4*)(codes + p);
                     uint32_t* u = (uint32_t*)&w;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t r = 0;
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) r |= (uint32_t)(rescaled((int8_t)(u[i] >> (8 * b)), ratio, s_old, s) & 0xFF) << (8 * b);
-                        u[i] = r;
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        u[i] = (uint32_t)table[u[i] & 0xFF] | (uint32_t)table[u[i] >> 8 & 0xFF] << 8 | (uint32_t)table[u[i] >> 16 & 0xFF] << 16 |
+                               (uint32_t)table[u[i] >> 24] << 24;
                 }
-                *(uint4*)(codes + at) = w;
+                *(uint4*)(codes + p) = w;
             }
-            if (lane == 0) *scale_at = s;
-            __threadfence();   // the new codes below are stored after these, which other lanes wrote
+            // the new codes below go where other threads have just stored: stores that have been waited for are in front of them
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
         }
         const float inv = s > 0.0f ? 1.0f / s : 0.0f;
-        for (int j = 0; j < n;) {
-            const int t = t0 + j;
-            if (page_at(t) != page) { ++j; continue; }
-            const int off = (int)(slots[t] & (P - 1));
-            const T* row = rows + (int64_t)t * stride;
-            // a whole run of sixteen values of a column is one store
-            if (values && (off & 15) == 0 && j + 16 <= n && __ballot(lane < 16 && slots[t + min(lane, 15)] != slots[t] + lane) == 0) {
+        for (int j0 = 0; straight && j0 < n; j0 += batch) {
+            if (n > batch) load(j0);
+            int c[ROWS_HELD][4];
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    uint32_t w[4] = {0, 0, 0, 0};
+            for (int i = 0; i < ROWS_HELD; ++i)
 #pragma unroll
-                    for (int b = 0; b < 16; ++b)
-                        w[b / 4] |= (uint32_t)(code_of(to_f32(row[b * stride + 64 * i]), s, inv) & 0xFF) << (8 * (b % 4));
-                    *(uint4*)(codes + ((off >> 4) * D + lane + 64 * i) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-                j += 16;
-                continue;
+                for (int e = 0; e < 4; ++e) c[i][e] = code_of(x[i][e], s, inv);
+            if (side == 0) {
+#pragma unroll
+                for (int i = 0; i < ROWS_HELD; ++i)
+                    if (off[i] >= 0) *(uint32_t*)(codes + off[i] * D + d0) = pack4(c[i][0], c[i][1], c[i][2], c[i][3]);
+            } else if (off[ROWS_HELD - 1] >= 0 && (off[0] & 7) == 0) {
+#pragma unroll
+                for (int h = 0; h < ROWS_HELD; h += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        *(uint2*)(codes + ((off[h] >> 4) * D + d0 + e) * 16 + (off[h] & 8)) =
+                            make_uint2(pack4(c[h][e], c[h + 1][e], c[h + 2][e], c[h + 3][e]), pack4(c[h + 4][e], c[h + 5][e], c[h + 6][e], c[h + 7][e]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < ROWS_HELD; ++i)
+                    if (off[i] >= 0)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) codes[((off[i] >> 4) * D + d0 + e) * 16 + (off[i] & 15)] = (int8_t)c[i][e];
             }
+        }
+        // Other runs may name a token twice, and the last row stays: one row after the other, a column always the same lane's.
+        for (int j = 0; !straight && wave == 0 && j < n; ++j) {
+            const int64_t slot = slots[t0 + j];
+            if (page_of(slot) != page || lane >= LANES) continue;
+            const T* row = rows + (int64_t)(t0 + j) * stride;
+            const int place = (int)(slot & (P - 1));
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int d = lane + 64 * i, c = code_of(to_f32(row[64 * i]), s, inv);
-                codes[values ? ((off >> 4) * D + d) * 16 + (off & 15) : off * D + d] = (int8_t)c;
+            for (int e = 0; e < 4; ++e) {
+                const int c = code_of(to_f32(row[e]), s, inv);
+                codes[side ? ((place >> 4) * D + d0 + e) * 16 + (place & 15) : place * D + d0 + e] = (int8_t)c;
             }
-            ++j;
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Rows of the cache as values: one wave to sixteen rows of a head and side.
+// Rows of the cache as values: a wave to sixteen rows of a head and side. Sixteen rows that are a run of the cache (sixteen tokens
+// in their order) are one load a column of the values.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D>
 __global__ __launch_bounds__(128) void kv_read_kernel(const int64_t* __restrict__ slots, int tokens, KvPool pool, T* __restrict__ k_out,
                                                       T* __restrict__ v_out) {
     constexpr int PER = D / 64;
-    const int lane = threadIdx.x & 63, head = blockIdx.y;
+    const int lane = threadIdx.x & 63, head = blockIdx.y, t0 = blockIdx.x * 16, n = min(tokens - t0, 16);
     const bool values = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) != 0;
     const int shift = pool.page_shift, mask = (1 << shift) - 1;
-    T* out = values ? v_out : k_out;
-    for (int t = blockIdx.x * 16; t < min(tokens, (int)blockIdx.x * 16 + 16); ++t) {
-        const int64_t slot = slots[t], page = slot >> shift;
-        const bool held = slot >= 0 && page < pool.pages;
-        const int off = (int)(slot & mask);
-        const int8_t* codes = (values ? pool.v : pool.k) + (((held ? page : 0) * pool.heads + head) << shift) * D;
-        const float s = (values ? pool.v_scales : pool.k_scales)[(held ? page : 0) * pool.heads + head];
+    const int8_t* codes = values ? pool.v : pool.k;
+    const float* scales = values ? pool.v_scales : pool.k_scales;
+    T* out = (values ? v_out : k_out) + ((int64_t)t0 * pool.heads + head) * D + lane;
+    const int64_t row = (int64_t)pool.heads * D;
+    // lanes 0 .. 15: a row's slot, where its codes start, and its scale
+    const int64_t slot = (lane & 15) < n ? slots[t0 + (lane & 15)] : -1, page = slot >> shift;
+    const bool held = slot >= 0 && page < pool.pages;
+    const int64_t at_page = (held ? page : 0) * pool.heads + head;
+    const int64_t start = (at_page << shift) * D;
+    const float s = held ? scales[at_page] : 0.0f;
+    const int off = held ? (int)(slot & mask) : 0;
+    const int64_t slot0 = __shfl((long long)slot, 0);
+    if (values && __ballot(!held || slot != slot0 + (lane & 15) || (slot0 & 15) != 0) == 0) {
+        const float s0 = __shfl(s, 0);
+        const int8_t* from = codes + __shfl((long long)start, 0) + ((int64_t)(__shfl(off, 0) >> 4) * D + lane) * 16;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint4 w = *(const uint4*)(from + 64 * 16 * i);
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 16; ++j) out[j * row + 64 * i] = from_f32<T>((float)(int8_t)(u[j / 4] >> (8 * (j % 4))) * s0);
+        }
+        return;
+    }
+    int8_t c[16][PER];   // all loads before the first store
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {   // (a row that is absent or none: of page 0, and not used)
+        const int offj = __shfl(off, j);
+        const int8_t* from = codes + __shfl((long long)start, j);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int d = lane + 64 * i;
-            const int8_t c = codes[values ? ((off >> 4) * D + d) * 16 + (off & 15) : off * D + d];
-            out[((int64_t)t * pool.heads + head) * D + d] = from_f32<T>(held ? (float)c * s : 0.0f);
+            c[j][i] = from[values ? ((offj >> 4) * D + d) * 16 + (offj & 15) : offj * D + d];
         }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const float sj = __shfl(s, j);   // 0 where the row is absent
+        const bool is = __shfl((int)held, j) != 0;
+        if (j < n)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) out[j * row + 64 * i] = from_f32<T>(is ? (float)c[j][i] * sj : 0.0f);
     }
 }
 
@@ -298,8 +395,11 @@ static int by_type_and_dim(int type, int head_dim, A... a) {
 template <typename T, int D>
 struct Write {
     static void run(const void* k, const void* v, int64_t ks, int64_t vs, const int64_t* slots, int tokens, KvPool pool, int window, hipStream_t s) {
-        hipLaunchKernelGGL((kv_write_kernel<T, D>), dim3((tokens + window - 1) / window, pool.heads), dim3(128), 0, s, (const T*)k, (const T*)v,
-                           ks, vs, slots, tokens, pool, window);
+        const int four = 4 * sizeof(T) - 1;
+        const bool aligned = (((uintptr_t)k | (uintptr_t)v | (uintptr_t)(ks * sizeof(T)) | (uintptr_t)(vs * sizeof(T))) & four) == 0;
+        const int of_wave = ROWS_HELD * 256 / D, waves = min(WRITE_WAVES, ((1 << pool.page_shift) + of_wave - 1) / of_wave);
+        hipLaunchKernelGGL((kv_write_kernel<T, D>), dim3((tokens + window - 1) / window, pool.heads, 2), dim3(64 * waves), 0, s, (const T*)k,
+                           (const T*)v, ks, vs, aligned, slots, tokens, pool, window);
     }
 };
 template <typename T, int D>
@@ -342,7 +442,9 @@ extern "C" int lk_kv_write_q8(const void* k, const void* v, int type, int64_t k_
         v_stride < row)
         return LK_ERR_ARG;
     const KvPool pool{(int8_t*)k_codes, (int8_t*)v_codes, k_scales, v_scales, pages, kv_heads, kv_log2(page_tokens)};
-    const int window = tokens <= 512 ? 1 : 16;
+    // Rows of which a workgroup writes the runs that start there, one after the other: single tokens' runs are a row each, a prompt's a
+    // page.
+    const int window = tokens <= 128 ? 1 : tokens <= 1024 ? 4 : 16;
     return by_type_and_dim<Write>(type, head_dim, k, v, k_stride, v_stride, slots, tokens, pool, window, (hipStream_t)stream);
 }
 
