@@ -17,6 +17,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "lk_common.h"
 #include "stream_scratch.h"
 
@@ -26,6 +28,7 @@ namespace {
 
 constexpr int BINS = 2048;        // steps of the histogram
 constexpr int LIST = 2048;        // words that are sorted in LDS
+constexpr int COUNTED = 256;      // words up to which each is counted to its place
 constexpr int SAMPLE_WG = 512, SAMPLE_WAVES = SAMPLE_WG / 64;
 constexpr int ONE_BITS = 42;      // a weight of 1 is 2^42
 constexpr float LIVE = 42.5f;     // words below 2^-42.5 weigh nothing
@@ -39,29 +42,42 @@ static __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key ^ ((int)key < 0 ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// Calls f(value, index) for the words begin .. end - 1 of a row, sixteen bytes a load, the loads of AHEAD out before the first is used.
+// Calls f(values, index of the first) for the words begin .. end - 1 of a row, sixteen bytes at a time (and single words behind the
+// last such piece), the loads of AHEAD pieces out before the first is used.
 template <int AHEAD, typename T, class F>
-static __device__ __forceinline__ void each_word(const T* __restrict__ row, int begin, int end, F f) {
+static __device__ __forceinline__ void each_piece(const T* __restrict__ row, int begin, int end, F f) {
     constexpr int VEC = 16 / sizeof(T);
     struct __attribute__((aligned(sizeof(T)))) Load { T v[VEC]; };   // rows start on any word
     const int step = SAMPLE_WG * VEC;
+    auto hand = [&](const Load& raw, int i) {
+        float v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = to_f32(raw.v[e]);
+        f(v, i);
+    };
     int i = begin + (int)threadIdx.x * VEC;
     for (; i + (AHEAD - 1) * step + VEC <= end; i += AHEAD * step) {
         Load raw[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) raw[j] = *(const Load*)(row + i + j * step);
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) f(to_f32(raw[j].v[e]), i + j * step + e);
+        for (int j = 0; j < AHEAD; ++j) hand(raw[j], i + j * step);
     }
-    for (; i + VEC <= end; i += step) {
-        const Load raw = *(const Load*)(row + i);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f(to_f32(raw.v[e]), i + e);
-    }
+    for (; i + VEC <= end; i += step) hand(*(const Load*)(row + i), i);
     const int rest = end - (end - begin) % VEC + (int)threadIdx.x;
-    if (rest < end) f(to_f32(row[rest]), rest);
+    if (rest < end) {
+        const float v[1] = {to_f32(row[rest])};
+        f(v, rest);
+    }
+}
+// The same word by word.
+template <int AHEAD, typename T, class F>
+static __device__ __forceinline__ void each_word(const T* __restrict__ row, int begin, int end, F f) {
+    each_piece<AHEAD>(row, begin, end, [&](const auto& v, int i) {
+        constexpr int N = sizeof(v) / sizeof(float);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f(v[e], i + e);
+    });
 }
 
 struct Peak {
@@ -124,20 +140,20 @@ __global__ __launch_bounds__(SAMPLE_WG) void sample_peak_kernel(Sampling a) {
     if (t == 0) a.peaks[(int64_t)row * a.chunks + c] = p;
 }
 
-// 2^x, -43 <= x <= 0, as an integer of 2^-42. x = n + r, |r| <= 1/2; of the series of e^(r ln 2) the terms up to the fifth in 64
+// 2^x, -43 <= x <= 0, as an integer of 2^-42. x = n + r, |r| <= 1/2; of 2^r = sum (ln 2)^k / k! r^k the terms up to the fifth in 64
 // bits, the sixth to the tenth, which are below 2.4e-6 of it, in 32; what is left out is below 2.2e-13.
 static __device__ __forceinline__ uint64_t weight_of(double x) {
     const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
     const double y = x + magic;
     const int n = (int)(uint32_t)__double_as_longlong(y);
-    const double r = (x - (y - magic)) * 0.6931471805599453;
+    const double r = x - (y - magic);
     const float s = (float)r;
-    const float high = fmaf(s, fmaf(s, fmaf(s, fmaf(s, 1.0f / 3628800.0f, 1.0f / 362880.0f), 1.0f / 40320.0f), 1.0f / 5040.0f), 1.0f / 720.0f);
-    double p = fma(r, (double)high, 1.0 / 120.0);
-    p = fma(r, p, 1.0 / 24.0);
-    p = fma(r, p, 1.0 / 6.0);
-    p = fma(r, p, 0.5);
-    p = fma(r, p, 1.0);
+    const float high = fmaf(s, fmaf(s, fmaf(s, fmaf(s, 7.05491162e-09f, 1.0178086e-07f), 1.32154868e-06f), 1.52527338e-05f), 0.000154035304f);
+    double p = fma(r, (double)high, 0.0013333558146428441);
+    p = fma(r, p, 0.009618129107628477);
+    p = fma(r, p, 0.055504108664821576);
+    p = fma(r, p, 0.2402265069591007);
+    p = fma(r, p, 0.6931471805599453);
     p = fma(r, p, 1.0);
     // times 2^n in the exponent; 1024 more, and the last place is 2^-42: what the sum rounds to is the integer
     const uint64_t scaled = (uint64_t)__double_as_longlong(p) + ((uint64_t)(uint32_t)(n << 20) << 32);
@@ -175,7 +191,10 @@ struct Scale {
     __device__ __forceinline__ bool live(float d) const { return d <= reach; }
     // The step of a live word, as a number that has not been cut to an integer.
     __device__ __forceinline__ float step(float d) const { return fminf(d * steps, (float)(BINS - 1)); }
-    __device__ __forceinline__ double power(float v) const { return infinite ? 0.0 : ((double)v - (double)top) * rate; }
+    // (v - M) log2(e) / T; at v = M 1e-15 off, which no weight shows
+    __device__ __forceinline__ double power(float v) const { return infinite ? 0.0 : fma((double)v, rate, -top_rate); }
+    // Whether min-p keeps a word d below the top.
+    __device__ __forceinline__ bool kept(float d, double power) const { return (d == 0.0f ? 0.0 : power) >= least; }
 };
 
 static __device__ __forceinline__ Peak peak_of_row(const Sampling& a, int row) {
@@ -205,7 +224,7 @@ static_assert(BINS <= LIST, "the finer histogram stands where the list does");
 struct Shared {
     uint64_t mass[BINS];      // running sums once scanned
     uint32_t count[BINS];
-    uint64_t list[LIST], sums[LIST];   // also a finer histogram, while there is no list
+    uint64_t list[LIST], sums[LIST];   // both also a finer histogram, while there is no list
     uint64_t meet[SAMPLE_WAVES][2];
     uint64_t found;
     uint32_t low, high;
@@ -261,19 +280,39 @@ static __device__ __forceinline__ int first_reaching(const V* sums, int n, uint6
 // what is compared, so the order the words came in does not show.
 static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale& sc) {
     const int t = threadIdx.x;
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + t; i < size; i += SAMPLE_WG) sh.list[i] = 0;
-    __syncthreads();
-    for (int run = 2; run <= size; run <<= 1)
-        for (int gap = run >> 1; gap > 0; gap >>= 1) {
-            for (int j = t; j < size / 2; j += SAMPLE_WG) {
-                const int lo = 2 * j - (j & (gap - 1)), hi = lo + gap;
-                const uint64_t x = sh.list[lo], y = sh.list[hi];
-                if ((x < y) == ((lo & run) == 0)) { sh.list[lo] = y; sh.list[hi] = x; }
-            }
-            __syncthreads();
+    if (n <= COUNTED) {
+        // a word a thread: its place is the number of words in front of it. 256 compares of 64 bits a thread take 2 us, exchanges with a
+        // barrier each 5; 1000 words the other way round, 25 and 10.
+        constexpr int AT_ONCE = 8;
+        if (t < AT_ONCE) sh.list[n + t] = 0;   // (the list has room for them)
+        __syncthreads();
+        const uint64_t mine = t < n ? sh.list[t] : ~0ull;
+        int place = 0;
+        for (int i = 0; i < n; i += AT_ONCE) {
+            uint64_t x[AT_ONCE];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) x[j] = sh.list[i + j];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) place += x[j] > mine;
         }
+        __syncthreads();
+        if (t < n) sh.list[place] = mine;
+        __syncthreads();
+    } else {
+        int size = 2 * COUNTED;
+        while (size < n) size <<= 1;
+        for (int i = n + t; i < size; i += SAMPLE_WG) sh.list[i] = 0;
+        __syncthreads();
+        for (int run = 2; run <= size; run <<= 1)
+            for (int gap = run >> 1; gap > 0; gap >>= 1) {
+                for (int j = t; j < size / 2; j += SAMPLE_WG) {
+                    const int lo = 2 * j - (j & (gap - 1)), hi = lo + gap;
+                    const uint64_t x = sh.list[lo], y = sh.list[hi];
+                    if ((x < y) == ((lo & run) == 0)) { sh.list[lo] = y; sh.list[hi] = x; }
+                }
+                __syncthreads();
+            }
+    }
     constexpr int PER = LIST / SAMPLE_WG;
     uint64_t m[PER], ms = 0;
 #pragma unroll
@@ -437,26 +476,40 @@ struct Searcher {
 };
 
 // The histogram of a piece of a row, into LDS arrays that are clear; the weight of what min-p keeps, of the thread's words.
-template <typename T>
-static __device__ __forceinline__ uint64_t weigh(const T* x, int begin, int end, const Scale& sc, const Wants& wants, uint64_t* mass, uint32_t* count) {
+template <bool COUNT, bool MASS, bool ABOVE, typename T>
+static __device__ __forceinline__ uint64_t weigh_as(const T* x, int begin, int end, const Scale& sc, uint64_t* mass, uint32_t* count) {
     uint64_t above = 0;
-    each_word<2>(x, begin, end, [&](float v, int) {
-        const float d = sc.below(v);
-        if (!sc.live(d)) return;
-        const int b = (int)sc.step(d);
-        if (wants.count) atomicAdd(&count[b], 1u);
-        if (wants.mass) {
-            const double power = sc.power(v);
-            const uint64_t w = weight_of(power);
-            atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w);
-            if (wants.above) above += power >= sc.least ? w : 0;
+    each_piece<2>(x, begin, end, [&](const auto& v, int) {
+        constexpr int N = sizeof(v) / sizeof(float);
+        // first all weights (of words that weigh nothing something that is not used), side by side
+        float d[N];
+        uint64_t w[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            d[e] = sc.below(v[e]);
+            const double power = MASS ? sc.power(v[e]) : 0.0;
+            w[e] = MASS ? weight_of(power) : 0;
+            if (ABOVE) above += sc.live(d[e]) && sc.kept(d[e], power) ? w[e] : 0;
         }
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (sc.live(d[e])) {
+                const int b = (int)sc.step(d[e]);
+                if (COUNT) atomicAdd(&count[b], 1u);
+                if (MASS) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w[e]);
+            }
     });
     return above;
 }
+template <typename T>
+static __device__ __forceinline__ uint64_t weigh(const T* x, int begin, int end, const Scale& sc, const Wants& wants, uint64_t* mass, uint32_t* count) {
+    if (!wants.mass) return weigh_as<true, false, false>(x, begin, end, sc, mass, count);
+    if (!wants.count && !wants.above) return weigh_as<false, true, false>(x, begin, end, sc, mass, count);
+    return weigh_as<true, true, true>(x, begin, end, sc, mass, count);   // (what is not asked for is not read)
+}
 
 template <typename T>
-__global__ __launch_bounds__(SAMPLE_WG) void sample_steps_kernel(Sampling a) {
+__global__ __launch_bounds__(SAMPLE_WG, 4) void sample_steps_kernel(Sampling a) {
     __shared__ uint64_t mass[BINS];
     __shared__ uint32_t count[BINS];
     const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
@@ -521,7 +574,7 @@ static __device__ __forceinline__ void choose_alone(const Sampling& a, int row, 
 }
 
 template <typename T>
-__global__ __launch_bounds__(SAMPLE_WG) void sample_choose_kernel(Sampling a) {
+__global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a) {
     __shared__ Shared sh;
     const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     const T* x = (const T*)a.logits + row * a.stride;
@@ -573,16 +626,43 @@ __global__ __launch_bounds__(SAMPLE_WG) void sample_choose_kernel(Sampling a) {
         if (b1 >= 0 && c1 >= b0 - 1) { b0 = min(b0, c0); c0 = BINS; c1 = -1; }
         else if (b1 < 0 && c1 >= a0 - 1) { a0 = min(a0, c0); c0 = BINS; c1 = -1; }
     }
-    const float fa = (float)a0, ta = (float)(a1 + 1), fb = (float)b0, tb = (float)(b1 + 1), fc = (float)c0, tc = (float)(c1 + 1);
+    // A word's step s is in a range where s - (its first step), a difference without rounding, is at least 0 and below its length:
+    // as bits, below that.
+    if (a1 < 0) {   // what there is of ranges comes first
+        a0 = b0; a1 = b1; b0 = BINS; b1 = -1;
+        if (a1 < 0) { a0 = c0; a1 = c1; c0 = BINS; c1 = -1; }
+    }
+    const float fa = (float)a0, fb = (float)b0, fc = (float)c0;
+    const uint32_t na = __float_as_uint((float)max(a1 + 1 - a0, 0)), nb = __float_as_uint((float)max(b1 + 1 - b0, 0)),
+                   nc = __float_as_uint((float)max(c1 + 1 - c0, 0));
     if (t == 0) sh.n = 0;
     __syncthreads();
-    each_word<4>(x, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](float v, int i) {
-        const float d = sc.below(v), s = sc.step(d);
-        if (sc.live(d) && ((s >= fa && s < ta) || (s >= fb && s < tb) || (s >= fc && s < tc))) {
-            const int at = atomicAdd(&sh.n, 1);
-            if (at < LIST) sh.list[at] = (uint64_t)key_of(sc.infinite ? 0.0f : v) << 32 | (uint32_t)~i;
-        }
-    });
+    auto take_words = [&](auto ranges) {
+        constexpr int R = decltype(ranges)::value;
+        each_piece<4>(x, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](const auto& v, int i) {
+            constexpr int N = sizeof(v) / sizeof(float);
+            uint32_t hit = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float d = sc.below(v[e]), s = fminf(d * sc.steps, (float)BINS);   // (past the last step: no range's)
+                bool in = __float_as_uint(s - fa) < na;
+                if (R > 1) in = in || __float_as_uint(s - fb) < nb || __float_as_uint(s - fc) < nc;
+                hit |= (uint32_t)in << e;
+            }
+            while (hit) {
+                const int e = __ffs((int)hit) - 1;
+                hit &= hit - 1;
+                float word = v[0];
+#pragma unroll
+                for (int j = 1; j < N; ++j) word = e == j ? v[j] : word;
+                if (!sc.live(sc.below(word))) continue;   // (of the last step's words some weigh nothing)
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < LIST) sh.list[at] = (uint64_t)key_of(sc.infinite ? 0.0f : word) << 32 | (uint32_t)~(i + e);
+            }
+        });
+    };
+    if (nb == 0 && nc == 0) take_words(std::integral_constant<int, 1>{});
+    else take_words(std::integral_constant<int, 3>{});
     __syncthreads();
     int n = sh.n;
     if (a.chunks > 1) {
@@ -650,7 +730,8 @@ __global__ __launch_bounds__(SAMPLE_WG) void sample_choose_kernel(Sampling a) {
         int lo = 1, hi = n;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (sc.power(value_of((uint32_t)(sh.list[mid] >> 32))) >= sc.least) lo = mid + 1;
+            const float v = value_of((uint32_t)(sh.list[mid] >> 32));
+            if (sc.kept(sc.infinite ? 0.0f : sc.top - v, sc.power(v))) lo = mid + 1;
             else hi = mid;
         }
         above = sh.sums[lo - 1];

@@ -25,26 +25,49 @@ PLAN_SEQS = 8192
 
 def _on_device(what: str, *tensors: torch.Tensor) -> None:
     """The launches go to the current device's current stream: the tensors have to be there."""
-    if not all(t.is_cuda for t in tensors) or {t.get_device() for t in tensors} != {torch._C._cuda_getDevice()}:
+    device = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError(f"{what}: tensors on several devices")
+    if device < 0 or device != torch._C._cuda_getDevice():
         raise ValueError(f"{what}: a tensor is not on the current device")
 
 
 def _vector(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, n: int | None = None) -> None:
-    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
+    if t.dtype is not dtype or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise ValueError(f"{what}: {name} is a contiguous {dtype} vector" + (f" of {n}" if n is not None else ""))
 
 
-def _rows(what: str, name: str, t: torch.Tensor, heads: int | None, head_dim: int) -> int:
-    """``[rows, heads, head_dim]`` with a token's values together; the distance between tokens."""
-    if t.dtype not in _X_TYPES or t.dim() != 3 or t.shape[2] != head_dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what}: {name} is [rows, {'heads' if heads is None else heads}, {head_dim}] of f32, f16 or bf16")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != head_dim)):
+def _rows(what: str, name: str, t: torch.Tensor, heads: int | None, head_dim: int):
+    """``[rows, heads, head_dim]`` with a token's values together: rows, heads, the distance between tokens."""
+    if t.dim() != 3 or t.dtype not in _X_TYPES:
+        raise ValueError(f"{what}: {name} is [rows, heads, {head_dim}] of f32, f16 or bf16")
+    n, h, d = t.shape
+    if d != head_dim or (heads is not None and h != heads):
+        raise ValueError(f"{what}: {name} is [rows, {'heads' if heads is None else heads}, {head_dim}]")
+    if t.is_contiguous():
+        return n, h, h * d
+    across, of_head, of_value = t.stride()
+    if n and (of_value != 1 or (h > 1 and of_head != d)):
         raise ValueError(f"{what}: the values of a token of {name} have to stand together")
-    row = t.shape[1] * t.shape[2]
-    stride = t.stride(0) if t.shape[0] > 1 else row
-    if stride < row:
+    if n <= 1:
+        return n, h, h * d
+    if across < h * d:
         raise ValueError(f"{what}: rows of {name} overlap")
-    return stride
+    return n, h, across
+
+
+def _table(what: str, table: torch.Tensor, seqs: int):
+    """int32 ``[sequences, columns]``: columns, the distance between rows."""
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != seqs:
+        raise ValueError(f"{what}: table is int32 [sequences, columns]")
+    cols = table.shape[1]
+    if table.is_contiguous():
+        return cols, cols
+    across, of_col = table.stride()
+    if (cols > 1 and of_col != 1) or (seqs > 1 and across < cols):
+        raise ValueError(f"{what}: table is int32 [sequences, columns], a row together")
+    return cols, across if seqs > 1 else cols
 
 
 class KvCacheQ8:
@@ -103,8 +126,7 @@ def kv_plan(past: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free_p
     _vector("kv_plan", "past", past, torch.int32)
     _vector("kv_plan", "fresh", fresh, torch.int32, seqs)
     _vector("kv_plan", "free_pages", free_pages, torch.int32)
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != seqs or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("kv_plan: table is int32 [sequences, columns]")
+    cols, across = _table("kv_plan", table, seqs)
     if page_tokens not in PAGE_TOKENS:
         raise ValueError(f"kv_plan: pages of {PAGE_TOKENS} tokens")
     if plan.lens.numel() != seqs:
@@ -114,24 +136,23 @@ def kv_plan(past: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free_p
         if taken.data_ptr() == plan.taken.data_ptr():
             raise ValueError("kv_plan: taken is the plan's own")
     _on_device("kv_plan", past, fresh, table, free_pages, plan.slots, *(() if taken is None else (taken,)))
-    cols = table.shape[1]
     _lib.check("lk_kv_plan", _lib.load().lk_kv_plan(
         past.data_ptr(), fresh.data_ptr(), seqs, page_tokens, free_pages.data_ptr(), free_pages.numel(),
-        None if taken is None else taken.data_ptr(), table.data_ptr(), table.stride(0) if seqs > 1 else cols, cols, plan.lens.data_ptr(),
+        None if taken is None else taken.data_ptr(), table.data_ptr(), across, cols, plan.lens.data_ptr(),
         plan.starts.data_ptr(), plan.slots.data_ptr(), plan.positions.data_ptr(), plan.slots.numel(), plan.taken.data_ptr(), _stream()))
     return plan
 
 
 def kv_write(cache: KvCacheQ8, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """New keys and values ``[tokens, kv_heads, head_dim]`` (f32, f16 or bf16; rows may be parts of wider ones) into the cache."""
-    if k.dtype != v.dtype or k.shape != v.shape:
+    tokens, _, ks = _rows("kv_write", "k", k, cache.kv_heads, cache.head_dim)
+    of_v, _, vs = _rows("kv_write", "v", v, cache.kv_heads, cache.head_dim)
+    if k.dtype is not v.dtype or of_v != tokens:
         raise ValueError("kv_write: keys and values are of one type and shape")
-    ks = _rows("kv_write", "k", k, cache.kv_heads, cache.head_dim)
-    vs = _rows("kv_write", "v", v, cache.kv_heads, cache.head_dim)
-    _vector("kv_write", "slots", slots, torch.int64, k.shape[0])
+    _vector("kv_write", "slots", slots, torch.int64, tokens)
     _on_device("kv_write", k, v, slots, cache.k)
     _lib.check("lk_kv_write_q8", _lib.load().lk_kv_write_q8(
-        k.data_ptr(), v.data_ptr(), _X_TYPES[k.dtype], ks, vs, slots.data_ptr(), k.shape[0], cache.kv_heads, cache.head_dim,
+        k.data_ptr(), v.data_ptr(), _X_TYPES[k.dtype], ks, vs, slots.data_ptr(), tokens, cache.kv_heads, cache.head_dim,
         cache.page_tokens, cache.pages, *cache._at, _stream()))
 
 
@@ -155,14 +176,12 @@ def kv_attention(q: torch.Tensor, cache: KvCacheQ8, table: torch.Tensor, lens: t
     ``window`` > 0: that many positions, the row's own among them. Rows behind the last sequence stay as they are in ``out``
     (without one: zeros). ``max_fresh``, ``max_len``: the most rows and tokens of a sequence as far as the caller knows them."""
     seqs = lens.numel()
-    stride = _rows("kv_attention", "q", q, None, cache.head_dim)
-    rows, heads = q.shape[0], q.shape[1]
+    rows, heads, stride = _rows("kv_attention", "q", q, None, cache.head_dim)
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError("kv_attention: the heads of q are a multiple of the cache's")
     _vector("kv_attention", "lens", lens, torch.int32)
     _vector("kv_attention", "starts", starts, torch.int32, seqs + 1)
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != seqs or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("kv_attention: table is int32 [sequences, columns]")
+    cols, across = _table("kv_attention", table, seqs)
     if max_fresh < 0 or max_len < 0 or window < 0:
         raise ValueError("kv_attention: sizes below zero")
     scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else scale
@@ -170,13 +189,12 @@ def kv_attention(q: torch.Tensor, cache: KvCacheQ8, table: torch.Tensor, lens: t
         raise ValueError("kv_attention: the scale is a number above zero")
     if out is None:
         out = torch.zeros((rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape:
+    of_out, _, out_stride = _rows("kv_attention", "out", out, heads, cache.head_dim)
+    if out.dtype is not q.dtype or of_out != rows:
         raise ValueError("kv_attention: out has the type and shape of q")
-    out_stride = _rows("kv_attention", "out", out, None, cache.head_dim)
     _on_device("kv_attention", q, out, table, lens, starts, cache.k)
-    cols = table.shape[1]
     _lib.check("lk_kv_attention_q8", _lib.load().lk_kv_attention_q8(
         q.data_ptr(), _X_TYPES[q.dtype], stride, out.data_ptr(), out_stride, *cache._at, cache.pages, cache.page_tokens, table.data_ptr(),
-        table.stride(0) if seqs > 1 else cols, cols, lens.data_ptr(), starts.data_ptr(), seqs, rows, min(max_fresh, 0x7FFFFFFF),
+        across, cols, lens.data_ptr(), starts.data_ptr(), seqs, rows, min(max_fresh, 0x7FFFFFFF),
         min(max_len, 0x7FFFFFFF), heads, cache.kv_heads, cache.head_dim, scale, min(window, 0x7FFFFFFF), _stream()))
     return out
