@@ -186,7 +186,8 @@ struct Scale {
         least = min_p > 0.0f ? log2((double)min_p) : -1e300;
         return true;
     }
-    // How far a word is below the top (not at all a number: for one that is none).
+    // How far a word is below the top (not at all a number: for one that is none). The launches over pieces leave rows with an
+    // infinite word to the workgroup that chooses alone, and ask less.
     __device__ __forceinline__ float below(float v) const { return infinite ? (v == INFINITY ? 0.0f : NAN) : top - v; }
     __device__ __forceinline__ bool live(float d) const { return d <= reach; }
     // The step of a live word, as a number that has not been cut to an integer.
@@ -476,7 +477,7 @@ struct Searcher {
 };
 
 // The histogram of a piece of a row, into LDS arrays that are clear; the weight of what min-p keeps, of the thread's words.
-template <bool COUNT, bool MASS, bool ABOVE, typename T>
+template <bool COUNT, bool MASS, bool ABOVE, bool ALONE, typename T>
 static __device__ __forceinline__ uint64_t weigh_as(const T* x, int begin, int end, const Scale& sc, uint64_t* mass, uint32_t* count) {
     uint64_t above = 0;
     each_piece<2>(x, begin, end, [&](const auto& v, int) {
@@ -486,15 +487,15 @@ static __device__ __forceinline__ uint64_t weigh_as(const T* x, int begin, int e
         uint64_t w[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            d[e] = sc.below(v[e]);
-            const double power = MASS ? sc.power(v[e]) : 0.0;
+            d[e] = ALONE ? sc.below(v[e]) : sc.top - v[e];
+            const double power = !MASS ? 0.0 : ALONE ? sc.power(v[e]) : fma((double)v[e], sc.rate, -sc.top_rate);
             w[e] = MASS ? weight_of(power) : 0;
             if (ABOVE) above += sc.live(d[e]) && sc.kept(d[e], power) ? w[e] : 0;
         }
 #pragma unroll
         for (int e = 0; e < N; ++e)
             if (sc.live(d[e])) {
-                const int b = (int)sc.step(d[e]);
+                const int b = (int)(d[e] * sc.steps);   // (of a live word: below BINS)
                 if (COUNT) atomicAdd(&count[b], 1u);
                 if (MASS) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w[e]);
             }
@@ -502,23 +503,21 @@ static __device__ __forceinline__ uint64_t weigh_as(const T* x, int begin, int e
     return above;
 }
 template <typename T>
-static __device__ __forceinline__ uint64_t weigh(const T* x, int begin, int end, const Scale& sc, const Wants& wants, uint64_t* mass, uint32_t* count) {
-    if (!wants.mass) return weigh_as<true, false, false>(x, begin, end, sc, mass, count);
-    if (!wants.count && !wants.above) return weigh_as<false, true, false>(x, begin, end, sc, mass, count);
-    return weigh_as<true, true, true>(x, begin, end, sc, mass, count);   // (what is not asked for is not read)
-}
-
-template <typename T>
 __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_steps_kernel(Sampling a) {
     __shared__ uint64_t mass[BINS];
     __shared__ uint32_t count[BINS];
     const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     Scale sc;
-    if (!sc.init(peak_of_row(a, row), a.temperature[row], a.min_p ? a.min_p[row] : 0.0f)) return;
+    if (!sc.init(peak_of_row(a, row), a.temperature[row], a.min_p ? a.min_p[row] : 0.0f) || sc.infinite) return;
     const Wants wants(a, row);
     for (int i = t; i < BINS; i += SAMPLE_WG) { mass[i] = 0; count[i] = 0; }
     __syncthreads();
-    uint64_t above = weigh((const T*)a.logits + row * a.stride, c * a.chunk, min((c + 1) * a.chunk, a.vocab), sc, wants, mass, count);
+    const T* x = (const T*)a.logits + row * a.stride;
+    const int begin = c * a.chunk, end = min((c + 1) * a.chunk, a.vocab);
+    uint64_t above = 0;
+    if (!wants.mass) weigh_as<true, false, false, false>(x, begin, end, sc, mass, count);
+    else if (!wants.count && !wants.above) weigh_as<false, true, false, false>(x, begin, end, sc, mass, count);
+    else above = weigh_as<true, true, true, false>(x, begin, end, sc, mass, count);   // (what is not asked for is not read)
     if (wants.above) {
         for (int o = 32; o; o >>= 1) above += __shfl_xor((unsigned long long)above, o);
         if ((t & 63) == 0 && above) atomicAdd((unsigned long long*)&a.floor_mass[row], (unsigned long long)above);
@@ -539,9 +538,7 @@ static __device__ __forceinline__ void choose_alone(const Sampling& a, int row, 
     for (int i = t; i < BINS; i += SAMPLE_WG) { sh.mass[i] = 0; sh.count[i] = 0; }
     if (t == 0) sh.found = 0;
     __syncthreads();
-    Wants wants(a, row);
-    wants.count = wants.mass = wants.above = true;
-    uint64_t above = weigh(x, 0, a.vocab, sc, wants, sh.mass, sh.count);
+    uint64_t above = weigh_as<true, true, true, true>(x, 0, a.vocab, sc, sh.mass, sh.count);
     for (int o = 32; o; o >>= 1) above += __shfl_xor((unsigned long long)above, o);
     if ((t & 63) == 0) atomicAdd((unsigned long long*)&sh.found, (unsigned long long)above);
     __syncthreads();
@@ -585,6 +582,10 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
             a.tokens[row] = peak.best ? (int)~(uint32_t)peak.best : -1;
             if (a.probs) a.probs[row] = peak.best ? 1.0f : 0.0f;
         }
+        return;
+    }
+    if (sc.infinite) {   // words beside infinite ones are none: as rare as it is, not worth asking for in the pieces
+        if (c == 0) choose_alone<T>(a, row, sc, sh);
         return;
     }
     const Wants wants(a, row);
@@ -644,7 +645,7 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
             uint32_t hit = 0;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const float d = sc.below(v[e]), s = fminf(d * sc.steps, (float)BINS);   // (past the last step: no range's)
+                const float s = fminf((sc.top - v[e]) * sc.steps, (float)BINS);   // (past the last step, or no number: no range's)
                 bool in = __float_as_uint(s - fa) < na;
                 if (R > 1) in = in || __float_as_uint(s - fb) < nb || __float_as_uint(s - fc) < nc;
                 hit |= (uint32_t)in << e;
@@ -655,9 +656,9 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
                 float word = v[0];
 #pragma unroll
                 for (int j = 1; j < N; ++j) word = e == j ? v[j] : word;
-                if (!sc.live(sc.below(word))) continue;   // (of the last step's words some weigh nothing)
+                if (!sc.live(sc.top - word)) continue;   // (of the last step's words some weigh nothing)
                 const int at = atomicAdd(&sh.n, 1);
-                if (at < LIST) sh.list[at] = (uint64_t)key_of(sc.infinite ? 0.0f : word) << 32 | (uint32_t)~(i + e);
+                if (at < LIST) sh.list[at] = (uint64_t)key_of(word) << 32 | (uint32_t)~(i + e);
             }
         });
     };
@@ -709,7 +710,7 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
         int lo = 0, hi = n;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (sc.step(sc.infinite ? 0.0f : sc.top - value_of((uint32_t)(sh.list[mid] >> 32))) >= (float)step) hi = mid;
+            if (sc.step(sc.top - value_of((uint32_t)(sh.list[mid] >> 32))) >= (float)step) hi = mid;
             else lo = mid + 1;
         }
         return lo;
@@ -731,7 +732,7 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             const float v = value_of((uint32_t)(sh.list[mid] >> 32));
-            if (sc.kept(sc.infinite ? 0.0f : sc.top - v, sc.power(v))) lo = mid + 1;
+            if (sc.kept(sc.top - v, sc.power(v))) lo = mid + 1;
             else hi = mid;
         }
         above = sh.sums[lo - 1];
