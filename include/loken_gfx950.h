@@ -816,7 +816,8 @@ int lk_kv_read_q8(const int64_t* slots, int tokens, int kv_heads, int head_dim, 
  * leaving out positions whose page is absent. A row that sees none gives zeros, one whose q holds a value that is not finite gives
  * values that are not numbers. Rows behind the last sequence are left as they were. `out` has q's type, out_stride elements from row
  * to row; it does not overlap q. max_fresh and max_len: the most rows and the most tokens of a sequence as the caller knows
- * them; they choose launch shapes only, a sequence with more is served too. table_cols * page_tokens up to 2^31 - 256, else LK_ERR_SIZE.
+ * them; they choose launch shapes only, a sequence with more is served too. table_cols * page_tokens up to 2^31 - 1024 and rows * heads / kv_heads up to
+ * 2^31 - 1, else LK_ERR_SIZE.
  * Scores, softmax and sums are held in f32 (sums of products of codes in int32 as long as they are exact). Partial results of a
  * context that is split over workgroups go through scratch of the stream (LK_ERR_NOMEM where there is none; while a
  * graph is recorded, where no call outside a recording has needed as much). */

@@ -13,23 +13,23 @@ struct PartsOf {
     int parts;
     int64_t base, step, first;
     __device__ __forceinline__ PartsOf(const Attend& a, const KvSeq& s, int seq, int tok, int head, int per) {
-        const int64_t all_rows = (int64_t)s.tokens() * a.group, r = (int64_t)tok * a.group + head % a.group;
+        const unsigned group = a.group, all_rows = (unsigned)s.tokens() * group, r = (unsigned)tok * group + (unsigned)head % group;   // below 2^31
         if (a.chunks) {
             parts = 1;
             base = step = first = 0;
-            if (all_rows > per) return;
+            if ((int)all_rows > per) return;
             const KvPieces pieces(a, per);
             const int at = KvPieces::first_of(a, per, seq), steps = kv_steps_of(a, seq, per);
             const int c0 = at / pieces.length, c1 = (at + steps - 1) / pieces.length;
             parts = c1 - c0 + 1;
             // the piece that the sequence starts in has it second, the others first
-            base = ((int64_t)(head / a.group) * a.chunks + c0) * 2 * per + r;
+            base = ((int64_t)((unsigned)head / group) * a.chunks + c0) * 2 * per + r;
             step = 2 * per;
             first = per;
             return;
         }
-        const int64_t r0 = r / per * per, r1 = min(r0 + per, all_rows) - 1;
-        parts = KvSpan(a, s, s.first + (int)(r0 / a.group), s.first + (int)(r1 / a.group)).parts;
+        const unsigned r0 = r / per * per, r1 = min(r0 + per, all_rows) - 1;
+        parts = KvSpan(a, s, s.first + (int)(r0 / group), s.first + (int)(r1 / group)).parts;
         base = (a.part_row(seq, s, s.first + tok) * a.heads + head) * a.splits;
         step = 1;
         first = 0;
@@ -109,21 +109,21 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_few_parts_kernel(Atte
     int seq = (int)(item / a.heads / tokens), tok = (int)(item / a.heads % tokens);
     if (!few) {   // the last sequence that starts at or before the row
         const int row = (int)(item / a.heads);
-        int lo = 0, hi = a.seqs - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (a.starts[mid] <= row) lo = mid;
-            else hi = mid - 1;
+        seq = 0;
+        for (int n = a.seqs; n > 1;) {
+            const int step = (n + 63) / 64;
+            const bool is = lane * step < n && a.starts[seq + lane * step] <= row;
+            const int back = max(__popcll(__ballot(is)) - 1, 0) * step;
+            seq += back;
+            n = min(step, n - back);
         }
-        seq = lo;
         tok = row - max(a.starts[seq], 0);
     }
     const KvSeq s(a, seq);
-    const int64_t all_rows = (int64_t)s.tokens() * a.group;
-    if ((all_rows <= a.few_rows) != few || tok < 0) return;
+    if (((int64_t)s.tokens() * a.group <= a.few_rows) != few || tok < 0) return;
     for (; tok < s.tokens(); tok += few ? tokens : 0x40000000) {
         const PartsOf of(a, s, seq, tok, head, per);
-        const int parts = of.parts;
+        const int parts = __builtin_amdgcn_readfirstlane(of.parts);
         if (parts > 1) {
             float m = -INFINITY, l = 0.f, acc[PER] = {};
             for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[of.at(p)].x);
@@ -131,12 +131,13 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_few_parts_kernel(Atte
                 float x[AHEAD][PER];
                 float2 ml[AHEAD];
 #pragma unroll
-                for (int j = 0; j < AHEAD; ++j) {
-                    const int64_t from = of.at(min(p0 + j, parts - 1));
-                    ml[j] = a.part_ml[from];
+                for (int j = 0; j < AHEAD; ++j)
+                    if (p0 + j < parts) {
+                        const int64_t from = of.at(p0 + j);
+                        ml[j] = a.part_ml[from];
 #pragma unroll
-                    for (int i = 0; i < PER; ++i) x[j][i] = a.part_o[from * D + lane + 64 * i];
-                }
+                        for (int i = 0; i < PER; ++i) x[j][i] = a.part_o[from * D + lane + 64 * i];
+                    }
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j)
                     if (p0 + j < parts) {
@@ -200,7 +201,7 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     if (!q || !out || !lens || !starts || (table_cols > 0 && !table) || (((uintptr_t)q | (uintptr_t)out) & (size - 1)) || q_stride < row ||
         out_stride < row)
         return LK_ERR_ARG;
-    if ((int64_t)table_cols * page_tokens > 0x7FFFFF00) return LK_ERR_SIZE;   // positions and what is added to them fit 32 bits
+    if ((int64_t)table_cols * page_tokens > 0x7FFFFC00 || (int64_t)rows * (heads / kv_heads) > 0x7FFFFFFF) return LK_ERR_SIZE;   // positions and what is added to them fit 32 bits
     hipStream_t s = (hipStream_t)stream;
     const int group = heads / kv_heads;
     const Attend a{q, out, q_stride, out_stride, {(int8_t*)k_codes, (int8_t*)v_codes, (float*)k_scales, (float*)v_scales, pages, kv_heads, kv_log2(page_tokens)},

@@ -1,7 +1,7 @@
 // Attention over the 8-bit cache for many rows of a sequence: prompts and prefill chunks.
 //
 // Rows are (token, head of the group) of one key / value head, so that the group's heads share the keys and values that are
-// read. A workgroup of four waves has 128 rows; a step is 64 positions, whose codes are turned into f16 (exactly) once for all
+// read. A team of four waves has 128 rows; a step is 64 positions, whose codes are turned into f16 (exactly) once for all
 // rows on their way into LDS, values with the positions of a column together as they lie in the cache. Products are
 // v_mfma_f32_32x32x16_f16, both turned round so that a lane keeps one row throughout:
 //     scores   (32 positions) x (32 rows): lane l holds row l % 32, and the positions of its half of the lanes stand in the order in
@@ -17,6 +17,12 @@
 //
 // The sums are put to a new maximum only where that lies 2^8 above the one they go by: weights up to 2^8 then, which stand
 // LIFT = 2^7 above one and stay below 2^15, f16's largest; a weight of 2^-21 still has all its bits, one of 2^-31 some.
+//
+// A wave's step is 32 products of 32 cycles (twice as many in f32) and some 400 other instructions, 32 of them exponentials, which
+// take four times as long. It is these that bound it, and what of them does not run beside products: so a product comes with
+// six of them in turn, its operands read from LDS a group ahead, and nothing that is loaded is looked at before the step after.
+// 2048 tokens of one prompt, 32 heads over 8 of 128 bf16 values: 69 us, 500 TFLOP/s of the causal half's products; 700 f32 rows over
+// 2200 positions beside eleven single rows: 137 us.
 
 #include "kv_attention.h"
 
@@ -25,8 +31,9 @@ namespace {
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
 
-constexpr int WAVES = 4, THREADS = 64 * WAVES, RUNS = KV_TILE / 16;
+constexpr int WAVES = 4, THREADS = 64 * WAVES, RUNS = KV_TILE / 16;   // of a team
 constexpr float LIFT = 7.f, SLACK = 8.f;   // powers of two
 
 // Sixteen codes as f16, as they lie: 0x6400 + (code + 128) is the f16 number 1152 + code.
@@ -46,6 +53,28 @@ static __device__ __forceinline__ void to_halves(uint4 w, uint4* out) {
     out[1] = make_uint4(r[4], r[5], r[6], r[7]);
 }
 
+// (the compiler takes a look at each operand for signalling NaN first)
+static __device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// What the four lanes of the runs have together.
+template <typename F>
+static __device__ __forceinline__ float across_runs(float x, F both) {
+    static_assert(RUNS == 4);
+    x = both(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xB1, 0xF, 0xF, true)));          // lanes 1, 0, 3, 2
+    return both(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x4E, 0xF, 0xF, true)));       // lanes 2, 3, 0, 1
+}
+
+// Teams of a workgroup, which take its steps in turn. Two, where the registers hold them, so that both waves of a SIMD have the same
+// rows' work to do to the end: a prompt of 2048 tokens, 32 heads over 8 of 128 bf16 values, took 80 us with one team and two
+// workgroups to a CU, of which the one with the longer rows ran on alone. f32 has no registers for the meeting of the teams
+// (700 rows over long contexts: 178 us against 140), 256 columns none for a second wave on a SIMD.
+constexpr int many_teams(bool fine, int head_dim) { return head_dim == 256 || fine ? 1 : 2; }
+constexpr int many_waves(int head_dim) { return head_dim == 256 ? 1 : 2; }   // on a SIMD
+
 template <typename T, int D>
 struct Many {
     static constexpr bool FINE = sizeof(T) == 4;
@@ -53,35 +82,43 @@ struct Many {
     static constexpr int KS = D / 16, NB = D / 32;
     static constexpr int K_PITCH = 2 * D + 16, V_PITCH = 2 * KV_TILE + 16;   // bytes; sixteen more: no bank conflicts
     static constexpr int K_BYTES = KV_TILE * K_PITCH, V_BYTES = D * V_PITCH;
-    static constexpr int BUFFERS = D < 256 ? 2 : 1;
     static constexpr int CHUNKS = KV_TILE * D / 16 / THREADS;   // of sixteen codes, a thread and side
-    static constexpr int LDS = BUFFERS * (K_BYTES + V_BYTES);
+    static constexpr int TEAMS = many_teams(FINE, D), TEAM_BYTES = 2 * (K_BYTES + V_BYTES);
+    static constexpr int LDS = TEAMS * TEAM_BYTES;
+    static_assert(TEAM_BYTES >= THREADS * D);   // half of the sums of a team, on their way to the other
 };
 
 // What a step's pages have for everybody.
 struct Step {
     float ks[RUNS];     // key scales; -1: the page is absent
-    float bias[RUNS];   // log2 of the value scale over `ref`, and LIFT; of a page whose values are all zero LIFT alone
-    float back[RUNS];   // 2^-bias
-    uint32_t live[RUNS];   // all bits, or none where the values are zero
+    float bias[RUNS];   // log2 of the value scale over `ref`, and LIFT; -infinity where the scale is zero
+    float back[RUNS];   // 2^-bias, 0 with a scale of zero
+    uint32_t dead;      // a bit for each page whose values are all zero
     float shrink;       // what `ref` before this step is of it now
     float ref;          // the largest value scale so far
     int absent;         // whether a page is
-    int pad;
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_kernel(Attend a, int row_tiles, int cus) {
+__global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves(D)) void kv_attention_many_kernel(Attend a, int row_tiles, int cus) {
     using M = Many<T, D>;
-    extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ Step steps[2];
-    __shared__ int pages[2][RUNS];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    extern __shared__ __align__(16) uint8_t lds_of_all[];
+    __shared__ Step steps_of_all[M::TEAMS][2];
+    __shared__ int pages_of_all[M::TEAMS][4][RUNS];
+    __shared__ int64_t starts_of_all[M::TEAMS][4][RUNS];   // of a run's codes in the pool, on either side
+    __shared__ float refs[M::TEAMS];
+    __shared__ float2 meet[M::TEAMS][32 * WAVES];
+    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
+    const int tid = threadIdx.x % THREADS, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint8_t* lds = lds_of_all + team * M::TEAM_BYTES;
+    Step* steps = steps_of_all[team];
+    auto pages = pages_of_all[team];
+    auto starts = starts_of_all[team];
     const int col = lane & 31, half = lane >> 5;
-    // Workgroups in rounds of one to a CU, every other round backwards: row tiles that see the most come first, and where two rounds are
-    // all there is a CU with much of one has little of the other.
+    // Row tiles that see the most come first, so that what comes last is short. Where a CU has two workgroups at once they come in
+    // rounds of one to a CU, every other one backwards: a CU with much of one has little of the other.
     unsigned at = blockIdx.x;
-    {
+    if (M::TEAMS == 1 && D < 256) {
         const unsigned round = at / cus, first = round * cus, size = min((unsigned)cus, gridDim.x - first);
         if (round & 1) at = first + (size - 1 - (at - first));
     }
@@ -91,53 +128,40 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
     at /= a.pool.heads;
     const int seq = at % a.seqs, tile0 = row_tiles - 1 - (int)(at / a.seqs);
     const KvSeq s(a, seq);
-    const int64_t all_rows = (int64_t)s.tokens() * a.group;
-    if (all_rows <= a.few_rows) return;
+    const unsigned all_rows = (unsigned)s.tokens() * (unsigned)a.group;   // below 2^31
+    if ((int)all_rows <= a.few_rows) return;
     const int shift = a.pool.page_shift;
     const int32_t* entries = a.table + seq * a.table_stride;
     auto k_lds = [&](int buffer) { return lds + buffer * (M::K_BYTES + M::V_BYTES); };
     auto v_lds = [&](int buffer) { return lds + buffer * (M::K_BYTES + M::V_BYTES) + M::K_BYTES; };
 
-    for (int64_t r_tile = (int64_t)tile0 * KV_MANY_ROWS; r_tile < all_rows; r_tile += (int64_t)row_tiles * KV_MANY_ROWS) {
-        const int64_t r_end = min(r_tile + KV_MANY_ROWS, all_rows);
-        const KvSpan span(a, s, s.first + (int)(r_tile / a.group), s.first + (int)((r_end - 1) / a.group));
+    for (uint64_t tile = tile0; tile * KV_MANY_ROWS < all_rows; tile += row_tiles) {
+        const unsigned r_tile = (unsigned)tile * KV_MANY_ROWS, group = a.group;
+        const unsigned r_end = min(r_tile + KV_MANY_ROWS, all_rows);
+        const KvSpan span(a, s, s.first + (int)(r_tile / group), s.first + (int)((r_end - 1) / group));
         const int per_part = span.per_part, parts = span.parts;
         if (part >= parts) continue;
-        const int t_begin = part * per_part, t_end = min(span.tiles, t_begin + per_part);
+        // a team has every other step; steps are counted from its first
+        const int t_begin = part * per_part, t_all = min(span.tiles, t_begin + per_part) - t_begin;
+        const int turns = (t_all + M::TEAMS - 1) / M::TEAMS, t_end = (t_all - team + M::TEAMS - 1) / M::TEAMS;
+        const int from_pos = span.lo + (t_begin + team) * KV_TILE;
+        auto base_of = [&](int t) { return from_pos + t * M::TEAMS * KV_TILE; };   // below 2^31: contexts end 1024 positions before
         // the lane's row, and what its wave sees
-        const int64_t r = r_tile + 32 * wave + col;
+        const unsigned r = r_tile + 32 * wave + col;
         const bool row_is = r < r_end;
-        const int64_t r_in = min(r, r_end - 1);
-        const int tok = s.first + (int)(r_in / a.group), head = kv * a.group + (int)(r_in % a.group);
+        const unsigned r_in = min(r, r_end - 1);
+        const int tok = s.first + (int)(r_in / group), head = kv * (int)group + (int)(r_in % group);
         const int pos = (int)max(s.pos_of_0 + tok, (int64_t)-1);
-        const int64_t w0 = min(r_tile + 32 * wave, r_end - 1), w1 = min(r_tile + 32 * wave + 31, r_end - 1);
-        const int pos_least = (int)max(s.pos_of_0 + s.first + w0 / a.group, (int64_t)-1), pos_most = (int)max(s.pos_of_0 + s.first + w1 / a.group, (int64_t)-1);
+        const unsigned w0 = min(r_tile + 32 * wave, r_end - 1), w1 = min(r_tile + 32 * wave + 31, r_end - 1);
+        const int pos_least = (int)max(s.pos_of_0 + s.first + w0 / group, (int64_t)-1), pos_most = (int)max(s.pos_of_0 + s.first + w1 / group, (int64_t)-1);
 
+        struct __attribute__((packed, aligned(sizeof(T)))) Eight { T of[8]; };   // (a row's alignment is its type's)
+        const Eight* row = (const Eight*)((const T*)a.q + tok * a.q_stride + (int64_t)head * D + 8 * half);
+        Eight in[M::KS];
+#pragma unroll
+        for (int k = 0; k < M::KS; ++k) in[k] = row[2 * k];
         h8 q[M::PARTS][M::KS];
-        float unit;
-        {
-            const T* row = (const T*)a.q + tok * a.q_stride + (int64_t)head * D + 8 * half;
-            uint32_t most = 0;
-#pragma unroll
-            for (int k = 0; k < M::KS; ++k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(to_f32(row[16 * k + e])) & 0x7FFFFFFFu);
-            most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-            const bool finite = most < 0x7F800000u;
-            int e2 = 0;
-            (void)frexpf(finite && most ? __uint_as_float(most) : 1.f, &e2);   // the row's largest is in [2^(e2 - 1), 2^e2)
-#pragma unroll
-            for (int k = 0; k < M::KS; ++k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = finite ? ldexpf(to_f32(row[16 * k + e]), 14 - e2) : 0.f;   // below 2^14
-                    const _Float16 hi = (_Float16)x;
-                    q[0][k][e] = hi;
-                    if (M::FINE) q[M::PARTS - 1][k][e] = (_Float16)(x - (float)hi);
-                }
-            // the scale first: powers that it makes up for may be far from one
-            unit = finite ? ldexpf(ldexpf(a.scale * 1.4426950408889634f, e2 / 2), e2 - e2 / 2 - 14) : NAN;
-        }
+        float unit = 0.f;
         v16f o[M::NB];
 #pragma unroll
         for (int b = 0; b < M::NB; ++b)
@@ -147,60 +171,59 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
 
         // A step's codes: thread tid has chunk tid, tid + 256, .. of sixteen. Its pages have been in LDS since the step before.
         uint4 kc[M::CHUNKS], vc[M::CHUNKS];
-        auto entry = [&](int t) {   // of run tid, in the first lanes
-            const int p0 = span.lo + t * KV_TILE + 16 * (tid & (RUNS - 1));
-            const int page = t < t_end && p0 < span.hi ? entries[p0 >> shift] : -1;
-            return (unsigned)page < (unsigned)a.pool.pages ? page : -1;
+        // Loads have no conditions and nothing of them is looked at before a step later: a wait for one would be a wait for all.
+        const int run = tid & (RUNS - 1);
+        auto entry = [&](int t) { return entries[min(base_of(t) + 16 * run, span.hi - 1) >> shift]; };   // (there is a step)
+        auto list = [&](int t, int entry) {   // by the first lanes
+            const int p0 = base_of(t) + 16 * run, off = p0 & ((1 << shift) - 1);
+            const int page = p0 < span.hi && (unsigned)entry < (unsigned)a.pool.pages ? entry : -1;
+            pages[t & 3][run] = page;
+            starts[t & 3][run] = ((((int64_t)max(page, 0) * a.pool.heads + kv) << shift) + off) * D;
         };
         float ks = -1.f, vs = 0.f, ref = 0.f;
+        int page_of_run = -1;
         auto fetch = [&](int t) {
-            const int* page = pages[t & 1];
+            const int64_t* start = starts[t & 3];
+            page_of_run = pages[t & 3][run];
+            const int64_t at_scale = (int64_t)max(page_of_run, 0) * a.pool.heads + kv;
 #pragma unroll
-            for (int c = 0; c < M::CHUNKS; ++c) {
+            for (int c = 0; c < M::CHUNKS; ++c) {   // (a run of either side is D chunks)
                 const int n = tid + c * THREADS;
-                const int token = n / (D / 16), run_v = n / D;
-                const int off_k = (span.lo + t * KV_TILE + token) & ((1 << shift) - 1);
-                kc[c] = *(const uint4*)(a.pool.k + ((((int64_t)max(page[token >> 4], 0) * a.pool.heads + kv) << shift) + off_k) * D + (n % (D / 16)) * 16);
-                const int off_v = (span.lo + t * KV_TILE + 16 * run_v) & ((1 << shift) - 1);
-                vc[c] = *(const uint4*)(a.pool.v + ((((int64_t)max(page[run_v], 0) * a.pool.heads + kv) << shift) + off_v) * D + (n % D) * 16);
+                kc[c] = *(const uint4*)(a.pool.k + start[n / D] + n % D * 16);
+                vc[c] = *(const uint4*)(a.pool.v + start[n / D] + n % D * 16);
             }
-            if (tid < RUNS) {
-                const int p = page[tid];
-                const int64_t at_scale = (int64_t)max(p, 0) * a.pool.heads + kv;
-                ks = a.pool.k_scales[at_scale];
-                vs = a.pool.v_scales[at_scale];
-                if (p < 0) { ks = -1.f; vs = 0.f; }
-            }
+            ks = a.pool.k_scales[at_scale];
+            vs = a.pool.v_scales[at_scale];
+        };
+        auto store_chunk = [&](int t, int i) {   // keys and values in turn
+            const int n = tid + i / 2 * THREADS;
+            uint4 w[2];
+            to_halves(i & 1 ? vc[i / 2] : kc[i / 2], w);
+            uint4* to = (uint4*)(i & 1 ? v_lds(t & 1) + (n % D) * M::V_PITCH + (n / D) * 32 : k_lds(t & 1) + (n / (D / 16)) * M::K_PITCH + (n % (D / 16)) * 32);
+            to[0] = w[0];
+            to[1] = w[1];
         };
         auto store = [&](int t) {
-            const int buffer = M::BUFFERS == 2 ? t & 1 : 0;
 #pragma unroll
-            for (int c = 0; c < M::CHUNKS; ++c) {
-                const int n = tid + c * THREADS;
-                uint4 w[2];
-                to_halves(kc[c], w);
-                uint4* to = (uint4*)(k_lds(buffer) + (n / (D / 16)) * M::K_PITCH + (n % (D / 16)) * 32);
-                to[0] = w[0];
-                to[1] = w[1];
-                to_halves(vc[c], w);
-                to = (uint4*)(v_lds(buffer) + (n % D) * M::V_PITCH + (n / D) * 32);
-                to[0] = w[0];
-                to[1] = w[1];
-            }
-            if (tid < RUNS) {
+            for (int i = 0; i < 2 * M::CHUNKS; ++i) store_chunk(t, i);
+        };
+        auto note = [&](int t) {
+            if (wave == 1 && lane < RUNS) {
                 Step& st = steps[t & 1];
-                float most = vs, least = ks;
-                for (int o = 1; o < RUNS; o <<= 1) { most = fmaxf(most, __shfl_xor(most, o)); least = fminf(least, __shfl_xor(least, o)); }
+                const float k1 = page_of_run < 0 ? -1.f : ks, v1 = page_of_run < 0 ? 0.f : vs;
+                const float most = across_runs(v1, [](float x, float y) { return fmaxf(x, y); });
+                const float least = across_runs(k1, [](float x, float y) { return fminf(x, y); });
                 const float now = fmaxf(ref, most);
-                st.ks[tid] = ks;
-                const float bias = vs > 0.f ? __builtin_amdgcn_logf(vs / now) + LIFT : LIFT;
-                st.bias[tid] = bias;
-                st.back[tid] = __builtin_amdgcn_exp2f(-bias);
-                st.live[tid] = vs > 0.f ? 0xFFFFFFFFu : 0u;
-                if (tid == 0) {
+                const float bias = v1 > 0.f ? __builtin_amdgcn_logf(v1 / now) + LIFT : -INFINITY;
+                st.ks[lane] = k1;
+                st.bias[lane] = bias;
+                st.back[lane] = v1 > 0.f ? __builtin_amdgcn_exp2f(-bias) : 0.f;
+                const uint32_t dead = (uint32_t)__ballot(!(v1 > 0.f));
+                if (lane == 0) {
                     st.shrink = ref > 0.f ? ref / now : 1.f;   // (up to then the sums are zeros)
                     st.ref = now;
                     st.absent = least < 0.f;
+                    st.dead = dead;
                 }
                 ref = now;
             }
@@ -208,51 +231,124 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
 
         __syncthreads();   // the last row tile's reads of LDS
         int next = -1;
-        if (tid < RUNS) {
-            pages[t_begin & 1][tid] = entry(t_begin);
-            next = entry(t_begin + 1);
-        }
-        __syncthreads();
-        if (t_begin < t_end) {
-            fetch(t_begin);
-            store(t_begin);
-        }
-        if (tid < RUNS) pages[(t_begin + 1) & 1][tid] = next;
-        __syncthreads();
-        float ref_of_sums = 0.f;
-        for (int t = t_begin; t < t_end; ++t) {
-            const int buffer = M::BUFFERS == 2 ? t & 1 : 0;
-            if (t + 1 < t_end) fetch(t + 1);
-            if (tid < RUNS) next = entry(t + 2);
-            const int base = span.lo + t * KV_TILE;
-            const Step& st = steps[t & 1];
-            ref_of_sums = st.ref;
-            if (st.shrink < 1.f) {
-                const float f = st.shrink;
+        if (t_all > 0) {   // (a team without a step: of no positions, and of page 0)
+            const int e0 = entry(0), e1 = entry(1), e2 = entry(2);
+            next = entry(3);
+            if (wave == 2 && lane < RUNS) {
+                list(0, e0);
+                list(1, e1);
+                list(2, e2);
+            }
+            __syncthreads();
+            fetch(0);
+            {
+                uint32_t most = 0;
 #pragma unroll
-                for (int b = 0; b < M::NB; ++b) o[b] *= f;
+                for (int k = 0; k < M::KS; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(to_f32(in[k].of[e])) & 0x7FFFFFFFu);
+                most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+                const bool finite = most < 0x7F800000u;
+                int e2 = 0;
+                (void)frexpf(finite && most ? __uint_as_float(most) : 1.f, &e2);   // the row's largest is in [2^(e2 - 1), 2^e2)
+#pragma unroll
+                for (int k = 0; k < M::KS; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = ldexpf(to_f32(in[k].of[e]), 14 - e2);   // below 2^14
+                        const _Float16 hi = (_Float16)x;
+                        q[0][k][e] = hi;
+                        if (M::FINE) q[M::PARTS - 1][k][e] = (_Float16)(x - (float)hi);
+                    }
+                // the scale first: powers that it makes up for may be far from one
+                unit = finite ? ldexpf(ldexpf(a.scale * 1.4426950408889634f, e2 / 2), e2 - e2 / 2 - 14) : NAN;
+            }
+            store(0);
+            note(0);
+            if (!M::FINE) fetch(1);
+            __syncthreads();
+        }
+        float ref_of_sums = 0.f;
+        for (int t = 0; t < turns; ++t) {
+            const bool is = t < t_end;   // the other team may have one step more
+            const int base = base_of(t);
+            const Step& st = steps[t & 1];
+            int after = -1;
+            if (M::FINE) {
+                after = entry(t + 4);
+                fetch(t + 1);
+            }
+            float shrink = 1.f;
+            if (is) {
+                ref_of_sums = st.ref;
+                shrink = st.shrink;
             }
             // a wave whose rows see nothing of the step leaves it
-            if (base <= pos_most && (a.window == 0 || base + KV_TILE - 1 > pos_least - a.window)) {
-                const uint8_t *kl = k_lds(buffer), *vl = v_lds(buffer);
-                v16f x[2];
+            const bool sees = is && base <= pos_most && (a.window == 0 || base + KV_TILE - 1 > pos_least - a.window);
+            v16f x[2];
+            float by[RUNS];
+            // First the scores, and the next step's codes into LDS meanwhile; then those of the step after it on their way. (f32 has no
+            // registers for that: its next step's codes are loaded here and put into LDS at the end. 142 us against 164.)
+            if (sees) {
+                // row i = 8 b + 4 h + j of the operand is position 16 (b / 2) + 8 h + 4 (b % 2) + j
+                const int from = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
+                const uint8_t* kr = k_lds(t & 1) + from * M::K_PITCH + 16 * half;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    // row i = 8 b + 4 h + j of the operand is position 16 (b / 2) + 8 h + 4 (b % 2) + j
-                    const int from = 32 * u + 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
-                    const uint8_t* kr = kl + from * M::K_PITCH + 16 * half;
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[u][e] = 0.f;
+                if constexpr (M::FINE) {
 #pragma unroll
-                    for (int k = 0; k < M::KS; ++k) {
-                        const h8 kk = *(const h8*)(kr + 32 * k);
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int p = 0; p < M::PARTS; ++p) x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk, q[p][k], x[u], 0, 0, 0);
+                        for (int k = 0; k < M::KS; ++k) {
+                            const h8 kk = *(const h8*)(kr + 32 * u * M::K_PITCH + 32 * k);
+#pragma unroll
+                            for (int p = 0; p < M::PARTS; ++p) x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk, q[p][k], x[u], 0, 0, 0);
+                        }
+                } else {
+                // a few products at a time, the next ones' operands on their way from LDS
+                constexpr int K_AT = M::FINE ? 1 : 2, TURNS = M::KS / K_AT, EACH = TURNS / (2 * M::CHUNKS);
+                h8 kk[2][2 * K_AT];
+                auto operands = [&](int i) {
+#pragma unroll
+                    for (int j = 0; j < 2 * K_AT; ++j) kk[i & 1][j] = *(const h8*)(kr + 32 * (j & 1) * M::K_PITCH + 32 * (K_AT * i + j / 2));
+                };
+                operands(0);
+#pragma unroll
+                for (int i = 0; i < TURNS; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (i + 1 < TURNS) operands(i + 1);
+                    if (i % EACH == EACH - 1) store_chunk(t + 1, i / EACH);
+#pragma unroll
+                    for (int j = 0; j < 2 * K_AT; ++j)
+#pragma unroll
+                        for (int p = 0; p < M::PARTS; ++p) x[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk[i & 1][j], q[p][K_AT * i + j / 2], x[j & 1], 0, 0, 0);
+                    if (i + 1 < TURNS) __builtin_amdgcn_sched_group_barrier(0x100, 2 * K_AT, 0);
+#pragma unroll
+                    for (int j = 0; j < 2 * K_AT * M::PARTS; ++j) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
                     }
+                    __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                }
+            } else if (!M::FINE) store(t + 1);
+            if (!M::FINE) {
+                note(t + 1);
+                if (wave == 2 && lane < RUNS) list(t + 3, next);
+                next = entry(t + 4);
+                fetch(t + 2);
+            }
+            if (shrink < 1.f) {
+#pragma unroll
+                for (int b = 0; b < M::NB; ++b) o[b] *= shrink;
+            }
+            if (sees) {
                 // scores in powers of two; element e of x[u]: position base + 32 u + 16 (e / 8) + 8 half + e % 8
                 const bool whole = base + KV_TILE - 1 <= pos_least && (a.window == 0 || base > pos_most - a.window) && !st.absent;
-                float by[RUNS], top = -INFINITY;
+                float top = -INFINITY;
 #pragma unroll
                 for (int n = 0; n < RUNS; ++n) by[n] = st.ks[n] * unit;
                 if (!whole) {
@@ -269,9 +365,9 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
                 }
 #pragma unroll
                 for (int n = 0; n < RUNS; ++n) {
-                    float part_top = x[n / 2][8 * (n % 2)];
-#pragma unroll
-                    for (int e = 1; e < 8; ++e) part_top = fmaxf(part_top, x[n / 2][8 * (n % 2) + e]);
+                    const v16f& y = x[n / 2];
+                    const int e = 8 * (n % 2);
+                    const float part_top = max3(max3(max3(y[e], y[e + 1], y[e + 2]), y[e + 3], y[e + 4]), y[e + 5], max3(y[e + 6], y[e + 7], y[e + 7]));
                     top = fmaxf(top, part_top * by[n]);
                 }
                 {
@@ -286,10 +382,25 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
                     for (int b = 0; b < M::NB; ++b) o[b] *= keep;
                     m = m_new;
                 }
-                const float m_base = m == -INFINITY ? 0.f : m;
+                if (st.dead) {   // positions of pages without values: in the sum of weights only
+                    const float m_base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-                for (int n = 0; n < RUNS; ++n) {
-                    h8 w[M::PARTS];
+                    for (int n = 0; n < RUNS; ++n)
+                        if (st.dead >> n & 1)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) l += __builtin_amdgcn_exp2f(fmaf(x[n / 2][8 * (n % 2) + e], by[n], -m_base));
+                }
+            }
+            // then the weights and sums
+            if (sees) {
+                const uint8_t* vl = v_lds(t & 1);
+                const float m_base = m == -INFINITY ? 0.f : m;
+                h8 w[2][M::PARTS], vv[2][M::NB];
+                auto operands = [&](int n) {
+#pragma unroll
+                    for (int b = 0; b < M::NB; ++b) vv[n & 1][b] = *(const h8*)(vl + (32 * b + col) * M::V_PITCH + 32 * n + 16 * half);
+                };
+                auto weights = [&](int n) {
                     const float add = st.bias[n] - m_base;
                     float sum = 0.f;
 #pragma unroll
@@ -299,53 +410,110 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void kv_attention_many_ke
                         sum += y[0];
                         sum += y[1];
                         const h2 hi = __builtin_convertvector(y, h2);
-                        w[0][e] = hi[0];
-                        w[0][e + 1] = hi[1];
+                        w[n & 1][0][e] = hi[0];
+                        w[n & 1][0][e + 1] = hi[1];
                         if (M::FINE) {
                             const f2 left = {y[0] - (float)hi[0], y[1] - (float)hi[1]};
                             const h2 lo = __builtin_convertvector(left, h2);
-                            w[M::PARTS - 1][e] = lo[0];
-                            w[M::PARTS - 1][e + 1] = lo[1];
+                            w[n & 1][M::PARTS - 1][e] = lo[0];
+                            w[n & 1][M::PARTS - 1][e + 1] = lo[1];
                         }
                     }
                     l = fmaf(sum, st.back[n], l);
-#pragma unroll
-                    for (int p = 0; p < M::PARTS; ++p) {   // values of a page whose scale is zero: zeros, whatever its codes are
-                        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-                        w[p] = __builtin_bit_cast(h8, __builtin_bit_cast(u4, w[p]) & st.live[n]);
-                    }
-#pragma unroll
-                    for (int b = 0; b < M::NB; ++b) {
-                        const h8 vv = *(const h8*)(vl + (32 * b + col) * M::V_PITCH + 32 * n + 16 * half);
-#pragma unroll
-                        for (int p = 0; p < M::PARTS; ++p) o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, w[p], o[b], 0, 0, 0);
-                    }
+                };
+                if constexpr (!M::FINE) {
+                    operands(0);
+                    weights(0);
                 }
+                // the next run's operands and weights while this one's products are on the matrix unit
+#pragma unroll
+                for (int n = 0; n < RUNS; ++n) {
+                    if (!M::FINE) __builtin_amdgcn_sched_barrier(0);
+                    if (M::FINE) {
+                        operands(n);
+                        weights(n);
+                    } else if (n + 1 < RUNS) {
+                        operands(n + 1);
+                        weights(n + 1);
+                    }
+#pragma unroll
+                    for (int b = 0; b < M::NB; ++b)
+#pragma unroll
+                        for (int p = 0; p < M::PARTS; ++p) o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[n & 1][b], w[n & 1][p], o[b], 0, 0, 0);
+                    if constexpr (!M::FINE)
+                        if (n + 1 < RUNS) {
+                            __builtin_amdgcn_sched_group_barrier(0x100, M::NB, 0);
+#pragma unroll
+                            for (int b = 0; b < M::NB; ++b) {
+                                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                                __builtin_amdgcn_sched_group_barrier(0x402, 36 / M::NB, 0);
+                            }
+                        }
+                }
+                if (!M::FINE) __builtin_amdgcn_sched_barrier(0);
             }
-            if (M::BUFFERS == 1) __syncthreads();
-            if (t + 1 < t_end) store(t + 1);
-            if (tid < RUNS) pages[t & 1][tid] = next;   // of step t + 2; those of t have been read
+            if (M::FINE) {
+                store(t + 1);
+                note(t + 1);
+                if (wave == 2 && lane < RUNS) list(t + 3, next);
+                next = after;
+            }
             __syncthreads();
         }
         l += __shfl_xor(l, 32);
-        const float back = ref_of_sums * 0.0078125f;   // 2^-LIFT
-        if (!row_is) continue;
         // element e of o[b]: column 32 b + 8 (e / 4) + 4 half + e % 4
+        constexpr int MINE = M::NB / M::TEAMS;
+        float back = ref_of_sums * 0.0078125f;   // 2^-LIFT
+        if (M::TEAMS == 2) {
+            // The teams' sums meet: each gives the other half of its columns. (The last step's end was a barrier.)
+            if (team == 1)
+#pragma unroll
+                for (int b = 0; b < MINE; ++b) {
+                    const v16f x = o[b];
+                    o[b] = o[MINE + b];
+                    o[MINE + b] = x;
+                }
+            auto slot = [&](int of, int n) { return (f4*)(lds_of_all + of * M::TEAM_BYTES) + n * THREADS + tid; };
+#pragma unroll
+            for (int b = 0; b < MINE; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) *slot(team, 4 * b + e / 4) = f4{o[MINE + b][e], o[MINE + b][e + 1], o[MINE + b][e + 2], o[MINE + b][e + 3]};
+            if (half == 0) meet[team][32 * wave + col] = make_float2(m, l);
+            if (tid == 0) refs[team] = back;
+            __syncthreads();
+            const float2 ml = meet[1 - team][32 * wave + col];
+            const float m_both = fmaxf(m, ml.x);
+            const float mine = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_both), other = ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m_both);
+            l = l * mine + ml.y * other;   // (what has no maximum has sums of zero, or none that is a number)
+            m = m_both;
+            const float mine_o = mine * back, other_o = other * refs[1 - team];
+            back = 1.f;
+#pragma unroll
+            for (int b = 0; b < MINE; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const f4 x = *slot(1 - team, 4 * b + e / 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[b][e + j] = o[b][e + j] * mine_o + x[j] * other_o;
+                }
+        }
+        if (!row_is) continue;
+        const int column = team * 32 * MINE + 4 * half;
         if (parts == 1) {
             const float f = l == 0.f ? 0.f : back / l;
-            T* out = (T*)a.out + tok * a.out_stride + (int64_t)head * D + 4 * half;
+            T* out = (T*)a.out + tok * a.out_stride + (int64_t)head * D + column;
 #pragma unroll
-            for (int b = 0; b < M::NB; ++b)
+            for (int b = 0; b < MINE; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) out[32 * b + 8 * (e / 4) + e % 4] = from_f32<T>(o[b][e] * f);
         } else {
             const int64_t to = (a.part_row(seq, s, tok) * a.heads + head) * a.splits + part;
-            float* out = a.part_o + to * D + 4 * half;
+            float* out = a.part_o + to * D + column;
 #pragma unroll
-            for (int b = 0; b < M::NB; ++b)
+            for (int b = 0; b < MINE; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) out[32 * b + 8 * (e / 4) + e % 4] = o[b][e] * back;
-            if (half == 0) a.part_ml[to] = make_float2(m, l);
+            if (half == 0 && team == 0) a.part_ml[to] = make_float2(m, l);
         }
     }
 }
@@ -362,7 +530,7 @@ static int launch(const Attend& a, int max_rows, hipStream_t s) {
         (void)hipGetLastError();
         return LK_ERR_LAUNCH;
     }
-    hipLaunchKernelGGL((kv_attention_many_kernel<T, D>), dim3((unsigned)blocks), dim3(THREADS), bytes, s, a, row_tiles, lk_device().cus);
+    hipLaunchKernelGGL((kv_attention_many_kernel<T, D>), dim3((unsigned)blocks), dim3(Many<T, D>::TEAMS * THREADS), bytes, s, a, row_tiles, lk_device().cus);
     return lk_launch_status();
 }
 
