@@ -110,6 +110,9 @@ def parse_args():
                     help="--workload decode-1p7b above 8 rows: auto = the host mirror's choice between the matrix-unit "
                          "rows kernels and the tiled matmul; matvec = mat-vec launches over slices of eight rows up to "
                          "32 rows; tiled = the tiled matmul")
+    ap.add_argument("--context", type=int, default=0,
+                    help="--workload decode-1p7b: every row is a sequence of so many tokens in a paged 8-bit cache, and the step has its "
+                         "plan of pages, cache writes, attention and the choice of the next token as well (0: linears only)")
     ap.add_argument("--launches", type=int, default=200, help="timed launches of the per-launch workloads")
     return ap.parse_args()
 

@@ -10,7 +10,9 @@
   moe         one Qwen3-30B-A3B-shaped expert block (128 experts, 2048 -> 768 -> 2048, top-8,
               Q4_K) at `--tokens` rows, path chosen as the layer code chooses it
   decode-1p7b every quantized linear of a Qwen3-1.7B-shaped decode step at `--batch` rows:
-              mat-vec launches at one row, the rows kernels or the tiled matmul above
+              mat-vec launches at one row, the rows kernels or the tiled matmul above; with
+              `--context` also what stands between them: the plan of pages, each layer's cache
+              write and attention over so many tokens a row, and the choice of the next token
 
 Timing: 20 warm-up launches, then `--launches` (default 200) launches each bracketed by its own
 pair of events on the launch stream; median, p10, p90, min and max are reported (the protocol of
@@ -23,7 +25,7 @@ import json
 import numpy as np
 import torch
 
-from . import lib, moe, ops, synth
+from . import kv, lib, moe, ops, synth
 
 HBM_PEAK_GBS = 8000.0
 INT8_PEAK_TOPS = 5000.0
@@ -451,6 +453,64 @@ def moe_block(args, dev):
                 extra)
 
 
+# ---------------------------------------------------------------------------- between the linears
+HEAD_DIM, PAGE_TOKENS = 128, 64
+
+
+class Between:
+    """What a decode step of ``seqs`` sequences does between its linears: the plan of pages once, each layer's cache write and
+    attention over ``context`` tokens and the new one, and the choice of the next token at the end; as items of a launch plan."""
+
+    def __init__(self, seqs, context, heads, kv_heads, mk):
+        cols = context // PAGE_TOKENS + 1
+        self.seqs, self.context, self.heads, self.kv_heads, self.mk = seqs, context, heads, kv_heads, mk
+        self.pages = seqs * cols
+        ids = torch.randperm(self.pages, device=mk.dev, generator=mk.gen).to(torch.int32).reshape(seqs, cols)
+        held = -(-context // PAGE_TOKENS)
+        self.table = ids.clone()
+        self.table[:, held:] = -1
+        self.free = ids[:, held:].reshape(-1).contiguous()
+        self.past = torch.full((seqs,), context, dtype=torch.int32, device=mk.dev)
+        self.fresh = torch.ones_like(self.past)
+        self.plan = kv.KvPlan(seqs, seqs, mk.dev)
+        self.rules = [torch.rand(seqs, device=mk.dev, generator=mk.gen), torch.full((seqs,), 0.8, device=mk.dev),
+                      torch.full((seqs,), 50, dtype=torch.int32, device=mk.dev), torch.full((seqs,), 0.95, device=mk.dev)]
+        self.caches, self.tokens, self.probs = [], torch.empty_like(self.past), torch.empty(seqs, device=mk.dev)
+
+    def bytes_read(self):
+        """Codes of the keys and values that a layer's attention reads."""
+        return 2 * self.seqs * (self.context + 1) * self.kv_heads * HEAD_DIM
+
+    def plan_item(self, s):
+        p, t = self.plan, self.table
+        return ("status", lib.load().lk_kv_plan, (
+            self.past.data_ptr(), self.fresh.data_ptr(), self.seqs, PAGE_TOKENS, self.free.data_ptr(), self.free.numel(), None, t.data_ptr(),
+            t.stride(0), t.shape[1], p.lens.data_ptr(), p.starts.data_ptr(), p.slots.data_ptr(), p.positions.data_ptr(), self.seqs,
+            p.taken.data_ptr(), s))
+
+    def attention_items(self, q, k, v, out, s):
+        """A layer's cache, the write of its ``k`` and ``v`` and the attention of ``q`` over it, into ``out``."""
+        L, f32, p, t = lib.load(), lib.TYPE_F32, self.plan, self.table
+        shape, dev = (self.pages, self.kv_heads, PAGE_TOKENS * HEAD_DIM), self.mk.dev
+        codes = [torch.randint(-127, 128, shape, dtype=torch.int8, device=dev, generator=self.mk.gen) for _ in "kv"]
+        scales = [torch.rand(shape[:2], device=dev, generator=self.mk.gen) * 0.01 + 0.005 for _ in "kv"]
+        c = kv.KvCacheQ8(codes[0].view(*shape[:2], PAGE_TOKENS, HEAD_DIM), codes[1].view(*shape[:2], PAGE_TOKENS // 16, HEAD_DIM, 16), *scales)
+        self.caches.append(c)
+        at = (c.k.data_ptr(), c.v.data_ptr(), c.k_scales.data_ptr(), c.v_scales.data_ptr())
+        return [("status", L.lk_kv_write_q8, (k.data_ptr(), v.data_ptr(), f32, k.stride(0), v.stride(0), p.slots.data_ptr(), self.seqs,
+                                              self.kv_heads, HEAD_DIM, PAGE_TOKENS, self.pages, *at, s)),
+                ("status", L.lk_kv_attention_q8, (
+                    q.data_ptr(), f32, q.stride(0), out.data_ptr(), out.stride(0), *at, self.pages, PAGE_TOKENS, t.data_ptr(), t.stride(0),
+                    t.shape[1], p.lens.data_ptr(), p.starts.data_ptr(), self.seqs, self.seqs, 1, self.context + 1, self.heads,
+                    self.kv_heads, HEAD_DIM, HEAD_DIM ** -0.5, 0, s))]
+
+    def sample_item(self, logits, vocab, s):
+        u, temperature, top_k, top_p = self.rules
+        return ("status", lib.load().lk_sample, (
+            logits.data_ptr(), lib.TYPE_F32, logits.stride(0), self.seqs, vocab, u.data_ptr(), temperature.data_ptr(), top_k.data_ptr(),
+            top_p.data_ptr(), None, self.tokens.data_ptr(), self.probs.data_ptr(), s))
+
+
 # ---------------------------------------------------------------------------- decode-1p7b
 def decode_1p7b(args, dev):
     L = lib.load()
@@ -464,6 +524,7 @@ def decode_1p7b(args, dev):
     acts = {g: mk.randn(b, k) for g, k, _, _ in groups}
     acts["final"] = mk.randn(b, hidden)
     keep, plan, total_bytes = [], [], 0
+    results = []   # of the group's linears, as they were added
     matvec = b <= 8
     used = {"rows": 0, "matvec": 0, "tiled": 0}
 
@@ -503,6 +564,7 @@ def decode_1p7b(args, dev):
         if g == "h":   # `down` reads the Q8_1 rows the gate + up launch wrote
             out = torch.empty((b, ns[0]), device=dev)
             keep.append(out)
+            results.append(out)
             if b <= 6 and ns[0] * k < (48 << 20):   # a small matrix at few rows: the mat-vec (host_qmatmul.hip's rule)
                 plan.append(("status", L.lk_mmvq, (wtype, weights[0].data_ptr(), rows_h_q81.data_ptr(), out.data_ptr(), lib.TYPE_F32,
                                                    k, ns[0], b, k // 32, ns[0], None, 0, s)))
@@ -518,6 +580,7 @@ def decode_1p7b(args, dev):
             for w, n in zip(weights, ns):
                 out = torch.empty((b, n), device=dev)
                 keep.append(out)
+                results.append(out)
                 plan.append(("status", L.lk_dense_q6k_rows, (w.data_ptr(), q.data_ptr(), out.data_ptr(), b, n, k, s)))
         elif g == "x2":
             plan.append(("status", L.lk_dense_q4k_rows_actmul_q8_1,
@@ -528,6 +591,7 @@ def decode_1p7b(args, dev):
             dst = (lib.C.c_void_p * len(ns))(*[o.data_ptr() for o in outs])
             nn = (lib.C.c_int * len(ns))(*ns)
             keep.extend(outs + [vx, dst, nn])
+            results.extend(outs)
             plan.append(("status", L.lk_dense_q4k_rows_multi, (vx, dst, nn, len(ns), q.data_ptr(), b, k, 0, s)))
 
     # one or two rows: gate + up as the pair launch that applies SiLU and writes the Q8_1 rows `down`
@@ -558,6 +622,7 @@ def decode_1p7b(args, dev):
         elif paired and g == "h":
             out = torch.empty((b, ns[0]), device=dev)
             keep.append(out)
+            results.append(out)
             plan.append(("status", L.lk_mmvq, (wtype, weights[0].data_ptr(), h_q81.data_ptr(), out.data_ptr(), lib.TYPE_F32, k,
                                                ns[0], b, h_q81.shape[1], ns[0], None, 0, s)))
         elif matvec and k <= 8192:
@@ -567,6 +632,7 @@ def decode_1p7b(args, dev):
             dst = (lib.C.c_void_p * len(ns))(*[o.data_ptr() for o in outs])
             nn = (lib.C.c_int * len(ns))(*ns)
             keep.extend(outs + [vx, dst, nn])
+            results.extend(outs)
             if from_norm:
                 plan.append(("status", L.lk_mmvq_multi, (wtype, len(ns), vx, qn.data_ptr(), dst, lib.TYPE_F32, k, nn, b, qn.shape[1],
                                                           stride, None, s)))
@@ -580,6 +646,7 @@ def decode_1p7b(args, dev):
             for w, n in zip(weights, ns):
                 out = torch.empty((b, n), device=dev)
                 keep.append(out)
+                results.append(out)
                 plan.append(("status", L.lk_mmvq, (wtype, w.data_ptr(), q.data_ptr(), out.data_ptr(), lib.TYPE_F32, k, n, b,
                                          q.shape[1], n, None, 0, s)))
         elif args.mid_rows == "auto" and all(rows_kernel_serves(wtype, n, k, b) for n in ns):
@@ -587,6 +654,7 @@ def decode_1p7b(args, dev):
             if g == "h" and mid_h_q81 is not None:   # `down` reads the Q8_1 rows the gate + up launch wrote
                 out = torch.empty((b, ns[0]), device=dev)
                 keep.append(out)
+                results.append(out)
                 plan.append(("status", L.lk_dense_q6k_rows, (weights[0].data_ptr(), mid_h_q81.data_ptr(), out.data_ptr(), b, ns[0], k, s)))
                 used["rows"] += 1
                 return
@@ -606,12 +674,14 @@ def decode_1p7b(args, dev):
                 dst = (lib.C.c_void_p * len(ns))(*[o.data_ptr() for o in outs])
                 nn = (lib.C.c_int * len(ns))(*ns)
                 keep.extend(outs + [vx, dst, nn])
+                results.extend(outs)
                 plan.append(("status", L.lk_dense_q4k_rows_multi, (vx, dst, nn, len(ns), q.data_ptr(), b, k, 0, s)))
                 used["rows"] += len(ns)
                 return
             for w, n in zip(weights, ns):
                 out = torch.empty((b, n), device=dev)
                 keep.append(out)
+                results.append(out)
                 plan.append(("status", L.lk_dense_q4k_rows if wtype == Q4K else L.lk_dense_q6k_rows,
                              (w.data_ptr(), q.data_ptr(), out.data_ptr(), b, n, k, s)))
                 used["rows"] += 1
@@ -624,6 +694,7 @@ def decode_1p7b(args, dev):
             for w, n in zip(weights, ns):
                 out = torch.empty((b, n), device=dev)
                 keep.append(out)
+                results.append(out)
                 for r0 in range(0, b, 8):
                     rows = min(8, b - r0)
                     plan.append(("status", L.lk_mmvq, (wtype, w.data_ptr(), q[r0].data_ptr(), out[r0].data_ptr(),
@@ -638,14 +709,24 @@ def decode_1p7b(args, dev):
             for w, n in zip(weights, ns):
                 out = torch.empty((b, n), device=dev)
                 keep.append(out)
+                results.append(out)
                 plan.append(("tile", getattr(L, ops.MMQ_LAUNCHER[wtype]),
                              (ops.mmq_fixup(dev).data_ptr(), w.data_ptr(), ws.data_ptr(), out.data_ptr(), k, n, b, k // 256, n, info["cc"],
                               info["nsm"], info["smpbo"], info["warp_size"], s)))
 
+    between = Between(b, args.context, hidden // HEAD_DIM, kv // HEAD_DIM, mk) if args.context else None
+    if between:
+        plan.append(between.plan_item(s))
     for _ in range(layers):
         for g, k, wtype, ns in groups:
+            results.clear()
             add_group(g, k, wtype, ns)
+            if between and g == "x":   # the attention's rows are what `o` reads
+                plan.extend(between.attention_items(*results, acts["attn"], s))
+    results.clear()
     add_group("final", hidden, Q6K, [vocab])
+    if between:
+        plan.append(between.sample_item(results[0], vocab, s))
     def run(items):
         for kind, fn, a in items:
             rc = fn(*a)
@@ -668,13 +749,15 @@ def decode_1p7b(args, dev):
     # at least 20 warm-up replays and 200 timed ones, each replay between its own pair of events
     us = time_replays(graph, max(200, args.steps), warm=max(20, args.warmup))
     ms = float(np.median(us)) * 1e-3
-    value = total_bytes / (ms * 1e-3) / 1e9
+    cache_bytes = layers * between.bytes_read() if between else 0
+    value = (total_bytes + cache_bytes) / (ms * 1e-3) / 1e9
     roofline = {"bound": "hbm", "achieved": round(value, 1), "peak": HBM_PEAK_GBS, "unit": "GB/s",
                 "frac": round(value / HBM_PEAK_GBS, 4), "traffic": None,
                 "kernel": "whole step (all launches of the graph)", "launches_per_step": len(plan)}
     return line(args, value, "GB/s", ms, "int8",
                 {"workload": f"qwen3-1.7b decode-step quantized linears (Q4_K attention and gate/up, Q6_K down and "
-                             f"lm_head), batch {b}, 28 layers",
+                             f"lm_head), batch {b}, 28 layers" + (f"; the plan of pages, cache write and attention of a layer over {args.context} "
+                             f"tokens a sequence, and the choice of the next token (value: weight and cache bytes)" if between else ""),
                  "path": "mat-vec (fused: q + k + v, o from f32 rows; gate + up as the pair launch that writes down's Q8_1 rows)" if paired
                          else "mat-vec (fused; own quantizer launch for rows over 8192 values)" if matvec
                          else "16-row tiles on the matrix unit: q + k + v in one launch, o, gate + up with SiLU in one launch that writes "
@@ -684,7 +767,8 @@ def decode_1p7b(args, dev):
                  "acts": "f32 rows into every group" if getattr(args, "acts", "f32") == "f32"
                          else "q + k + v and gate + up read Q8_1 rows as the model's RMSNorm launches that also quantize leave them "
                               "(those launches are not timed); o and lm_head from f32 rows",
-                 "weight_bytes_per_step": total_bytes, "launches_per_step": len(plan), "hip_graph": True}, roofline,
+                 "weight_bytes_per_step": total_bytes, **({"cache_bytes_per_step": cache_bytes} if between else {}),
+                 "launches_per_step": len(plan), "hip_graph": True}, roofline,
                 {"step_spread": spread(us), "ms_per_step_is": "median of the timed replays"})
 
 
