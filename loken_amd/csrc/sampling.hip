@@ -265,16 +265,22 @@ static __device__ __forceinline__ void scan_bins(uint64_t* mass, uint32_t* count
     __syncthreads();
 }
 
-// The first of n >= 1 running sums that reaches `target`, n - 1 if none does. Every thread looks for itself.
+// The first of 0 .. n - 1 for which `is` holds, as it does for all behind it; n if for none. Each wave looks for itself, all its lanes
+// at once: two looks into LDS, one after the other, where halves would take eleven.
+static_assert(BINS <= 64 * 64 && LIST <= 64 * 64);
+template <class F>
+static __device__ __forceinline__ int first_where(int n, F is) {
+    const int lane = threadIdx.x & 63, run = (n + 63) >> 6;
+    uint64_t all = __ballot(lane * run < n && is(min(lane * run + run, n) - 1));
+    if (!all) return n;
+    const int from = (__ffsll((unsigned long long)all) - 1) * run;
+    all = __ballot(lane < run && from + lane < n && is(min(from + lane, n - 1)));
+    return from + __ffsll((unsigned long long)all) - 1;
+}
+// The first of n >= 1 running sums that reaches `target`, n - 1 if none does.
 template <typename V>
 static __device__ __forceinline__ int first_reaching(const V* sums, int n, uint64_t target) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (sums[mid] >= target) hi = mid;
-        else lo = mid + 1;
-    }
-    return lo;
+    return min(first_where(n, [&](int i) { return sums[i] >= target; }), n - 1);
 }
 
 // Sorts the n <= LIST words of the list, the largest first, and gives their running sums of weights. A word's number is part of
@@ -707,13 +713,7 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
     sort_list(sh, n, sc);
     // The list's running sums as the row's: each range starts at the weight of what lies in front of it.
     auto first_at = [&](int step) {   // the first word of the list whose step is not in front of `step`
-        int lo = 0, hi = n;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (sc.step(sc.top - value_of((uint32_t)(sh.list[mid] >> 32))) >= (float)step) hi = mid;
-            else lo = mid + 1;
-        }
-        return lo;
+        return first_where(n, [&](int i) { return sc.step(sc.top - value_of((uint32_t)(sh.list[i] >> 32))) >= (float)step; });
     };
     auto shift_of = [&](int step, int first) {
         return (wants.mass && step > 0 && step < BINS ? sh.mass[min(max(step - 1, 0), BINS - 1)] : 0) - (first > 0 ? sh.sums[max(first - 1, 0)] : 0);
@@ -728,14 +728,11 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
     if (top_p < 1.0f) kept = sh.sums[first_reaching(sh.sums, n, nucleus_sum(top_p, kept))];
     uint64_t above = kept_m;
     if (!wants.mass && a.min_p && a.min_p[row] > 0.0f) {   // what min-p keeps of the list, which is a prefix
-        int lo = 1, hi = n;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            const float v = value_of((uint32_t)(sh.list[mid] >> 32));
-            if (sc.kept(sc.top - v, sc.power(v))) lo = mid + 1;
-            else hi = mid;
-        }
-        above = sh.sums[lo - 1];
+        const int past = first_where(n, [&](int i) {
+            const float v = value_of((uint32_t)(sh.list[i] >> 32));
+            return !sc.kept(sc.top - v, sc.power(v));
+        });
+        above = sh.sums[max(past, 1) - 1];
     }
     kept = min(kept, above);
     const int at = first_reaching(sh.sums, n, drawn_sum(u, kept));
