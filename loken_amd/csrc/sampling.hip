@@ -247,22 +247,25 @@ static __device__ __forceinline__ uint64_t sum_before(uint64_t mine, uint64_t (*
     return before;
 }
 
-// The histogram's running sums, in place.
-static __device__ __forceinline__ void scan_bins(uint64_t* mass, uint32_t* count, uint64_t (*meet)[2]) {
-    constexpr int PER = BINS / SAMPLE_WG;
+// Running sums over the steps, of what the thread has of them (PER from PER t on), into `mass` and `count`.
+constexpr int PER = BINS / SAMPLE_WG;
+static __device__ __forceinline__ void scan_held(uint64_t (&m)[PER], uint32_t (&c)[PER], uint64_t* mass, uint32_t* count, uint64_t (*meet)[2]) {
     const int t = threadIdx.x;
-    uint64_t m[PER], ms = 0;
-    uint32_t c[PER], cs = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        m[i] = (ms += mass[t * PER + i]);
-        c[i] = (cs += count[t * PER + i]);
-    }
-    const uint64_t mb = sum_before(ms, meet, 0);
-    const uint32_t cb = (uint32_t)sum_before(cs, meet, 1);
+    for (int i = 1; i < PER; ++i) { m[i] += m[i - 1]; c[i] += c[i - 1]; }
+    const uint64_t mb = sum_before(m[PER - 1], meet, 0);
+    const uint32_t cb = (uint32_t)sum_before(c[PER - 1], meet, 1);
 #pragma unroll
     for (int i = 0; i < PER; ++i) { mass[t * PER + i] = mb + m[i]; count[t * PER + i] = cb + c[i]; }
     __syncthreads();
+}
+// The same of a histogram in LDS, in place.
+static __device__ __forceinline__ void scan_bins(uint64_t* mass, uint32_t* count, uint64_t (*meet)[2]) {
+    uint64_t m[PER];
+    uint32_t c[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { m[i] = mass[threadIdx.x * PER + i]; c[i] = count[threadIdx.x * PER + i]; }
+    scan_held(m, c, mass, count, meet);
 }
 
 // The first of 0 .. n - 1 for which `is` holds, as it does for all behind it; n if for none. Each wave looks for itself, all its lanes
@@ -294,6 +297,7 @@ static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale&
         if (t < AT_ONCE) sh.list[n + t] = 0;   // (the list has room for them)
         __syncthreads();
         const uint64_t mine = t < n ? sh.list[t] : ~0ull;
+        const uint64_t weight = weight_of(sc.power(t < n ? value_of((uint32_t)(mine >> 32)) : sc.top));
         int place = 0;
         for (int i = 0; i < n; i += AT_ONCE) {
             uint64_t x[AT_ONCE];
@@ -303,8 +307,15 @@ static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale&
             for (int j = 0; j < AT_ONCE; ++j) place += x[j] > mine;
         }
         __syncthreads();
-        if (t < n) sh.list[place] = mine;
+        if (t < n) {
+            sh.list[place] = mine;
+            sh.sums[place] = weight;
+        }
         __syncthreads();
+        const uint64_t here = t < n ? sh.sums[t] : 0, before = sum_before(here, sh.meet, 0);
+        if (t < n) sh.sums[t] = before + here;
+        __syncthreads();
+        return;
     } else {
         int size = 2 * COUNTED;
         while (size < n) size <<= 1;
@@ -320,7 +331,7 @@ static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale&
                 __syncthreads();
             }
     }
-    constexpr int PER = LIST / SAMPLE_WG;
+    static_assert(PER * SAMPLE_WG == LIST);
     uint64_t m[PER], ms = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -581,6 +592,15 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
     __shared__ Shared sh;
     const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     const T* x = (const T*)a.logits + row * a.stride;
+    // everything that is read of the row's other launches, at once
+    uint64_t mass[PER];
+    uint32_t count[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        mass[i] = a.mass[(int64_t)row * BINS + t * PER + i];
+        count[i] = a.count[(int64_t)row * BINS + t * PER + i];
+    }
+    const uint64_t floor_mass = a.floor_mass[row];
     const Peak peak = peak_of_row(a, row);
     Scale sc;
     if (!sc.init(peak, a.temperature[row], a.min_p ? a.min_p[row] : 0.0f)) {   // no words, or the first of them
@@ -595,13 +615,8 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
         return;
     }
     const Wants wants(a, row);
-    for (int i = t; i < BINS; i += SAMPLE_WG) {
-        sh.mass[i] = wants.mass ? a.mass[(int64_t)row * BINS + i] : 0;
-        sh.count[i] = wants.count ? a.count[(int64_t)row * BINS + i] : 0;
-    }
-    __syncthreads();
-    scan_bins(sh.mass, sh.count, sh.meet);
-    const uint64_t one = 1ull << ONE_BITS, kept_m = wants.above ? max((uint64_t)a.floor_mass[row], one) : ~0ull;
+    scan_held(mass, count, sh.mass, sh.count, sh.meet);   // (what is not counted or weighed is zeros)
+    const uint64_t one = 1ull << ONE_BITS, kept_m = wants.above ? max(floor_mass, one) : ~0ull;
     const float top_p = a.top_p ? a.top_p[row] : 1.0f, u = a.uniform[row];
     const int k = wants.count ? a.top_k[row] : 0;
     const bool cut_k = wants.count && (uint32_t)k < sh.count[BINS - 1];
