@@ -29,6 +29,7 @@ namespace {
 constexpr int BINS = 2048;        // steps of the histogram
 constexpr int LIST = 2048;        // words that are sorted in LDS
 constexpr int COUNTED = 256;      // words up to which each is counted to its place
+constexpr int CROWD = 64;         // words of a step up to which they are
 constexpr int SAMPLE_WG = 512, SAMPLE_WAVES = SAMPLE_WG / 64;
 constexpr int ONE_BITS = 42;      // a weight of 1 is 2^42
 constexpr float LIVE = 42.5f;     // words below 2^-42.5 weigh nothing
@@ -291,8 +292,7 @@ static __device__ __forceinline__ int first_reaching(const V* sums, int n, uint6
 static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale& sc) {
     const int t = threadIdx.x;
     if (n <= COUNTED) {
-        // a word a thread: its place is the number of words in front of it. 256 compares of 64 bits a thread take 2 us, exchanges with a
-        // barrier each 5; 1000 words the other way round, 25 and 10.
+        // a word a thread: its place is the number of words in front of it
         constexpr int AT_ONCE = 8;
         if (t < AT_ONCE) sh.list[n + t] = 0;   // (the list has room for them)
         __syncthreads();
@@ -316,7 +316,30 @@ static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale&
         if (t < n) sh.sums[t] = before + here;
         __syncthreads();
         return;
-    } else {
+    }
+    // More words: to their steps first, and then, among the words of a step, as above. 1000 words take 3 us; exchanges with a
+    // barrier each, as for words of which many share a step, 16.
+    static_assert(PER * SAMPLE_WG == LIST && PER % 2 == 0);
+    uint32_t* start = (uint32_t*)sh.sums;   // of a step's words, while there are no sums
+    uint64_t word[PER];
+    int step[PER], slot[PER];
+    for (int i = t; i < BINS; i += SAMPLE_WG) start[i] = 0;
+    __syncthreads();
+    bool crowd = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = i * SAMPLE_WG + t;
+        word[i] = at < n ? sh.list[at] : 0;
+        step[i] = at < n ? (int)sc.step(sc.below(value_of((uint32_t)(word[i] >> 32)))) : 0;
+        slot[i] = at < n ? (int)atomicAdd(&start[step[i]], 1u) : 0;
+        crowd = crowd || slot[i] >= CROWD;
+    }
+    const uint64_t crowds = __ballot(crowd);
+    if ((t & 63) == 0) sh.meet[t >> 6][1] = crowds;
+    __syncthreads();
+    uint64_t any = 0;
+    for (int w = 0; w < SAMPLE_WAVES; ++w) any |= sh.meet[w][1];
+    if (any) {
         int size = 2 * COUNTED;
         while (size < n) size <<= 1;
         for (int i = n + t; i < size; i += SAMPLE_WG) sh.list[i] = 0;
@@ -330,8 +353,38 @@ static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale&
                 }
                 __syncthreads();
             }
+    } else {
+        uint32_t held[PER], all = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) { held[i] = start[t * PER + i]; all += held[i]; }
+        uint32_t before = (uint32_t)sum_before(all, sh.meet, 0);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            start[t * PER + i] = before;
+            before += held[i];
+        }
+        __syncthreads();
+        int from[PER], to[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            from[i] = (int)start[step[i]];
+            to[i] = step[i] + 1 < BINS ? (int)start[min(step[i] + 1, BINS - 1)] : n;
+            if (i * SAMPLE_WG + t < n) sh.list[from[i] + slot[i]] = word[i];
+        }
+        __syncthreads();
+        int place[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            place[i] = from[i];
+            if (i * SAMPLE_WG + t < n)
+                for (int j = from[i]; j < to[i]; ++j) place[i] += sh.list[j] > word[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (i * SAMPLE_WG + t < n) sh.list[place[i]] = word[i];
+        __syncthreads();
     }
-    static_assert(PER * SAMPLE_WG == LIST);
     uint64_t m[PER], ms = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {

@@ -157,3 +157,12 @@ def test_the_same_call_gives_the_same_bits():
     for _ in range(5):
         again = sampling.sample(x, u, t)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("top_k", [200, 255, 256, 257, 300, 511, 512, 513, 777, 1000, 1023, 1024, 1025, 2047])
+@pytest.mark.parametrize("coarse", [0, 64, 4, 1])
+def test_lists_of_every_length(top_k, coarse):
+    """Words sorted by counting, by their steps, and (many of a value) by exchanges; the draw anywhere among them."""
+    x = normal(6, 50000, top_k + coarse)
+    x = x if not coarse else (x * coarse).round() / coarse
+    check(x, [0.0, 0.3, 0.9, 0.999, 0.99999, 0.5], 3.0, top_k=top_k, top_p=[1, 1, 1, 1, 0.99, 0.7])
