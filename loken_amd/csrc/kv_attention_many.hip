@@ -22,7 +22,7 @@
 // take four times as long. It is these that bound it, and what of them does not run beside products: so a product comes with
 // six of them in turn, its operands read from LDS a group ahead, and nothing that is loaded is looked at before the step after.
 // 2048 tokens of one prompt, 32 heads over 8 of 128 bf16 values: 69 us, 500 TFLOP/s of the causal half's products; 700 f32 rows over
-// 2200 positions beside eleven single rows: 137 us.
+// 2200 positions beside eleven single rows: 109 us.
 
 #include "kv_attention.h"
 
@@ -71,7 +71,7 @@ static __device__ __forceinline__ float across_runs(float x, F both) {
 // Teams of a workgroup, which take its steps in turn. Two, where the registers hold them, so that both waves of a SIMD have the same
 // rows' work to do to the end: a prompt of 2048 tokens, 32 heads over 8 of 128 bf16 values, took 80 us with one team and two
 // workgroups to a CU, of which the one with the longer rows ran on alone. f32 has no registers for the meeting of the teams
-// (700 rows over long contexts: 178 us against 140), 256 columns none for a second wave on a SIMD.
+// (700 rows over 2200 positions: 178 us against 140), 256 columns none for a second wave on a SIMD.
 constexpr int many_teams(bool fine, int head_dim) { return head_dim == 256 || fine ? 1 : 2; }
 constexpr int many_waves(int head_dim) { return head_dim == 256 ? 1 : 2; }   // on a SIMD
 
@@ -99,8 +99,35 @@ struct Step {
     int absent;         // whether a page is
 };
 
+// The row tile of that number among those of all sequences, from the last one on; false: there are fewer. Found by each wave.
+static __device__ __forceinline__ bool tile_at(const Attend& a, int number, int& seq, int& tile) {
+    const int lane = threadIdx.x & 63;
+    auto tiles_of = [&](int i) {
+        if (i >= a.seqs) return 0;
+        const unsigned rows = (unsigned)KvSeq(a, i).tokens() * (unsigned)a.group;
+        return (int)rows <= a.few_rows ? 0 : (int)((rows + KV_MANY_ROWS - 1) / KV_MANY_ROWS);
+    };
+    for (int base = (a.seqs - 1) & ~63; base >= 0; base -= 64) {
+        const int mine = tiles_of(base + lane);
+        int behind = mine;   // of this sequence and those behind it
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_down(behind, o);
+            if (lane + o < 64) behind += v;
+        }
+        const uint64_t over = __ballot(behind > number);
+        if (over) {
+            const int l = 63 - __clzll((long long)over);
+            seq = base + l;
+            tile = __builtin_amdgcn_readlane(behind, l) - 1 - number;
+            return true;
+        }
+        number -= __builtin_amdgcn_readfirstlane(behind);
+    }
+    return false;
+}
+
 template <typename T, int D>
-__global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves(D)) void kv_attention_many_kernel(Attend a, int row_tiles, int cus) {
+__global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves(D)) void kv_attention_many_kernel(Attend a, int row_tiles, int listed, int cus) {
     using M = Many<T, D>;
     extern __shared__ __align__(16) uint8_t lds_of_all[];
     __shared__ Step steps_of_all[M::TEAMS][2];
@@ -126,7 +153,8 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
     at /= a.splits;
     const int kv = at % a.pool.heads;
     at /= a.pool.heads;
-    const int seq = at % a.seqs, tile0 = row_tiles - 1 - (int)(at / a.seqs);
+    int seq = at % a.seqs, tile0 = row_tiles - 1 - (int)(at / a.seqs);
+    if (listed && !tile_at(a, (int)at, seq, tile0)) return;
     const KvSeq s(a, seq);
     const unsigned all_rows = (unsigned)s.tokens() * (unsigned)a.group;   // below 2^31
     if ((int)all_rows <= a.few_rows) return;
@@ -520,8 +548,13 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
 
 template <typename T, int D>
 static int launch(const Attend& a, int max_rows, hipStream_t s) {
+    // Workgroups to row tiles: as many to every sequence as the longest is said to have, or, where that is more, the tiles of all as a list
+    // (at most one each that is not full). One prompt of 700 beside eleven single rows in f32: 816 workgroups and 109 us, 6336 otherwise, of
+    // which each that finds nothing to do still holds a CU's LDS a while, and 137 us.
     const int row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / KV_MANY_ROWS + 1;
-    const int64_t blocks = (int64_t)a.seqs * a.pool.heads * row_tiles * a.splits;
+    const int64_t spread = (int64_t)a.seqs * row_tiles, all = ((int64_t)a.rows * a.group - 1) / KV_MANY_ROWS + 1 + a.seqs;
+    const bool listed = all < spread;
+    const int64_t blocks = (listed ? all : spread) * a.pool.heads * a.splits;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
     constexpr int bytes = Many<T, D>::LDS;
     // a kernel gets 64 KB of LDS unless the runtime is told otherwise
@@ -530,7 +563,7 @@ static int launch(const Attend& a, int max_rows, hipStream_t s) {
         (void)hipGetLastError();
         return LK_ERR_LAUNCH;
     }
-    hipLaunchKernelGGL((kv_attention_many_kernel<T, D>), dim3((unsigned)blocks), dim3(Many<T, D>::TEAMS * THREADS), bytes, s, a, row_tiles, lk_device().cus);
+    hipLaunchKernelGGL((kv_attention_many_kernel<T, D>), dim3((unsigned)blocks), dim3(Many<T, D>::TEAMS * THREADS), bytes, s, a, listed ? 1 << 25 : row_tiles, listed, lk_device().cus);
     return lk_launch_status();
 }
 

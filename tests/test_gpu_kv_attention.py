@@ -260,3 +260,15 @@ def test_many_contexts_are_cut_into_equal_pieces(what, dtype):
     b = Batch(lens, fresh, 2, 1, 64, 16, dtype, seed=41, pad=3)
     out = b.check(window=700 if what == "window" else 0, max_fresh=2 if what != "beside a prompt" else 70, max_len=9000)
     assert (out[-3:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("seqs,longest", [(70, 150), (130, 40), (200, 300)])
+def test_long_and_short_sequences_of_a_batch(seqs, longest, dtype):
+    """Row tiles of a few sequences among many that have none, in more than one look's worth of sequences; hints too small as well."""
+    g = np.random.default_rng(seqs)
+    fresh = [int(g.integers(0, longest)) if i % 9 == 4 else int(g.integers(0, 3)) for i in range(seqs)]
+    fresh[-1] = longest
+    b = Batch([f + int(g.integers(0, 30)) for f in fresh], fresh, 4, 2, 64, 16, dtype, seed=seqs, pad=3)
+    assert (b.check()[-3:] == 7).all()
+    b.check(max_fresh=17, max_len=5)
