@@ -12,7 +12,7 @@ constexpr int MOST_PARTS = 1024, JOIN_WAVES = 4;
 struct PartsOf {
     int parts;
     int64_t base, step, first;
-    __device__ __forceinline__ PartsOf(const Attend& a, const KvSeq& s, int seq, int tok, int head, int per) {
+    __device__ __forceinline__ void set(const Attend& a, const KvSeq& s, int seq, int tok, int head, int per) {
         const unsigned group = a.group, all_rows = (unsigned)s.tokens() * group, r = (unsigned)tok * group + (unsigned)head % group;   // below 2^31
         if (a.chunks) {
             parts = 1;
@@ -50,7 +50,8 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_kernel(Attend a, int 
     const int64_t all_rows = (int64_t)s.tokens() * a.group;
     if ((all_rows <= a.few_rows) != few) return;
     for (int tok = blockIdx.x / a.heads % tokens; tok < s.tokens(); tok += tokens) {
-        const PartsOf of(a, s, seq, tok, head, per);
+        PartsOf of;
+        of.set(a, s, seq, tok, head, per);
         const int parts = of.parts;   // at most MOST_PARTS
         if (parts == 1) continue;
         float m = -INFINITY;
@@ -98,17 +99,18 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_kernel(Attend a, int 
     }
 }
 
-// The same for a few parts: a wave to a row and head. `few`: items are (sequence, one of `tokens`, head); else (row of the batch, head).
-template <typename T, int D>
+// The same for a few parts: a wave to a row and AT heads, whose loads are in flight together. `few`: items are (sequence, one of
+// `tokens`, head); else (row of the batch, heads AT at a time).
+template <typename T, int D, int AT>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_few_parts_kernel(Attend a, int per, bool few, int tokens, int64_t items) {
-    constexpr int PER = D / 64, AHEAD = 8;
+    constexpr int PER = D / 64, AHEAD = AT == 1 ? 8 : 4;
     const int lane = threadIdx.x & 63;
     const int64_t item = (int64_t)blockIdx.x * JOIN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= items) return;
-    const int head = (int)(item % a.heads);
-    int seq = (int)(item / a.heads / tokens), tok = (int)(item / a.heads % tokens);
+    const int of_row = (a.heads + AT - 1) / AT, head0 = AT * (int)(item % of_row);
+    int seq = (int)(item / of_row / tokens), tok = (int)(item / of_row % tokens);
     if (!few) {   // the last sequence that starts at or before the row
-        const int row = (int)(item / a.heads);
+        const int row = (int)(item / of_row);
         seq = 0;
         for (int n = a.seqs; n > 1;) {
             const int step = (n + 63) / 64;
@@ -122,47 +124,75 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_few_parts_kernel(Atte
     const KvSeq s(a, seq);
     if (((int64_t)s.tokens() * a.group <= a.few_rows) != few || tok < 0) return;
     for (; tok < s.tokens(); tok += few ? tokens : 0x40000000) {
-        const PartsOf of(a, s, seq, tok, head, per);
-        const int parts = __builtin_amdgcn_readfirstlane(of.parts);
-        if (parts > 1) {
-            float m = -INFINITY, l = 0.f, acc[PER] = {};
-            for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[of.at(p)].x);
-            for (int p0 = 0; p0 < parts; p0 += AHEAD) {
-                float x[AHEAD][PER];
-                float2 ml[AHEAD];
+        int parts[AT], most = 0;
+        PartsOf of[AT];
+#pragma unroll
+        for (int h = 0; h < AT; ++h) {
+            of[h].set(a, s, seq, tok, min(head0 + h, a.heads - 1), per);
+            parts[h] = head0 + h < a.heads ? __builtin_amdgcn_readfirstlane(of[h].parts) : 0;
+            most = max(most, parts[h]);
+        }
+        if (most < 2) continue;
+        float m[AT], l[AT], acc[AT][PER] = {};
+#pragma unroll
+        for (int h = 0; h < AT; ++h) {
+            m[h] = -INFINITY;
+            l[h] = 0.f;
+        }
+        // sums relative to the largest maximum so far
+        for (int p0 = 0; p0 < most; p0 += AHEAD) {
+            float x[AT][AHEAD][PER];
+            float2 ml[AT][AHEAD];
+#pragma unroll
+            for (int h = 0; h < AT; ++h)
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j)
-                    if (p0 + j < parts) {
-                        const int64_t from = of.at(p0 + j);
-                        ml[j] = a.part_ml[from];
+                    if (p0 + j < parts[h]) {
+                        const int64_t from = of[h].at(p0 + j);
+                        ml[h][j] = a.part_ml[from];
 #pragma unroll
-                        for (int i = 0; i < PER; ++i) x[j][i] = a.part_o[from * D + lane + 64 * i];
+                        for (int i = 0; i < PER; ++i) x[h][j][i] = a.part_o[from * D + lane + 64 * i];
                     }
 #pragma unroll
-                for (int j = 0; j < AHEAD; ++j)
-                    if (p0 + j < parts) {
-                        const float f = ml[j].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[j].x - m);
-                        l += ml[j].x == -INFINITY ? ml[j].y : ml[j].y * f;
+            for (int h = 0; h < AT; ++h) {
+                float now = m[h];
 #pragma unroll
-                        for (int i = 0; i < PER; ++i) acc[i] = fmaf(x[j][i], f, acc[i]);
+                for (int j = 0; j < AHEAD; ++j) now = p0 + j < parts[h] ? fmaxf(now, ml[h][j].x) : now;
+                const float back = m[h] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[h] - now);   // (what has no maximum is zeros, or no number)
+                l[h] *= back;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) acc[h][i] *= back;
+                m[h] = now;
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j)
+                    if (p0 + j < parts[h]) {
+                        const float f = ml[h][j].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[h][j].x - now);
+                        l[h] += ml[h][j].x == -INFINITY ? ml[h][j].y : ml[h][j].y * f;
+#pragma unroll
+                        for (int i = 0; i < PER; ++i) acc[h][i] = fmaf(x[h][j][i], f, acc[h][i]);
                     }
             }
-            T* out = (T*)a.out + (int64_t)(s.first + tok) * a.out_stride + (int64_t)head * D + lane;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) out[64 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
         }
+        T* out = (T*)a.out + (int64_t)(s.first + tok) * a.out_stride + (int64_t)head0 * D + lane;
+#pragma unroll
+        for (int h = 0; h < AT; ++h)
+            if (parts[h] > 1)
+#pragma unroll
+                for (int i = 0; i < PER; ++i) out[h * D + 64 * i] = from_f32<T>(l[h] == 0.f ? 0.f : acc[h][i] / l[h]);
     }
 }
 
 template <typename T, int D>
 static int join_of(const Attend& a, int per, bool few, int tokens, hipStream_t s) {
-    const int64_t items = few ? (int64_t)a.seqs * tokens * a.heads : (int64_t)a.rows * a.heads;
+    constexpr int AT = 4;   // heads of a row together: 700 rows of 32 heads in three parts 17 us, 19 one by one
+    const int64_t items = few ? (int64_t)a.seqs * tokens * a.heads : (int64_t)a.rows * ((a.heads + AT - 1) / AT);
     const bool wide = few && (a.chunks ? a.chunks > 8 * a.seqs : a.splits > 8);   // four waves to a row from nine parts on
     const int64_t blocks = wide ? items : (items + JOIN_WAVES - 1) / JOIN_WAVES;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
     const dim3 grid((unsigned)blocks), threads(64 * JOIN_WAVES);
     if (wide) hipLaunchKernelGGL((kv_join_kernel<T, D>), grid, threads, 0, s, a, per, few, tokens);
-    else hipLaunchKernelGGL((kv_join_few_parts_kernel<T, D>), grid, threads, 0, s, a, per, few, tokens, items);
+    else if (few) hipLaunchKernelGGL((kv_join_few_parts_kernel<T, D, 1>), grid, threads, 0, s, a, per, few, tokens, items);
+    else hipLaunchKernelGGL((kv_join_few_parts_kernel<T, D, AT>), grid, threads, 0, s, a, per, few, tokens, items);
     return lk_launch_status();
 }
 
