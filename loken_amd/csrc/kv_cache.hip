@@ -126,8 +126,8 @@ __global__ __launch_bounds__(PLAN_WG) void kv_plan_kernel(const int32_t* __restr
 //
 // What it costs is latency: slots, then rows and scale, then (where a scale grows) the page. A lane holds four columns of eight
 // consecutive rows, whose loads are all in flight together: four codes of a key row are one store, eight of a value column another.
-// 64 single tokens of 8 heads of 128 in f32: 6 us; 4400 rows in bf16: 10 us. (Slots looked up row by row, with a fence before the new
-// codes: 12 and 51 us.)
+// 64 single tokens of 8 heads of 128 in f32: 6 us; 1504 rows of a prompt in bf16, 16 tokens a page: 8 us. (With slots looked up row by
+// row and a fence before the new codes the single tokens took 12.)
 // ---------------------------------------------------------------------------------------------
 constexpr int ROWS_HELD = 8, WRITE_WAVES = 8;
 
@@ -443,8 +443,9 @@ extern "C" int lk_kv_write_q8(const void* k, const void* v, int type, int64_t k_
         return LK_ERR_ARG;
     const KvPool pool{(int8_t*)k_codes, (int8_t*)v_codes, k_scales, v_scales, pages, kv_heads, kv_log2(page_tokens)};
     // Rows of which a workgroup writes the runs that start there, one after the other: single tokens' runs are a row each, a prompt's a
-    // page.
-    const int window = tokens <= 128 ? 1 : tokens <= 1024 ? 4 : 16;
+    // page, and a workgroup that finds none costs 3 ns. 1504 rows of a prompt in bf16, 16 and 32 rows to a workgroup: 7.7 and 11.3 us
+    // with pages of 16 tokens, 9.2 and 7.7 of 32, 10.1 and 8.3 of 64, 16.2 and 9.9 of 128.
+    const int window = tokens <= 128 ? 1 : tokens <= 1024 ? 4 : page_tokens < 32 ? page_tokens : 32;
     return by_type_and_dim<Write>(type, head_dim, k, v, k_stride, v_stride, slots, tokens, pool, window, (hipStream_t)stream);
 }
 
