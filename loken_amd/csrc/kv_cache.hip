@@ -58,9 +58,9 @@ __global__ __launch_bounds__(PLAN_WG) void kv_plan_kernel(const int32_t* __restr
                                                           int table_cols, int32_t* __restrict__ lens, int32_t* __restrict__ starts,
                                                           int64_t* __restrict__ slots, int32_t* __restrict__ positions, int rows,
                                                           int32_t* __restrict__ taken_out) {
-    extern __shared__ int plan_lds[];   // [seqs] first row, [seqs] first new page
+    extern __shared__ int plan_lds[];   // [seqs] first row, [seqs] first new page, [seqs] past
     __shared__ int64_t meet[PLAN_WG / 64][2];
-    int *row0 = plan_lds, *page0 = plan_lds + seqs;
+    int *row0 = plan_lds, *page0 = plan_lds + seqs, *had = plan_lds + 2 * seqs;
     const int t = threadIdx.x, P = 1 << page_shift;
     const bool writes = blockIdx.x == 0;
     const int per = (seqs + PLAN_WG - 1) / PLAN_WG, i0 = t * per, i1 = min(i0 + per, seqs);
@@ -75,6 +75,7 @@ __global__ __launch_bounds__(PLAN_WG) void kv_plan_kernel(const int32_t* __restr
     for (int i = i0; i < i1; ++i) {
         const int64_t p = max(past[i], 0), f = max(fresh[i], 0);
         row0[i] = clamp_i32(tokens);
+        had[i] = (int)p;
         page0[i] = clamp_i32(pages);
         if (writes) {
             starts[i] = clamp_i32(tokens);
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(PLAN_WG) void kv_plan_kernel(const int32_t* __restr
     const int n_pages = clamp_i32(all_pages), n_rows = clamp_i32(all_tokens);
     for (int64_t j = (int64_t)blockIdx.x * PLAN_WG + t; j < n_pages; j += (int64_t)gridDim.x * PLAN_WG) {
         const int i = last_not_above(page0, seqs, (int)j);
-        const int64_t col = (((int64_t)max(past[i], 0) + P - 1) >> page_shift) + j - page0[i];
+        const int64_t col = (((int64_t)had[i] + P - 1) >> page_shift) + j - page0[i];
         if (col < table_cols) table[i * table_stride + col] = page_of(j);
     }
     // the rows; a new page's number comes from the free list, where no workgroup waits for another's store
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(PLAN_WG) void kv_plan_kernel(const int32_t* __restr
         int64_t slot = -1, at = 0;
         if (r < n_rows) {
             const int i = last_not_above(row0, seqs, (int)r);
-            const int64_t p = max(past[i], 0);
+            const int64_t p = had[i];
             at = p + r - row0[i];
             const int64_t col = at >> page_shift, have = (p + P - 1) >> page_shift;
             if (col < table_cols) {
@@ -420,13 +421,13 @@ extern "C" int lk_kv_plan(const int32_t* past, const int32_t* fresh, int seqs, i
         return LK_ERR_ARG;
     if (seqs > LK_KV_PLAN_SEQS) return LK_ERR_SIZE;
     // a kernel gets 64 KB of LDS unless the runtime is told otherwise
-    if (seqs * 8 > 60 * 1024 &&
-        hipFuncSetAttribute((const void*)kv_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, seqs * 8) != hipSuccess) {
+    if (seqs * 12 > 60 * 1024 &&
+        hipFuncSetAttribute((const void*)kv_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, seqs * 12) != hipSuccess) {
         (void)hipGetLastError();
         return LK_ERR_LAUNCH;
     }
     const int blocks = rows > 0 ? (rows + PLAN_ROWS - 1) / PLAN_ROWS : 1;
-    hipLaunchKernelGGL(kv_plan_kernel, dim3(blocks), dim3(PLAN_WG), seqs * 8, (hipStream_t)stream, past, fresh, seqs, kv_log2(page_tokens),
+    hipLaunchKernelGGL(kv_plan_kernel, dim3(blocks), dim3(PLAN_WG), seqs * 12, (hipStream_t)stream, past, fresh, seqs, kv_log2(page_tokens),
                        free_pages, n_free, taken, table, table_stride, table_cols, lens, starts, slots, positions, rows, taken_out);
     return lk_launch_status();
 }
