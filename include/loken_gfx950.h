@@ -816,9 +816,11 @@ int lk_kv_read_q8(const int64_t* slots, int tokens, int kv_heads, int head_dim, 
  * leaving out positions whose page is absent. A row that sees none gives zeros, one whose q holds a value that is not finite gives
  * values that are not numbers. Rows behind the last sequence are left as they were. `out` has q's type, out_stride elements from row
  * to row; it does not overlap q. max_fresh and max_len: the most rows and the most tokens of a sequence as the caller knows
- * them; they choose launch shapes only, a sequence with more is served too. table_cols * page_tokens up to 2^31 - 1024 and rows * heads / kv_heads up to
- * 2^31 - 1, else LK_ERR_SIZE.
- * Scores, softmax and sums are held in f32 (sums of products of codes in int32 as long as they are exact). Partial results of a
+ * them; they choose launch shapes only, a sequence with more is served too. table_cols * page_tokens up to 2^31 - 1024 and
+ * rows * heads / kv_heads up to 2^31 - 1, else LK_ERR_SIZE.
+ * Scores, softmax and sums are held in f32 (sums of products of codes in int32 as long as they are exact). In the products a
+ * query value of f32 is held to 2^-22 of its row's largest, one of f16 or bf16 to 2^-15, and a softmax weight to as much of the largest of
+ * 64 positions, or as f16 (f32: as two). Partial results of a
  * context that is split over workgroups go through scratch of the stream (LK_ERR_NOMEM where there is none; while a
  * graph is recorded, where no call outside a recording has needed as much). */
 int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, void* out, int64_t out_stride, const void* k_codes,
@@ -842,7 +844,7 @@ int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, void* out, int
 int lk_sample(const void* logits, int type, int64_t stride, int rows, int vocab, const float* uniform, const float* temperature,
               const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, float* probs, void* stream);
 
-/* Frees what the expert launchers, the expert block, the router and the f16 tiles hold on the current device, for
+/* Frees what the expert launchers, the expert block, the router, the f16 tiles, attention and sampling hold on the current device, for
  * every stream and every recorded graph: none recorded over them may be replayed after. The host linears' workspaces
  * stay (lkh_release_workspaces). Synchronizes the device (cuda/moe/moe_gguf.cu:104-118). */
 void loken_stream_scratch_release(void);
