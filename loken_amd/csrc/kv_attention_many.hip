@@ -21,8 +21,8 @@
 // A wave's step is 32 products of 32 cycles (twice as many in f32) and some 400 other instructions, 32 of them exponentials, which
 // take four times as long. It is these that bound it, and what of them does not run beside products: so a product comes with
 // six of them in turn, its operands read from LDS a group ahead, and nothing that is loaded is looked at before the step after.
-// 2048 tokens of one prompt, 32 heads over 8 of 128 bf16 values: 69 us, 500 TFLOP/s of the causal half's products; 700 f32 rows over
-// 2200 positions beside eleven single rows: 109 us.
+// 2048 tokens of one prompt, 32 heads over 8 of 128 bf16 values: 69 us, 500 TFLOP/s of the causal half's products (two starts of 5 us a
+// CU in it); the same behind 16384 tokens 683 us, 850 TFLOP/s, in f32 1060; 700 f32 rows over 2200 positions beside eleven single rows: 108 us.
 
 #include "kv_attention.h"
 
@@ -314,7 +314,6 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
             // a wave whose rows see nothing of the step leaves it
             const bool sees = is && base <= pos_most && (a.window == 0 || base + KV_TILE - 1 > pos_least - a.window);
             v16f x[2];
-            float by[RUNS];
             // First the scores, and the next step's codes into LDS meanwhile; then those of the step after it on their way. (f32 has no
             // registers for that: its next step's codes are loaded here and put into LDS at the end. 142 us against 164.)
             if (sees) {
@@ -334,33 +333,31 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
 #pragma unroll
                             for (int p = 0; p < M::PARTS; ++p) x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk, q[p][k], x[u], 0, 0, 0);
                         }
-                } else {
-                // a few products at a time, the next ones' operands on their way from LDS
-                constexpr int K_AT = M::FINE ? 1 : 2, TURNS = M::KS / K_AT, EACH = TURNS / (2 * M::CHUNKS);
-                h8 kk[2][2 * K_AT];
-                auto operands = [&](int i) {
+                } else {   // four products at a time, the next ones' operands on their way from LDS
+                    constexpr int FOURS = M::KS / 2;
+                    static_assert(FOURS == 2 * M::CHUNKS);
+                    h8 kk[2][4];
+                    auto operands = [&](int i) {
 #pragma unroll
-                    for (int j = 0; j < 2 * K_AT; ++j) kk[i & 1][j] = *(const h8*)(kr + 32 * (j & 1) * M::K_PITCH + 32 * (K_AT * i + j / 2));
-                };
-                operands(0);
+                        for (int j = 0; j < 4; ++j) kk[i & 1][j] = *(const h8*)(kr + 32 * (j & 1) * M::K_PITCH + 32 * (2 * i + j / 2));
+                    };
+                    operands(0);
 #pragma unroll
-                for (int i = 0; i < TURNS; ++i) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (i + 1 < TURNS) operands(i + 1);
-                    if (i % EACH == EACH - 1) store_chunk(t + 1, i / EACH);
+                    for (int i = 0; i < FOURS; ++i) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i + 1 < FOURS) operands(i + 1);
+                        store_chunk(t + 1, i);
 #pragma unroll
-                    for (int j = 0; j < 2 * K_AT; ++j)
+                        for (int j = 0; j < 4; ++j) x[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk[i & 1][j], q[0][2 * i + j / 2], x[j & 1], 0, 0, 0);
+                        if (i + 1 < FOURS) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-                        for (int p = 0; p < M::PARTS; ++p) x[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk[i & 1][j], q[p][K_AT * i + j / 2], x[j & 1], 0, 0, 0);
-                    if (i + 1 < TURNS) __builtin_amdgcn_sched_group_barrier(0x100, 2 * K_AT, 0);
-#pragma unroll
-                    for (int j = 0; j < 2 * K_AT * M::PARTS; ++j) {
-                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                        for (int j = 0; j < 4; ++j) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                        }
+                        __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);
                     }
-                    __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             } else if (!M::FINE) store(t + 1);
             if (!M::FINE) {
@@ -376,7 +373,7 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
             if (sees) {
                 // scores in powers of two; element e of x[u]: position base + 32 u + 16 (e / 8) + 8 half + e % 8
                 const bool whole = base + KV_TILE - 1 <= pos_least && (a.window == 0 || base > pos_most - a.window) && !st.absent;
-                float top = -INFINITY;
+                float by[RUNS], top = -INFINITY;
 #pragma unroll
                 for (int n = 0; n < RUNS; ++n) by[n] = st.ks[n] * unit;
                 if (!whole) {
@@ -410,19 +407,16 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                     for (int b = 0; b < M::NB; ++b) o[b] *= keep;
                     m = m_new;
                 }
+                const float m_base = m == -INFINITY ? 0.f : m;
                 if (st.dead) {   // positions of pages without values: in the sum of weights only
-                    const float m_base = m == -INFINITY ? 0.f : m;
 #pragma unroll
                     for (int n = 0; n < RUNS; ++n)
                         if (st.dead >> n & 1)
 #pragma unroll
                             for (int e = 0; e < 8; ++e) l += __builtin_amdgcn_exp2f(fmaf(x[n / 2][8 * (n % 2) + e], by[n], -m_base));
                 }
-            }
-            // then the weights and sums
-            if (sees) {
+                // then the weights and sums
                 const uint8_t* vl = v_lds(t & 1);
-                const float m_base = m == -INFINITY ? 0.f : m;
                 h8 w[2][M::PARTS], vv[2][M::NB];
                 auto operands = [&](int n) {
 #pragma unroll
