@@ -839,7 +839,8 @@ int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, void* out, int
  * sum; tokens[r] its number, probs[r] (nullable) its weight over that sum. temperature <= 0 (or not a number): the first word of the order,
  * probability 1. A row without words: -1 and 0. Arrays top_k, top_p, min_p may be null (no such rule).
  * Weights are summed as integers of 2^-42, so results do not depend on the order of execution; a word whose weight
- * rounds to none is not drawn. vocab up to LK_SAMPLE_VOCAB, else LK_ERR_SIZE. */
+ * rounds to none is not drawn. vocab up to LK_SAMPLE_VOCAB, else LK_ERR_SIZE; up to 65535 rows, else LK_ERR_ARG. Works in scratch of
+ * the stream, as attention does. */
 #define LK_SAMPLE_VOCAB (1 << 20)
 int lk_sample(const void* logits, int type, int64_t stride, int rows, int vocab, const float* uniform, const float* temperature,
               const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, float* probs, void* stream);

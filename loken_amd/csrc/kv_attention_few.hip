@@ -32,6 +32,8 @@ struct Few {
     static constexpr int PER = DIGITS == 3 ? 1 : 2;     // rows whose sums a lane holds, per operand
     // The largest numbers the digits are made of. They hold 127 * (65536 + 256 + 1) and 127 * (256 + 1); the first leaves room for a last place of f32.
     static constexpr float Q_MAX = DIGITS == 3 ? 127.f * 65536 : 127.f * 256 + 127;
+    static constexpr int Q_BITS = DIGITS == 3 ? 23 : 15;   // Q_MAX is just below 2^Q_BITS
+    static constexpr float Q_ROUND = 1 << Q_BITS;
     static constexpr float P_MAX = DIGITS == 3 ? 63.f * 65536 + 127 * 256 + 127 : 127.f * 256 + 127;   // below 2^22: see cut()
     static constexpr int BALANCE = DIGITS == 3 ? 0x808080 : 0x8080;
 };
@@ -190,11 +192,11 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 && !(D == 128 && NT == 2) ? 2 :
             most = max(most, (uint32_t)__shfl_xor((int)most, 16));
             most = max(most, (uint32_t)__shfl_xor((int)most, 32));
             const bool finite = most < 0x7F800000u;
-            const float largest = __uint_as_float(most);
             int e2 = 0;
-            const float mant = frexpf(finite && most ? largest : 1.f, &e2);   // in [1/2, 1)
+            const float mant = frexpf(finite && most ? __uint_as_float(most) : 1.f, &e2);   // in [1/2, 1)
             const float f = F::Q_MAX / mant;
-            unit[n] = finite ? (largest * a.scale) * (1.4426950408889634f / F::Q_MAX) : NAN;
+            // (the row's power of two last: what it makes up for may be far from one)
+            unit[n] = finite ? ldexpf(mant * (a.scale * (1.4426950408889634f * F::Q_ROUND / F::Q_MAX)), e2 - F::Q_BITS) : NAN;
 #pragma unroll
             for (int kk = 0; kk < F::KK; ++kk) {
                 uint32_t w[4];

@@ -714,6 +714,8 @@ def decode_1p7b(args, dev):
                              (ops.mmq_fixup(dev).data_ptr(), w.data_ptr(), ws.data_ptr(), out.data_ptr(), k, n, b, k // 256, n, info["cc"],
                               info["nsm"], info["smpbo"], info["warp_size"], s)))
 
+    if args.context < 0:
+        raise SystemExit("--context: tokens of a sequence, 0 or more")
     between = Between(b, args.context, hidden // HEAD_DIM, kv // HEAD_DIM, mk) if args.context else None
     if between:
         plan.append(between.plan_item(s))

@@ -272,3 +272,18 @@ def test_long_and_short_sequences_of_a_batch(seqs, longest, dtype):
     b = Batch([f + int(g.integers(0, 30)) for f in fresh], fresh, 4, 2, 64, 16, dtype, seed=seqs, pad=3)
     assert (b.check()[-3:] == 7).all()
     b.check(max_fresh=17, max_len=5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fresh", [1, 30])
+def test_queries_whose_scale_alone_would_overflow(fresh, dtype):
+    """Scores of ordinary size from queries at the end of the type's range and keys at the beginning of it."""
+    b = Batch([200], [fresh], 4, 2, 64, 16, dtype, seed=31)
+    g = np.random.default_rng(31)
+    shape = b.want.scales["k"].shape
+    b.want.codes["k"] = g.integers(-3, 4, b.want.codes["k"].shape)
+    b.want.scales["k"] = g.uniform(1.2e-38, 2e-38, shape).astype(np.float32)
+    b.q = (b.q.float() * 7e37).clamp(-3e38, 3e38)
+    b.q[..., 5] = 3e38
+    b.q = b.q.to(TYPES[dtype])
+    b.check(scale=1.3)
