@@ -75,7 +75,7 @@ def attention_args(**change):
     (dict(scale=math.inf), lib.LK_ERR_ARG), (dict(window=-1), lib.LK_ERR_ARG), (dict(fresh=-1), lib.LK_ERR_ARG), (dict(len=-1), lib.LK_ERR_ARG),
     (dict(rows=-1), lib.LK_ERR_ARG), (dict(seqs=-1), lib.LK_ERR_ARG), (dict(stride=4), lib.LK_ERR_ARG), (dict(q=None), lib.LK_ERR_ARG),
     (dict(out=P + 2), lib.LK_ERR_ARG), (dict(lens=None), lib.LK_ERR_ARG), (dict(starts=None), lib.LK_ERR_ARG), (dict(table=None), lib.LK_ERR_ARG),
-    (dict(cols=1 << 27, stride=1 << 27), lib.LK_ERR_SIZE), (dict(rows=0), lib.LK_OK), (dict(seqs=0), lib.LK_OK)])
+    (dict(cols=1 << 27, stride=1 << 27), lib.LK_ERR_SIZE), (dict(rows=1 << 30), lib.LK_ERR_SIZE), (dict(rows=0), lib.LK_OK), (dict(seqs=0), lib.LK_OK)])
 def test_attention(change, status):
     assert lib.load().lk_kv_attention_q8(*attention_args(**change)) == status
 
