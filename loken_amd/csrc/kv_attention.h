@@ -29,6 +29,10 @@ struct Attend {
     int chunks;
     // The few-rows kernel takes the sequences of up to so many rows (token, head of the group), the other kernel the rest.
     int few_rows;
+    // Row / group for rows below 2^31: ceil(2^shift / group), shift = 31 + ceil(log2 group).
+    uint32_t group_inverse;
+    int group_shift;
+    __device__ __forceinline__ int token_of(unsigned row) const { return (int)(((uint64_t)row * group_inverse) >> group_shift); }
     __device__ __forceinline__ int64_t part_row(int seq, const struct KvSeq& s, int row) const;
 };
 
@@ -60,9 +64,12 @@ struct KvSpan {
         hi = (int)max((int64_t)0, min(pb + 1, s.limit));
         lo = a.window > 0 ? (int)max((int64_t)0, pa - a.window + 1) & ~(KV_TILE - 1) : 0;
         tiles = hi > lo ? (hi - lo + KV_TILE - 1) / KV_TILE : 0;
-        const bool whole = a.splits == 1 || (a.part_seq && s.tokens() > a.part_seq);
-        per_part = whole ? max(tiles, 1) : max(a.least_tiles, (tiles + a.splits - 1) / a.splits);
-        parts = max(1, (tiles + per_part - 1) / per_part);
+        per_part = max(tiles, 1);
+        parts = 1;
+        if (a.splits > 1 && !(a.part_seq && s.tokens() > a.part_seq)) {
+            per_part = max(a.least_tiles, (tiles + a.splits - 1) / a.splits);
+            parts = max(1, (tiles + per_part - 1) / per_part);
+        }
     }
 };
 

@@ -13,7 +13,7 @@ struct PartsOf {
     int parts;
     int64_t base, step, first;
     __device__ __forceinline__ void set(const Attend& a, const KvSeq& s, int seq, int tok, int head, int per) {
-        const unsigned group = a.group, all_rows = (unsigned)s.tokens() * group, r = (unsigned)tok * group + (unsigned)head % group;   // below 2^31
+        const unsigned group = a.group, all_rows = (unsigned)s.tokens() * group, r = (unsigned)tok * group + (head - a.token_of(head) * group);   // below 2^31
         if (a.chunks) {
             parts = 1;
             base = step = first = 0;
@@ -23,13 +23,13 @@ struct PartsOf {
             const int c0 = at / pieces.length, c1 = (at + steps - 1) / pieces.length;
             parts = c1 - c0 + 1;
             // the piece that the sequence starts in has it second, the others first
-            base = ((int64_t)((unsigned)head / group) * a.chunks + c0) * 2 * per + r;
+            base = ((int64_t)a.token_of(head) * a.chunks + c0) * 2 * per + r;
             step = 2 * per;
             first = per;
             return;
         }
         const unsigned r0 = r / per * per, r1 = min(r0 + per, all_rows) - 1;
-        parts = KvSpan(a, s, s.first + (int)(r0 / group), s.first + (int)(r1 / group)).parts;
+        parts = KvSpan(a, s, s.first + a.token_of(r0), s.first + a.token_of(r1)).parts;
         base = (a.part_row(seq, s, s.first + tok) * a.heads + head) * a.splits;
         step = 1;
         first = 0;
@@ -234,8 +234,11 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     if ((int64_t)table_cols * page_tokens > 0x7FFFFC00 || (int64_t)rows * (heads / kv_heads) > 0x7FFFFFFF) return LK_ERR_SIZE;   // positions and what is added to them fit 32 bits
     hipStream_t s = (hipStream_t)stream;
     const int group = heads / kv_heads;
+    int group_shift = 31;
+    while ((1 << (group_shift - 31)) < group) ++group_shift;
     const Attend a{q, out, q_stride, out_stride, {(int8_t*)k_codes, (int8_t*)v_codes, (float*)k_scales, (float*)v_scales, pages, kv_heads, kv_log2(page_tokens)},
-                   table, lens, starts, table_stride, table_cols, seqs, rows, heads, group, window, scale, (((uintptr_t)q | (uintptr_t)(q_stride * size)) & 15) == 0, 1, 1, 0, nullptr, nullptr, 0, 0};
+                   table, lens, starts, table_stride, table_cols, seqs, rows, heads, group, window, scale, (((uintptr_t)q | (uintptr_t)(q_stride * size)) & 15) == 0, 1, 1, 0, nullptr, nullptr, 0, 0,
+                   (uint32_t)(((1ull << group_shift) + group - 1) / group), group_shift};
     // What the caller says of the sizes chooses launches; whatever the sequences are, one of the kernels takes each.
     const int tokens = max_fresh < 1 ? 1 : max_fresh < rows ? max_fresh : rows;
     const int64_t most_rows = (int64_t)tokens * group;

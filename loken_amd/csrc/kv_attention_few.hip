@@ -103,7 +103,7 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 && !(D == 128 && NT == 2) ? 2 :
       const int all_rows = (int)rows_of_all;
       for (int tile = tile0; tile * F::ROWS < all_rows; tile += row_tiles) {
         const int r0 = tile * F::ROWS, r1 = min(r0 + F::ROWS, all_rows) - 1;
-        const KvSpan span(a, s, s.first + r0 / a.group, s.first + r1 / a.group);
+        const KvSpan span(a, s, s.first + a.token_of(r0), s.first + a.token_of(r1));
         int t_begin = 0, t_end = span.tiles;
         int64_t to = -1;   // the first row of the sums' place among the parts; -1: they are not a part
         if (a.chunks) {
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 && !(D == 128 && NT == 2) ? 2 :
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int r = r0 + n * F::RPT + i / F::SLOTS;
-            const int tok = s.first + min(r, r1) / a.group, head = kv * a.group + min(r, r1) % a.group;
+            const int of_seq = a.token_of(min(r, r1)), tok = s.first + of_seq, head = kv * a.group + min(r, r1) - of_seq * a.group;
             pos[n] = r <= r1 ? (int)max(s.pos_of_0 + tok, (int64_t)-1) : -1;
             const T* row = (const T*)a.q + tok * a.q_stride + (int64_t)head * D + 16 * g;
             float x[F::KK][16];
@@ -363,8 +363,8 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 && !(D == 128 && NT == 2) ? 2 :
                 // (a part whose scores are no numbers has no maximum and a sum that is none)
                 lw += tops[w][r] == -INFINITY ? weights[w][r] : weights[w][r] * __builtin_amdgcn_exp2f(tops[w][r] - top);
             }
-            const int64_t row = s.first + (r0 + r) / a.group;
-            const int head = kv * a.group + (r0 + r) % a.group;
+            const int of_seq = a.token_of(r0 + r), head = kv * a.group + r0 + r - of_seq * a.group;
+            const int64_t row = s.first + of_seq;
             if (to < 0) {
                 ((T*)a.out)[row * a.out_stride + (int64_t)head * D + d] = from_f32<T>(lw == 0.f ? 0.f : total / lw);
             } else {

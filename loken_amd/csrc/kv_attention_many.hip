@@ -164,9 +164,9 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
     auto v_lds = [&](int buffer) { return lds + buffer * (M::K_BYTES + M::V_BYTES) + M::K_BYTES; };
 
     for (uint64_t tile = tile0; tile * KV_MANY_ROWS < all_rows; tile += row_tiles) {
-        const unsigned r_tile = (unsigned)tile * KV_MANY_ROWS, group = a.group;
+        const unsigned r_tile = (unsigned)tile * KV_MANY_ROWS;
         const unsigned r_end = min(r_tile + KV_MANY_ROWS, all_rows);
-        const KvSpan span(a, s, s.first + (int)(r_tile / group), s.first + (int)((r_end - 1) / group));
+        const KvSpan span(a, s, s.first + a.token_of(r_tile), s.first + a.token_of(r_end - 1));
         const int per_part = span.per_part, parts = span.parts;
         if (part >= parts) continue;
         // a team has every other step; steps are counted from its first
@@ -178,10 +178,10 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
         const unsigned r = r_tile + 32 * wave + col;
         const bool row_is = r < r_end;
         const unsigned r_in = min(r, r_end - 1);
-        const int tok = s.first + (int)(r_in / group), head = kv * (int)group + (int)(r_in % group);
+        const int of_seq = a.token_of(r_in), tok = s.first + of_seq, head = kv * a.group + (int)r_in - of_seq * a.group;
         const int pos = (int)max(s.pos_of_0 + tok, (int64_t)-1);
         const unsigned w0 = min(r_tile + 32 * wave, r_end - 1), w1 = min(r_tile + 32 * wave + 31, r_end - 1);
-        const int pos_least = (int)max(s.pos_of_0 + s.first + w0 / group, (int64_t)-1), pos_most = (int)max(s.pos_of_0 + s.first + w1 / group, (int64_t)-1);
+        const int pos_least = (int)max(s.pos_of_0 + s.first + a.token_of(w0), (int64_t)-1), pos_most = (int)max(s.pos_of_0 + s.first + a.token_of(w1), (int64_t)-1);
 
         struct __attribute__((packed, aligned(sizeof(T)))) Eight { T of[8]; };   // (a row's alignment is its type's)
         const Eight* row = (const Eight*)((const T*)a.q + tok * a.q_stride + (int64_t)head * D + 8 * half);
