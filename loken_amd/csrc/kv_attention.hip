@@ -184,14 +184,18 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void kv_join_few_parts_kernel(Atte
 
 template <typename T, int D>
 static int join_of(const Attend& a, int per, bool few, int tokens, hipStream_t s) {
-    constexpr int AT = 4;   // heads of a row together: 700 rows of 32 heads in three parts 17 us, 19 one by one
-    const int64_t items = few ? (int64_t)a.seqs * tokens * a.heads : (int64_t)a.rows * ((a.heads + AT - 1) / AT);
+    // Heads of a row together where there are more rows and heads than waves run at once: 700 rows of 32 heads in three parts 15 us, 18
+    // one by one; 64 rows behind 4096 tokens
+    // (32 us in all) four longer that way
+    constexpr int AT = 4;
+    const bool together = !few && (int64_t)a.rows * a.heads > 32 * lk_device().cus;
+    const int64_t items = few ? (int64_t)a.seqs * tokens * a.heads : (int64_t)a.rows * (together ? (a.heads + AT - 1) / AT : a.heads);
     const bool wide = few && (a.chunks ? a.chunks > 8 * a.seqs : a.splits > 8);   // four waves to a row from nine parts on
     const int64_t blocks = wide ? items : (items + JOIN_WAVES - 1) / JOIN_WAVES;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
     const dim3 grid((unsigned)blocks), threads(64 * JOIN_WAVES);
     if (wide) hipLaunchKernelGGL((kv_join_kernel<T, D>), grid, threads, 0, s, a, per, few, tokens);
-    else if (few) hipLaunchKernelGGL((kv_join_few_parts_kernel<T, D, 1>), grid, threads, 0, s, a, per, few, tokens, items);
+    else if (!together) hipLaunchKernelGGL((kv_join_few_parts_kernel<T, D, 1>), grid, threads, 0, s, a, per, few, tokens, items);
     else hipLaunchKernelGGL((kv_join_few_parts_kernel<T, D, AT>), grid, threads, 0, s, a, per, few, tokens, items);
     return lk_launch_status();
 }
