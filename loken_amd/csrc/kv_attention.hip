@@ -217,6 +217,31 @@ static void cut(Attend& a, int64_t groups, int tiles, int want, int least) {
     a.least_tiles = tiles > a.splits ? (tiles + a.splits - 1) / a.splits : 1;
 }
 
+// Parts of the many-rows kernel's contexts, of `tiles` steps for `groups` row tiles and heads: those that take the least time where
+// a workgroup takes 6 us to start and `step` us a step, as many at once as the CUs hold, and each row and head's part 0.35 ns to be stored
+// and joined, 4 us in all beside. In bf16 (us measured, and by this rule's sum): 64 rows behind 4096 tokens 5 / 9 / 17 parts 32 / 29 / 38
+// (30 / 26 / 38); 200 behind 4096 5 / 9 parts 59 / 52 (62 / 55), both more than one round; four sequences of 500 behind 1000 whole / in two
+// 79 / 144 (73 / 134).
+static void cut_many(Attend& a, int64_t groups, int tiles, bool f32, int head_dim, int cus) {
+    const int64_t slots = (int64_t)cus * (f32 && head_dim < 256 ? 2 : 1);
+    const double rows = (double)a.rows * a.heads;
+    double least = 1e30;
+    for (int parts = 1, of = 0; parts <= 64 && parts <= tiles / 2 + 1; ++parts) {
+        const int per = (tiles + parts - 1) / parts;
+        if (per == of) continue;
+        of = per;
+        const int64_t rounds = (groups * parts + slots - 1) / slots;
+        // f32 of up to 128 columns: two workgroups to a CU, each slower for it
+        const double step = head_dim == 256 ? (f32 ? 8.0 : 4.8) : (!f32 ? 1.28 : groups * parts <= cus ? 2.8 : 3.6) * head_dim / 128;
+        const double time = (double)rounds * (per * step + 6.0) + (parts > 1 ? 4.0 + rows * parts * 0.35e-3 : 0.0);
+        if (time < least) {
+            least = time;
+            a.splits = parts;
+            a.least_tiles = per > 1 ? per : 1;
+        }
+    }
+}
+
 }  // namespace
 
 extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, void* out, int64_t out_stride, const void* k_codes,
@@ -277,11 +302,7 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     int64_t part_rows_m = 0;
     if (many) {
         am.few_rows = few ? FEW_ROWS : 0;
-// Parts of at least 16 steps until there are two workgroups to a CU, and, where every CU has one as it is, of at least 64. 512
-        // bf16 rows behind 4096 tokens: 81 us, with parts of 8 steps and twice as many 106; four sequences of 500 rows behind 1000: 79 us,
-        // in two parts each 144.
-        const int64_t groups = ((int64_t)rows * group + KV_MANY_ROWS - 1) / KV_MANY_ROWS * kv_heads;
-        cut(am, groups, tiles, 2 * cus, groups < cus ? 16 : 64);
+        cut_many(am, ((int64_t)rows * group + KV_MANY_ROWS - 1) / KV_MANY_ROWS * kv_heads, tiles, type == LK_TYPE_F32, head_dim, cus);
         if (am.splits > 1) part_rows_m = (int64_t)rows * heads * am.splits;
     }
     LkScratch scratch(s);
