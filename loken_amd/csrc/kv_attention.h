@@ -43,8 +43,9 @@ struct KvSeq {
     int64_t limit;         // positions that the table has columns for
     __device__ __forceinline__ KvSeq(const Attend& a, int seq) {
         const int s = a.starts[seq], e = a.starts[seq + 1];
-        first = max(s, 0);
-        end = min(e, a.rows);
+        // both within the batch, whatever stands there: a difference of what does not would pass 32 bits
+        first = min(max(s, 0), a.rows);
+        end = min(max(e, 0), a.rows);
         pos_of_0 = (int64_t)a.lens[seq] - e;
         limit = (int64_t)a.table_cols << a.pool.page_shift;
     }

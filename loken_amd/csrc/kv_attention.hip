@@ -20,7 +20,7 @@ struct PartsOf {
             if ((int)all_rows > per) return;
             const KvPieces pieces(a, per);
             const int at = KvPieces::first_of(a, per, seq), steps = kv_steps_of(a, seq, per);
-            const int c0 = at / pieces.length, c1 = (at + steps - 1) / pieces.length;
+            const int c0 = min(at / pieces.length, a.chunks - 1), c1 = min((at + steps - 1) / pieces.length, a.chunks - 1);
             parts = c1 - c0 + 1;
             // the piece that the sequence starts in has it second, the others first
             base = ((int64_t)a.token_of(head) * a.chunks + c0) * 2 * per + r;

@@ -287,3 +287,17 @@ def test_queries_whose_scale_alone_would_overflow(fresh, dtype):
     b.q[..., 5] = 3e38
     b.q = b.q.to(TYPES[dtype])
     b.check(scale=1.3)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("hint", [1, 40])
+def test_first_rows_far_outside_the_batch(hint, dtype):
+    """Rows that a sequence claims are those of the batch at most, whatever `starts` holds: one that ends before it starts has none,
+    even where the difference passes 32 bits; one whose positions are all below zero sees nothing."""
+    b = Batch([300, 200, 100], [0, 0, 0], 4, 2, 64, 16, dtype, pad=40)
+    out = torch.full((b.rows, b.heads, b.dim), 7.0, dtype=TYPES[dtype], device="cuda")
+    for starts, want in (([2000000000, -2000000000, -2147483648, -2147483648], 7.0), ([2147483647, -2147483648, 2147483647, -2147483648], 0.0),
+                         ([2147483647, -5, -2147483648, 0], 7.0)):
+        out.fill_(7.0)
+        kv.kv_attention(b.q.cuda(), b.cache(), i32(b.table), i32(b.lens), i32(starts), max_fresh=hint, max_len=300, out=out)
+        assert (out == want).all()
