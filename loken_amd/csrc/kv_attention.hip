@@ -302,7 +302,9 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     int64_t part_rows_m = 0;
     if (many) {
         am.few_rows = few ? FEW_ROWS : 0;
-        cut_many(am, ((int64_t)rows * group + KV_MANY_ROWS - 1) / KV_MANY_ROWS * kv_heads, tiles, type == LK_TYPE_F32, head_dim, cus);
+        // as many sequences as fill the batch with the most rows that one has
+        const int64_t long_seqs = min((int64_t)seqs, (rows + (int64_t)tokens / 2) / tokens);
+        cut_many(am, long_seqs * ((max_rows - 1) / KV_MANY_ROWS + 1) * kv_heads, tiles, type == LK_TYPE_F32, head_dim, cus);
         if (am.splits > 1) part_rows_m = (int64_t)rows * heads * am.splits;
     }
     LkScratch scratch(s);
