@@ -277,34 +277,40 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     const int64_t seen = window > 0 && window < max_len ? (int64_t)window + tokens : max_len;
     const int tiles = (int)((min(seen, table_tokens) + KV_TILE - 1) / KV_TILE);
     Attend af = a, am = a;
-    const int few_max = many ? FEW_ROWS : max_rows, few_per = kv_few_rows(type == LK_TYPE_F32, head_dim, few_max);
+    const bool f32 = type == LK_TYPE_F32;
+    // Beside a sequence of many rows the few-rows kernel takes what one of its workgroups holds, if that is a token's.
+    const int one_wg = kv_few_rows(f32, head_dim, FEW_ROWS), few_limit = group <= one_wg ? one_wg : FEW_ROWS;
+    const int few_max = many ? few_limit : max_rows, few_per = kv_few_rows(f32, head_dim, few_max);
     const int cus = lk_device().cus;
+    // Workgroups of the few-rows kernel that run at once: one to a CU where its registers leave a SIMD one wave. 64 sequences of 4000
+    // tokens, 32 heads over 4 of 128 f32 values, in pieces or parts for one / two to a CU: 55 / 71 us; eight of them 18 / 26.
+    const int few_slots = head_dim == 256 || (head_dim == 128 && few_per > kv_few_rows(f32, head_dim, 1)) ? cus : 2 * cus;
     if (few) {
-        af.few_rows = many ? FEW_ROWS : 0x7FFFFFFF;
+        af.few_rows = many ? few_limit : 0x7FFFFFFF;
         const int64_t groups = (int64_t)seqs * kv_heads * ((few_max + few_per - 1) / few_per);
-        // Long contexts of several sequences whose rows fit a workgroup each: pieces of equal length, two to a CU (as many as run at
-        // once). 64 sequences of 1 to 8010 tokens, 32 heads over 8 of 128 f32 values: 116 us against 139 with parts per sequence; all of
+        // Long contexts of several sequences whose rows fit a workgroup each: pieces of equal length, as many as run at
+        // once. 64 sequences of 1 to 8010 tokens, 32 heads over 8 of 128 f32 values: 116 us against 139 with parts per sequence; all of
         // 4096 104 against 107. With more than four heads and sequences to a CU parts per sequence balance by themselves (256 of 1024
         // tokens: 108 us, 121 in pieces, whose every sequence costs a start of 3 us).
         const int64_t most_steps = (int64_t)seqs * ((table_tokens + KV_TILE - 1) / KV_TILE + 1);
         if (seqs > 1 && few_max <= few_per && groups <= 4 * cus && groups * tiles > 16 * cus && most_steps < 0x7FFFFFFF) {
-            af.chunks = (2 * cus + kv_heads - 1) / kv_heads;
+            af.chunks = (few_slots + kv_heads - 1) / kv_heads;
             af.least_tiles = 4;
         } else {
             // A context of up to 1024 positions stays in one launch; a longer one in parts of at least a step for each wave. One sequence
             // of 1024 / 2048 / 8192 tokens: 12.1 / 13.6 / 13.9 us a call, with parts of 16 steps 12.0 / 16.7 / 17.9, of 4 steps from
             // the start 13.8 / 13.6 / 13.9.
-            cut(af, groups, tiles, 2 * cus, tiles <= 16 ? 16 : 4);
-            af.part_seq = many ? FEW_ROWS / group : tokens;
+            cut(af, groups, tiles, few_slots, tiles <= 16 ? 16 : 4);
+            af.part_seq = many ? few_limit / group : tokens;
         }
     }
     const int64_t part_rows_f = !few ? 0 : af.chunks ? (int64_t)kv_heads * af.chunks * 2 * few_per : af.splits > 1 ? (int64_t)seqs * af.part_seq * heads * af.splits : 0;
     int64_t part_rows_m = 0;
     if (many) {
-        am.few_rows = few ? FEW_ROWS : 0;
+        am.few_rows = few ? few_limit : 0;
         // as many sequences as fill the batch with the most rows that one has
         const int64_t long_seqs = min((int64_t)seqs, (rows + (int64_t)tokens / 2) / tokens);
-        cut_many(am, long_seqs * ((max_rows - 1) / KV_MANY_ROWS + 1) * kv_heads, tiles, type == LK_TYPE_F32, head_dim, cus);
+        cut_many(am, long_seqs * ((max_rows - 1) / KV_MANY_ROWS + 1) * kv_heads, tiles, f32, head_dim, cus);
         if (am.splits > 1) part_rows_m = (int64_t)rows * heads * am.splits;
     }
     LkScratch scratch(s);
@@ -326,6 +332,6 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
     if (many) status = kv_attention_many(am, type, head_dim, max_rows, s);
     if (status == LK_OK && few) status = kv_attention_few(af, type, head_dim, few_max, s);
     if (status == LK_OK && part_rows_m) status = join_parts(am, KV_MANY_ROWS, false, tokens);
-    if (status == LK_OK && part_rows_f) status = join_parts(af, few_per, true, many ? FEW_ROWS / group : tokens);
+    if (status == LK_OK && part_rows_f) status = join_parts(af, few_per, true, many ? few_limit / group : tokens);
     return status;
 }
