@@ -683,7 +683,8 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
     const int k = wants.count ? a.top_k[row] : 0;
     const bool cut_k = wants.count && (uint32_t)k < sh.count[BINS - 1];
     // The steps that are gathered: up to three ranges, [a0, a1] around the end of the top-k words, [b0, b1] around that of top-p's, which
-    // is nearer to the top or touches it, [c0, c1] around the draw, nearer still. A range that touches the next one is part of it.
+    // is nearer to the top or touches it, [c0, c1] around the draw, nearer still. A range that touches the next one, where there is one
+    // (its end is not below 0), is part of it.
     int a0 = BINS, a1 = -1, b0 = BINS, b1 = -1, c0 = BINS, c1 = -1;
     if (!wants.mass) {   // the top-k words and the rest of their last step
         a0 = 0;
@@ -701,14 +702,14 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
             b1 = first_reaching(sh.mass, BINS, nucleus_sum(top_p, most));
             least = before(b0) + 1;
             most = sh.mass[b1];
-            if (b1 >= a0 - 1) { a0 = min(a0, b0); b0 = BINS; b1 = -1; }
+            if (a1 >= 0 && b1 >= a0 - 1) { a0 = min(a0, b0); b0 = BINS; b1 = -1; }
         }
         least = min(least, kept_m);
         most = min(most, kept_m);
         c0 = first_reaching(sh.mass, BINS, drawn_sum(u, least));
         c1 = first_reaching(sh.mass, BINS, drawn_sum(u, most));
         if (b1 >= 0 && c1 >= b0 - 1) { b0 = min(b0, c0); c0 = BINS; c1 = -1; }
-        else if (b1 < 0 && c1 >= a0 - 1) { a0 = min(a0, c0); c0 = BINS; c1 = -1; }
+        else if (b1 < 0 && a1 >= 0 && c1 >= a0 - 1) { a0 = min(a0, c0); c0 = BINS; c1 = -1; }
     }
     // A word's step s is in a range where s - (its first step), a difference without rounding, is at least 0 and below its length:
     // as bits, below that.

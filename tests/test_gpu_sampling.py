@@ -166,3 +166,19 @@ def test_lists_of_every_length(top_k, coarse):
     x = normal(6, 50000, top_k + coarse)
     x = x if not coarse else (x * coarse).round() / coarse
     check(x, [0.0, 0.3, 0.9, 0.999, 0.99999, 0.5], 3.0, top_k=top_k, top_p=[1, 1, 1, 1, 0.99, 0.7])
+
+
+@pytest.mark.parametrize("top_p", [0.5, 0.9, 0.95, 0.99, 0.9999])
+@pytest.mark.parametrize("spread", [0.01, 0.3, 1.0])
+def test_a_nucleus_that_ends_with_the_last_words(spread, top_p):
+    """Rows of a few words, whose smallest one is the end of the histogram, alone and among masked ones; draws all over [0, 1)."""
+    g = np.random.default_rng(int(spread * 100))
+    for words in (2, 3, 4, 8, 16):
+        x = normal(33, words, words, spread=spread)
+        u = ((np.arange(33) + g.random(33)) / 33).astype(np.float32)
+        check(x, u, 1.0, top_p=top_p)
+        masked = torch.full((33, 5003), float("-inf"))
+        masked[:, torch.tensor(np.sort(g.choice(5003, words, replace=False)))] = x
+        check(masked, u, 1.0, top_p=top_p)
+        check(masked, u, 1.0, top_p=top_p, top_k=10 ** 6, min_p=1e-6)
+    check(normal(9, 3001, 2, spread=spread), ((np.arange(9) + 0.5) / 9).astype(np.float32), 1.0, top_p=top_p)
