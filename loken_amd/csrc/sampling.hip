@@ -149,14 +149,14 @@ static __device__ __forceinline__ double fma_by(double a, double b, double c) {
     return r;
 }
 
-// 2^x, -43 <= x <= 0, as an integer of 2^-42. x = n + r, |r| <= 1/2; 2^r = 1 + r f(r), f the polynomial of degree 8 through
-// (2^r - 1) / r at the nine Chebyshev points of [-1/2, 1/2]: off by 2.8e-14. Its terms from r^5 on, which are below 2.4e-6 of
+// 2^x, x = below * rate, -43 <= x <= 0, as an integer of 2^-42. x = n + r, |r| <= 1/2; 2^r = 1 + r f(r), f the polynomial of degree 8
+// through (2^r - 1) / r at the nine Chebyshev points of [-1/2, 1/2]: off by 2.8e-14. Its terms from r^5 on, which are below 2.4e-6 of
 // the result, are made in 32 bits: off by 2e-13.
-static __device__ __forceinline__ uint64_t weight_of(double x) {
+static __device__ __forceinline__ uint64_t weight_of(double below, double rate) {
     const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
-    const double y = x + magic;
+    const double y = fma(below, rate, magic);
     const int n = (int)(uint32_t)__double_as_longlong(y);
-    const double r = x - (y - magic);
+    const double r = fma(below, rate, magic - y);
     const float s = (float)r;
     const float high = fmaf(s, fmaf(s, fmaf(s, 1.0203121e-07f, 1.3255225e-06f), 1.5252687e-05f), 0.00015403455f);
     double p = fma_by(r, (double)high, 0.0013333558179043112);
@@ -174,7 +174,6 @@ static __device__ __forceinline__ uint64_t weight_of(double x) {
 struct Scale {
     float top;        // M; where it is infinite the words that are too count as 0, all others as none
     double rate;      // log2(e) / T
-    double top_rate;  // M times that
     float reach;      // words further below the top weigh nothing
     float steps;      // steps of the histogram per unit of the logit
     double least;     // log2(min_p)
@@ -188,7 +187,6 @@ struct Scale {
         float lowest = value_of(peak.lowest);
         if (infinite) top = lowest = 0.0f;
         rate = 1.4426950408889634 / (double)temperature;
-        top_rate = (double)top * rate;
         reach = fminf((float)(LIVE / rate), 3.402823466e38f);
         const float range = fminf(reach, top - lowest);
         steps = range > 0.0f ? (float)(BINS - 1) / range : 0.0f;
@@ -202,10 +200,13 @@ struct Scale {
     __device__ __forceinline__ bool live(float d) const { return d <= reach; }
     // The step of a live word, as a number that has not been cut to an integer.
     __device__ __forceinline__ float step(float d) const { return fminf(d * steps, (float)(BINS - 1)); }
-    // (v - M) log2(e) / T; at v = M 1e-15 off, which no weight shows
-    __device__ __forceinline__ double power(float v) const { return infinite ? 0.0 : fma((double)v, rate, -top_rate); }
-    // Whether min-p keeps a word d below the top.
-    __device__ __forceinline__ bool kept(float d, double power) const { return (d == 0.0f ? 0.0 : power) >= least; }
+    // v - M, to 64 bits, and its product with log2(e) / T: the difference first. Of v log2(e) / T - M log2(e) / T the rounding of the
+    // second product stays, 2^-53 |M| / T, which is any size where |M| / T is: at M = 12.5 and T = 1e-17 the first word's power was -96.
+    __device__ __forceinline__ double from_top(float v) const { return infinite ? 0.0 : (double)v - (double)top; }
+    __device__ __forceinline__ double power(float v) const { return from_top(v) * rate; }
+    __device__ __forceinline__ uint64_t weight(float v) const { return weight_of(from_top(v), rate); }
+    // Whether min-p keeps a word.
+    __device__ __forceinline__ bool kept(double power) const { return power >= least; }
 };
 
 static __device__ __forceinline__ Peak peak_of_row(const Sampling& a, int row) {
@@ -306,7 +307,7 @@ static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale&
         if (t < AT_ONCE) sh.list[n + t] = 0;   // (the list has room for them)
         __syncthreads();
         const uint64_t mine = t < n ? sh.list[t] : ~0ull;
-        const uint64_t weight = weight_of(sc.power(t < n ? value_of((uint32_t)(mine >> 32)) : sc.top));
+        const uint64_t weight = sc.weight(t < n ? value_of((uint32_t)(mine >> 32)) : sc.top);
         int place = 0;
         for (int i = 0; i < n; i += AT_ONCE) {
             uint64_t x[AT_ONCE];
@@ -398,7 +399,7 @@ static __device__ __forceinline__ void sort_list(Shared& sh, int n, const Scale&
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int at = t * PER + i;
-        if (at < n) ms += weight_of(sc.power(value_of((uint32_t)(sh.list[at] >> 32))));
+        if (at < n) ms += sc.weight(value_of((uint32_t)(sh.list[at] >> 32)));
         m[i] = ms;
     }
     const uint64_t before = sum_before(ms, sh.meet, 0);
@@ -501,7 +502,7 @@ struct Searcher {
                         const float d = sc.below(v);
                         if (sc.live(d) && (int)sc.step(d) == b && key >= low && key <= high) {
                             const uint32_t at = (high - key) >> shift;   // below BINS
-                            atomicAdd((unsigned long long*)&sub_mass[at], (unsigned long long)weight_of(sc.power(v)));
+                            atomicAdd((unsigned long long*)&sub_mass[at], (unsigned long long)sc.weight(v));
                             atomicAdd(&sub_count[at], 1u);
                         }
                     });
@@ -528,7 +529,7 @@ struct Searcher {
     // More equal words than the list takes: the one whose turn it is, counted in the order of their numbers.
     __device__ __forceinline__ Place equal(Shared& sh, uint32_t key, bool by_mass, uint64_t target) {
         const int t = threadIdx.x;
-        const uint64_t w = weight_of(sc.power(value_of(key)));
+        const uint64_t w = sc.weight(value_of(key));
         const uint32_t turn = (uint32_t)(by_mass ? (target - base_mass + w - 1) / w : target - base_count);
         uint32_t passed = 0;
         b0 = b1 = -1;
@@ -567,9 +568,9 @@ static __device__ __forceinline__ uint64_t weigh_as(const T* x, int begin, int e
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             d[e] = ALONE ? sc.below(v[e]) : sc.top - v[e];
-            const double power = !MASS ? 0.0 : ALONE ? sc.power(v[e]) : fma((double)v[e], sc.rate, -sc.top_rate);
-            w[e] = MASS ? weight_of(power) : 0;
-            if (ABOVE) above += sc.live(d[e]) && sc.kept(d[e], power) ? w[e] : 0;
+            const double from_top = !MASS ? 0.0 : ALONE ? sc.from_top(v[e]) : (double)v[e] - (double)sc.top;
+            w[e] = MASS ? weight_of(from_top, sc.rate) : 0;
+            if (ABOVE) above += sc.live(d[e]) && sc.kept(from_top * sc.rate) ? w[e] : 0;
         }
 #pragma unroll
         for (int e = 0; e < N; ++e)
@@ -808,7 +809,7 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
     if (!wants.mass && a.min_p && a.min_p[row] > 0.0f) {   // what min-p keeps of the list, which is a prefix
         const int past = first_where(n, [&](int i) {
             const float v = value_of((uint32_t)(sh.list[i] >> 32));
-            return !sc.kept(sc.top - v, sc.power(v));
+            return !sc.kept(sc.power(v));
         });
         above = sh.sums[max(past, 1) - 1];
     }
@@ -816,7 +817,7 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a)
     const int at = first_reaching(sh.sums, n, drawn_sum(u, kept));
     if (t == 0) {
         a.tokens[row] = (int)~(uint32_t)sh.list[at];
-        if (a.probs) a.probs[row] = (float)((double)weight_of(sc.power(value_of((uint32_t)(sh.list[at] >> 32)))) / (double)kept);
+        if (a.probs) a.probs[row] = (float)((double)sc.weight(value_of((uint32_t)(sh.list[at] >> 32))) / (double)kept);
     }
 }
 

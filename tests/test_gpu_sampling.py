@@ -182,3 +182,37 @@ def test_a_nucleus_that_ends_with_the_last_words(spread, top_p):
         check(masked, u, 1.0, top_p=top_p)
         check(masked, u, 1.0, top_p=top_p, top_k=10 ** 6, min_p=1e-6)
     check(normal(9, 3001, 2, spread=spread), ((np.arange(9) + 0.5) / 9).astype(np.float32), 1.0, top_p=top_p)
+
+
+@pytest.mark.parametrize("temperature", [1e-14, 1e-15, 1e-16, 1e-17, 3e-18, 1e-18, 1e-19, 1e-20, 1e-22, 1e-24, 1e-38, 1e-44])
+@pytest.mark.parametrize("rules", [dict(), dict(top_k=3), dict(top_k=2000), dict(top_p=0.6), dict(min_p=0.5)], ids=str)
+def test_temperatures_far_below_the_logits(temperature, rules):
+    """Only words equal to the largest are left, each with a weight of one: alone, and as one of a few or of thousands."""
+    x = normal(8, 5003, 17)
+    for r, n in enumerate((1, 2, 3, 7, 300, 2500, 1, 2)):
+        at = np.random.default_rng(r).choice(5003, n, replace=False)
+        x[r, torch.tensor(at)] = [11.37, 12.5, 14.0, 9.1, 15.999, 8.3, 1e5, 65504.0][r]
+    for u in (0.0, 0.37, 0.99999994):
+        check(x, u, temperature, **rules)
+
+
+@pytest.mark.parametrize("size", [1e8, 1e12, 1e16, 1e17, 1e18, 1e20, 1e22, 1e26, 1e29, 3e38])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("rules", [dict(), dict(top_k=3), dict(top_p=0.6), dict(min_p=0.5)], ids=str)
+def test_logits_far_from_zero(size, sign, rules):
+    """Rows of large logits: equal ones, neighbours in their type, and words far behind them."""
+    g = np.random.default_rng(18)
+    top = np.float32(sign * size)
+    x = np.full((6, 4001), -np.inf, np.float32)
+    near = [top]
+    for _ in range(6):
+        near.append(np.nextafter(near[-1], np.float32(-np.inf)))
+    for r in range(6):
+        x[r] = np.array(near)[g.integers(0, 1 + r, 4001)]
+        x[r, g.random(4001) < 0.9] = [-np.inf, np.float32(-3.4e38), near[-1], -np.inf, -np.inf, near[2]][r]
+        x[r, 17] = top
+    if sign > 0:
+        x[0, ::7] = 0.5
+    for temperature in (1.0, float(near[0]) - float(near[1])):
+        for u in (0.0, 0.37, 0.99999994):
+            check(torch.tensor(x), u, temperature, **rules)
