@@ -35,6 +35,9 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES, RUNS = KV_TILE / 16;   // of a team
 constexpr float LIFT = 7.f, SLACK = 8.f;   // powers of two
+// Pages whose value scale is this share of the largest so far, or less, are as those without values: their weights, at most
+// 2^(SLACK + LIFT) of it, are zeros in f16 (2^-25 and below), high or low half. The share itself goes down to 2^-247, and 2^-bias past f32.
+constexpr float LEAST_SHARE = 0x1p-40f;
 
 // Sixteen codes as f16, as they lie: 0x6400 + (code + 128) is the f16 number 1152 + code.
 static __device__ __forceinline__ void to_halves(uint4 w, uint4* out) {
@@ -91,9 +94,9 @@ struct Many {
 // What a step's pages have for everybody.
 struct Step {
     float ks[RUNS];     // key scales; -1: the page is absent
-    float bias[RUNS];   // log2 of the value scale over `ref`, and LIFT; -infinity where the scale is zero
-    float back[RUNS];   // 2^-bias, 0 with a scale of zero
-    uint32_t dead;      // a bit for each page whose values are all zero
+    float bias[RUNS];   // log2 of the value scale over `ref`, and LIFT; -infinity where the values do not show
+    float back[RUNS];   // 2^-bias, 0 where the values do not show
+    uint32_t dead;      // a bit for each page whose values do not show: all zero, or LEAST_SHARE of `ref` at most
     float shrink;       // what `ref` before this step is of it now
     float ref;          // the largest value scale so far
     int absent;         // whether a page is
@@ -242,11 +245,12 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                 const float most = across_runs(v1, [](float x, float y) { return fmaxf(x, y); });
                 const float least = across_runs(k1, [](float x, float y) { return fminf(x, y); });
                 const float now = fmaxf(ref, most);
-                const float bias = v1 > 0.f ? __builtin_amdgcn_logf(v1 / now) + LIFT : -INFINITY;
+                const bool shows = v1 > now * LEAST_SHARE;
+                const float bias = shows ? __builtin_amdgcn_logf(v1 / now) + LIFT : -INFINITY;
                 st.ks[lane] = k1;
                 st.bias[lane] = bias;
-                st.back[lane] = v1 > 0.f ? __builtin_amdgcn_exp2f(-bias) : 0.f;
-                const uint32_t dead = (uint32_t)__ballot(!(v1 > 0.f));
+                st.back[lane] = shows ? __builtin_amdgcn_exp2f(-bias) : 0.f;
+                const uint32_t dead = (uint32_t)__ballot(!shows);
                 if (lane == 0) {
                     st.shrink = ref > 0.f ? ref / now : 1.f;   // (up to then the sums are zeros)
                     st.ref = now;
@@ -408,7 +412,7 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                     m = m_new;
                 }
                 const float m_base = m == -INFINITY ? 0.f : m;
-                if (st.dead) {   // positions of pages without values: in the sum of weights only
+                if (st.dead) {   // positions of pages whose values do not show: in the sum of weights only
 #pragma unroll
                     for (int n = 0; n < RUNS; ++n)
                         if (st.dead >> n & 1)

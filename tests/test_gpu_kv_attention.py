@@ -301,3 +301,25 @@ def test_first_rows_far_outside_the_batch(hint, dtype):
         out.fill_(7.0)
         kv.kv_attention(b.q.cuda(), b.cache(), i32(b.table), i32(b.lens), i32(starts), max_fresh=hint, max_len=300, out=out)
         assert (out == want).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("fresh", [1, 40])
+@pytest.mark.parametrize("largest", ["first", "last", "in the middle"])
+@pytest.mark.parametrize("ratio", [-20, -36, -39, -40, -41, -44, -60, -100, -120, -126])
+def test_value_scales_of_any_ratio(ratio, largest, fresh, dtype):
+    """One page of large values among pages of values that do not show beside them: their weights count all the same."""
+    b = Batch([300], [fresh], 4, 2, 64, 16, dtype, seed=50)
+    b.want.scales["v"][:] = np.float32(2.0 ** ratio)
+    b.want.scales["v"][b.table[0, {"first": 0, "last": 16, "in the middle": 9}[largest]]] = 1.0
+    for scale in (0.125, 1.5):
+        b.check(scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fresh", [1, 40])
+def test_value_scales_at_both_ends_of_what_a_page_may_have(fresh, dtype):
+    b = Batch([300], [fresh], 4, 2, 64, 16, dtype, seed=51)
+    b.want.scales["v"][:] = np.float32(2.0 ** -126)
+    b.want.scales["v"][b.table[0, ::5]] = np.float32(2.0 ** 14)
+    b.check()
