@@ -786,7 +786,9 @@ void loken_argsort_small_u32(const uint32_t* in, uint32_t* sorted_out, uint32_t*
  *   lens[seqs]         past + fresh
  *   starts[seqs + 1]   the first row of each sequence in the batch, and their number
  *   slots[rows], positions[rows]   of each row: -1 and the position where its page is absent; -1 and 0 behind the last sequence
- *   *taken_out         *taken + the pages asked for (above n_free: that many more are wanted); not the address of `taken`
+ *   *taken_out         *taken + the pages asked for (above n_free: that many more are wanted)
+ * What is written shares no memory with what is read, nor with anything else that is written (else LK_ERR_ARG): the next step's
+ * past and taken are copies of lens and *taken_out, or two steps' arrays are used in turn.
  * Rows past `rows` are left out of slots and positions. Sums past 2^31 - 1 stay there. More than LK_KV_PLAN_SEQS sequences: LK_ERR_SIZE. */
 int lk_kv_plan(const int32_t* past, const int32_t* fresh, int seqs, int page_tokens, const int32_t* free_pages, int n_free,
                const int32_t* taken, int32_t* table, int64_t table_stride, int table_cols, int32_t* lens, int32_t* starts,

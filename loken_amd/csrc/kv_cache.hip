@@ -412,6 +412,20 @@ struct Read {
 
 }  // namespace
 
+// Whether any two of the arrays, the first `inputs` of which are only read, share memory that one of them is written to.
+struct Bytes {
+    const void* at;
+    int64_t size;
+};
+static bool written_together(const Bytes* a, int inputs, int all) {
+    for (int j = inputs; j < all; ++j)
+        for (int i = 0; i < j; ++i) {
+            const uintptr_t p = (uintptr_t)a[i].at, q = (uintptr_t)a[j].at;
+            if (a[i].size > 0 && a[j].size > 0 && (p < q ? q - p < (uint64_t)a[i].size : p - q < (uint64_t)a[j].size)) return true;
+        }
+    return false;
+}
+
 extern "C" int lk_kv_plan(const int32_t* past, const int32_t* fresh, int seqs, int page_tokens, const int32_t* free_pages, int n_free,
                           const int32_t* taken, int32_t* table, int64_t table_stride, int table_cols, int32_t* lens, int32_t* starts,
                           int64_t* slots, int32_t* positions, int rows, int32_t* taken_out, void* stream) {
@@ -420,6 +434,11 @@ extern "C" int lk_kv_plan(const int32_t* past, const int32_t* fresh, int seqs, i
         (rows > 0 && (!slots || !positions)) || (n_free > 0 && !free_pages) || ((uintptr_t)slots & 7))
         return LK_ERR_ARG;
     if (seqs > LK_KV_PLAN_SEQS) return LK_ERR_SIZE;
+    // every workgroup reads all lengths while the first one writes its sums
+    const Bytes arrays[] = {{past, 4 * (int64_t)seqs}, {fresh, 4 * (int64_t)seqs}, {free_pages, 4 * (int64_t)n_free}, {taken, taken ? 4 : 0},
+                            {table, seqs > 0 && table_cols > 0 ? 4 * ((seqs - 1) * table_stride + table_cols) : 0}, {lens, 4 * (int64_t)seqs},
+                            {starts, 4 * ((int64_t)seqs + 1)}, {slots, 8 * (int64_t)rows}, {positions, 4 * (int64_t)rows}, {taken_out, 4}};
+    if (written_together(arrays, 4, 10)) return LK_ERR_ARG;
     // a kernel gets 64 KB of LDS unless the runtime is told otherwise
     if (seqs * 12 > 60 * 1024 &&
         hipFuncSetAttribute((const void*)kv_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, seqs * 12) != hipSuccess) {

@@ -121,7 +121,8 @@ class KvPlan:
 def kv_plan(past: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, page_tokens: int, plan: KvPlan,
             taken: torch.Tensor | None = None) -> KvPlan:
     """Pages for the tokens that each sequence brings (into ``table`` [seqs, columns], in place) and, in ``plan``, lengths, first
-    rows, the slot and position of every row, and how many pages of ``free_pages`` are gone by then; ``taken``: how many were before."""
+    rows, the slot and position of every row, and how many pages of ``free_pages`` are gone by then; ``taken``: how many were before.
+    None of what it reads is the plan's own: the next step's ``past`` is a copy of ``plan.lens``, or two plans are used in turn."""
     seqs = past.numel()
     _vector("kv_plan", "past", past, torch.int32)
     _vector("kv_plan", "fresh", fresh, torch.int32, seqs)
@@ -135,6 +136,8 @@ def kv_plan(past: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free_p
         _vector("kv_plan", "taken", taken, torch.int32, 1)
         if taken.data_ptr() == plan.taken.data_ptr():
             raise ValueError("kv_plan: taken is the plan's own")
+    if past.data_ptr() == plan.lens.data_ptr() and seqs:
+        raise ValueError("kv_plan: past is the plan's own")
     _on_device("kv_plan", past, fresh, table, free_pages, plan.slots, *(() if taken is None else (taken,)))
     _lib.check("lk_kv_plan", _lib.load().lk_kv_plan(
         past.data_ptr(), fresh.data_ptr(), seqs, page_tokens, free_pages.data_ptr(), free_pages.numel(),

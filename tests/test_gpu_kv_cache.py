@@ -70,6 +70,42 @@ def test_the_largest_plan():
     check_plan(past, fresh, 16, int(fresh.sum()) + 70, 4, g.permutation(seqs))
 
 
+@pytest.mark.parametrize("seqs,most_fresh", [(3, 5), (700, 4)])
+def test_plan_of_arrays_side_by_side(seqs, most_fresh):
+    """All arrays of a plan in one allocation, each starting where another ends; and past and taken from the plan before."""
+    g = np.random.default_rng(seqs)
+    past, fresh, cols = g.integers(0, 60, seqs), g.integers(0, most_fresh + 1, seqs), 6
+    rows, free = int(fresh.sum()) + 7, g.permutation(seqs * 9)
+    sizes = dict(slots=2 * rows, past=seqs, lens=seqs, fresh=seqs, taken=1, out=1, free=len(free), table=seqs * cols, starts=seqs + 1, positions=rows)
+    whole, at = torch.full((sum(sizes.values()),), -99, dtype=torch.int32, device="cuda"), {}
+    for name, n in sizes.items():
+        first = sum(v.numel() for v in at.values())
+        at[name] = whole[first:first + n]
+    table = np.full((seqs, cols), -1, np.int32)
+    for i, p in enumerate(past):
+        table[i, :-(-p // 16)] = np.arange(-(-p // 16)) + 10 * i
+    for name, v in (("past", past), ("fresh", fresh), ("free", free), ("table", table.reshape(-1)), ("taken", [2])):
+        at[name].copy_(i32(v))
+    L = lib.load()
+
+    def plan(a):
+        lib.check("lk_kv_plan", L.lk_kv_plan(a["past"].data_ptr(), a["fresh"].data_ptr(), seqs, 16, a["free"].data_ptr(), len(free), a["taken"].data_ptr(),
+                                             a["table"].data_ptr(), cols, cols, a["lens"].data_ptr(), a["starts"].data_ptr(), a["slots"].data_ptr(),
+                                             a["positions"].data_ptr(), rows, a["out"].data_ptr(), torch.cuda.current_stream().cuda_stream))
+
+    taken, lens = 2, past
+    other = {n: torch.empty_like(v) for n, v in at.items()}
+    for step in range(4):   # what was written is read by the next one, which writes the other arrays
+        a, b = (at, other) if step % 2 == 0 else (other, at)
+        plan(a)
+        table, lens, starts, slots, positions, taken = ref.plan(lens, fresh, table, free, 16, rows, taken)
+        for name, want in (("table", table.reshape(-1)), ("lens", lens), ("starts", starts), ("positions", positions), ("out", [taken])):
+            assert np.array_equal(a[name].cpu().numpy(), want), (step, name)
+        assert np.array_equal(a["slots"].view(torch.int64).cpu().numpy(), slots)
+        for name, v in (("past", a["lens"]), ("taken", a["out"]), ("fresh", a["fresh"]), ("free", a["free"]), ("table", a["table"])):
+            b[name].copy_(v)
+
+
 # ------------------------------------------------------------------------------------------ the cache
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 

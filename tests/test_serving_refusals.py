@@ -146,3 +146,28 @@ def test_tensors_of_another_place_or_shape_are_refused():
     for args in ((logits, u, u), (logits.double(), u, u), (logits, u[:1], u), (logits, u, u, u), (logits[:, ::2], u, u), (logits[:1].expand(2, 10), u, u)):
         with pytest.raises(ValueError):
             sampling.sample(*args)
+
+
+# arrays of a plan of 100 sequences and 700 rows, far from each other
+APART = dict(past=1 << 20, fresh=2 << 20, seqs=100, page=16, free=3 << 20, n_free=50, taken=4 << 20, table=5 << 20, stride=12, cols=8, lens=6 << 20,
+             starts=7 << 20, slots=8 << 20, positions=9 << 20, rows=700, out=10 << 20)
+# bytes of each: the table's last row ends with its columns
+SIZES = dict(past=400, fresh=400, free=200, taken=4, table=4 * (99 * 12 + 8), lens=400, starts=404, slots=5600, positions=2800, out=4)
+
+
+@pytest.mark.parametrize("written", ["table", "lens", "starts", "slots", "positions", "out"])
+@pytest.mark.parametrize("other", sorted(SIZES))
+def test_a_plan_does_not_write_what_it_reads(written, other):
+    """The first and the last byte's word in common are enough; slots stand on eight bytes."""
+    if other == written:
+        return
+    word = 8 if written == "slots" else 4
+    for at in (APART[other], APART[other] + (SIZES[other] - 4) // word * word, APART[other] - SIZES[written] + word):
+        assert lib.load().lk_kv_plan(*plan_args(**{**APART, written: at})) == lib.LK_ERR_ARG, at
+
+
+def test_lengths_of_the_plan_itself_are_refused():
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    plan = kv.KvPlan(2, 8, device="cpu")
+    with pytest.raises(ValueError, match="plan's own"):
+        kv.kv_plan(plan.lens, i32(1, 1), torch.zeros(2, 4, dtype=torch.int32), i32(1), 16, plan)
