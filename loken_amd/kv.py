@@ -72,7 +72,8 @@ def _table(what: str, table: torch.Tensor, seqs: int):
 
 class KvCacheQ8:
     """Pages of one layer's cache: codes ``k`` int8 [pages, kv_heads, page_tokens, head_dim] and ``v`` int8
-    [pages, kv_heads, page_tokens / 16, head_dim, 16], scales f32 [pages, kv_heads]."""
+    [pages, kv_heads, page_tokens / 16, head_dim, 16], scales f32 [pages, kv_heads]. Other tensors are another cache: these four are not
+    assigned anew."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor):
         if k.dim() != 4 or k.dtype != torch.int8 or v.dtype != torch.int8:
@@ -89,10 +90,19 @@ class KvCacheQ8:
             raise ValueError("kv cache: its tensors are on several devices")
         if not all(t.is_contiguous() for t in (k, v, k_scales, v_scales)):
             raise ValueError("kv cache: its tensors are contiguous")
-        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
-        self._at = (k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
-        if (self._at[0] | self._at[1]) & 15:
+        self._tensors = (k, v, k_scales, v_scales)
+        if (k.data_ptr() | v.data_ptr()) & 15:
             raise ValueError("kv cache: codes start on 16 bytes")
+
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scales = property(lambda self: self._tensors[2])
+    v_scales = property(lambda self: self._tensors[3])
+
+    def _at(self):
+        """Where the tensors are now: a program may have given one other memory since."""
+        k, v, k_scales, v_scales = self._tensors
+        return k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr()
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page_tokens: int = 16, device="cuda") -> "KvCacheQ8":
@@ -156,7 +166,7 @@ def kv_write(cache: KvCacheQ8, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
     _on_device("kv_write", k, v, slots, cache.k)
     _lib.check("lk_kv_write_q8", _lib.load().lk_kv_write_q8(
         k.data_ptr(), v.data_ptr(), _X_TYPES[k.dtype], ks, vs, slots.data_ptr(), tokens, cache.kv_heads, cache.head_dim,
-        cache.page_tokens, cache.pages, *cache._at, _stream()))
+        cache.page_tokens, cache.pages, *cache._at(), _stream()))
 
 
 def kv_read(cache: KvCacheQ8, slots: torch.Tensor, dtype: torch.dtype = torch.float32):
@@ -168,7 +178,7 @@ def kv_read(cache: KvCacheQ8, slots: torch.Tensor, dtype: torch.dtype = torch.fl
     k = torch.empty((slots.numel(), cache.kv_heads, cache.head_dim), dtype=dtype, device=slots.device)
     v = torch.empty_like(k)
     _lib.check("lk_kv_read_q8", _lib.load().lk_kv_read_q8(
-        slots.data_ptr(), slots.numel(), cache.kv_heads, cache.head_dim, cache.page_tokens, cache.pages, *cache._at, k.data_ptr(),
+        slots.data_ptr(), slots.numel(), cache.kv_heads, cache.head_dim, cache.page_tokens, cache.pages, *cache._at(), k.data_ptr(),
         v.data_ptr(), _X_TYPES[dtype], _stream()))
     return k, v
 
@@ -197,7 +207,7 @@ def kv_attention(q: torch.Tensor, cache: KvCacheQ8, table: torch.Tensor, lens: t
         raise ValueError("kv_attention: out has the type and shape of q")
     _on_device("kv_attention", q, out, table, lens, starts, cache.k)
     _lib.check("lk_kv_attention_q8", _lib.load().lk_kv_attention_q8(
-        q.data_ptr(), _X_TYPES[q.dtype], stride, out.data_ptr(), out_stride, *cache._at, cache.pages, cache.page_tokens, table.data_ptr(),
+        q.data_ptr(), _X_TYPES[q.dtype], stride, out.data_ptr(), out_stride, *cache._at(), cache.pages, cache.page_tokens, table.data_ptr(),
         across, cols, lens.data_ptr(), starts.data_ptr(), seqs, rows, min(max_fresh, 0x7FFFFFFF),
         min(max_len, 0x7FFFFFFF), heads, cache.kv_heads, cache.head_dim, scale, min(window, 0x7FFFFFFF), _stream()))
     return out

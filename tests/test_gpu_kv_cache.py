@@ -255,3 +255,20 @@ def test_pages_behind_2_to_the_31_bytes():
     gk, gv = kv.kv_read(cache, i64(slots))
     assert torch.equal(gk, gv) and (gk.cpu() - x).abs().max() <= x.abs().max() / 127 / 2 * 1.001
     assert not k[:pages - 2].any() and not k[pages - 1, 0, 4:].any()
+
+
+def test_calls_go_to_where_the_tensors_are():
+    """A tensor of the cache that has been given other memory: rows go there, and come from there."""
+    g = np.random.default_rng(5)
+    cache, want = both(4, 2, 16, 64)
+    old = [getattr(cache, n).data for n in ("k", "v", "k_scales", "v_scales")]   # (their memory stays)
+    write(cache, want, rows_of(g, 20, 2, 64, torch.float32), rows_of(g, 20, 2, 64, torch.float32), range(20))
+    before = [t.clone() for t in old]
+    for n in ("k", "v", "k_scales", "v_scales"):
+        getattr(cache, n).data = getattr(cache, n).clone()
+    write(cache, want, rows_of(g, 9, 2, 64, torch.float32), rows_of(g, 9, 2, 64, torch.float32), range(20, 29))
+    check_cache(cache, want)
+    assert all(torch.equal(a, b) for a, b in zip(old, before))
+    gk, gv = kv.kv_read(cache, i64(range(16, 29)))
+    for side, got in (("k", gk), ("v", gv)):
+        assert np.allclose(got.cpu().numpy(), want.values(side, 1)[:, :13].transpose(1, 0, 2), rtol=2.0 ** -23, atol=0)

@@ -171,3 +171,11 @@ def test_lengths_of_the_plan_itself_are_refused():
     plan = kv.KvPlan(2, 8, device="cpu")
     with pytest.raises(ValueError, match="plan's own"):
         kv.kv_plan(plan.lens, i32(1, 1), torch.zeros(2, 4, dtype=torch.int32), i32(1), 16, plan)
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_scales", "v_scales"])
+def test_the_tensors_of_a_cache_are_not_assigned_anew(name):
+    """Without checks of the new ones, and with calls that go on with the old ones' memory."""
+    c = cpu_cache()
+    with pytest.raises(AttributeError):
+        setattr(c, name, getattr(c, name).clone())
