@@ -35,6 +35,8 @@ struct Few {
     static constexpr int Q_BITS = DIGITS == 3 ? 23 : 15;   // Q_MAX is just below 2^Q_BITS
     static constexpr float Q_ROUND = 1 << Q_BITS;
     static constexpr float P_MAX = DIGITS == 3 ? 63.f * 65536 + 127 * 256 + 127 : 127.f * 256 + 127;   // below 2^22: see cut()
+    // Whole numbers of weights are brought to size before a scale comes in: with the scale alone a small one's quotient would be subnormal.
+    static constexpr float P_UNIT = DIGITS == 3 ? 0x1p-22f : 0x1p-15f, P_LEFT = 1.f / (P_MAX * P_UNIT);   // just above 1
     static constexpr int BALANCE = DIGITS == 3 ? 0x808080 : 0x8080;
 };
 
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 && !(D == 128 && NT == 2) ? 2 :
                 const float g0 = __builtin_amdgcn_exp2f(base - m_base);
                 const float part_gain = top == -INFINITY ? 1.f : g0;
                 l[n] = l[n] * keep[n] + sum * part_gain;
-                gain[n] = top == -INFINITY ? 0.f : g0 * (vs_most / F::P_MAX);
+                gain[n] = top == -INFINITY ? 0.f : g0 * (vs_most * F::P_LEFT);
                 m[n] = m_new;
             }
 #pragma unroll
@@ -319,12 +321,12 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 && !(D == 128 && NT == 2) ? 2 :
                 for (int b = 0; b < F::NB; ++b) {
                     const v4i c = mfma(p_op[n], v[b], (v4i){0, 0, 0, 0});
                     if (F::DIGITS == 3) {
-                        const float x = fmaf((float)c[0], 65536.f, fmaf((float)c[1], 256.f, (float)c[2]));
+                        const float x = fmaf((float)c[0], 65536.f * F::P_UNIT, fmaf((float)c[1], 256.f * F::P_UNIT, (float)c[2] * F::P_UNIT));
                         acc[n][0][b] = fmaf(x, gr[0], acc[n][0][b] * kr[0]);
                     } else {
 #pragma unroll
                         for (int p = 0; p < F::PER; ++p) {
-                            const float x = (float)(c[2 * p] * 256 + c[2 * p + 1]);
+                            const float x = (float)(c[2 * p] * 256 + c[2 * p + 1]) * F::P_UNIT;
                             acc[n][p][b] = fmaf(x, gr[p], acc[n][p][b] * kr[p]);
                         }
                     }

@@ -323,3 +323,21 @@ def test_value_scales_at_both_ends_of_what_a_page_may_have(fresh, dtype):
     b.want.scales["v"][:] = np.float32(2.0 ** -126)
     b.want.scales["v"][b.table[0, ::5]] = np.float32(2.0 ** 14)
     b.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fresh,length", [(1, 300), (40, 300), (1, 9000), (40, 9000)])
+@pytest.mark.parametrize("power", [-126, -120, -110, -100])
+def test_values_near_the_smallest(power, fresh, length, dtype):
+    """Pages whose scales are the smallest that a page may have, alike: outputs keep the bits that their type has there."""
+    b = Batch([length], [fresh], 2, 1, 64, 16, dtype, seed=52)
+    b.want.scales["v"] = (b.want.scales["v"].astype(np.float64) * 50 * 2.0 ** power).clip(2.0 ** -126).astype(np.float32)
+    out = torch.zeros((b.rows, b.heads, b.dim), dtype=TYPES[dtype], device="cuda")
+    kv.kv_attention(b.q.cuda(), b.cache(), i32(b.table), i32(b.lens), i32(b.starts), max_fresh=fresh, max_len=length, out=out)
+    want, reach, most = ref.attention(b.q.float().numpy(), b.want, b.table, b.lens, b.starts, b.dim ** -0.5, 0, np.zeros(out.shape))
+    fine = dtype == "f32"
+    bound = most * (2 * reach * 2.0 ** (-22 if fine else -15) + 2.0 ** (-17 if fine else -10) + 2.0 ** -20)
+    step = 2.0 ** -24 if fine else torch.finfo(TYPES[dtype]).eps / 2
+    least = 2.0 ** -150 if fine else 2.0 ** -134   # half of the type's smallest step, which a rounding below the normal numbers goes by
+    off = np.abs(out.double().cpu().numpy() - want) - step * np.abs(want) - bound[..., None] - least
+    assert (off <= 0).all(), off.max() / most.max()
