@@ -260,8 +260,9 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 && !(D == 128 && NT == 2) ? 2 :
             kp_next = page_of(t + 2 * WAVES, i >> 2);
             vp_next = page_of(t + 2 * WAVES, g);
 
-            const float vs_most = max_over_groups(vs_now);
-            const float cut = vs_most > 0.f ? vs_now / vs_most * F::P_MAX : 0.f;
+            // a row's weights go by the largest value scale of the pages that it sees
+            auto share_of = [&](float mine, float most) { return most > 0.f ? mine / most * F::P_MAX : 0.f; };
+            const float vs_all = max_over_groups(vs_now), cut_all = share_of(vs_now, vs_all);
             uint4 p_op[NT];
             float keep[NT], gain[NT];
 #pragma unroll
@@ -276,8 +277,12 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 && !(D == 128 && NT == 2) ? 2 :
                     if (F::SLOTS == 4) f += dpp_f32<0x4E>(f);
                     x[e] = f * by;
                 }
+                float vs_most = vs_all, cut = cut_all;
                 if (!whole) {
                     const int last = vp_now < 0 ? -1 : pos[n] - p0, first = a.window > 0 ? pos[n] - a.window - p0 : -1;
+                    const float vs_seen = last >= 0 && first < 15 ? vs_now : 0.f;
+                    vs_most = max_over_groups(vs_seen);
+                    cut = share_of(vs_seen, vs_most);
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         if (e > last || e <= first) x[e] = -INFINITY;

@@ -341,3 +341,14 @@ def test_values_near_the_smallest(power, fresh, length, dtype):
     least = 2.0 ** -150 if fine else 2.0 ** -134   # half of the type's smallest step, which a rounding below the normal numbers goes by
     off = np.abs(out.double().cpu().numpy() - want) - step * np.abs(want) - bound[..., None] - least
     assert (off <= 0).all(), off.max() / most.max()
+
+
+@pytest.mark.parametrize("dtype,ratio", [(d, r) for d in sorted(TYPES) for r in (-8, -12, -20, -40, -100) if d != "f16" or r >= -12])   # (f16: normal numbers)
+@pytest.mark.parametrize("length,fresh,window,hidden", [(300, 1, 70, (12, 13)), (300, 3, 70, (12, 13)), (300, 1, 33, (0, 16)), (290, 4, 0, (18,)), (290, 4, 20, (16, 18)),
+                                                        (2000, 1, 300, (104, 105))])
+def test_pages_that_a_row_does_not_see_do_not_cost_it_bits(length, fresh, window, hidden, dtype, ratio):
+    """Large values behind a window's border, or of the sequence's later rows: what is lost of a row goes by the values that it sees."""
+    b = Batch([length], [fresh], 4, 2, 64, 16, dtype, seed=53)
+    b.want.scales["v"] *= np.float32(2.0 ** ratio)
+    b.want.scales["v"][b.table[0, list(hidden)]] = 1.0
+    b.check(window=window)
