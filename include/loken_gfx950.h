@@ -821,8 +821,9 @@ int lk_kv_read_q8(const int64_t* slots, int tokens, int kv_heads, int head_dim, 
  * them; they choose launch shapes only, a sequence with more is served too. table_cols * page_tokens up to 2^31 - 1024 and
  * rows * heads / kv_heads up to 2^31 - 1, else LK_ERR_SIZE.
  * Scores, softmax and sums are held in f32 (sums of products of codes in int32 as long as they are exact). In the products a
- * query value of f32 is held to 2^-22 of its row's largest, one of f16 or bf16 to 2^-15, and a softmax weight to as much of the largest of
- * 64 positions, or as f16 (f32: as two). Partial results of a
+ * query value of f32 is held to 2^-22 of its row's largest, one of f16 or bf16 to 2^-15, and a softmax weight with its page's value
+ * scale to as much of the largest weight and the largest scale that the row sees among 64 positions, or as f16 (f32: as two) of the
+ * largest such product. A sum of weights times values has to be a number of f32 before it is divided by the weights. Partial results of a
  * context that is split over workgroups go through scratch of the stream (LK_ERR_NOMEM where there is none; while a
  * graph is recorded, where no call outside a recording has needed as much). */
 int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, void* out, int64_t out_stride, const void* k_codes,

@@ -11,12 +11,14 @@
 //
 // Queries come in f16 scaled by a power of two of their row (bf16 fits with its 8 bits, f16 as it is); f32 ones as a high and a
 // low half, two products each, as are its weights: 22 bits. A page's key scale goes onto the scores. Its value scale goes onto the
-// weights, relative to the largest value scale so far, so that no scale is too small for f16: as its logarithm, in the exponent that
+// weights, as a share of `ref`, a power of two above the largest value scale so far: as its logarithm, in the exponent that
 // the weight is made from (off by 5e-7 of the weight at most, a last place of the logarithm), and back out of the sum of
 // weights run by run.
 //
-// The sums are put to a new maximum only where that lies 2^8 above the one they go by: weights up to 2^8 then, which stand
-// LIFT = 2^7 above one and stay below 2^15, f16's largest; a weight of 2^-21 still has all its bits, one of 2^-31 some.
+// A row's sums go by 2^m, m a whole number about the largest of score + logarithm of the share among the positions that the row sees: so
+// neither small scales nor large ones of pages that it does not see cost its weights bits in f16. They are put to a new m only where
+// that lies 2^8 above: weights times shares up to 2^8 then, which stand LIFT = 2^7 above one and stay below 2^15, f16's largest; one of
+// 2^-21 still has all its bits, one of 2^-31 some. Where `ref` grows, m falls by as much and the sums of values stay as they are.
 //
 // A wave's step is 32 products of 32 cycles (twice as many in f32) and some 400 other instructions, 32 of them exponentials, which
 // take four times as long. It is these that bound it, and what of them does not run beside products: so a product comes with
@@ -35,9 +37,9 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES, RUNS = KV_TILE / 16;   // of a team
 constexpr float LIFT = 7.f, SLACK = 8.f;   // powers of two
-// Pages whose value scale is this share of the largest so far, or less, are as those without values: their weights, at most
-// 2^(SLACK + LIFT) of it, are zeros in f16 (2^-25 and below), high or low half. The share itself goes down to 2^-247, and 2^-bias past f32.
-constexpr float LEAST_SHARE = 0x1p-40f;
+// Pages whose value scale is a share of 2^-FAR or less are as those without values: in the sum of weights, at a share of 2^-FAR. (A share
+// goes down to 2^-247, and what it is taken back out with would leave f32.)
+constexpr float FAR = 90.f, LEAST_SHARE = 0x1p-90f;
 
 // Sixteen codes as f16, as they lie: 0x6400 + (code + 128) is the f16 number 1152 + code.
 static __device__ __forceinline__ void to_halves(uint4 w, uint4* out) {
@@ -94,11 +96,13 @@ struct Many {
 // What a step's pages have for everybody.
 struct Step {
     float ks[RUNS];     // key scales; -1: the page is absent
-    float bias[RUNS];   // log2 of the value scale over `ref`, and LIFT; -infinity where the values do not show
+    float share[RUNS];  // log2 of the value scale over `ref`; -FAR where the values do not show
+    float bias[RUNS];   // that, and LIFT; -infinity where the values do not show
     float back[RUNS];   // 2^-bias, 0 where the values do not show
     uint32_t dead;      // a bit for each page whose values do not show: all zero, or LEAST_SHARE of `ref` at most
-    float shrink;       // what `ref` before this step is of it now
-    float ref;          // the largest value scale so far
+    float ref;          // a power of two, at least the largest value scale so far
+    float drop, grow;   // log2 of how much `ref` has grown with this step, up to 100, and 2^drop
+    float shrink;       // 2^-that of the rest
     int absent;         // whether a page is
 };
 
@@ -244,15 +248,27 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                 const float k1 = page_of_run < 0 ? -1.f : ks, v1 = page_of_run < 0 ? 0.f : vs;
                 const float most = across_runs(v1, [](float x, float y) { return fmaxf(x, y); });
                 const float least = across_runs(k1, [](float x, float y) { return fminf(x, y); });
-                const float now = fmaxf(ref, most);
+                int e2 = 0;
+                (void)frexpf(most, &e2);
+                const float now = most > 0.f ? fmaxf(ref, ldexpf(1.f, min(e2, 127))) : ref;
                 const bool shows = v1 > now * LEAST_SHARE;
-                const float bias = shows ? __builtin_amdgcn_logf(v1 / now) + LIFT : -INFINITY;
+                const float share = shows ? __builtin_amdgcn_logf(v1 / now) : -FAR, bias = shows ? share + LIFT : -INFINITY;
                 st.ks[lane] = k1;
+                st.share[lane] = share;
                 st.bias[lane] = bias;
                 st.back[lane] = shows ? __builtin_amdgcn_exp2f(-bias) : 0.f;
                 const uint32_t dead = (uint32_t)__ballot(!shows);
                 if (lane == 0) {
-                    st.shrink = ref > 0.f ? ref / now : 1.f;   // (up to then the sums are zeros)
+                    int grown = 0;   // (up to the first scale the sums are zeros)
+                    if (ref > 0.f) {
+                        (void)frexpf(ref, &grown);
+                        int e3 = 0;
+                        (void)frexpf(now, &e3);
+                        grown = e3 - grown;
+                    }
+                    st.drop = (float)min(grown, 100);
+                    st.grow = ldexpf(1.f, min(grown, 100));
+                    st.shrink = ldexpf(1.f, min(100 - grown, 0));
                     st.ref = now;
                     st.absent = least < 0.f;
                     st.dead = dead;
@@ -310,10 +326,10 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                 after = entry(t + 4);
                 fetch(t + 1);
             }
-            float shrink = 1.f;
+            float grow = 1.f;
             if (is) {
                 ref_of_sums = st.ref;
-                shrink = st.shrink;
+                grow = st.grow;
             }
             // a wave whose rows see nothing of the step leaves it
             const bool sees = is && base <= pos_most && (a.window == 0 || base + KV_TILE - 1 > pos_least - a.window);
@@ -370,9 +386,14 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                 next = entry(t + 4);
                 fetch(t + 2);
             }
-            if (shrink < 1.f) {
+            if (grow > 1.f) {
+                m -= st.drop;
+                l = fminf(l * grow, 0x1p126f);
+                const float shrink = st.shrink;
+                if (shrink < 1.f) {
 #pragma unroll
-                for (int b = 0; b < M::NB; ++b) o[b] *= shrink;
+                    for (int b = 0; b < M::NB; ++b) o[b] *= shrink;
+                }
             }
             if (sees) {
                 // scores in powers of two; element e of x[u]: position base + 32 u + 16 (e / 8) + 8 half + e % 8
@@ -397,14 +418,14 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                     const v16f& y = x[n / 2];
                     const int e = 8 * (n % 2);
                     const float part_top = max3(max3(max3(y[e], y[e + 1], y[e + 2]), y[e + 3], y[e + 4]), y[e + 5], max3(y[e + 6], y[e + 7], y[e + 7]));
-                    top = fmaxf(top, part_top * by[n]);
+                    top = fmaxf(top, fmaf(part_top, by[n], st.share[n]));
                 }
                 {
                     const auto r2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                     top = fmaxf(__uint_as_float(r2[0]), __uint_as_float(r2[1]));
                 }
                 if (__ballot(top > m + SLACK || (m == -INFINITY && top > m)) != 0) {
-                    const float m_new = fmaxf(m, top);
+                    const float m_new = fmaxf(m, ceilf(top));
                     const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
                     l *= keep;
 #pragma unroll

@@ -352,3 +352,28 @@ def test_pages_that_a_row_does_not_see_do_not_cost_it_bits(length, fresh, window
     b.want.scales["v"] *= np.float32(2.0 ** ratio)
     b.want.scales["v"][b.table[0, list(hidden)]] = 1.0
     b.check(window=window)
+
+
+@pytest.mark.parametrize("dtype,ratio", [(d, r) for d in sorted(TYPES) for r in (-4, -8, -12, -16, -20, -28, -40, -60) if d != "f16" or r >= -12])   # (f16: normal numbers)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("length,fresh,window,hidden", [(300, 40, 0, (18,)), (300, 40, 0, (17,)), (400, 40, 70, (16, 17, 18)), (400, 40, 70, (18, 19)), (400, 100, 0, (20, 21, 22, 23, 24)),
+                                                        (3000, 33, 500, (156, 157, 186)), (3000, 300, 0, (170, 186))])
+def test_pages_that_a_row_of_a_prompt_does_not_see_do_not_cost_it_bits(length, fresh, window, hidden, dim, dtype, ratio):
+    b = Batch([length], [fresh], 2, 1, dim, 16, dtype, seed=54)
+    b.want.scales["v"] *= np.float32(2.0 ** ratio)
+    b.want.scales["v"][b.table[0, list(hidden)]] = 1.0
+    b.check(window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fresh", [1, 40])
+def test_value_scales_that_grow_again_and_again(fresh, dtype):
+    """Each page's values a multiple of the ones before: every step's sums are put to another size, up to what f32 holds."""
+    for step in (0.5, 3.0, 12.0):
+        b = Batch([500], [fresh], 4, 2, 64, 16, dtype, seed=55)
+        n = int((b.table[0] >= 0).sum())
+        powers = np.minimum(-120 + step * np.arange(n), 90)
+        b.want.scales["v"][b.table[0, :n]] = (2.0 ** powers)[:, None].astype(np.float32)
+        b.check()
+        b.want.scales["v"][b.table[0, :n]] = (2.0 ** powers[::-1])[:, None].astype(np.float32)
+        b.check()
