@@ -192,21 +192,24 @@ __global__ __launch_bounds__(64 * WRITE_WAVES) void kv_write_kernel(const T* __r
                 break;
             }
         if (inside) continue;
-        // The run's length; whether it holds the page's first token; whether its rows are the page's tokens in their order.
-        int n = 0;
+        // The run's rows, up to the last present one (a batch's padding may follow); whether it holds the page's first token; whether its
+        // rows are the page's tokens in their order.
+        int n = 0, rows_there = 0;
         bool anew = false, straight = true;
-        for (int skip = at;; skip = 0) {
-            const int t = n == 0 ? base + lane : t0 + n + lane;
-            const int64_t slot = n == 0 ? my_slot : slot_at(t), here = page_of(slot);
+        for (int skip = at, t_here = base;; skip = 0, t_here += 64) {
+            const int t = t_here + lane;
+            const int64_t slot = t_here == base ? my_slot : slot_at(t), here = page_of(slot);
             const uint64_t from = ~0ull << skip;
             const uint64_t ends = __ballot(t >= tokens || (here >= 0 && here != page)) & from;
             const int stop = ends ? __ffsll((unsigned long long)ends) - 1 : 64;
-            const uint64_t in = from & (stop == 64 ? ~0ull : (1ull << stop) - 1);
-            anew = anew || (__ballot(here == page && (slot & (P - 1)) == 0) & in) != 0;
-            straight = straight && (__ballot(slot != slot0 + (t - t0)) & in) == 0;
-            n += stop - skip;
+            const uint64_t there = __ballot(here == page) & from & (stop == 64 ? ~0ull : (1ull << stop) - 1);
+            anew = anew || (__ballot((slot & (P - 1)) == 0) & there) != 0;
+            straight = straight && (__ballot(slot != slot0 + (t - t0)) & there) == 0;
+            rows_there += __popcll(there);
+            if (there) n = t_here + 64 - __clzll((long long)there) - t0;
             if (stop < 64) break;
         }
+        straight = straight && rows_there == n;
         const bool whole = straight && n == P;   // (then it starts with the first)
         float x[ROWS_HELD][4];
         int64_t off[ROWS_HELD];   // the token's place in the page; -1: not the page's
