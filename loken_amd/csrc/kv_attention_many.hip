@@ -17,14 +17,14 @@
 //
 // A row's sums go by 2^m, m a whole number about the largest of score + logarithm of the share among the positions that the row sees: so
 // neither small scales nor large ones of pages that it does not see cost its weights bits in f16. They are put to a new m only where
-// that lies 2^8 above: weights times shares up to 2^8 then, which stand LIFT = 2^7 above one and stay below 2^15, f16's largest; one of
+// that lies 2^8 above: weights times shares up to 2^8 then, which stand LIFT = 2^7 above one and stay within 2^15, which f16 holds; one of
 // 2^-21 still has all its bits, one of 2^-31 some. Where `ref` grows, m falls by as much and the sums of values stay as they are.
 //
 // A wave's step is 32 products of 32 cycles (twice as many in f32) and some 400 other instructions, 32 of them exponentials, which
 // take four times as long. It is these that bound it, and what of them does not run beside products: so a product comes with
 // six of them in turn, its operands read from LDS a group ahead, and nothing that is loaded is looked at before the step after.
-// 2048 tokens of one prompt, 32 heads over 8 of 128 bf16 values: 69 us, 500 TFLOP/s of the causal half's products (two starts of 5 us a
-// CU in it); the same behind 16384 tokens 683 us, 850 TFLOP/s, in f32 1060; 700 f32 rows over 2200 positions beside eleven single rows: 108 us.
+// 2048 tokens of one prompt, 32 heads over 8 of 128 bf16 values: 70 us, 490 TFLOP/s of the causal half's products (two starts of 5 us a
+// CU in it); the same behind 16384 tokens 700 us, 830 TFLOP/s, in f32 1110; 700 f32 rows over 2200 positions beside eleven single rows: 108 us.
 
 #include "kv_attention.h"
 
@@ -94,7 +94,7 @@ struct Many {
 };
 
 // What a step's pages have for everybody.
-struct Step {
+struct __attribute__((aligned(16))) Step {
     float ks[RUNS];     // key scales; -1: the page is absent
     float share[RUNS];  // log2 of the value scale over `ref`; -FAR where the values do not show
     float bias[RUNS];   // that, and LIFT; -infinity where the values do not show
@@ -248,9 +248,8 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                 const float k1 = page_of_run < 0 ? -1.f : ks, v1 = page_of_run < 0 ? 0.f : vs;
                 const float most = across_runs(v1, [](float x, float y) { return fmaxf(x, y); });
                 const float least = across_runs(k1, [](float x, float y) { return fminf(x, y); });
-                int e2 = 0;
-                (void)frexpf(most, &e2);
-                const float now = most > 0.f ? fmaxf(ref, ldexpf(1.f, min(e2, 127))) : ref;
+                // the power of two above `most`, from its exponent
+                const float now = most > 0.f ? fmaxf(ref, __uint_as_float(min((__float_as_uint(most) & 0x7F800000u) + 0x00800000u, 0x7F000000u))) : ref;
                 const bool shows = v1 > now * LEAST_SHARE;
                 const float share = shows ? __builtin_amdgcn_logf(v1 / now) : -FAR, bias = shows ? share + LIFT : -INFINITY;
                 st.ks[lane] = k1;
@@ -259,16 +258,11 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                 st.back[lane] = shows ? __builtin_amdgcn_exp2f(-bias) : 0.f;
                 const uint32_t dead = (uint32_t)__ballot(!shows);
                 if (lane == 0) {
-                    int grown = 0;   // (up to the first scale the sums are zeros)
-                    if (ref > 0.f) {
-                        (void)frexpf(ref, &grown);
-                        int e3 = 0;
-                        (void)frexpf(now, &e3);
-                        grown = e3 - grown;
-                    }
-                    st.drop = (float)min(grown, 100);
-                    st.grow = ldexpf(1.f, min(grown, 100));
-                    st.shrink = ldexpf(1.f, min(100 - grown, 0));
+                    // (up to the first scale the sums are zeros)
+                    const int grown = ref > 0.f ? (int)((__float_as_uint(now) - __float_as_uint(ref)) >> 23) : 0, drop = min(grown, 100);
+                    st.drop = (float)drop;
+                    st.grow = __uint_as_float((uint32_t)(127 + drop) << 23);
+                    st.shrink = grown - drop > 126 ? 0.f : __uint_as_float((uint32_t)(127 - (grown - drop)) << 23);
                     st.ref = now;
                     st.absent = least < 0.f;
                     st.dead = dead;
@@ -398,9 +392,12 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
             if (sees) {
                 // scores in powers of two; element e of x[u]: position base + 32 u + 16 (e / 8) + 8 half + e % 8
                 const bool whole = base + KV_TILE - 1 <= pos_least && (a.window == 0 || base > pos_most - a.window) && !st.absent;
-                float by[RUNS], top = -INFINITY;
+                float by[RUNS], share[RUNS], top = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < RUNS; ++n) by[n] = st.ks[n] * unit;
+                for (int n = 0; n < RUNS; ++n) {
+                    by[n] = st.ks[n] * unit;
+                    share[n] = st.share[n];
+                }
                 if (!whole) {
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
@@ -418,7 +415,7 @@ __global__ __launch_bounds__(many_teams(sizeof(T) == 4, D) * THREADS, many_waves
                     const v16f& y = x[n / 2];
                     const int e = 8 * (n % 2);
                     const float part_top = max3(max3(max3(y[e], y[e + 1], y[e + 2]), y[e + 3], y[e + 4]), y[e + 5], max3(y[e + 6], y[e + 7], y[e + 7]));
-                    top = fmaxf(top, fmaf(part_top, by[n], st.share[n]));
+                    top = fmaxf(top, fmaf(part_top, by[n], share[n]));
                 }
                 {
                     const auto r2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
