@@ -5,8 +5,9 @@
 // its own in a 16-row operand that a few rows would leave mostly empty: three digits for f32 (24 bits with the sign), two for f16
 // and bf16 (a key's code holds 7 bits of its page's largest value, the query's two digits 15 of its row's). So
 //     q . k = s_q s_k sum_i 256^i (digit_i . code),    sum_j p_j v_j = (v_max / F) sum_i 256^i (digit_i(p_j F s_v,j / v_max) . code_j)
-// where every product in parentheses is exact in int32, over the head dimension or over a step of 64 positions. Weights are taken
-// relative to the step's own maximum before they are cut into digits, so a step far below the row's maximum loses no bits.
+// where every product in parentheses is exact in int32, over the head dimension or over a step of 64 positions, and v_max is the largest value
+// scale that the row sees in the step. Weights are taken relative to the step's own maximum before they are cut into digits, so a step far
+// below the row's maximum loses no bits.
 //
 // One wave takes a step: 64 positions as four runs of sixteen. v_mfma_i32_16x16x64_i8 gives the scores as (16 positions) x
 // (16 slots); the positions of its operand are chosen so that lane group g ends with the sixteen of run g, which is how the second
