@@ -13,7 +13,7 @@ Head layouts and vocabularies are those of the benchmark's configurations (32 he
 151936 words) and generic ones. Activations are N(0, 1); logits N(0, 3) with a few words well ahead of the others.
 
 The cache: blocks of 32 neighbouring values of a token and head share a power of two, 2^(byte - 127); a value is a sign
-and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 times that. A byte holds two neighbours, the first in its low half.
+and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 times that. Powers written are 2^-96 and above. A byte holds two neighbours, the first in its low half.
   keys    [pages, kv_heads, page, dim / 2], their powers [pages, kv_heads, page, dim / 32]
   values  [pages, kv_heads, page / 4, 16, 4, dim / 32]: four tokens, a sixteenth of the head of each together;
           their powers [pages, kv_heads, dim / 32, page]
@@ -278,7 +278,7 @@ def _held(x):
     """Rows [rows, heads, dim] as the cache's values, in 64 bits: borders of codes and powers are not to be missed."""
     blocks = x.double().unflatten(-1, (-1, 32))
     part, power = torch.frexp(blocks.abs().amax(-1, keepdim=True))
-    power = torch.where(part == 0, -124, power - 3 + (part >= 0.875).int()).clamp(-124, 125)
+    power = torch.where(part == 0, -96, power - 3 + (part >= 0.875).int()).clamp(-96, 125)
     power = torch.tensor(POWERS, dtype=torch.float64, device=DEV)[power.long() + 127]
     ladder = torch.tensor(LADDER + tuple(-v for v in LADDER), dtype=torch.float64, device=DEV)
     return (ladder[_nearest(blocks / power).long()] * power).flatten(-2)
@@ -465,7 +465,7 @@ def _held_exact(x):
     for b in range(0, x.shape[-1], 32):
         block = x[..., b:b + 32]
         peak = block.abs().amax(-1, keepdim=True)
-        unit = torch.full_like(peak, 2.0 ** -124)
+        unit = torch.full_like(peak, 2.0 ** -96)
         while bool((peak >= 7 * unit).any()):
             unit = torch.where(peak >= 7 * unit, 2 * unit, unit)
         steps = torch.tensor(LADDER, dtype=torch.float64, device=DEV)
