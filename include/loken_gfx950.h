@@ -848,6 +848,65 @@ int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, void* out, int
 int lk_sample(const void* logits, int type, int64_t stride, int rows, int vocab, const float* uniform, const float* temperature,
               const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, float* probs, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Norms of the query and key heads and their rotation in one pass; the cache in 4 bits and attention over it. No counterparts in the
+ * reference.
+ * ------------------------------------------------------------------------------------- */
+#define LK_ROTARY_AXES 4
+
+/* Rows of queries [rows][heads][head_dim] and keys [rows][kv_heads][head_dim] of `type` (*_stride elements from row to row), head_dim 64, 128
+ * or 256, into q_out and k_out (the same rows, or rows that share nothing with any input):
+ *   y = x / sqrt(mean x^2 + eps) * weight       (weights f32 [head_dim]; null: y = x)
+ *   pairs i < `pairs` of y, (i, i + pairs), or with `neighbours` (2 i, 2 i + 1):  (a, b) -> factor * (a cos - b sin, a sin + b cos)
+ *   angle = positions[axis[i] * axis_stride + row] * frequencies[i]           (radians; made in 64 bits)
+ * Values past 2 * pairs are not rotated. pairs: a multiple of 4, up to head_dim / 2. positions: int32, `axes` (1 .. LK_ROTARY_AXES) runs of
+ * rows; axis: uint8 [pairs], null: axis 0 for all (one past the last counts as the last). Computed in f32, rounded once. */
+int lk_qk_norm_rope(const void* q, const void* k, int type, int64_t q_stride, int64_t k_stride, void* q_out, void* k_out,
+                    int64_t q_out_stride, int64_t k_out_stride, int rows, int heads, int kv_heads, int head_dim, const float* q_weight,
+                    const float* k_weight, float eps, const int32_t* positions, int64_t axis_stride, int axes, const float* frequencies,
+                    const uint8_t* axis, int pairs, int neighbours, float factor, void* stream);
+
+/* The cache in 4 bits: MXFP4 blocks of 32 neighbouring values of a token and head, 2^(power - 127) times codes e2m1 (bit 3 the sign; 0, 1/2, 1,
+ * 3/2, 2, 3, 4, 6), two to a byte, the first in its low half. Pages, slots and tables as above:
+ *   k_codes    [pages][kv_heads][page_tokens][head_dim / 2]
+ *   v_codes    [pages][kv_heads][page_tokens / 4][16][4][head_dim / 32]    of four tokens a sixteenth of the row each, together
+ *   k_powers   [pages][kv_heads][page_tokens][head_dim / 32]
+ *   v_powers   [pages][kv_heads][head_dim / 32][page_tokens]
+ * all 16-byte aligned.
+ *
+ * New rows into the slots that `slots` names, as lk_kv_write_q8 takes them, but in any order: a token's bytes are its own. Where a slot is
+ * named twice, what it holds then is not defined. Per block, over its finite x:
+ *   E = the least with max |x| < 7 * 2^E, within -96 .. 125; power = E + 127
+ *   codes: the nearest to x / 2^E, halves to the even code, +-6 past it
+ * An infinite x is stored as +-6, one that is not a number as 0. */
+int lk_kv_write_mxfp4(const void* k, const void* v, int type, int64_t k_stride, int64_t v_stride, const int64_t* slots, int tokens,
+                      int kv_heads, int head_dim, int page_tokens, int pages, void* k_codes, void* v_codes, void* k_powers, void* v_powers,
+                      void* stream);
+
+/* Rows of the cache as values, zeros where a slot is absent. Any power is read (255: no number). */
+int lk_kv_read_mxfp4(const int64_t* slots, int tokens, int kv_heads, int head_dim, int page_tokens, int pages, const void* k_codes,
+                     const void* v_codes, const void* k_powers, const void* v_powers, void* k_out, void* v_out, int type, void* stream);
+
+/* lk_qk_norm_rope whose keys go into the cache in place of k_out, and with them the rows v (not rotated), as lk_kv_write_mxfp4 writes them. The
+ * keys' norm and rotation are computed in 64 bits, and their codes made of those: no key comes out as a border's other code for a rounding
+ * before it. A row whose slot is absent writes its queries alone. */
+int lk_qk_norm_rope_kv_mxfp4(const void* q, const void* k, const void* v, int type, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                             void* q_out, int64_t q_out_stride, const int64_t* slots, int rows, int heads, int kv_heads, int head_dim,
+                             const float* q_weight, const float* k_weight, float eps, const int32_t* positions, int64_t axis_stride,
+                             int axes, const float* frequencies, const uint8_t* axis, int pairs, int neighbours, float factor,
+                             int page_tokens, int pages, void* k_codes, void* v_codes, void* k_powers, void* v_powers, void* stream);
+
+/* Attention of the batch's rows over the 4-bit cache: lk_kv_attention_q8's arguments, rows, masks, absent pages and limits, and
+ *   cap > 0: scores are cap * tanh(scale * q . k / cap) before the softmax   (0: as they are)
+ * Powers below 31 and above 252, which nothing here writes, are not defined at positions that some row sees. Products are exact but for the softmax weights, which
+ * are held to 24 bits in f32 and 16 in f16 and bf16 (8 where bf16 comes in many rows of a sequence); sums are f32. A query value keeps all its bits down to 2^-126. A product of a
+ * row and a key, and a sum of weights times values, have to be numbers of f32. Scratch as for lk_kv_attention_q8. */
+int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, void* out, int64_t out_stride, const void* k_codes, const void* v_codes,
+                          const void* k_powers, const void* v_powers, int pages, int page_tokens, const int32_t* table,
+                          int64_t table_stride, int table_cols, const int32_t* lens, const int32_t* starts, int seqs, int rows,
+                          int max_fresh, int max_len, int heads, int kv_heads, int head_dim, float scale, int window, float cap,
+                          void* stream);
+
 /* Frees what the expert launchers, the expert block, the router, the f16 tiles, attention and sampling hold on the current device, for
  * every stream and every recorded graph: none recorded over them may be replayed after. The host linears' workspaces
  * stay (lkh_release_workspaces). Synchronizes the device (cuda/moe/moe_gguf.cu:104-118). */

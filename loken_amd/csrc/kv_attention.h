@@ -1,4 +1,4 @@
-// What the kernels of lk_kv_attention_q8 share: the call, which rows and positions a workgroup has, and partial results.
+// What the attention kernels over the paged caches share: the call, which rows and positions a workgroup has, and partial results.
 #pragma once
 #include <math.h>
 
@@ -137,3 +137,6 @@ constexpr int kv_few_rows(bool f32, int head_dim, int max_rows) {
 
 int kv_attention_few(const Attend& a, int type, int head_dim, int max_rows, hipStream_t stream);
 int kv_attention_many(const Attend& a, int type, int head_dim, int max_rows, hipStream_t stream);
+// Joins the parts of a launch before it: of the few-rows kernel's sequences (`few`), `tokens` of whose rows a launch counts on, or of the others;
+// `per` rows of a workgroup had the same parts.
+int kv_attention_join(const Attend& a, int type, int head_dim, int per, bool few, int tokens, hipStream_t stream);

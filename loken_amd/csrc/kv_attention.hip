@@ -205,6 +205,16 @@ static int join(const Attend& a, int head_dim, int per, bool few, int tokens, hi
     return head_dim == 64 ? join_of<T, 64>(a, per, few, tokens, s) : head_dim == 128 ? join_of<T, 128>(a, per, few, tokens, s) : join_of<T, 256>(a, per, few, tokens, s);
 }
 
+}  // namespace
+
+int kv_attention_join(const Attend& a, int type, int head_dim, int per, bool few, int tokens, hipStream_t s) {
+    if (type == LK_TYPE_F32) return join<float>(a, head_dim, per, few, tokens, s);
+    if (type == LK_TYPE_F16) return join<__half>(a, head_dim, per, few, tokens, s);
+    return join<__hip_bfloat16>(a, head_dim, per, few, tokens, s);
+}
+
+namespace {
+
 // Sequences of up to this many rows (token, head of a group) are the few-rows kernel's.
 constexpr int FEW_ROWS = 16;
 
@@ -323,15 +333,10 @@ extern "C" int lk_kv_attention_q8(const void* q, int type, int64_t q_stride, voi
         af.part_o = mem + 2 * (part_rows_f + part_rows_m);
         am.part_o = af.part_o + part_rows_f * head_dim;
     }
-    auto join_parts = [&](const Attend& x, int per, bool is_few, int toks) {
-        if (type == LK_TYPE_F32) return join<float>(x, head_dim, per, is_few, toks, s);
-        if (type == LK_TYPE_F16) return join<__half>(x, head_dim, per, is_few, toks, s);
-        return join<__hip_bfloat16>(x, head_dim, per, is_few, toks, s);
-    };
     int status = LK_OK;
     if (many) status = kv_attention_many(am, type, head_dim, max_rows, s);
     if (status == LK_OK && few) status = kv_attention_few(af, type, head_dim, few_max, s);
-    if (status == LK_OK && part_rows_m) status = join_parts(am, KV_MANY_ROWS, false, tokens);
-    if (status == LK_OK && part_rows_f) status = join_parts(af, few_per, true, many ? few_limit / group : tokens);
+    if (status == LK_OK && part_rows_m) status = kv_attention_join(am, type, head_dim, KV_MANY_ROWS, false, tokens, s);
+    if (status == LK_OK && part_rows_f) status = kv_attention_join(af, type, head_dim, few_per, true, many ? few_limit / group : tokens, s);
     return status;
 }

@@ -1,0 +1,66 @@
+// What the kernels of lk_kv_attention_mxfp4 share: the call, and how 4-bit codes become operands of the matrix unit.
+#pragma once
+#include "kv_attention.h"
+#include "kv_mxfp4.h"
+
+// Parts, pieces and rows are those of the 8-bit cache's attention; `pool` of it holds sizes alone.
+struct AttendMx : Attend {
+    MxPool mx;
+    float cap;   // above 0: scores are cap * tanh(score / cap)
+};
+
+typedef __bf16 mx_b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 mx_b8 __attribute__((ext_vector_type(8)));
+typedef float mx_f2 __attribute__((ext_vector_type(2)));
+
+// Byte `SEL` of `w`, two codes, times a power of two: as two bf16, exactly.
+template <int SEL>
+static __device__ __forceinline__ uint32_t mx_two(uint32_t w, float power) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, power, SEL));
+}
+// A word, eight codes, as an operand of eight bf16.
+static __device__ __forceinline__ mx_b8 mx_eight(uint32_t w, float power) {
+    return __builtin_bit_cast(mx_b8, make_uint4(mx_two<0>(w, power), mx_two<1>(w, power), mx_two<2>(w, power), mx_two<3>(w, power)));
+}
+// Byte `I` of a word of powers, 2^(byte - 127).
+template <int I>
+static __device__ __forceinline__ float mx_power_of(uint32_t w) {
+    return __uint_as_float((I == 3 ? w >> 1 : w << (23 - 8 * I)) & 0x7F800000u);
+}
+
+static __device__ __forceinline__ uint32_t mx_pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((mx_f2){a, b}, mx_b2));   // the nearest
+}
+// Two numbers as PIECES pairs of bf16 whose sums they are: to 8, 16 or 24 bits.
+template <int PIECES>
+static __device__ __forceinline__ void mx_pieces(float a, float b, uint32_t (&out)[PIECES]) {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        out[p] = mx_pack(a, b);
+        if (p + 1 < PIECES) {
+            a -= __uint_as_float(out[p] << 16);
+            b -= __uint_as_float(out[p] & 0xFFFF0000u);
+        }
+    }
+}
+
+// A score in powers of two from a product: `by` = scale * log2(e), or with a cap scale / cap.
+template <bool FINE>
+static __device__ __forceinline__ float mx_score(float product, float by, float cap) {
+    const float x = product * by;
+    if (!(cap > 0.f)) return x;
+    // tanh x = 1 - 2 / (e^2x + 1), off by 1.2e-7; below a quarter, for f32, by its series: to a few last places of x
+    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.8853900817779268f) + 1.f);
+    float t = far;
+    if (FINE) {
+        const float s = x * x;
+        const float near = fmaf(x * s, fmaf(s, fmaf(s, fmaf(s, 0.021869488f, -0.053968254f), 0.13333334f), -0.33333334f), x);
+        t = fabsf(x) < 0.25f ? near : far;
+    }
+    return t * (cap * 1.4426950408889634f);
+}
+
+// Rows of a workgroup of the few-rows kernel: one or two operands of sixteen.
+constexpr int mx_few_rows(int head_dim, int max_rows) { return head_dim < 256 && max_rows > 16 ? 32 : 16; }
+
+int kv_attention_mxfp4_few(const AttendMx& a, int type, int head_dim, int max_rows, hipStream_t stream);

@@ -1,0 +1,395 @@
+// Attention over the 4-bit cache for a few rows of a sequence: single tokens, and the handful a draft brings.
+//
+// Both products run on v_mfma_f32_16x16x32_bf16: a code times its block's power of two is a bf16 exactly, two codes an instruction, and so are
+// queries and softmax weights as sums of bf16 pieces (bf16 queries one, f16 two, f32 three; weights two, f32 three). Products are then exact but for
+// weights of 16 bits, sums are f32.
+//
+// One wave takes a step: 64 positions as four tiles of sixteen. Scores come as (16 positions) x (16 rows): a lane holds row l % 16 and four positions
+// of each tile, which are, two tiles together, what the second product wants of the weights in that lane: nothing crosses lanes but maxima.
+// The values' operand is (16 columns) x (32 positions): the cache has the values of four tokens that a lane takes in one piece; codes of one token
+// become bf16 by its block's power, and halves of words change places to bring a column's positions together.
+// Sums come as (16 columns) x (16 rows): a lane's row again, so maxima and corrections are the lane's own.
+//
+// Loads of the next step's keys go out once the scores have been taken, its values' once the sums have been: both are in flight through the other
+// half of the step. Four waves take steps in turn and meet in LDS; long contexts are cut into parts, which a second launch joins.
+
+#include "kv_attention_mxfp4.h"
+
+namespace {
+
+constexpr int WAVES = 4;
+
+static __device__ __forceinline__ float max_over_groups(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+static __device__ __forceinline__ float sum_over_groups(float v) { return swap_add32(swap_add16(v)); }
+
+template <int WORDS>
+struct __attribute__((aligned(WORDS >= 4 ? 16 : 8))) Words { uint32_t w[WORDS]; };
+
+template <typename T, int D, int NT>
+struct Few {
+    static constexpr int PIECES = sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1;   // of a query value
+    static constexpr int SHARES = sizeof(T) == 4 ? 3 : 2;                                         // of a weight
+    static constexpr int ROWS = 16 * NT, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
+    // waves of a SIMD that the registers leave room for
+    static constexpr int ON_SIMD = D == 256 || (D == 128 && NT == 2) ? 1 : 2;
+};
+
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_kernel(AttendMx a, int row_tiles) {
+    using F = Few<T, D, NT>;
+    __shared__ float sums[WAVES][16][D + 4];
+    __shared__ float tops[WAVES][F::ROWS], weights[WAVES][F::ROWS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int shift = a.mx.page_shift;
+    // The workgroup's place: (part, row tile, head, sequence), the part fastest; or (head, piece), a piece being of one or
+    // several sequences.
+    int kv, seq, seq_end, tile0 = 0, part = 0;
+    int first_step = 0, at_step = 0, end_step = 0, length = 1;   // the first step of `seq`, the piece's steps, and how many a piece has
+    if (a.chunks) {
+        kv = blockIdx.x % a.mx.heads;
+        part = blockIdx.x / a.mx.heads;
+        const KvPieces pieces(a, F::ROWS);
+        length = pieces.length;
+        if ((int64_t)part * length >= pieces.total) return;
+        at_step = part * length;
+        end_step = (int)min((int64_t)at_step + length, (int64_t)pieces.total);
+        seq = __builtin_amdgcn_readfirstlane(KvPieces::sequence_at(a, F::ROWS, at_step, first_step));
+        first_step = __builtin_amdgcn_readfirstlane(first_step);
+        seq_end = a.seqs;
+        row_tiles = 1;
+    } else {
+        unsigned at = blockIdx.x;
+        part = at % a.splits;
+        at /= a.splits;
+        tile0 = at % row_tiles;
+        at /= row_tiles;
+        kv = at % a.mx.heads;
+        seq = at / a.mx.heads;
+        seq_end = seq + 1;
+    }
+    for (int steps = 0; seq < seq_end && (a.chunks == 0 || first_step < end_step); ++seq, first_step += steps) {
+      const KvSeq s(a, seq);
+      const int64_t rows_of_all = (int64_t)s.tokens() * a.group;
+      steps = 0;
+      if (rows_of_all == 0 || rows_of_all > a.few_rows) continue;
+      const int all_rows = (int)rows_of_all;
+      for (int tile = tile0; tile * F::ROWS < all_rows; tile += row_tiles) {
+        const int r0 = tile * F::ROWS, r1 = min(r0 + F::ROWS, all_rows) - 1;
+        const KvSpan span(a, s, s.first + a.token_of(r0), s.first + a.token_of(r1));
+        int t_begin = 0, t_end = span.tiles;
+        int64_t to = -1;   // the first row of the sums' place among the parts; -1: they are not a part
+        if (a.chunks) {
+            steps = all_rows > F::ROWS ? 1 : max(1, span.tiles);   // as kv_steps_of
+            if (all_rows <= F::ROWS) {
+                t_begin = max(at_step - first_step, 0);
+                t_end = min(end_step - first_step, span.tiles);
+                if (first_step < at_step || first_step + steps > end_step)
+                    to = (((int64_t)kv * a.chunks + part) * 2 + (first_step / length == part ? 1 : 0)) * F::ROWS;
+            }
+        } else {
+            if (part >= span.parts) continue;
+            t_begin = part * span.per_part;
+            t_end = min(span.tiles, t_begin + span.per_part);
+            if (span.parts > 1) to = 0;
+        }
+        // positions that some row of the tile sees: [seen_from, span.hi)
+        const int seen_from = a.window > 0 ? (int)max((int64_t)0, s.pos_of_0 + s.first + a.token_of(r0) - a.window + 1) : 0;
+
+        const int32_t* entries = a.table + seq * a.table_stride;
+        // the page of a step's tile; -1: absent, or behind the last position
+        auto page_of = [&](int t, int b) {
+            const int p0 = span.lo + t * KV_TILE + 16 * b;
+            const int page = t < t_end && p0 < span.hi ? entries[p0 >> shift] : -1;
+            return (unsigned)page < (unsigned)a.mx.pages ? page : -1;
+        };
+        Words<F::W> k[4], v[4];
+        uint32_t kp[4], vp[4];   // powers: of the lane's block or two of a key; of four tokens' values
+        auto load_keys = [&](int t, const int (&pages)[4]) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int64_t page = (int64_t)max(pages[b], 0) * a.mx.heads + kv;
+                const int64_t tok = (page << shift) + ((span.lo + t * KV_TILE + 16 * b) & ((1 << shift) - 1)) + i;
+                k[b] = *(const Words<F::W>*)(a.mx.k + tok * (D / 2) + g * (D / 8));
+                if (D == 256) kp[b] = *(const uint16_t*)(a.mx.k_powers + tok * F::PART + 2 * g);
+                else kp[b] = a.mx.k_powers[tok * F::PART + (D == 64 ? g >> 1 : g)];
+            }
+        };
+        auto load_values = [&](int t, const int (&pages)[4]) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int64_t page = (int64_t)max(pages[b], 0) * a.mx.heads + kv;
+                const int at = ((span.lo + t * KV_TILE + 16 * b) & ((1 << shift) - 1)) + 4 * g;
+                v[b] = *(const Words<F::W>*)(a.mx.v + (page << shift) * (D / 2) + ((at >> 2) * 16 + i) * (D / 8));
+                vp[b] = *(const uint32_t*)(a.mx.v_powers + (page << shift) * F::PART + ((i * F::PART / 16) << shift) + at);
+            }
+        };
+        int t = t_begin + wave;
+        int pages[4];   // of the step whose keys are loaded next
+#pragma unroll
+        for (int b = 0; b < 4; ++b) pages[b] = page_of(t, b);
+        if (t < t_end) {
+            load_keys(t, pages);
+            load_values(t, pages);
+        }
+
+        // the rows' pieces, and what a product is in scores
+        mx_b8 q[NT][F::KS][F::PIECES];
+        float unit[NT];
+        int pos[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = r0 + 16 * n + i;
+            const int of_seq = a.token_of(min(r, r1)), tok = s.first + of_seq, head = kv * a.group + min(r, r1) - of_seq * a.group;
+            pos[n] = r <= r1 ? (int)max(s.pos_of_0 + tok, (int64_t)-1) : -1;
+            const T* row = (const T*)a.q + tok * a.q_stride + (int64_t)head * D + g * (D / 4);
+            bool finite = true;
+#pragma unroll
+            for (int ks = 0; ks < F::KS; ++ks) {
+                const MxEight<T> raw = *(const MxEight<T>*)(row + 8 * ks);
+                uint32_t w[F::PIECES][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = to_f32(raw.v[2 * e]), y = to_f32(raw.v[2 * e + 1]);
+                    finite = finite && fabsf(x) < INFINITY && fabsf(y) < INFINITY;
+                    uint32_t both[F::PIECES];
+                    mx_pieces<F::PIECES>(x, y, both);
+#pragma unroll
+                    for (int p = 0; p < F::PIECES; ++p) w[p][e] = both[p];
+                }
+#pragma unroll
+                for (int p = 0; p < F::PIECES; ++p) q[n][ks][p] = __builtin_bit_cast(mx_b8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
+            }
+            const uint64_t odd = __ballot(!finite);
+            finite = (odd >> i & 0x0001000100010001ull) == 0;
+            unit[n] = finite ? (a.cap > 0.f ? a.scale / a.cap : a.scale * 1.4426950408889634f) : NAN;
+        }
+        int pos_least = 0x7FFFFFFF, pos_most = -1;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (r0 + 16 * n + i <= r1) { pos_least = min(pos_least, pos[n]); pos_most = max(pos_most, pos[n]); }
+        }
+        for (int o = 1; o < 16; o <<= 1) {
+            pos_least = min(pos_least, __shfl_xor(pos_least, o));
+            pos_most = max(pos_most, __shfl_xor(pos_most, o));
+        }
+
+        float m[NT], l[NT];
+        v4f acc[NT][F::NB];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n] = -INFINITY;
+            l[n] = 0.f;
+#pragma unroll
+            for (int b = 0; b < F::NB; ++b) acc[n][b] = (v4f){0.f, 0.f, 0.f, 0.f};
+        }
+
+        for (; t < t_end; t += WAVES) {
+            const int p0 = span.lo + t * KV_TILE;
+            // whether every row sees every position of the step
+            const bool here = pages[0] >= 0 && pages[1] >= 0 && pages[2] >= 0 && pages[3] >= 0;
+            const bool whole = p0 + KV_TILE - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && here;
+            v4f sc[NT][4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                v4f c[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) c[n] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < F::KS; ++ks) {
+                    const float power = D == 256 && ks >= F::KS / 2 ? mx_power_of<1>(kp[b]) : mx_power_of<0>(kp[b]);
+                    const mx_b8 op = mx_eight(k[b].w[ks], power);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int p = 0; p < F::PIECES; ++p) c[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, q[n][ks][p], c[n], 0, 0, 0);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sc[n][b] = c[n];
+            }
+            int next[4], absent = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                absent |= (pages[b] < 0) << b;
+                next[b] = page_of(t + WAVES, b);
+            }
+            if (t + WAVES < t_end) load_keys(t + WAVES, next);
+
+            uint32_t share[NT][F::SHARES][4][2];   // weights: of a tile's four positions
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float x[16], top = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = mx_score<sizeof(T) == 4>(sc[n][e >> 2][e & 3], unit[n], a.cap);
+                if (!whole) {
+                    const int last = pos[n] - p0 - 4 * g, first = a.window > 0 ? last - a.window : -0x40000000;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int at = 16 * (e >> 2) + (e & 3);
+                        if (at > last || at <= first || (absent >> (e >> 2) & 1)) x[e] = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
+                top = max_over_groups(top);
+                const float now = fmaxf(m[n], top), base = now == -INFINITY ? 0.f : now;   // (a row that is not finite has no top and stays that way)
+                if (__ballot(now > m[n])) {
+                    const float keep = __builtin_amdgcn_exp2f(m[n] - base);
+                    l[n] = m[n] == -INFINITY ? l[n] : l[n] * keep;
+#pragma unroll
+                    for (int b = 0; b < F::NB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[n][b][e] = m[n] == -INFINITY ? acc[n][b][e] : acc[n][b][e] * keep;
+                    m[n] = now;
+                }
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p[e] = __builtin_amdgcn_exp2f(x[4 * b + e] - base);
+                        l[n] += p[e];
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t both[F::SHARES];
+                        mx_pieces<F::SHARES>(p[2 * h], p[2 * h + 1], both);
+#pragma unroll
+                        for (int j = 0; j < F::SHARES; ++j) share[n][j][b][h] = both[j];
+                    }
+                }
+            }
+            if (!whole) {
+                // what no row sees may hold anything: its values count as zeros
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t seen = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int at = p0 + 16 * b + 4 * g + j;
+                        if (at >= seen_from && at < span.hi && !(absent >> b & 1)) seen |= 0xFFu << (8 * j);
+                    }
+                    vp[b] &= seen;
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int b0 = 2 * half;
+                float power[8];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    power[4 * b] = mx_power_of<0>(vp[b0 + b]);
+                    power[4 * b + 1] = mx_power_of<1>(vp[b0 + b]);
+                    power[4 * b + 2] = mx_power_of<2>(vp[b0 + b]);
+                    power[4 * b + 3] = mx_power_of<3>(vp[b0 + b]);
+                }
+                mx_b8 w[NT][F::SHARES];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < F::SHARES; ++j)
+                        w[n][j] = __builtin_bit_cast(mx_b8, make_uint4(share[n][j][b0][0], share[n][j][b0][1], share[n][j][b0 + 1][0], share[n][j][b0 + 1][1]));
+#pragma unroll
+                for (int byte = 0; byte < F::PART; ++byte) {   // columns 2 byte and 2 byte + 1 of the lane's sixteenth
+                    uint32_t c[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int at = (j & 3) * F::PART + byte;
+                        const uint32_t word = v[b0 + (j >> 2)].w[at >> 2];
+                        const int sel = at & 3;
+                        c[j] = sel == 0 ? mx_two<0>(word, power[j]) : sel == 1 ? mx_two<1>(word, power[j]) : sel == 2 ? mx_two<2>(word, power[j]) : mx_two<3>(word, power[j]);
+                    }
+                    uint32_t even[4], odd[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        even[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x05040100u);
+                        odd[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x07060302u);
+                    }
+                    const mx_b8 op0 = __builtin_bit_cast(mx_b8, make_uint4(even[0], even[1], even[2], even[3]));
+                    const mx_b8 op1 = __builtin_bit_cast(mx_b8, make_uint4(odd[0], odd[1], odd[2], odd[3]));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < F::SHARES; ++j) {
+                            acc[n][2 * byte] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op0, w[n][j], acc[n][2 * byte], 0, 0, 0);
+                            acc[n][2 * byte + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op1, w[n][j], acc[n][2 * byte + 1], 0, 0, 0);
+                        }
+                }
+            }
+            if (t + WAVES < t_end) load_values(t + WAVES, next);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) pages[b] = next[b];
+        }
+
+        // the four waves' sums relative to their common maximum, sixteen rows at a time
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float lw = sum_over_groups(l[n]);
+            if (g == 0) { tops[wave][16 * n + i] = m[n]; weights[wave][16 * n + i] = lw; }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (n) __syncthreads();
+            const int r = 16 * n + i;
+            const float top = fmaxf(fmaxf(tops[0][r], tops[1][r]), fmaxf(tops[2][r], tops[3][r]));
+            const float f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
+            // column of the sums: the lane's rows 4 g + e of the operand are sixteenths of the head
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int b = 0; b < F::NB; ++b) sums[wave][i][(4 * g + e) * (D / 16) + b] = acc[n][b][e] * f;
+            __syncthreads();
+            for (int at = threadIdx.x; at < min(r1 - r0 + 1 - 16 * n, 16) * D; at += 64 * WAVES) {
+                const int rr = at / D, d = at % D, row_of = 16 * n + rr;
+                const float most = fmaxf(fmaxf(tops[0][row_of], tops[1][row_of]), fmaxf(tops[2][row_of], tops[3][row_of]));
+                float total = 0.f, lw = 0.f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    total += sums[w][rr][d];
+                    // (a part whose scores are no numbers has no maximum and a sum that is none)
+                    lw += tops[w][row_of] == -INFINITY ? weights[w][row_of] : weights[w][row_of] * __builtin_amdgcn_exp2f(tops[w][row_of] - most);
+                }
+                const int of_seq = a.token_of(r0 + row_of), head = kv * a.group + r0 + row_of - of_seq * a.group;
+                const int64_t row = s.first + of_seq;
+                if (to < 0) {
+                    ((T*)a.out)[row * a.out_stride + (int64_t)head * D + d] = from_f32<T>(lw == 0.f ? 0.f : total / lw);
+                } else {
+                    const int64_t place = a.chunks ? to + row_of : (a.part_row(seq, s, (int)row) * a.heads + head) * a.splits + part;
+                    a.part_o[place * D + d] = total;
+                    if (d == 0) a.part_ml[place] = make_float2(most, lw);
+                }
+            }
+        }
+        __syncthreads();
+      }
+    }
+}
+
+template <typename T, int D>
+static int launch(const AttendMx& a, int max_rows, hipStream_t s) {
+    const int per = mx_few_rows(D, max_rows), row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / per + 1;
+    const int64_t blocks = a.chunks ? (int64_t)a.chunks * a.mx.heads : (int64_t)a.seqs * a.mx.heads * row_tiles * a.splits;
+    if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
+    if (per == 32) hipLaunchKernelGGL((mx_few_kernel<T, D, (D < 256 ? 2 : 1)>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a, row_tiles);
+    else hipLaunchKernelGGL((mx_few_kernel<T, D, 1>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a, row_tiles);
+    return lk_launch_status();
+}
+
+template <typename T>
+static int by_dim(const AttendMx& a, int head_dim, int max_rows, hipStream_t s) {
+    return head_dim == 64 ? launch<T, 64>(a, max_rows, s) : head_dim == 128 ? launch<T, 128>(a, max_rows, s) : launch<T, 256>(a, max_rows, s);
+}
+
+}  // namespace
+
+int kv_attention_mxfp4_few(const AttendMx& a, int type, int head_dim, int max_rows, hipStream_t s) {
+    if (type == LK_TYPE_F32) return by_dim<float>(a, head_dim, max_rows, s);
+    if (type == LK_TYPE_F16) return by_dim<__half>(a, head_dim, max_rows, s);
+    return by_dim<__hip_bfloat16>(a, head_dim, max_rows, s);
+}

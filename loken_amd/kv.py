@@ -1,4 +1,4 @@
-"""The paged 8-bit key / value cache of a served step, and attention over it.
+"""The paged key / value caches of a served step, in 8 and in 4 bits, and attention over them.
 
 Torch holds device memory and the current stream only; every computation goes through ``libloken_gfx950.so``
 (``lk_kv_*`` in ``include/loken_gfx950.h``, which states the formulas and what is done with absent pages). Per step:
@@ -114,6 +114,51 @@ class KvCacheQ8:
                    torch.zeros((pages, kv_heads), dtype=torch.float32, device=device))
 
 
+class KvCacheMxfp4:
+    """Pages of one layer's cache in 4 bits, blocks of 32 values of a token and head with a power of two each: uint8 ``k``
+    [pages, kv_heads, page_tokens, head_dim / 2], ``v`` [pages, kv_heads, page_tokens / 4, 16, 4, head_dim / 32], ``k_powers``
+    [pages, kv_heads, page_tokens, head_dim / 32], ``v_powers`` [pages, kv_heads, head_dim / 32, page_tokens]. These four are not
+    assigned anew. A row's bytes are its own: rows are written in any order."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_powers: torch.Tensor, v_powers: torch.Tensor):
+        if k.dim() != 4:
+            raise ValueError("kv cache: k is uint8 [pages, kv_heads, page_tokens, head_dim / 2]")
+        self.pages, self.kv_heads, self.page_tokens, self.head_dim = *k.shape[:3], 2 * k.shape[3]
+        if self.page_tokens not in PAGE_TOKENS or self.head_dim not in HEAD_DIMS or self.pages < 1 or self.kv_heads < 1:
+            raise ValueError(f"kv cache: pages of {PAGE_TOKENS} tokens, heads of {HEAD_DIMS} values")
+        of_page, blocks = (self.pages, self.kv_heads), self.head_dim // 32
+        if tuple(v.shape) != (*of_page, self.page_tokens // 4, 16, 4, blocks):
+            raise ValueError("kv cache: v is [pages, kv_heads, page_tokens / 4, 16, 4, head_dim / 32]")
+        if tuple(k_powers.shape) != (*of_page, self.page_tokens, blocks) or tuple(v_powers.shape) != (*of_page, blocks, self.page_tokens):
+            raise ValueError("kv cache: powers are [pages, kv_heads, page_tokens, head_dim / 32] and [pages, kv_heads, head_dim / 32, page_tokens]")
+        self._tensors = (k, v, k_powers, v_powers)
+        if any(t.dtype is not torch.uint8 for t in self._tensors):
+            raise ValueError("kv cache: its tensors are uint8")
+        if len({t.device for t in self._tensors}) != 1:
+            raise ValueError("kv cache: its tensors are on several devices")
+        if not all(t.is_contiguous() for t in self._tensors):
+            raise ValueError("kv cache: its tensors are contiguous")
+        if any(t.data_ptr() & 15 for t in self._tensors):
+            raise ValueError("kv cache: its tensors start on 16 bytes")
+
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_powers = property(lambda self: self._tensors[2])
+    v_powers = property(lambda self: self._tensors[3])
+
+    def _at(self):
+        """Where the tensors are now: a program may have given one other memory since."""
+        return tuple(t.data_ptr() for t in self._tensors)
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, head_dim: int, page_tokens: int = 16, device="cuda") -> "KvCacheMxfp4":
+        if page_tokens not in PAGE_TOKENS or head_dim not in HEAD_DIMS:
+            raise ValueError(f"kv cache: pages of {PAGE_TOKENS} tokens, heads of {HEAD_DIMS} values")
+        make = lambda *shape: torch.zeros((pages, kv_heads, *shape), dtype=torch.uint8, device=device)  # noqa: E731
+        return cls(make(page_tokens, head_dim // 2), make(page_tokens // 4, 16, 4, head_dim // 32), make(page_tokens, head_dim // 32),
+                   make(head_dim // 32, page_tokens))
+
+
 class KvPlan:
     """What ``kv_plan`` writes for ``seqs`` sequences and a batch of ``rows`` rows; kept from step to step (a recorded step
     holds its addresses)."""
@@ -156,7 +201,7 @@ def kv_plan(past: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free_p
     return plan
 
 
-def kv_write(cache: KvCacheQ8, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+def kv_write(cache: KvCacheQ8 | KvCacheMxfp4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """New keys and values ``[tokens, kv_heads, head_dim]`` (f32, f16 or bf16; rows may be parts of wider ones) into the cache."""
     tokens, _, ks = _rows("kv_write", "k", k, cache.kv_heads, cache.head_dim)
     of_v, _, vs = _rows("kv_write", "v", v, cache.kv_heads, cache.head_dim)
@@ -164,12 +209,13 @@ def kv_write(cache: KvCacheQ8, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
         raise ValueError("kv_write: keys and values are of one type and shape")
     _vector("kv_write", "slots", slots, torch.int64, tokens)
     _on_device("kv_write", k, v, slots, cache.k)
-    _lib.check("lk_kv_write_q8", _lib.load().lk_kv_write_q8(
+    name = "lk_kv_write_mxfp4" if isinstance(cache, KvCacheMxfp4) else "lk_kv_write_q8"
+    _lib.check(name, getattr(_lib.load(), name)(
         k.data_ptr(), v.data_ptr(), _X_TYPES[k.dtype], ks, vs, slots.data_ptr(), tokens, cache.kv_heads, cache.head_dim,
         cache.page_tokens, cache.pages, *cache._at(), _stream()))
 
 
-def kv_read(cache: KvCacheQ8, slots: torch.Tensor, dtype: torch.dtype = torch.float32):
+def kv_read(cache: KvCacheQ8 | KvCacheMxfp4, slots: torch.Tensor, dtype: torch.dtype = torch.float32):
     """Rows of the cache as values: keys and values ``[tokens, kv_heads, head_dim]``; zeros where a slot is absent."""
     if dtype not in _X_TYPES:
         raise ValueError("kv_read: f32, f16 or bf16")
@@ -177,17 +223,19 @@ def kv_read(cache: KvCacheQ8, slots: torch.Tensor, dtype: torch.dtype = torch.fl
     _on_device("kv_read", slots, cache.k)
     k = torch.empty((slots.numel(), cache.kv_heads, cache.head_dim), dtype=dtype, device=slots.device)
     v = torch.empty_like(k)
-    _lib.check("lk_kv_read_q8", _lib.load().lk_kv_read_q8(
+    name = "lk_kv_read_mxfp4" if isinstance(cache, KvCacheMxfp4) else "lk_kv_read_q8"
+    _lib.check(name, getattr(_lib.load(), name)(
         slots.data_ptr(), slots.numel(), cache.kv_heads, cache.head_dim, cache.page_tokens, cache.pages, *cache._at(), k.data_ptr(),
         v.data_ptr(), _X_TYPES[dtype], _stream()))
     return k, v
 
 
-def kv_attention(q: torch.Tensor, cache: KvCacheQ8, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor, *, max_fresh: int,
-                 max_len: int, scale: float | None = None, window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+def kv_attention(q: torch.Tensor, cache: KvCacheQ8 | KvCacheMxfp4, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor, *, max_fresh: int,
+                 max_len: int, scale: float | None = None, window: int = 0, softcap: float = 0.0,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the rows ``q`` ``[rows, heads, head_dim]`` over the cache, causal, each sequence's rows being its last positions;
     ``window`` > 0: that many positions, the row's own among them. Rows behind the last sequence stay as they are in ``out``
-    (without one: zeros). ``max_fresh``, ``max_len``: the most rows and tokens of a sequence as far as the caller knows them."""
+    (without one: zeros). ``softcap`` > 0 (the 4-bit cache alone): scores are softcap * tanh(score / softcap). ``max_fresh``, ``max_len``: the most rows and tokens of a sequence as far as the caller knows them."""
     seqs = lens.numel()
     rows, heads, stride = _rows("kv_attention", "q", q, None, cache.head_dim)
     if heads == 0 or heads % cache.kv_heads:
@@ -200,14 +248,19 @@ def kv_attention(q: torch.Tensor, cache: KvCacheQ8, table: torch.Tensor, lens: t
     scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else scale
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError("kv_attention: the scale is a number above zero")
+    in_4_bits = isinstance(cache, KvCacheMxfp4)
+    if not (softcap >= 0.0 and math.isfinite(softcap)) or (softcap and not in_4_bits):
+        raise ValueError("kv_attention: softcap is a number from zero on, and zero over the 8-bit cache")
     if out is None:
         out = torch.zeros((rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
     of_out, _, out_stride = _rows("kv_attention", "out", out, heads, cache.head_dim)
     if out.dtype is not q.dtype or of_out != rows:
         raise ValueError("kv_attention: out has the type and shape of q")
     _on_device("kv_attention", q, out, table, lens, starts, cache.k)
-    _lib.check("lk_kv_attention_q8", _lib.load().lk_kv_attention_q8(
+    name = "lk_kv_attention_mxfp4" if in_4_bits else "lk_kv_attention_q8"
+    _lib.check(name, getattr(_lib.load(), name)(
         q.data_ptr(), _X_TYPES[q.dtype], stride, out.data_ptr(), out_stride, *cache._at(), cache.pages, cache.page_tokens, table.data_ptr(),
         across, cols, lens.data_ptr(), starts.data_ptr(), seqs, rows, min(max_fresh, 0x7FFFFFFF),
-        min(max_len, 0x7FFFFFFF), heads, cache.kv_heads, cache.head_dim, scale, min(window, 0x7FFFFFFF), _stream()))
+        min(max_len, 0x7FFFFFFF), heads, cache.kv_heads, cache.head_dim, scale, min(window, 0x7FFFFFFF),
+        *((softcap,) if in_4_bits else ()), _stream()))
     return out

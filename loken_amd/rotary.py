@@ -1,0 +1,113 @@
+"""Norms of the query and key heads and their rotation in one pass (``lk_qk_norm_rope`` in ``include/loken_gfx950.h``, which states the
+formulas), and the same with keys and values going straight into the 4-bit cache. All of it can be recorded into a graph.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import lib as _lib
+from .kv import HEAD_DIMS, KvCacheMxfp4, _on_device, _rows, _vector
+from .ops import _X_TYPES, _stream
+
+MAX_AXES = 4
+
+
+class Rotary:
+    """A model's rotation: ``frequencies`` f32 [pairs], radians a position, scaled as the model wants them; ``axis`` uint8 [pairs], which
+    run of the positions turns a pair (time, height, width); pairs of ``neighbours`` (2 i, 2 i + 1) instead of (i, i + pairs); ``factor`` on
+    what is turned. Other tensors are another rotation: these two are not assigned anew."""
+
+    def __init__(self, frequencies: torch.Tensor, axis: torch.Tensor | None = None, neighbours: bool = False, factor: float = 1.0):
+        _vector("rotary", "frequencies", frequencies, torch.float32)
+        if frequencies.numel() % 4 or frequencies.numel() > max(HEAD_DIMS) // 2:
+            raise ValueError(f"rotary: a multiple of 4 pairs, up to {max(HEAD_DIMS) // 2}")
+        if axis is not None:
+            _vector("rotary", "axis", axis, torch.uint8, frequencies.numel())
+            if axis.device != frequencies.device:
+                raise ValueError("rotary: its tensors are on several devices")
+        if not math.isfinite(factor):
+            raise ValueError("rotary: the factor is a number")
+        self._tensors, self.neighbours, self.factor = (frequencies, axis), bool(neighbours), float(factor)
+
+    frequencies = property(lambda self: self._tensors[0])
+    axis = property(lambda self: self._tensors[1])
+
+
+def _arguments(what, q, k, positions, rotary, q_weight, k_weight, eps):
+    """Head dimension and sizes, what is checked of both calls' arguments, and the arguments that they share."""
+    if q.dim() != 3 or q.shape[2] not in HEAD_DIMS:
+        raise ValueError(f"{what}: heads of {HEAD_DIMS} values")
+    dim = q.shape[2]
+    rows, heads, qs = _rows(what, "q", q, None, dim)
+    of_k, kv_heads, ks = _rows(what, "k", k, None, dim)
+    if of_k != rows or k.dtype is not q.dtype or heads == 0 or kv_heads == 0:
+        raise ValueError(f"{what}: queries and keys are of one type and number of rows")
+    frequencies, axis = rotary.frequencies, rotary.axis
+    if 2 * frequencies.numel() > dim:
+        raise ValueError(f"{what}: more pairs than a head has")
+    if positions.dtype is not torch.int32 or positions.dim() not in (1, 2) or positions.shape[-1] != rows:
+        raise ValueError(f"{what}: positions are int32 [rows] or [axes, rows]")
+    axes = positions.shape[0] if positions.dim() == 2 else 1
+    if not 1 <= axes <= MAX_AXES or (rows > 1 and positions.stride(-1) != 1):
+        raise ValueError(f"{what}: positions are int32 [rows] or [axes, rows], an axis together, up to {MAX_AXES} axes")
+    across = positions.stride(0) if axes > 1 else rows
+    if across < rows:
+        raise ValueError(f"{what}: axes of positions overlap")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _vector(what, name, w, torch.float32, dim)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"{what}: eps is a number from zero on")
+    on = [t for t in (q, k, positions, frequencies, axis, q_weight, k_weight) if t is not None]
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    tail = (at(q_weight), at(k_weight), eps, positions.data_ptr(), across, axes, frequencies.data_ptr(), at(axis), frequencies.numel(),
+            int(rotary.neighbours), rotary.factor)
+    return dim, rows, heads, kv_heads, qs, ks, on, tail
+
+
+def _output(what, name, out, like, rows, heads, dim):
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=like.dtype, device=like.device)
+    of_out, _, stride = _rows(what, name, out, heads, dim)
+    if out.dtype is not like.dtype or of_out != rows:
+        raise ValueError(f"{what}: {name} has the type and shape of {name[0]}")
+    return out, stride
+
+
+def rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary: Rotary, *, q_weight: torch.Tensor | None = None,
+           k_weight: torch.Tensor | None = None, eps: float = 1e-6, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """``q`` [rows, heads, head_dim] and ``k`` [rows, kv_heads, head_dim] (f32, f16 or bf16; rows may be parts of wider ones), normed head by
+    head where there is a weight (f32 [head_dim]) and turned by ``positions`` (int32 [rows] or [axes, rows]); into ``q_out`` and ``k_out``
+    (new ones without; ``q`` and ``k`` themselves may be given)."""
+    dim, rows, heads, kv_heads, qs, ks, on, tail = _arguments("rotate", q, k, positions, rotary, q_weight, k_weight, eps)
+    q_out, qo = _output("rotate", "q_out", q_out, q, rows, heads, dim)
+    k_out, ko = _output("rotate", "k_out", k_out, k, rows, kv_heads, dim)
+    _on_device("rotate", *on, q_out, k_out)
+    _lib.check("lk_qk_norm_rope", _lib.load().lk_qk_norm_rope(
+        q.data_ptr(), k.data_ptr(), _X_TYPES[q.dtype], qs, ks, q_out.data_ptr(), k_out.data_ptr(), qo, ko, rows, heads, kv_heads, dim, *tail,
+        _stream()))
+    return q_out, k_out
+
+
+def rotate_into(cache: KvCacheMxfp4, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
+                rotary: Rotary, *, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``rotate`` whose keys go into ``cache`` at ``slots`` (int64 [rows], as ``kv_plan`` gives them), and the values ``v`` with them; returns
+    the queries."""
+    if not isinstance(cache, KvCacheMxfp4):
+        raise ValueError("rotate_into: a 4-bit cache (for another: rotate, then kv_write)")
+    dim, rows, heads, kv_heads, qs, ks, on, tail = _arguments("rotate_into", q, k, positions, rotary, q_weight, k_weight, eps)
+    if dim != cache.head_dim or kv_heads != cache.kv_heads:
+        raise ValueError("rotate_into: heads of the cache")
+    of_v, _, vs = _rows("rotate_into", "v", v, kv_heads, dim)
+    if v.dtype is not q.dtype or of_v != rows:
+        raise ValueError("rotate_into: queries, keys and values are of one type and number of rows")
+    _vector("rotate_into", "slots", slots, torch.int64, rows)
+    q_out, qo = _output("rotate_into", "q_out", q_out, q, rows, heads, dim)
+    _on_device("rotate_into", *on, v, slots, q_out, cache.k)
+    _lib.check("lk_qk_norm_rope_kv_mxfp4", _lib.load().lk_qk_norm_rope_kv_mxfp4(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _X_TYPES[q.dtype], qs, ks, vs, q_out.data_ptr(), qo, slots.data_ptr(), rows, heads, kv_heads,
+        dim, *tail, cache.page_tokens, cache.pages, *cache._at(), _stream()))
+    return q_out
