@@ -907,6 +907,24 @@ int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, void* out, 
                           int max_fresh, int max_len, int heads, int kv_heads, int head_dim, float scale, int window, float cap,
                           void* stream);
 
+/* Drafted tokens against the target's distribution, and the token that follows the accepted ones. Rows starts[i] .. starts[i + 1] - 1 of the
+ * logits ([rows][vocab] of `type`, `stride` elements from row to row) are sequence i's: its drafted tokens and one more. p of a row is what
+ * lk_sample would draw from, by the row's temperature, top_k, top_p and min_p. Row r (but a sequence's last) judges drafted[r], which came from the
+ * distribution draft[r] (of `draft_type`, [rows][vocab], draft_stride elements from row to row); draft null: for certain. In the order of rows
+ *   drafted[r] is accepted if uniform[r] * draft[r][drafted[r]] < p[drafted[r]]     (draft null: uniform[r] < p)
+ * up to the first that is not (a number outside the vocabulary is not). There the sequence's next token is drawn from max(p - draft[r], 0) (draft null: p
+ * without the drafted word; where nothing is left: p), at a sequence whose drafts are all accepted from p of its last row: the first word in the order of
+ * their numbers at which the running sum exceeds draw[i] (0 <= draw < 1) of the whole.
+ *   tokens[rows]     the accepted drafts of each sequence, its next token (-1 where that row has no words), -1 behind it and in rows of no sequence
+ *   probs[rows]      p of these tokens (nullable), 0 where there is none
+ *   accepted[seqs]   how many drafts were
+ * Of a sequence's last row uniform, drafted and draft are not looked at; a sequence without rows gets accepted 0. Weights are summed as lk_sample's are, what is left as
+ * integers of 2^-62. Limits and scratch as lk_sample's; up to 65535 sequences. Without rows or sequences nothing is written. */
+int lk_verify(const void* logits, int type, int64_t stride, int rows, int vocab, const int32_t* drafted, const int32_t* starts, int seqs,
+              const void* draft, int draft_type, int64_t draft_stride, const float* uniform, const float* draw, const float* temperature,
+              const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, int32_t* accepted, float* probs,
+              void* stream);
+
 /* Frees what the expert launchers, the expert block, the router, the f16 tiles, attention and sampling hold on the current device, for
  * every stream and every recorded graph: none recorded over them may be replayed after. The host linears' workspaces
  * stay (lkh_release_workspaces). Synchronizes the device (cuda/moe/moe_gguf.cu:104-118). */

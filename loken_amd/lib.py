@@ -169,6 +169,7 @@ SIGNATURES.update({
     "lk_kv_read_q8": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
     "lk_kv_attention_q8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _vp, _i64, _i, _vp, _vp] + [_i] * 7 + [_f, _i, _vp]),
     "lk_sample": (_i, [_vp, _i, _i64, _i, _i] + [_vp] * 8),
+    "lk_verify": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _i, _vp, _i, _i64] + [_vp] * 10),
     "lk_qk_norm_rope": (_i, [_vp, _vp, _i, _i64, _i64, _vp, _vp, _i64, _i64] + [_i] * 4 + [_vp, _vp, _f, _vp, _i64, _i, _vp, _vp, _i, _i, _f, _vp]),
     "lk_kv_write_mxfp4": (_i, [_vp, _vp, _i, _i64, _i64, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "lk_kv_read_mxfp4": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
