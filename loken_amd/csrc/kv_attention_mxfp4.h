@@ -22,10 +22,10 @@ static __device__ __forceinline__ uint32_t mx_two(uint32_t w, float power) {
 static __device__ __forceinline__ mx_b8 mx_eight(uint32_t w, float power) {
     return __builtin_bit_cast(mx_b8, make_uint4(mx_two<0>(w, power), mx_two<1>(w, power), mx_two<2>(w, power), mx_two<3>(w, power)));
 }
-// Byte `I` of a word of powers, 2^(byte - 127).
+// Byte `I` of a word of powers where the conversion looks for it: it takes a number's exponent alone.
 template <int I>
 static __device__ __forceinline__ float mx_power_of(uint32_t w) {
-    return __uint_as_float((I == 3 ? w >> 1 : w << (23 - 8 * I)) & 0x7F800000u);
+    return __uint_as_float(I == 3 ? w >> 1 : w << (23 - 8 * I));
 }
 
 static __device__ __forceinline__ uint32_t mx_pack(float a, float b) {
@@ -44,23 +44,27 @@ static __device__ __forceinline__ void mx_pieces(float a, float b, uint32_t (&ou
     }
 }
 
-// A score in powers of two from a product: `by` = scale * log2(e), or with a cap scale / cap.
+// tanh x = 1 - 2 / (e^2x + 1), off by 1.2e-7; below a quarter, for f32, by its series: to a few last places of x.
 template <bool FINE>
-static __device__ __forceinline__ float mx_score(float product, float by, float cap) {
-    const float x = product * by;
-    if (!(cap > 0.f)) return x;
-    // tanh x = 1 - 2 / (e^2x + 1), off by 1.2e-7; below a quarter, for f32, by its series: to a few last places of x
+static __device__ __forceinline__ float mx_tanh(float x) {
     const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.8853900817779268f) + 1.f);
-    float t = far;
-    if (FINE) {
-        const float s = x * x;
-        const float near = fmaf(x * s, fmaf(s, fmaf(s, fmaf(s, 0.021869488f, -0.053968254f), 0.13333334f), -0.33333334f), x);
-        t = fabsf(x) < 0.25f ? near : far;
-    }
-    return t * (cap * 1.4426950408889634f);
+    if (!FINE) return far;
+    const float s = x * x;
+    const float near = fmaf(x * s, fmaf(s, fmaf(s, fmaf(s, 0.021869488f, -0.053968254f), 0.13333334f), -0.33333334f), x);
+    return fabsf(x) < 0.25f ? near : far;
 }
 
-// Rows of a workgroup of the few-rows kernel: one or two operands of sixteen.
-constexpr int mx_few_rows(int head_dim, int max_rows) { return head_dim < 256 && max_rows > 16 ? 32 : 16; }
+// Rows of a workgroup of the few-rows kernel: with slots for the pieces while these fit, else sixteen, or two operands of them.
+constexpr int mx_few_rows(bool f32, int head_dim, int max_rows) {
+    if (max_rows <= (f32 ? 4 : 8)) return f32 ? 4 : 8;
+    if (f32 && max_rows <= 8 && head_dim < 256) return 8;
+    return head_dim < 256 && max_rows > 16 ? 32 : 16;
+}
+
+// Its waves on a SIMD, for that many rows: two where the registers hold them.
+constexpr int mx_few_on_simd(bool f32, int head_dim, int rows) {
+    const bool two = rows == 32 || (f32 && rows == 8);   // two operands
+    return head_dim == 256 || (two && (head_dim == 128 || (f32 && rows == 32))) ? 1 : 2;
+}
 
 int kv_attention_mxfp4_few(const AttendMx& a, int type, int head_dim, int max_rows, hipStream_t stream);

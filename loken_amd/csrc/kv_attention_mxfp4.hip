@@ -51,9 +51,9 @@ extern "C" int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, 
     const int64_t table_tokens = (int64_t)table_cols * page_tokens;
     const int64_t seen = window > 0 && window < max_len ? (int64_t)window + tokens : max_len;
     const int tiles = (int)((min(seen, table_tokens) + KV_TILE - 1) / KV_TILE);
-    const int per = mx_few_rows(head_dim, max_rows), cus = lk_device().cus;
+    const int per = mx_few_rows(type == LK_TYPE_F32, head_dim, max_rows), cus = lk_device().cus;
     const int64_t groups = (int64_t)seqs * kv_heads * ((max_rows - 1) / per + 1);
-    const int slots = head_dim == 256 || (head_dim == 128 && per == 32) ? cus : 2 * cus;   // workgroups that run at once
+    const int slots = cus * mx_few_on_simd(type == LK_TYPE_F32, head_dim, per);   // workgroups that run at once
     const int64_t most_steps = (int64_t)seqs * ((table_tokens + KV_TILE - 1) / KV_TILE + 1);
     if (seqs > 1 && max_rows <= per && groups <= 4 * cus && groups * tiles > 16 * cus && most_steps < 0x7FFFFFFF) {
         a.chunks = (slots + kv_heads - 1) / kv_heads;

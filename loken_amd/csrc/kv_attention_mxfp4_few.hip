@@ -2,16 +2,16 @@
 //
 // Both products run on v_mfma_f32_16x16x32_bf16: a code times its block's power of two is a bf16 exactly, two codes an instruction, and so are
 // queries and softmax weights as sums of bf16 pieces (bf16 queries one, f16 two, f32 three; weights two, f32 three). Products are then exact but for
-// weights of 16 bits, sums are f32.
+// weights of 16 bits, sums are f32. Up to four rows (f32; eight else) leave room for the pieces in the operand of sixteen columns: a slot of a row takes
+// one piece, and a product is one instruction; more rows take a column each and an instruction a piece.
 //
-// One wave takes a step: 64 positions as four tiles of sixteen. Scores come as (16 positions) x (16 rows): a lane holds row l % 16 and four positions
+// One wave takes a step: 64 positions as four tiles of sixteen. Scores come as (16 positions) x (16 columns): a lane holds column l % 16 and four positions
 // of each tile, which are, two tiles together, what the second product wants of the weights in that lane: nothing crosses lanes but maxima.
 // The values' operand is (16 columns) x (32 positions): the cache has the values of four tokens that a lane takes in one piece; codes of one token
 // become bf16 by its block's power, and halves of words change places to bring a column's positions together.
 // Sums come as (16 columns) x (16 rows): a lane's row again, so maxima and corrections are the lane's own.
 //
-// Loads of the next step's keys go out once the scores have been taken, its values' once the sums have been: both are in flight through the other
-// half of the step. Four waves take steps in turn and meet in LDS; long contexts are cut into parts, which a second launch joins.
+// The next step's loads are in flight through a whole step, the pages of the one behind it too. Four waves take steps in turn and meet in LDS; long contexts are cut into parts, which a second launch joins.
 
 #include "kv_attention_mxfp4.h"
 
@@ -30,22 +30,32 @@ static __device__ __forceinline__ float sum_over_groups(float v) { return swap_a
 template <int WORDS>
 struct __attribute__((aligned(WORDS >= 4 ? 16 : 8))) Words { uint32_t w[WORDS]; };
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int SLOTS>
 struct Few {
     static constexpr int PIECES = sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1;   // of a query value
     static constexpr int SHARES = sizeof(T) == 4 ? 3 : 2;                                         // of a weight
-    static constexpr int ROWS = 16 * NT, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
-    // waves of a SIMD that the registers leave room for
-    static constexpr int ON_SIMD = D == 256 || (D == 128 && NT == 2) ? 1 : 2;
+    static constexpr int QP = SLOTS == 1 ? PIECES : 1, SP = SLOTS == 1 ? SHARES : 1;              // operands of them
+    static constexpr int RPT = 16 / SLOTS, ROWS = RPT * NT, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
+    static constexpr int ON_SIMD = mx_few_on_simd(sizeof(T) == 4, D, ROWS);
 };
 
-template <typename T, int D, int NT>
-__global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_kernel(AttendMx a, int row_tiles) {
-    using F = Few<T, D, NT>;
-    __shared__ float sums[WAVES][16][D + 4];
+// What the slots of a row have together.
+template <int SLOTS>
+static __device__ __forceinline__ float sum_of_slots(float v) {
+    if (SLOTS >= 2) v += dpp_f32<0xB1>(v);   // lanes 1, 0, 3, 2
+    if (SLOTS >= 4) v += dpp_f32<0x4E>(v);   // lanes 2, 3, 0, 1
+    return v;
+}
+
+template <typename T, int D, int NT, int SLOTS>
+__global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void mx_few_kernel(AttendMx a, int row_tiles) {
+    using F = Few<T, D, NT, SLOTS>;
+    __shared__ float sums[WAVES][F::RPT][D + 4];
     __shared__ float tops[WAVES][F::ROWS], weights[WAVES][F::ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
+    const int slot = i % SLOTS;
+    const float second = slot >= 1 ? 1.f : 0.f, third = slot >= 2 ? 1.f : 0.f;   // whether the slot's piece is behind the first, the second
     const int shift = a.mx.page_shift;
     // The workgroup's place: (part, row tile, head, sequence), the part fastest; or (head, piece), a piece being of one or
     // several sequences.
@@ -98,53 +108,63 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_k
             t_end = min(span.tiles, t_begin + span.per_part);
             if (span.parts > 1) to = 0;
         }
-        // positions that some row of the tile sees: [seen_from, span.hi)
+        t_begin = __builtin_amdgcn_readfirstlane(t_begin);
+        t_end = __builtin_amdgcn_readfirstlane(t_end);
+        const int lo = __builtin_amdgcn_readfirstlane(span.lo), hi = __builtin_amdgcn_readfirstlane(span.hi);
+        // positions that some row of the tile sees: [seen_from, hi)
         const int seen_from = a.window > 0 ? (int)max((int64_t)0, s.pos_of_0 + s.first + a.token_of(r0) - a.window + 1) : 0;
 
-        const int32_t* entries = a.table + seq * a.table_stride;
+        // (as memory that nobody writes, which scalar loads read: what a wave's vector loads wait for stays theirs)
+        const auto* entries = (const __attribute__((address_space(4))) int32_t*)(uint64_t)(a.table + seq * a.table_stride);
         // the page of a step's tile; -1: absent, or behind the last position
         auto page_of = [&](int t, int b) {
-            const int p0 = span.lo + t * KV_TILE + 16 * b;
-            const int page = t < t_end && p0 < span.hi ? entries[p0 >> shift] : -1;
+            const int p0 = lo + t * KV_TILE + 16 * b;
+            const int page = t < t_end && p0 < hi ? entries[p0 >> shift] : -1;
             return (unsigned)page < (unsigned)a.mx.pages ? page : -1;
         };
-        Words<F::W> k[4], v[4];
-        uint32_t kp[4], vp[4];   // powers: of the lane's block or two of a key; of four tokens' values
-        auto load_keys = [&](int t, const int (&pages)[4]) {
+        // (a page's address is the wave's own, a lane's place in a tile always the same)
+        const uint32_t key_at = i * (D / 2) + g * (D / 8), key_power_at = i * F::PART + (D == 256 ? 2 * g : D == 64 ? g >> 1 : g);
+        const uint32_t value_at = (g * 16 + i) * (D / 8), value_power_at = ((i * F::PART / 16) << shift) + 4 * g;
+        // A step's codes and powers. Two of them: the next step's are loaded while this one's are at work.
+        struct Loaded {
+            Words<F::W> k[4], v[4];
+            uint32_t kp[4], vp[4];   // powers: of the lane's block or two of a key; of four tokens' values
+        } loaded[2];
+        auto load = [&](Loaded& into, int t, const int (&pages)[4]) {
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const int64_t page = (int64_t)max(pages[b], 0) * a.mx.heads + kv;
-                const int64_t tok = (page << shift) + ((span.lo + t * KV_TILE + 16 * b) & ((1 << shift) - 1)) + i;
-                k[b] = *(const Words<F::W>*)(a.mx.k + tok * (D / 2) + g * (D / 8));
-                if (D == 256) kp[b] = *(const uint16_t*)(a.mx.k_powers + tok * F::PART + 2 * g);
-                else kp[b] = a.mx.k_powers[tok * F::PART + (D == 64 ? g >> 1 : g)];
+                const int64_t page = ((int64_t)max(pages[b], 0) * a.mx.heads + kv) << shift;
+                const int at = (lo + t * KV_TILE + 16 * b) & ((1 << shift) - 1);
+                const uint8_t *codes = a.mx.k + (page + at) * (D / 2), *powers = a.mx.k_powers + (page + at) * F::PART;
+                into.k[b] = *(const Words<F::W>*)(codes + key_at);
+                if (D == 256) into.kp[b] = *(const uint16_t*)(powers + key_power_at);
+                else into.kp[b] = powers[key_power_at];
             }
-        };
-        auto load_values = [&](int t, const int (&pages)[4]) {
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const int64_t page = (int64_t)max(pages[b], 0) * a.mx.heads + kv;
-                const int at = ((span.lo + t * KV_TILE + 16 * b) & ((1 << shift) - 1)) + 4 * g;
-                v[b] = *(const Words<F::W>*)(a.mx.v + (page << shift) * (D / 2) + ((at >> 2) * 16 + i) * (D / 8));
-                vp[b] = *(const uint32_t*)(a.mx.v_powers + (page << shift) * F::PART + ((i * F::PART / 16) << shift) + at);
+                const int64_t page = ((int64_t)max(pages[b], 0) * a.mx.heads + kv) << shift;
+                const int at = (lo + t * KV_TILE + 16 * b) & ((1 << shift) - 1);
+                const uint8_t *codes = a.mx.v + (page + at) * (D / 2), *powers = a.mx.v_powers + page * F::PART + at;
+                into.v[b] = *(const Words<F::W>*)(codes + value_at);
+                into.vp[b] = *(const uint32_t*)(powers + value_power_at);
             }
         };
         int t = t_begin + wave;
-        int pages[4];   // of the step whose keys are loaded next
+        int pages[4], next[4];   // of this step and of the wave's next one
 #pragma unroll
         for (int b = 0; b < 4; ++b) pages[b] = page_of(t, b);
-        if (t < t_end) {
-            load_keys(t, pages);
-            load_values(t, pages);
-        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) next[b] = page_of(t + WAVES, b);
+        if (t < t_end) load(loaded[0], t, pages);
 
-        // the rows' pieces, and what a product is in scores
-        mx_b8 q[NT][F::KS][F::PIECES];
+        const float capped = a.cap > 0.f ? a.scale / a.cap : 0.f;   // what a product is under the tanh
+        // the rows' pieces, and what a product, or its tanh, is in powers of two
+        mx_b8 q[NT][F::KS][F::QP];
         float unit[NT];
         int pos[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int r = r0 + 16 * n + i;
+            const int r = r0 + n * F::RPT + i / SLOTS;
             const int of_seq = a.token_of(min(r, r1)), tok = s.first + of_seq, head = kv * a.group + min(r, r1) - of_seq * a.group;
             pos[n] = r <= r1 ? (int)max(s.pos_of_0 + tok, (int64_t)-1) : -1;
             const T* row = (const T*)a.q + tok * a.q_stride + (int64_t)head * D + g * (D / 4);
@@ -162,35 +182,54 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_k
 #pragma unroll
                     for (int p = 0; p < F::PIECES; ++p) w[p][e] = both[p];
                 }
+                if (SLOTS > 1) {   // the slot's piece alone
 #pragma unroll
-                for (int p = 0; p < F::PIECES; ++p) q[n][ks][p] = __builtin_bit_cast(mx_b8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t mine = slot == 0 ? w[0][e] : 0;
+#pragma unroll
+                        for (int p = 1; p < F::PIECES; ++p) mine = slot == p ? w[p][e] : mine;
+                        w[0][e] = mine;
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < F::QP; ++p) q[n][ks][p] = __builtin_bit_cast(mx_b8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
             }
             const uint64_t odd = __ballot(!finite);
             finite = (odd >> i & 0x0001000100010001ull) == 0;
-            unit[n] = finite ? (a.cap > 0.f ? a.scale / a.cap : a.scale * 1.4426950408889634f) : NAN;
+            unit[n] = finite ? (a.cap > 0.f ? a.cap : a.scale) * 1.4426950408889634f : NAN;
         }
         int pos_least = 0x7FFFFFFF, pos_most = -1;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            if (r0 + 16 * n + i <= r1) { pos_least = min(pos_least, pos[n]); pos_most = max(pos_most, pos[n]); }
+            if (r0 + n * F::RPT + i / SLOTS <= r1) { pos_least = min(pos_least, pos[n]); pos_most = max(pos_most, pos[n]); }
         }
         for (int o = 1; o < 16; o <<= 1) {
             pos_least = min(pos_least, __shfl_xor(pos_least, o));
             pos_most = max(pos_most, __shfl_xor(pos_most, o));
         }
 
-        float m[NT], l[NT];
+        float m[NT], base[NT], l[NT];   // the largest product or tanh, that as a score, and the sum of weights relative to it
         v4f acc[NT][F::NB];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             m[n] = -INFINITY;
-            l[n] = 0.f;
+            base[n] = l[n] = 0.f;
 #pragma unroll
             for (int b = 0; b < F::NB; ++b) acc[n][b] = (v4f){0.f, 0.f, 0.f, 0.f};
         }
 
-        for (; t < t_end; t += WAVES) {
-            const int p0 = span.lo + t * KV_TILE;
+        auto step = [&](Loaded& now, Loaded& then) {
+            const int p0 = lo + t * KV_TILE;
+            // (Behind the last step this one's are loaded again, out of the cache: a load that is left out at times would be waited for at the
+            // next use of any.)
+            const bool more = t + WAVES < t_end;
+            int from[4], behind[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                from[b] = more ? next[b] : pages[b];
+                behind[b] = page_of(t + 2 * WAVES, b);
+            }
+            load(then, t + WAVES, from);
             // whether every row sees every position of the step
             const bool here = pages[0] >= 0 && pages[1] >= 0 && pages[2] >= 0 && pages[3] >= 0;
             const bool whole = p0 + KV_TILE - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && here;
@@ -202,30 +241,30 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_k
                 for (int n = 0; n < NT; ++n) c[n] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int ks = 0; ks < F::KS; ++ks) {
-                    const float power = D == 256 && ks >= F::KS / 2 ? mx_power_of<1>(kp[b]) : mx_power_of<0>(kp[b]);
-                    const mx_b8 op = mx_eight(k[b].w[ks], power);
+                    const float power = D == 256 && ks >= F::KS / 2 ? mx_power_of<1>(now.kp[b]) : mx_power_of<0>(now.kp[b]);
+                    const mx_b8 op = mx_eight(now.k[b].w[ks], power);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int p = 0; p < F::PIECES; ++p) c[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, q[n][ks][p], c[n], 0, 0, 0);
+                        for (int p = 0; p < F::QP; ++p) c[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, q[n][ks][p], c[n], 0, 0, 0);
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) sc[n][b] = c[n];
             }
-            int next[4], absent = 0;
+            int absent = 0;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                absent |= (pages[b] < 0) << b;
-                next[b] = page_of(t + WAVES, b);
-            }
-            if (t + WAVES < t_end) load_keys(t + WAVES, next);
+            for (int b = 0; b < 4; ++b) absent |= (pages[b] < 0) << b;
 
-            uint32_t share[NT][F::SHARES][4][2];   // weights: of a tile's four positions
+            uint32_t share[NT][F::SP][4][2];   // weights: of a tile's four positions
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float x[16], top = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = mx_score<sizeof(T) == 4>(sc[n][e >> 2][e & 3], unit[n], a.cap);
+                for (int e = 0; e < 16; ++e) x[e] = sum_of_slots<SLOTS>(sc[n][e >> 2][e & 3]);
+                if (a.cap > 0.f) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = mx_tanh<sizeof(T) == 4>(x[e] * capped);
+                }
                 if (!whole) {
                     const int last = pos[n] - p0 - 4 * g, first = a.window > 0 ? last - a.window : -0x40000000;
 #pragma unroll
@@ -237,30 +276,43 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_k
 #pragma unroll
                 for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
                 top = max_over_groups(top);
-                const float now = fmaxf(m[n], top), base = now == -INFINITY ? 0.f : now;   // (a row that is not finite has no top and stays that way)
-                if (__ballot(now > m[n])) {
-                    const float keep = __builtin_amdgcn_exp2f(m[n] - base);
-                    l[n] = m[n] == -INFINITY ? l[n] : l[n] * keep;
+                if (__ballot(top > m[n])) {
+                    const float most = fmaxf(m[n], top), to = most == -INFINITY ? 0.f : most * unit[n];
+                    const float keep = m[n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base[n] - to);
+                    l[n] *= keep;
 #pragma unroll
                     for (int b = 0; b < F::NB; ++b)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[n][b][e] = m[n] == -INFINITY ? acc[n][b][e] : acc[n][b][e] * keep;
-                    m[n] = now;
+                        for (int e = 0; e < 4; ++e) acc[n][b][e] *= keep;
+                    m[n] = most;
+                    base[n] = to;
                 }
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     float p[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[e] = __builtin_amdgcn_exp2f(x[4 * b + e] - base);
+                        p[e] = __builtin_amdgcn_exp2f(fmaf(x[4 * b + e], unit[n], -base[n]));
                         l[n] += p[e];
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        uint32_t both[F::SHARES];
-                        mx_pieces<F::SHARES>(p[2 * h], p[2 * h + 1], both);
+                        if (SLOTS > 1) {
+                            uint32_t piece = mx_pack(p[2 * h], p[2 * h + 1]);
 #pragma unroll
-                        for (int j = 0; j < F::SHARES; ++j) share[n][j][b][h] = both[j];
+                            for (int j = 1; j < F::SHARES; ++j) {
+                                const float less = j == 1 ? second : third;
+                                p[2 * h] = fmaf(__uint_as_float(piece << 16), -less, p[2 * h]);
+                                p[2 * h + 1] = fmaf(__uint_as_float(piece & 0xFFFF0000u), -less, p[2 * h + 1]);
+                                piece = mx_pack(p[2 * h], p[2 * h + 1]);
+                            }
+                            share[n][0][b][h] = piece;
+                        } else {
+                            uint32_t both[F::SHARES];
+                            mx_pieces<F::SHARES>(p[2 * h], p[2 * h + 1], both);
+#pragma unroll
+                            for (int j = 0; j < F::SP; ++j) share[n][j][b][h] = both[j];
+                        }
                     }
                 }
             }
@@ -272,9 +324,9 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_k
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int at = p0 + 16 * b + 4 * g + j;
-                        if (at >= seen_from && at < span.hi && !(absent >> b & 1)) seen |= 0xFFu << (8 * j);
+                        if (at >= seen_from && at < hi && !(absent >> b & 1)) seen |= 0xFFu << (8 * j);
                     }
-                    vp[b] &= seen;
+                    now.vp[b] &= seen;
                 }
             }
 #pragma unroll
@@ -283,16 +335,16 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_k
                 float power[8];
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    power[4 * b] = mx_power_of<0>(vp[b0 + b]);
-                    power[4 * b + 1] = mx_power_of<1>(vp[b0 + b]);
-                    power[4 * b + 2] = mx_power_of<2>(vp[b0 + b]);
-                    power[4 * b + 3] = mx_power_of<3>(vp[b0 + b]);
+                    power[4 * b] = mx_power_of<0>(now.vp[b0 + b]);
+                    power[4 * b + 1] = mx_power_of<1>(now.vp[b0 + b]);
+                    power[4 * b + 2] = mx_power_of<2>(now.vp[b0 + b]);
+                    power[4 * b + 3] = mx_power_of<3>(now.vp[b0 + b]);
                 }
-                mx_b8 w[NT][F::SHARES];
+                mx_b8 w[NT][F::SP];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int j = 0; j < F::SHARES; ++j)
+                    for (int j = 0; j < F::SP; ++j)
                         w[n][j] = __builtin_bit_cast(mx_b8, make_uint4(share[n][j][b0][0], share[n][j][b0][1], share[n][j][b0 + 1][0], share[n][j][b0 + 1][1]));
 #pragma unroll
                 for (int byte = 0; byte < F::PART; ++byte) {   // columns 2 byte and 2 byte + 1 of the lane's sixteenth
@@ -300,7 +352,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_k
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const int at = (j & 3) * F::PART + byte;
-                        const uint32_t word = v[b0 + (j >> 2)].w[at >> 2];
+                        const uint32_t word = now.v[b0 + (j >> 2)].w[at >> 2];
                         const int sel = at & 3;
                         c[j] = sel == 0 ? mx_two<0>(word, power[j]) : sel == 1 ? mx_two<1>(word, power[j]) : sel == 2 ? mx_two<2>(word, power[j]) : mx_two<3>(word, power[j]);
                     }
@@ -315,44 +367,60 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_k
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int j = 0; j < F::SHARES; ++j) {
+                        for (int j = 0; j < F::SP; ++j) {
                             acc[n][2 * byte] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op0, w[n][j], acc[n][2 * byte], 0, 0, 0);
                             acc[n][2 * byte + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op1, w[n][j], acc[n][2 * byte + 1], 0, 0, 0);
                         }
                 }
             }
-            if (t + WAVES < t_end) load_values(t + WAVES, next);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) pages[b] = next[b];
+            for (int b = 0; b < 4; ++b) {
+                pages[b] = next[b];
+                next[b] = behind[b];
+            }
+            t += WAVES;
+        };
+        while (t < t_end) {
+            step(loaded[0], loaded[1]);
+            if (t < t_end) step(loaded[1], loaded[0]);
         }
 
-        // the four waves' sums relative to their common maximum, sixteen rows at a time
+        // the slots' sums, and the four waves' relative to their common maximum, an operand's rows at a time
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const float lw = sum_over_groups(l[n]);
-            if (g == 0) { tops[wave][16 * n + i] = m[n]; weights[wave][16 * n + i] = lw; }
+            m[n] = m[n] == -INFINITY ? m[n] : base[n];
+            if (g == 0 && slot == 0) { tops[wave][n * F::RPT + i / SLOTS] = m[n]; weights[wave][n * F::RPT + i / SLOTS] = lw; }
+            if (SLOTS > 1) {
+#pragma unroll
+                for (int b = 0; b < F::NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[n][b][e] = sum_of_slots<SLOTS>(slot < F::SHARES ? acc[n][b][e] : 0.f);
+            }
         }
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             if (n) __syncthreads();
-            const int r = 16 * n + i;
+            const int r = n * F::RPT + i / SLOTS;
             const float top = fmaxf(fmaxf(tops[0][r], tops[1][r]), fmaxf(tops[2][r], tops[3][r]));
             const float f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
             // column of the sums: the lane's rows 4 g + e of the operand are sixteenths of the head
+            if (slot == 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+                for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int b = 0; b < F::NB; ++b) sums[wave][i][(4 * g + e) * (D / 16) + b] = acc[n][b][e] * f;
+                    for (int b = 0; b < F::NB; ++b) sums[wave][i / SLOTS][(4 * g + e) * (D / 16) + b] = acc[n][b][e] * f;
+            }
             __syncthreads();
-            for (int at = threadIdx.x; at < min(r1 - r0 + 1 - 16 * n, 16) * D; at += 64 * WAVES) {
-                const int rr = at / D, d = at % D, row_of = 16 * n + rr;
+            for (int at = threadIdx.x; at < min(r1 - r0 + 1 - n * F::RPT, F::RPT) * D; at += 64 * WAVES) {
+                const int rr = at / D, d = at % D, row_of = n * F::RPT + rr;
                 const float most = fmaxf(fmaxf(tops[0][row_of], tops[1][row_of]), fmaxf(tops[2][row_of], tops[3][row_of]));
                 float total = 0.f, lw = 0.f;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) {
                     total += sums[w][rr][d];
-                    // (a part whose scores are no numbers has no maximum and a sum that is none)
+                    // (a part whose scores are no numbers has a sum that is none, and may have no maximum)
                     lw += tops[w][row_of] == -INFINITY ? weights[w][row_of] : weights[w][row_of] * __builtin_amdgcn_exp2f(tops[w][row_of] - most);
                 }
                 const int of_seq = a.token_of(r0 + row_of), head = kv * a.group + r0 + row_of - of_seq * a.group;
@@ -373,11 +441,19 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT>::ON_SIMD)) void mx_few_k
 
 template <typename T, int D>
 static int launch(const AttendMx& a, int max_rows, hipStream_t s) {
-    const int per = mx_few_rows(D, max_rows), row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / per + 1;
+    constexpr int SLOTS = sizeof(T) == 4 ? 4 : 2, TWO = D < 256 ? 2 : 1;
+    const int per = mx_few_rows(sizeof(T) == 4, D, max_rows), row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / per + 1;
     const int64_t blocks = a.chunks ? (int64_t)a.chunks * a.mx.heads : (int64_t)a.seqs * a.mx.heads * row_tiles * a.splits;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
-    if (per == 32) hipLaunchKernelGGL((mx_few_kernel<T, D, (D < 256 ? 2 : 1)>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a, row_tiles);
-    else hipLaunchKernelGGL((mx_few_kernel<T, D, 1>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a, row_tiles);
+    const dim3 grid((unsigned)blocks), threads(64 * WAVES);
+    if constexpr (sizeof(T) == 4 && D < 256)
+        if (per == 8) {
+            hipLaunchKernelGGL((mx_few_kernel<T, D, 2, SLOTS>), grid, threads, 0, s, a, row_tiles);
+            return lk_launch_status();
+        }
+    if (per == Few<T, D, 1, SLOTS>::ROWS) hipLaunchKernelGGL((mx_few_kernel<T, D, 1, SLOTS>), grid, threads, 0, s, a, row_tiles);
+    else if (per == 16) hipLaunchKernelGGL((mx_few_kernel<T, D, 1, 1>), grid, threads, 0, s, a, row_tiles);
+    else hipLaunchKernelGGL((mx_few_kernel<T, D, TWO, 1>), grid, threads, 0, s, a, row_tiles);
     return lk_launch_status();
 }
 
