@@ -54,17 +54,19 @@ static __device__ __forceinline__ float mx_tanh(float x) {
     return fabsf(x) < 0.25f ? near : far;
 }
 
-// Rows of a workgroup of the few-rows kernel: with slots for the pieces while these fit, else sixteen, or two operands of them.
+// Sequences of up to so many rows (token, head of a group) are the few-rows kernel's, and rows of its workgroups: with slots for the pieces while
+// these fit (in one operand, or f32 in two), else sixteen.
+constexpr int MX_FEW_ROWS = 16;
 constexpr int mx_few_rows(bool f32, int head_dim, int max_rows) {
     if (max_rows <= (f32 ? 4 : 8)) return f32 ? 4 : 8;
-    if (f32 && max_rows <= 8 && head_dim < 256) return 8;
-    return head_dim < 256 && max_rows > 16 ? 32 : 16;
+    return f32 && max_rows <= 8 && head_dim < 256 ? 8 : 16;
 }
-
 // Its waves on a SIMD, for that many rows: two where the registers hold them.
-constexpr int mx_few_on_simd(bool f32, int head_dim, int rows) {
-    const bool two = rows == 32 || (f32 && rows == 8);   // two operands
-    return head_dim == 256 || (two && (head_dim == 128 || (f32 && rows == 32))) ? 1 : 2;
-}
+constexpr int mx_few_on_simd(bool f32, int head_dim, int rows) { return head_dim == 256 || (head_dim == 128 && f32 && rows == 8) ? 1 : 2; }
+
+// Rows of a workgroup of the many-rows kernel, and its waves on a SIMD.
+constexpr int mx_many_rows(bool f32, int head_dim) { return head_dim == 256 && f32 ? 16 : 32; }
+constexpr int mx_many_on_simd(bool f32, bool f16, int head_dim) { return head_dim == 256 || (head_dim == 128 && (f32 || f16)) ? 1 : 2; }
 
 int kv_attention_mxfp4_few(const AttendMx& a, int type, int head_dim, int max_rows, hipStream_t stream);
+int kv_attention_mxfp4_many(const AttendMx& a, int type, int head_dim, hipStream_t stream);

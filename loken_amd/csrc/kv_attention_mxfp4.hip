@@ -16,6 +16,25 @@ static void cut(Attend& a, int64_t groups, int tiles, int want, int least) {
     a.least_tiles = tiles > a.splits ? (tiles + a.splits - 1) / a.splits : 1;
 }
 
+// Parts of the many-rows kernel's contexts, of `tiles` steps for `groups` row tiles and heads, `slots` workgroups at once: those that take the least
+// time where a workgroup takes 5 us to start and 0.8 us a step, and each row and head's part 0.35 ns to be stored and joined, 4 us in all beside.
+static void cut_many(Attend& a, int64_t groups, int tiles, int64_t slots) {
+    const double rows = (double)a.rows * a.heads;
+    double least = 1e30;
+    for (int parts = 1, of = 0; parts <= 64 && parts <= tiles / 2 + 1; ++parts) {
+        const int per = (tiles + parts - 1) / parts;
+        if (per == of) continue;
+        of = per;
+        const int64_t rounds = (groups * parts + slots - 1) / slots;
+        const double time = (double)rounds * (per * 0.8 + 5.0) + (parts > 1 ? 4.0 + rows * parts * 0.35e-3 : 0.0);
+        if (time < least) {
+            least = time;
+            a.splits = parts;
+            a.least_tiles = per > 1 ? per : 1;
+        }
+    }
+}
+
 }  // namespace
 
 extern "C" int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, void* out, int64_t out_stride, const void* k_codes,
@@ -44,33 +63,55 @@ extern "C" int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, 
                 nullptr, nullptr, 0, 0x7FFFFFFF, (uint32_t)(((1ull << group_shift) + group - 1) / group), group_shift},
                {(uint8_t*)k_codes, (uint8_t*)v_codes, (uint8_t*)k_powers, (uint8_t*)v_powers, pages, kv_heads, kv_log2(page_tokens)},
                cap};
-    // What the caller says of the sizes chooses launches; whatever the sequences are, the kernel takes each.
+    // What the caller says of the sizes chooses launches; whatever the sequences are, one of the kernels takes each.
+    const bool f32 = type == LK_TYPE_F32, f16 = type == LK_TYPE_F16;
     const int tokens = max_fresh < 1 ? 1 : max_fresh < rows ? max_fresh : rows;
     const int64_t most_rows = (int64_t)tokens * group;
     const int max_rows = most_rows < 0x7FFFFFFF ? (int)most_rows : 0x7FFFFFFF;
+    const bool many = max_rows > MX_FEW_ROWS, few = group <= MX_FEW_ROWS && (!many || seqs > 1);
     const int64_t table_tokens = (int64_t)table_cols * page_tokens;
     const int64_t seen = window > 0 && window < max_len ? (int64_t)window + tokens : max_len;
-    const int tiles = (int)((min(seen, table_tokens) + KV_TILE - 1) / KV_TILE);
-    const int per = mx_few_rows(type == LK_TYPE_F32, head_dim, max_rows), cus = lk_device().cus;
-    const int64_t groups = (int64_t)seqs * kv_heads * ((max_rows - 1) / per + 1);
-    const int slots = cus * mx_few_on_simd(type == LK_TYPE_F32, head_dim, per);   // workgroups that run at once
-    const int64_t most_steps = (int64_t)seqs * ((table_tokens + KV_TILE - 1) / KV_TILE + 1);
-    if (seqs > 1 && max_rows <= per && groups <= 4 * cus && groups * tiles > 16 * cus && most_steps < 0x7FFFFFFF) {
-        a.chunks = (slots + kv_heads - 1) / kv_heads;
-        a.least_tiles = 4;
-    } else {
-        cut(a, groups, tiles, slots, tiles <= 16 ? 16 : 4);
-        a.part_seq = tokens;
+    const int tiles = (int)((min(seen, table_tokens) + KV_TILE - 1) / KV_TILE), cus = lk_device().cus;
+    AttendMx af = a, am = a;
+    // Beside a sequence of many rows the few-rows kernel takes what one of its workgroups holds for a token's rows.
+    const int few_max = many ? mx_few_rows(f32, head_dim, group) : max_rows, per = mx_few_rows(f32, head_dim, few_max);
+    const int few_tokens = many ? few_max / group : tokens;
+    if (few) {
+        af.few_rows = many ? few_max : 0x7FFFFFFF;
+        const int64_t groups = (int64_t)seqs * kv_heads * ((few_max - 1) / per + 1);
+        const int slots = cus * mx_few_on_simd(f32, head_dim, per);   // workgroups that run at once
+        const int64_t most_steps = (int64_t)seqs * ((table_tokens + KV_TILE - 1) / KV_TILE + 1);
+        if (seqs > 1 && few_max <= per && groups <= 4 * cus && groups * tiles > 16 * cus && most_steps < 0x7FFFFFFF) {
+            af.chunks = (slots + kv_heads - 1) / kv_heads;
+            af.least_tiles = 4;
+        } else {
+            cut(af, groups, tiles, slots, tiles <= 16 ? 16 : 4);
+            af.part_seq = few_tokens;
+        }
     }
-    const int64_t part_rows = a.chunks ? (int64_t)kv_heads * a.chunks * 2 * per : a.splits > 1 ? (int64_t)seqs * a.part_seq * heads * a.splits : 0;
+    const int64_t part_rows_f = !few ? 0 : af.chunks ? (int64_t)kv_heads * af.chunks * 2 * per : af.splits > 1 ? (int64_t)seqs * af.part_seq * heads * af.splits : 0;
+    int64_t part_rows_m = 0;
+    const int many_rows = mx_many_rows(f32, head_dim);
+    if (many) {
+        am.few_rows = few ? few_max : 0;
+        // as many sequences as fill the batch with the most rows that one has
+        const int64_t long_seqs = min((int64_t)seqs, (rows + (int64_t)tokens / 2) / tokens);
+        cut_many(am, long_seqs * ((max_rows - 1) / many_rows + 1) * kv_heads, tiles, 2 * cus * mx_many_on_simd(f32, f16, head_dim));
+        if (am.splits > 1) part_rows_m = (int64_t)rows * heads * am.splits;
+    }
     LkScratch scratch(s);
-    if (part_rows) {
-        float* mem = (float*)scratch.get(LK_SCRATCH_ATTENTION, (size_t)part_rows * (head_dim + 2) * 4);
+    if (part_rows_f + part_rows_m) {
+        float* mem = (float*)scratch.get(LK_SCRATCH_ATTENTION, (size_t)(part_rows_f + part_rows_m) * (head_dim + 2) * 4);
         if (!mem) return LK_ERR_NOMEM;
-        a.part_ml = (float2*)mem;
-        a.part_o = mem + 2 * part_rows;
+        af.part_ml = (float2*)mem;
+        am.part_ml = af.part_ml + part_rows_f;
+        af.part_o = mem + 2 * (part_rows_f + part_rows_m);
+        am.part_o = af.part_o + part_rows_f * head_dim;
     }
-    int status = kv_attention_mxfp4_few(a, type, head_dim, max_rows, s);
-    if (status == LK_OK && part_rows) status = kv_attention_join(a, type, head_dim, per, true, tokens, s);
+    int status = LK_OK;
+    if (many) status = kv_attention_mxfp4_many(am, type, head_dim, s);
+    if (status == LK_OK && few) status = kv_attention_mxfp4_few(af, type, head_dim, few_max, s);
+    if (status == LK_OK && part_rows_m) status = kv_attention_join(am, type, head_dim, many_rows, false, tokens, s);
+    if (status == LK_OK && part_rows_f) status = kv_attention_join(af, type, head_dim, per, true, few_tokens, s);
     return status;
 }

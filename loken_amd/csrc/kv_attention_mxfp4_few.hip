@@ -441,7 +441,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
 
 template <typename T, int D>
 static int launch(const AttendMx& a, int max_rows, hipStream_t s) {
-    constexpr int SLOTS = sizeof(T) == 4 ? 4 : 2, TWO = D < 256 ? 2 : 1;
+    constexpr int SLOTS = sizeof(T) == 4 ? 4 : 2;
     const int per = mx_few_rows(sizeof(T) == 4, D, max_rows), row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / per + 1;
     const int64_t blocks = a.chunks ? (int64_t)a.chunks * a.mx.heads : (int64_t)a.seqs * a.mx.heads * row_tiles * a.splits;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
@@ -452,8 +452,7 @@ static int launch(const AttendMx& a, int max_rows, hipStream_t s) {
             return lk_launch_status();
         }
     if (per == Few<T, D, 1, SLOTS>::ROWS) hipLaunchKernelGGL((mx_few_kernel<T, D, 1, SLOTS>), grid, threads, 0, s, a, row_tiles);
-    else if (per == 16) hipLaunchKernelGGL((mx_few_kernel<T, D, 1, 1>), grid, threads, 0, s, a, row_tiles);
-    else hipLaunchKernelGGL((mx_few_kernel<T, D, TWO, 1>), grid, threads, 0, s, a, row_tiles);
+    else hipLaunchKernelGGL((mx_few_kernel<T, D, 1, 1>), grid, threads, 0, s, a, row_tiles);
     return lk_launch_status();
 }
 

@@ -1,0 +1,379 @@
+// Attention over the 4-bit cache for many rows of a sequence: prompts and prefill chunks.
+//
+// As for a few rows (the operands and what a lane holds are the same), but a row's pieces are instructions of their own, and a workgroup's two waves
+// have 16 NT rows (token, head of the group, so that the group's heads share what is read) and take steps of 32 positions in turn; they meet in
+// LDS at the end. Nothing is shared before: no barrier, and each wave converts the codes for itself.
+//
+// A row's weights are taken relative to a maximum that is put up only where a score lies 2^SLACK above it: bf16 has f32's range, so that costs no
+// bits, and a step without such a score needs no exchange between lanes and no correction. The sum of weights is a product with ones, of
+// the weights as they went into the sums of values: their roundings cancel.
+
+#include "kv_attention_mxfp4.h"
+
+namespace {
+
+constexpr int WAVES = 2, STEP = 32, TILES = STEP / 16;
+constexpr float SLACK = 8.f;   // a power of two
+
+static __device__ __forceinline__ float max_over_groups(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int WORDS>
+struct __attribute__((aligned(WORDS >= 4 ? 16 : 8))) Words { uint32_t w[WORDS]; };
+
+template <typename T, int D>
+struct Many {
+    static constexpr bool FINE = sizeof(T) == 4;
+    static constexpr int QP = FINE ? 3 : std::is_same<T, __half>::value ? 2 : 1;   // pieces of a query value
+    static constexpr int SP = QP;                                                  // and of a weight: 8 bits beside bf16, 16, 24
+    static constexpr int ROWS = mx_many_rows(FINE, D), NT = ROWS / 16, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
+};
+
+// The row tile of that number among those of all sequences, from the last one on; false: there are fewer. Found by each wave.
+static __device__ __forceinline__ bool tile_at(const Attend& a, int rows_of_tile, int number, int& seq, int& tile) {
+    const int lane = threadIdx.x & 63;
+    auto tiles_of = [&](int i) {
+        if (i >= a.seqs) return 0;
+        const unsigned rows = (unsigned)KvSeq(a, i).tokens() * (unsigned)a.group;
+        return (int)rows <= a.few_rows ? 0 : (int)((rows + rows_of_tile - 1) / rows_of_tile);
+    };
+    for (int base = (a.seqs - 1) & ~63; base >= 0; base -= 64) {
+        const int mine = tiles_of(base + lane);
+        int behind = mine;   // of this sequence and those behind it
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_down(behind, o);
+            if (lane + o < 64) behind += v;
+        }
+        const uint64_t over = __ballot(behind > number);
+        if (over) {
+            const int l = 63 - __clzll((long long)over);
+            seq = base + l;
+            tile = __builtin_amdgcn_readlane(behind, l) - 1 - number;
+            return true;
+        }
+        number -= __builtin_amdgcn_readfirstlane(behind);
+    }
+    return false;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof(T) == 2 && std::is_same<T, __half>::value, D))) void mx_many_kernel(AttendMx a) {
+    using M = Many<T, D>;
+    __shared__ float sums[16][D + 4];
+    __shared__ float tops[WAVES][M::ROWS], weights[WAVES][M::ROWS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4, shift = a.mx.page_shift;
+    unsigned block = blockIdx.x;
+    const int kv = block % a.mx.heads;
+    block /= a.mx.heads;
+    const int part = block % a.splits;
+    int seq = 0, tile = 0;
+    if (!tile_at(a, M::ROWS, block / a.splits, seq, tile)) return;
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    const KvSeq s(a, seq);
+    const unsigned all_rows = (unsigned)s.tokens() * (unsigned)a.group, r0 = (unsigned)tile * M::ROWS, r1 = min(r0 + M::ROWS, all_rows) - 1;
+    const KvSpan span(a, s, s.first + a.token_of(r0), s.first + a.token_of(r1));
+    if (part >= span.parts) return;
+    const int lo = __builtin_amdgcn_readfirstlane(span.lo), hi = __builtin_amdgcn_readfirstlane(span.hi);
+    const int t_end = __builtin_amdgcn_readfirstlane(min(span.tiles, (part + 1) * span.per_part)) * (KV_TILE / STEP);
+    int t = __builtin_amdgcn_readfirstlane(part * span.per_part) * (KV_TILE / STEP) + wave;
+    // positions that some row of the tile sees: [seen_from, hi)
+    const int seen_from = a.window > 0 ? (int)max((int64_t)0, s.pos_of_0 + s.first + a.token_of(r0) - a.window + 1) : 0;
+
+    // (as memory that nobody writes, which scalar loads read: what a wave's vector loads wait for stays theirs)
+    const auto* entries = (const __attribute__((address_space(4))) int32_t*)(uint64_t)(a.table + seq * a.table_stride);
+    auto page_of = [&](int t, int b) {
+        const int p0 = lo + t * STEP + 16 * b;
+        const int page = t < t_end && p0 < hi ? entries[p0 >> shift] : -1;
+        return (unsigned)page < (unsigned)a.mx.pages ? page : -1;
+    };
+    // (a page's address is the wave's own, a lane's place in a tile always the same)
+    const uint32_t key_at = i * (D / 2) + g * (D / 8), key_power_at = i * M::PART + (D == 256 ? 2 * g : D == 64 ? g >> 1 : g);
+    const uint32_t value_at = (g * 16 + i) * (D / 8), value_power_at = ((i * M::PART / 16) << shift) + 4 * g;
+    // A step's codes and powers. Two of them: the next step's are loaded while this one's are at work.
+    struct Loaded {
+        Words<M::W> k[TILES], v[TILES];
+        uint32_t kp[TILES], vp[TILES];   // powers: of the lane's block or two of a key; of four tokens' values
+    } loaded[2];
+    auto load = [&](Loaded& into, int t, const int (&pages)[TILES]) {
+#pragma unroll
+        for (int b = 0; b < TILES; ++b) {
+            const int64_t page = ((int64_t)max(pages[b], 0) * a.mx.heads + kv) << shift;
+            const int at = (lo + t * STEP + 16 * b) & ((1 << shift) - 1);
+            const uint8_t *codes = a.mx.k + (page + at) * (D / 2), *powers = a.mx.k_powers + (page + at) * M::PART;
+            into.k[b] = *(const Words<M::W>*)(codes + key_at);
+            if (D == 256) into.kp[b] = *(const uint16_t*)(powers + key_power_at);
+            else into.kp[b] = powers[key_power_at];
+        }
+#pragma unroll
+        for (int b = 0; b < TILES; ++b) {
+            const int64_t page = ((int64_t)max(pages[b], 0) * a.mx.heads + kv) << shift;
+            const int at = (lo + t * STEP + 16 * b) & ((1 << shift) - 1);
+            const uint8_t *codes = a.mx.v + (page + at) * (D / 2), *powers = a.mx.v_powers + page * M::PART + at;
+            into.v[b] = *(const Words<M::W>*)(codes + value_at);
+            into.vp[b] = *(const uint32_t*)(powers + value_power_at);
+        }
+    };
+    int pages[TILES], next[TILES];   // of this step and of the wave's next one
+#pragma unroll
+    for (int b = 0; b < TILES; ++b) {
+        pages[b] = page_of(t, b);
+        next[b] = page_of(t + WAVES, b);
+    }
+    if (t < t_end) load(loaded[0], t, pages);
+
+    const float capped = a.cap > 0.f ? a.scale / a.cap : 0.f;   // what a product is under the tanh
+    // the rows' pieces, and what a product, or its tanh, is in powers of two
+    mx_b8 q[M::NT][M::KS][M::QP];
+    float unit[M::NT];
+    int pos[M::NT];
+#pragma unroll
+    for (int n = 0; n < M::NT; ++n) {
+        const unsigned r = r0 + 16 * n + i;
+        const int of_seq = a.token_of(min(r, r1)), tok = s.first + of_seq, head = kv * a.group + (int)(min(r, r1) - (unsigned)of_seq * a.group);
+        pos[n] = r <= r1 ? (int)max(s.pos_of_0 + tok, (int64_t)-1) : -1;
+        const T* row = (const T*)a.q + tok * a.q_stride + (int64_t)head * D + g * (D / 4);
+        bool finite = true;
+#pragma unroll
+        for (int ks = 0; ks < M::KS; ++ks) {
+            const MxEight<T> raw = *(const MxEight<T>*)(row + 8 * ks);
+            uint32_t w[M::QP][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = to_f32(raw.v[2 * e]), y = to_f32(raw.v[2 * e + 1]);
+                finite = finite && fabsf(x) < INFINITY && fabsf(y) < INFINITY;
+                uint32_t both[M::QP];
+                mx_pieces<M::QP>(x, y, both);
+#pragma unroll
+                for (int p = 0; p < M::QP; ++p) w[p][e] = both[p];
+            }
+#pragma unroll
+            for (int p = 0; p < M::QP; ++p) q[n][ks][p] = __builtin_bit_cast(mx_b8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
+        }
+        const uint64_t odd = __ballot(!finite);
+        finite = (odd >> i & 0x0001000100010001ull) == 0;
+        unit[n] = finite ? (a.cap > 0.f ? a.cap : a.scale) * 1.4426950408889634f : NAN;
+    }
+    // positions that all rows see (of a window: behind the last one's first)
+    const int pos_least = (int)max(s.pos_of_0 + s.first + a.token_of(r0), (int64_t)-1), pos_most = (int)max(s.pos_of_0 + s.first + a.token_of(r1), (int64_t)-1);
+
+    float top[M::NT], base[M::NT];   // the product or tanh that weights are put to a new maximum above, and that maximum as a score
+    v4f l[M::NT], acc[M::NT][M::NB];
+#pragma unroll
+    for (int n = 0; n < M::NT; ++n) {
+        top[n] = -INFINITY;
+        base[n] = 0.f;
+        l[n] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < M::NB; ++b) acc[n][b] = (v4f){0.f, 0.f, 0.f, 0.f};
+    }
+    const mx_b8 ones = __builtin_bit_cast(mx_b8, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
+
+    auto step = [&](Loaded& now, Loaded& then) {
+        const int p0 = lo + t * STEP;
+        // (Behind the last step this one's are loaded again, out of the cache: a load that is left out at times would be waited for at the
+        // next use of any.)
+        const bool more = t + WAVES < t_end;
+        int from[TILES], behind[TILES], absent = 0;
+#pragma unroll
+        for (int b = 0; b < TILES; ++b) {
+            from[b] = more ? next[b] : pages[b];
+            behind[b] = page_of(t + 2 * WAVES, b);
+            absent |= (pages[b] < 0) << b;
+        }
+        load(then, t + WAVES, from);
+        // whether every row sees every position of the step
+        const bool whole = p0 + STEP - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && absent == 0;
+        v4f sc[M::NT][TILES];
+#pragma unroll
+        for (int b = 0; b < TILES; ++b) {
+#pragma unroll
+            for (int n = 0; n < M::NT; ++n) sc[n][b] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < M::KS; ++ks) {
+                const float power = D == 256 && ks >= M::KS / 2 ? mx_power_of<1>(now.kp[b]) : mx_power_of<0>(now.kp[b]);
+                const mx_b8 op = mx_eight(now.k[b].w[ks], power);
+#pragma unroll
+                for (int n = 0; n < M::NT; ++n)
+#pragma unroll
+                    for (int p = 0; p < M::QP; ++p) sc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, q[n][ks][p], sc[n][b], 0, 0, 0);
+            }
+        }
+        mx_b8 share[M::NT][M::SP];
+#pragma unroll
+        for (int n = 0; n < M::NT; ++n) {
+            float x[4 * TILES], most = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4 * TILES; ++e) x[e] = sc[n][e >> 2][e & 3];
+            if (a.cap > 0.f) {
+#pragma unroll
+                for (int e = 0; e < 4 * TILES; ++e) x[e] = mx_tanh<M::FINE>(x[e] * capped);
+            }
+            if (!whole) {
+                const int last = pos[n] - p0 - 4 * g, first = a.window > 0 ? last - a.window : -0x40000000;
+#pragma unroll
+                for (int e = 0; e < 4 * TILES; ++e) {
+                    const int at = 16 * (e >> 2) + (e & 3);
+                    if (at > last || at <= first || (absent >> (e >> 2) & 1)) x[e] = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4 * TILES; ++e) most = fmaxf(most, x[e]);
+            if (__ballot(most > top[n])) {
+                most = max_over_groups(most);
+                const bool first = top[n] == -INFINITY, up = most > top[n];
+                const float to = up ? most * unit[n] : base[n], keep = first ? 1.f : __builtin_amdgcn_exp2f(base[n] - to);
+                l[n] *= keep;
+#pragma unroll
+                for (int b = 0; b < M::NB; ++b) acc[n][b] *= keep;
+                base[n] = to;
+                top[n] = up ? most + SLACK / unit[n] : top[n];
+            }
+            uint32_t w[M::SP][2 * TILES];
+#pragma unroll
+            for (int e = 0; e < 2 * TILES; ++e) {
+                uint32_t both[M::SP];
+                mx_pieces<M::SP>(__builtin_amdgcn_exp2f(fmaf(x[2 * e], unit[n], -base[n])), __builtin_amdgcn_exp2f(fmaf(x[2 * e + 1], unit[n], -base[n])), both);
+#pragma unroll
+                for (int j = 0; j < M::SP; ++j) w[j][e] = both[j];
+            }
+#pragma unroll
+            for (int j = 0; j < M::SP; ++j) share[n][j] = __builtin_bit_cast(mx_b8, make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]));
+        }
+        if (!whole) {
+            // what no row sees may hold anything: its values count as zeros
+#pragma unroll
+            for (int b = 0; b < TILES; ++b) {
+                uint32_t seen = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = p0 + 16 * b + 4 * g + j;
+                    if (at >= seen_from && at < hi && !(absent >> b & 1)) seen |= 0xFFu << (8 * j);
+                }
+                now.vp[b] &= seen;
+            }
+        }
+        float power[4 * TILES];
+#pragma unroll
+        for (int b = 0; b < TILES; ++b) {
+            power[4 * b] = mx_power_of<0>(now.vp[b]);
+            power[4 * b + 1] = mx_power_of<1>(now.vp[b]);
+            power[4 * b + 2] = mx_power_of<2>(now.vp[b]);
+            power[4 * b + 3] = mx_power_of<3>(now.vp[b]);
+        }
+#pragma unroll
+        for (int n = 0; n < M::NT; ++n)
+#pragma unroll
+            for (int j = 0; j < M::SP; ++j) l[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, share[n][j], l[n], 0, 0, 0);
+#pragma unroll
+        for (int byte = 0; byte < M::PART; ++byte) {   // columns 2 byte and 2 byte + 1 of the lane's sixteenth
+            uint32_t c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = (j & 3) * M::PART + byte;
+                const uint32_t word = now.v[j >> 2].w[at >> 2];
+                const int sel = at & 3;
+                c[j] = sel == 0 ? mx_two<0>(word, power[j]) : sel == 1 ? mx_two<1>(word, power[j]) : sel == 2 ? mx_two<2>(word, power[j]) : mx_two<3>(word, power[j]);
+            }
+            uint32_t even[4], odd[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                even[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x05040100u);
+                odd[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x07060302u);
+            }
+            const mx_b8 op0 = __builtin_bit_cast(mx_b8, make_uint4(even[0], even[1], even[2], even[3]));
+            const mx_b8 op1 = __builtin_bit_cast(mx_b8, make_uint4(odd[0], odd[1], odd[2], odd[3]));
+#pragma unroll
+            for (int n = 0; n < M::NT; ++n)
+#pragma unroll
+                for (int j = 0; j < M::SP; ++j) {
+                    acc[n][2 * byte] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op0, share[n][j], acc[n][2 * byte], 0, 0, 0);
+                    acc[n][2 * byte + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op1, share[n][j], acc[n][2 * byte + 1], 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int b = 0; b < TILES; ++b) {
+            pages[b] = next[b];
+            next[b] = behind[b];
+        }
+        t += WAVES;
+    };
+    while (t < t_end) {
+        step(loaded[0], loaded[1]);
+        if (t < t_end) step(loaded[1], loaded[0]);
+    }
+
+    // the two waves' sums relative to their common maximum, sixteen rows at a time
+#pragma unroll
+    for (int n = 0; n < M::NT; ++n)
+        if (g == 0) {
+            tops[wave][16 * n + i] = top[n] == -INFINITY ? -INFINITY : base[n];
+            weights[wave][16 * n + i] = l[n][0];
+        }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < M::NT; ++n) {
+        const int r = 16 * n + i;
+        const float most = fmaxf(tops[0][r], tops[1][r]);
+        const float f = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base[n] - most);
+        // column of the sums: the lane's rows 4 g + e of the operand are sixteenths of the head
+        if (wave == 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int b = 0; b < M::NB; ++b) sums[i][(4 * g + e) * (D / 16) + b] = acc[n][b][e] * f;
+        }
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int b = 0; b < M::NB; ++b) sums[i][(4 * g + e) * (D / 16) + b] += acc[n][b][e] * f;
+        }
+        __syncthreads();
+        for (int at = threadIdx.x; at < min((int)(r1 - r0) + 1 - 16 * n, 16) * D; at += 64 * WAVES) {
+            const int rr = at / D, d = at % D, row_of = 16 * n + rr;
+            const float m0 = tops[0][row_of], m1 = tops[1][row_of], m = fmaxf(m0, m1);
+            // (a part whose scores are no numbers has a sum that is none, and may have no maximum)
+            const float lw = (m0 == -INFINITY ? weights[0][row_of] : weights[0][row_of] * __builtin_amdgcn_exp2f(m0 - m)) +
+                             (m1 == -INFINITY ? weights[1][row_of] : weights[1][row_of] * __builtin_amdgcn_exp2f(m1 - m));
+            const float total = sums[rr][d];
+            const int of_seq = a.token_of(r0 + row_of), head = kv * a.group + (int)(r0 + row_of - (unsigned)of_seq * a.group);
+            const int64_t row = s.first + of_seq;
+            if (span.parts == 1) {
+                ((T*)a.out)[row * a.out_stride + (int64_t)head * D + d] = from_f32<T>(lw == 0.f ? 0.f : total / lw);
+            } else {
+                const int64_t place = (a.part_row(seq, s, (int)row) * a.heads + head) * a.splits + part;
+                a.part_o[place * D + d] = total;
+                if (d == 0) a.part_ml[place] = make_float2(m, lw);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int D>
+static int launch(const AttendMx& a, hipStream_t s) {
+    const int64_t tiles = ((int64_t)a.rows * a.group + Many<T, D>::ROWS - 1) / Many<T, D>::ROWS + a.seqs, blocks = tiles * a.mx.heads * a.splits;
+    if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
+    hipLaunchKernelGGL((mx_many_kernel<T, D>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a);
+    return lk_launch_status();
+}
+
+template <typename T>
+static int by_dim(const AttendMx& a, int head_dim, hipStream_t s) {
+    return head_dim == 64 ? launch<T, 64>(a, s) : head_dim == 128 ? launch<T, 128>(a, s) : launch<T, 256>(a, s);
+}
+
+}  // namespace
+
+int kv_attention_mxfp4_many(const AttendMx& a, int type, int head_dim, hipStream_t s) {
+    if (type == LK_TYPE_F32) return by_dim<float>(a, head_dim, s);
+    if (type == LK_TYPE_F16) return by_dim<__half>(a, head_dim, s);
+    return by_dim<__hip_bfloat16>(a, head_dim, s);
+}
