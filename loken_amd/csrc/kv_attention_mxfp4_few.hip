@@ -47,7 +47,8 @@ static __device__ __forceinline__ float sum_of_slots(float v) {
     return v;
 }
 
-template <typename T, int D, int NT, int SLOTS>
+// CAP: whether scores are capped (as a branch at run time the compiler takes the tanh always, and the result where it is asked for)
+template <typename T, int D, int NT, int SLOTS, bool CAP>
 __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void mx_few_kernel(AttendMx a, int row_tiles) {
     using F = Few<T, D, NT, SLOTS>;
     __shared__ float sums[WAVES][F::RPT][D + 4];
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
         for (int b = 0; b < 4; ++b) next[b] = page_of(t + WAVES, b);
         if (t < t_end) load(loaded[0], t, pages);
 
-        const float capped = a.cap > 0.f ? a.scale / a.cap : 0.f;   // what a product is under the tanh
+        const float capped = CAP ? a.scale / a.cap : 0.f;   // what a product is under the tanh
         // the rows' pieces, and what a product, or its tanh, is in powers of two
         mx_b8 q[NT][F::KS][F::QP];
         float unit[NT];
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             }
             const uint64_t odd = __ballot(!finite);
             finite = (odd >> i & 0x0001000100010001ull) == 0;
-            unit[n] = finite ? (a.cap > 0.f ? a.cap : a.scale) * 1.4426950408889634f : NAN;
+            unit[n] = finite ? (CAP ? a.cap : a.scale) * 1.4426950408889634f : NAN;
         }
         int pos_least = 0x7FFFFFFF, pos_most = -1;
 #pragma unroll
@@ -261,11 +262,12 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
                 float x[16], top = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[e] = sum_of_slots<SLOTS>(sc[n][e >> 2][e & 3]);
-                if (a.cap > 0.f) {
+                if (CAP) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[e] = mx_tanh<sizeof(T) == 4>(x[e] * capped);
                 }
                 if (!whole) {
+                    asm volatile("");   // (stays a branch: the looks at sixteen positions would else be made in every step)
                     const int last = pos[n] - p0 - 4 * g, first = a.window > 0 ? last - a.window : -0x40000000;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
@@ -439,7 +441,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool CAP>
 static int launch(const AttendMx& a, int max_rows, hipStream_t s) {
     constexpr int SLOTS = sizeof(T) == 4 ? 4 : 2;
     const int per = mx_few_rows(sizeof(T) == 4, D, max_rows), row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / per + 1;
@@ -448,17 +450,22 @@ static int launch(const AttendMx& a, int max_rows, hipStream_t s) {
     const dim3 grid((unsigned)blocks), threads(64 * WAVES);
     if constexpr (sizeof(T) == 4 && D < 256)
         if (per == 8) {
-            hipLaunchKernelGGL((mx_few_kernel<T, D, 2, SLOTS>), grid, threads, 0, s, a, row_tiles);
+            hipLaunchKernelGGL((mx_few_kernel<T, D, 2, SLOTS, CAP>), grid, threads, 0, s, a, row_tiles);
             return lk_launch_status();
         }
-    if (per == Few<T, D, 1, SLOTS>::ROWS) hipLaunchKernelGGL((mx_few_kernel<T, D, 1, SLOTS>), grid, threads, 0, s, a, row_tiles);
-    else hipLaunchKernelGGL((mx_few_kernel<T, D, 1, 1>), grid, threads, 0, s, a, row_tiles);
+    if (per == 16 / SLOTS) hipLaunchKernelGGL((mx_few_kernel<T, D, 1, SLOTS, CAP>), grid, threads, 0, s, a, row_tiles);
+    else hipLaunchKernelGGL((mx_few_kernel<T, D, 1, 1, CAP>), grid, threads, 0, s, a, row_tiles);
     return lk_launch_status();
+}
+
+template <typename T, int D>
+static int by_cap(const AttendMx& a, int max_rows, hipStream_t s) {
+    return a.cap > 0.f ? launch<T, D, true>(a, max_rows, s) : launch<T, D, false>(a, max_rows, s);
 }
 
 template <typename T>
 static int by_dim(const AttendMx& a, int head_dim, int max_rows, hipStream_t s) {
-    return head_dim == 64 ? launch<T, 64>(a, max_rows, s) : head_dim == 128 ? launch<T, 128>(a, max_rows, s) : launch<T, 256>(a, max_rows, s);
+    return head_dim == 64 ? by_cap<T, 64>(a, max_rows, s) : head_dim == 128 ? by_cap<T, 128>(a, max_rows, s) : by_cap<T, 256>(a, max_rows, s);
 }
 
 }  // namespace

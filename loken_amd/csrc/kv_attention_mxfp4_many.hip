@@ -60,10 +60,11 @@ static __device__ __forceinline__ bool tile_at(const Attend& a, int rows_of_tile
     return false;
 }
 
-template <typename T, int D>
+// CAP: whether scores are capped (as a branch at run time the compiler takes the tanh always, and the result where it is asked for)
+template <typename T, int D, bool CAP>
 __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof(T) == 2 && std::is_same<T, __half>::value, D))) void mx_many_kernel(AttendMx a) {
     using M = Many<T, D>;
-    __shared__ float sums[16][D + 4];
+    __shared__ __attribute__((aligned(16))) float handed[M::NT][16][D + 4];
     __shared__ float tops[WAVES][M::ROWS], weights[WAVES][M::ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4, shift = a.mx.page_shift;
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
     }
     if (t < t_end) load(loaded[0], t, pages);
 
-    const float capped = a.cap > 0.f ? a.scale / a.cap : 0.f;   // what a product is under the tanh
+    const float capped = CAP ? a.scale / a.cap : 0.f;   // what a product is under the tanh
     // the rows' pieces, and what a product, or its tanh, is in powers of two
     mx_b8 q[M::NT][M::KS][M::QP];
     float unit[M::NT];
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
         }
         const uint64_t odd = __ballot(!finite);
         finite = (odd >> i & 0x0001000100010001ull) == 0;
-        unit[n] = finite ? (a.cap > 0.f ? a.cap : a.scale) * 1.4426950408889634f : NAN;
+        unit[n] = finite ? (CAP ? a.cap : a.scale) * 1.4426950408889634f : NAN;
     }
     // positions that all rows see (of a window: behind the last one's first)
     const int pos_least = (int)max(s.pos_of_0 + s.first + a.token_of(r0), (int64_t)-1), pos_most = (int)max(s.pos_of_0 + s.first + a.token_of(r1), (int64_t)-1);
@@ -210,11 +211,12 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             float x[4 * TILES], most = -INFINITY;
 #pragma unroll
             for (int e = 0; e < 4 * TILES; ++e) x[e] = sc[n][e >> 2][e & 3];
-            if (a.cap > 0.f) {
+            if (CAP) {
 #pragma unroll
                 for (int e = 0; e < 4 * TILES; ++e) x[e] = mx_tanh<M::FINE>(x[e] * capped);
             }
             if (!whole) {
+                asm volatile("");   // (stays a branch: the looks at eight positions would else be made in every step)
                 const int last = pos[n] - p0 - 4 * g, first = a.window > 0 ? last - a.window : -0x40000000;
 #pragma unroll
                 for (int e = 0; e < 4 * TILES; ++e) {
@@ -308,52 +310,53 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
         if (t < t_end) step(loaded[1], loaded[0]);
     }
 
-    // the two waves' sums relative to their common maximum, sixteen rows at a time
+    // The two waves' sums relative to their common maximum: each wave hands the other the half of the rows that it does not finish.
 #pragma unroll
     for (int n = 0; n < M::NT; ++n)
         if (g == 0) {
             tops[wave][16 * n + i] = top[n] == -INFINITY ? -INFINITY : base[n];
             weights[wave][16 * n + i] = l[n][0];
         }
+#pragma unroll
+    for (int n = 0; n < M::NT; ++n)
+        if (n != wave) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int b = 0; b < M::NB; b += 4)
+                    *(float4*)&handed[n][i][(4 * g + e) * (D / 16) + b] = make_float4(acc[n][b][e], acc[n][b + 1][e], acc[n][b + 2][e], acc[n][b + 3][e]);
+        }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < M::NT; ++n) {
-        const int r = 16 * n + i;
-        const float most = fmaxf(tops[0][r], tops[1][r]);
-        const float f = top[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base[n] - most);
-        // column of the sums: the lane's rows 4 g + e of the operand are sixteenths of the head
-        if (wave == 1) {
+        const unsigned r = r0 + 16 * n + i;
+        if (n != wave || r > r1) continue;
+        const float m0 = tops[0][16 * n + i], m1 = tops[1][16 * n + i], m = fmaxf(m0, m1);
+        // (a part whose scores are no numbers has a sum that is none, and may have no maximum)
+        const float f0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - m), f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
+        const float w0 = weights[0][16 * n + i], w1 = weights[1][16 * n + i], lw = (m0 == -INFINITY ? w0 : w0 * f0) + (m1 == -INFINITY ? w1 : w1 * f1);
+        const float mine = n == 0 ? f0 : f1, others = n == 0 ? f1 : f0;
+        const int of_seq = a.token_of(r), head = kv * a.group + (int)(r - (unsigned)of_seq * a.group);
+        const int64_t row = s.first + of_seq, place = (a.part_row(seq, s, (int)row) * a.heads + head) * a.splits + part;
+        const float by = span.parts > 1 ? 1.f : lw == 0.f ? 0.f : 1.f / lw;
+        // the lane's rows 4 g + e of the operand are sixteenths of the head
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e) {
+            const int d0 = (4 * g + e) * (D / 16);
+            float x[M::NB];
 #pragma unroll
-                for (int b = 0; b < M::NB; ++b) sums[i][(4 * g + e) * (D / 16) + b] = acc[n][b][e] * f;
-        }
-        __syncthreads();
-        if (wave == 0) {
+            for (int b = 0; b < M::NB; ++b) x[b] = fmaf(handed[n][i][d0 + b], others, acc[n][b][e] * mine) * by;
+            if (span.parts > 1) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int b = 0; b < M::NB; ++b) sums[i][(4 * g + e) * (D / 16) + b] += acc[n][b][e] * f;
-        }
-        __syncthreads();
-        for (int at = threadIdx.x; at < min((int)(r1 - r0) + 1 - 16 * n, 16) * D; at += 64 * WAVES) {
-            const int rr = at / D, d = at % D, row_of = 16 * n + rr;
-            const float m0 = tops[0][row_of], m1 = tops[1][row_of], m = fmaxf(m0, m1);
-            // (a part whose scores are no numbers has a sum that is none, and may have no maximum)
-            const float lw = (m0 == -INFINITY ? weights[0][row_of] : weights[0][row_of] * __builtin_amdgcn_exp2f(m0 - m)) +
-                             (m1 == -INFINITY ? weights[1][row_of] : weights[1][row_of] * __builtin_amdgcn_exp2f(m1 - m));
-            const float total = sums[rr][d];
-            const int of_seq = a.token_of(r0 + row_of), head = kv * a.group + (int)(r0 + row_of - (unsigned)of_seq * a.group);
-            const int64_t row = s.first + of_seq;
-            if (span.parts == 1) {
-                ((T*)a.out)[row * a.out_stride + (int64_t)head * D + d] = from_f32<T>(lw == 0.f ? 0.f : total / lw);
+                for (int b = 0; b < M::NB; ++b) a.part_o[place * D + d0 + b] = x[b];
             } else {
-                const int64_t place = (a.part_row(seq, s, (int)row) * a.heads + head) * a.splits + part;
-                a.part_o[place * D + d] = total;
-                if (d == 0) a.part_ml[place] = make_float2(m, lw);
+                struct __attribute__((aligned(sizeof(T)))) Run { T v[M::NB]; } run;   // rows of out start on any value
+#pragma unroll
+                for (int b = 0; b < M::NB; ++b) run.v[b] = from_f32<T>(x[b]);
+                *(Run*)((T*)a.out + row * a.out_stride + (int64_t)head * D + d0) = run;
             }
         }
-        __syncthreads();
+        if (span.parts > 1 && g == 0) a.part_ml[place] = make_float2(m, lw);
     }
 }
 
@@ -361,7 +364,8 @@ template <typename T, int D>
 static int launch(const AttendMx& a, hipStream_t s) {
     const int64_t tiles = ((int64_t)a.rows * a.group + Many<T, D>::ROWS - 1) / Many<T, D>::ROWS + a.seqs, blocks = tiles * a.mx.heads * a.splits;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
-    hipLaunchKernelGGL((mx_many_kernel<T, D>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a);
+    if (a.cap > 0.f) hipLaunchKernelGGL((mx_many_kernel<T, D, true>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a);
+    else hipLaunchKernelGGL((mx_many_kernel<T, D, false>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a);
     return lk_launch_status();
 }
 
