@@ -919,7 +919,7 @@ int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, void* out, 
  *   probs[rows]      p of these tokens (nullable), 0 where there is none
  *   accepted[seqs]   how many drafts were
  * Of a sequence's last row uniform, drafted and draft are not looked at; a sequence without rows gets accepted 0. Weights are summed as lk_sample's are, what is left as
- * integers of 2^-62. Limits and scratch as lk_sample's; up to 65535 sequences. Without rows or sequences nothing is written. */
+ * integers of 2^-51. Limits and scratch as lk_sample's; up to 65535 sequences. Without rows or sequences nothing is written. */
 int lk_verify(const void* logits, int type, int64_t stride, int rows, int vocab, const int32_t* drafted, const int32_t* starts, int seqs,
               const void* draft, int draft_type, int64_t draft_stride, const float* uniform, const float* draw, const float* temperature,
               const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, int32_t* accepted, float* probs,

@@ -19,6 +19,41 @@
 
 namespace {
 
+// The largest and the smallest word of a piece of a row; clears the row's histogram on the way.
+template <typename T>
+__global__ __launch_bounds__(SAMPLE_WG) void sample_peak_kernel(Sampling a) {
+    __shared__ Peak meet[SAMPLE_WAVES];
+    const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
+    float best = -INFINITY, lowest = INFINITY;
+    int at = 0x7FFFFFFF;
+    each_word<4>((const T*)a.logits + row * a.stride, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](float v, int i) {
+        const bool more = v > best;   // a thread meets the words in rising order
+        best = more ? v : best;
+        at = more ? i : at;
+        lowest = v > -INFINITY ? fminf(lowest, v) : lowest;   // (fminf passes over what is not a number)
+    });
+    for (int i = c * SAMPLE_WG + t; i < BINS; i += a.chunks * SAMPLE_WG) {
+        a.mass[(int64_t)row * BINS + i] = 0;
+        a.count[(int64_t)row * BINS + i] = 0;
+    }
+    if (c == 0 && t == 0) { a.floor_mass[row] = 0; a.arrived[row] = 0; }
+    Peak p{best > -INFINITY ? (uint64_t)key_of(best) << 32 | (uint32_t)~at : 0, key_of(lowest), 0};
+    wave_peak(p);
+    if ((t & 63) == 0) meet[t >> 6] = p;
+    __syncthreads();
+    if (t >= 64) return;
+    p = t < SAMPLE_WAVES ? meet[t] : Peak{0, 0xFFFFFFFFu, 0};
+    wave_peak(p);
+    if (t == 0) a.peaks[(int64_t)row * a.pieces + c] = p;
+}
+
+template <typename T>
+__global__ __launch_bounds__(SAMPLE_WG, 4) void sample_steps_kernel(Sampling a) {
+    __shared__ uint64_t mass[BINS];
+    __shared__ uint32_t count[BINS];
+    steps_of_row<T>(a, mass, count);
+}
+
 template <typename T>
 __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a) {
     __shared__ Shared sh;
@@ -43,7 +78,7 @@ extern "C" int lk_sample(const void* logits, int type, int64_t stride, int rows,
     if (vocab > LK_SAMPLE_VOCAB) return LK_ERR_SIZE;
     if (rows == 0) return LK_OK;
     if (!logits || !uniform || !temperature || !tokens || ((uintptr_t)logits & (size - 1))) return LK_ERR_ARG;
-    Sampling a{logits, stride, vocab, 0, 0, uniform, temperature, top_p, min_p, top_k, tokens, probs, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+    Sampling a{logits, stride, vocab, 0, 0, 0, uniform, temperature, top_p, min_p, top_k, tokens, probs, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     cut_rows(a, rows, size);
     LkScratch scratch((hipStream_t)stream);
     uint8_t* mem = (uint8_t*)scratch.get(LK_SCRATCH_SAMPLE, (size_t)rows * bytes_of_row(a));

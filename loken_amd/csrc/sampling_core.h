@@ -85,12 +85,12 @@ static __device__ __forceinline__ void wave_peak(Peak& p) {
 struct Sampling {
     const void* logits;
     int64_t stride;
-    int vocab, chunk, chunks;
+    int vocab, chunk, chunks, pieces;   // words of a piece, pieces of a row, and pieces whose peaks are taken by themselves
     const float *uniform, *temperature, *top_p, *min_p;
     const int32_t* top_k;
     int32_t* tokens;
     float* probs;
-    Peak* peaks;          // [rows][chunks]
+    Peak* peaks;          // [rows][pieces]
     uint64_t* mass;       // [rows][BINS]
     uint32_t* count;      // [rows][BINS]
     uint64_t* floor_mass; // [rows]: what min-p keeps
@@ -105,34 +105,6 @@ struct Kept {
     uint64_t best, last, kept;
 };
 
-// The largest and the smallest word of a piece of a row; clears the row's histogram on the way.
-template <typename T>
-__global__ __launch_bounds__(SAMPLE_WG) void sample_peak_kernel(Sampling a) {
-    __shared__ Peak meet[SAMPLE_WAVES];
-    const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
-    float best = -INFINITY, lowest = INFINITY;
-    int at = 0x7FFFFFFF;
-    each_word<4>((const T*)a.logits + row * a.stride, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](float v, int i) {
-        const bool more = v > best;   // a thread meets the words in rising order
-        best = more ? v : best;
-        at = more ? i : at;
-        lowest = v > -INFINITY ? fminf(lowest, v) : lowest;   // (fminf passes over what is not a number)
-    });
-    for (int i = c * SAMPLE_WG + t; i < BINS; i += a.chunks * SAMPLE_WG) {
-        a.mass[(int64_t)row * BINS + i] = 0;
-        a.count[(int64_t)row * BINS + i] = 0;
-    }
-    if (c == 0 && t == 0) { a.floor_mass[row] = 0; a.arrived[row] = 0; }
-    Peak p{best > -INFINITY ? (uint64_t)key_of(best) << 32 | (uint32_t)~at : 0, key_of(lowest), 0};
-    wave_peak(p);
-    if ((t & 63) == 0) meet[t >> 6] = p;
-    __syncthreads();
-    if (t >= 64) return;
-    p = t < SAMPLE_WAVES ? meet[t] : Peak{0, 0xFFFFFFFFu, 0};
-    wave_peak(p);
-    if (t == 0) a.peaks[(int64_t)row * a.chunks + c] = p;
-}
-
 // a b + c, c the same for all lanes: from scalar registers, where the compiler would copy it to the sum's register first: five of forty
 // instructions a word, 256 rows of 151936 in bf16 47 us instead of 40.
 static __device__ __forceinline__ double fma_by(double a, double b, double c) {
@@ -141,10 +113,10 @@ static __device__ __forceinline__ double fma_by(double a, double b, double c) {
     return r;
 }
 
-// 2^x, x = below * rate, -43 <= x <= 0, as an integer of 2^-42. x = n + r, |r| <= 1/2; 2^r = 1 + r f(r), f the polynomial of degree 8
+// 2^x, x = below * rate, -43 <= x <= 0. x = n + r, |r| <= 1/2; 2^r = 1 + r f(r), f the polynomial of degree 8
 // through (2^r - 1) / r at the nine Chebyshev points of [-1/2, 1/2]: off by 2.8e-14. Its terms from r^5 on, which are below 2.4e-6 of
 // the result, are made in 32 bits: off by 2e-13.
-static __device__ __forceinline__ uint64_t weight_of(double below, double rate) {
+static __device__ __forceinline__ double power_of(double below, double rate) {
     const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
     const double y = fma(below, rate, magic);
     const int n = (int)(uint32_t)__double_as_longlong(y);
@@ -157,9 +129,12 @@ static __device__ __forceinline__ uint64_t weight_of(double below, double rate) 
     p = fma_by(r, p, 0.2402265069581299);
     p = fma_by(r, p, 0.6931471805599453);
     p = fma(r, p, 1.0);
-    // times 2^n in the exponent; 1024 more, and the last place is 2^-42: what the sum rounds to is the integer
-    const uint64_t scaled = (uint64_t)__double_as_longlong(p) + ((uint64_t)(uint32_t)(n << 20) << 32);
-    return (uint64_t)__double_as_longlong(__longlong_as_double((long long)scaled) + 1024.0) - 0x4090000000000000ull;
+    // times 2^n in the exponent
+    return __longlong_as_double((long long)((uint64_t)__double_as_longlong(p) + ((uint64_t)(uint32_t)(n << 20) << 32)));
+}
+// The same as an integer of 2^-42: 1024 more, and the last place is 2^-42: what the sum rounds to is the integer.
+static __device__ __forceinline__ uint64_t weight_of(double below, double rate) {
+    return (uint64_t)__double_as_longlong(power_of(below, rate) + 1024.0) - 0x4090000000000000ull;
 }
 
 // What a row's weights and steps go by.
@@ -203,8 +178,8 @@ struct Scale {
 
 static __device__ __forceinline__ Peak peak_of_row(const Sampling& a, int row) {
     Peak peak{0, 0xFFFFFFFFu, 0};
-    for (int i = threadIdx.x & 63; i < a.chunks; i += 64) {
-        const Peak p = a.peaks[(int64_t)row * a.chunks + i];
+    for (int i = threadIdx.x & 63; i < a.pieces; i += 64) {
+        const Peak p = a.peaks[(int64_t)row * a.pieces + i];
         peak.best = p.best > peak.best ? p.best : peak.best;
         peak.lowest = p.lowest < peak.lowest ? p.lowest : peak.lowest;
     }
@@ -575,9 +550,7 @@ static __device__ __forceinline__ uint64_t weigh_as(const T* x, int begin, int e
     return above;
 }
 template <typename T>
-__global__ __launch_bounds__(SAMPLE_WG, 4) void sample_steps_kernel(Sampling a) {
-    __shared__ uint64_t mass[BINS];
-    __shared__ uint32_t count[BINS];
+static __device__ __forceinline__ void steps_of_row(const Sampling& a, uint64_t (&mass)[BINS], uint32_t (&count)[BINS]) {
     const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     Scale sc;
     if (!sc.init(peak_of_row(a, row), a.temperature[row], a.min_p ? a.min_p[row] : 0.0f) || sc.infinite) return;
@@ -844,15 +817,15 @@ static void cut_rows(Sampling& a, int rows, int size) {
     int chunks = (2 * lk_device().cus + rows - 1) / rows;
     if (chunks > (a.vocab + 4095) / 4096) chunks = (a.vocab + 4095) / 4096;
     a.chunk = ((a.vocab + chunks - 1) / chunks + vec - 1) / vec * vec;
-    a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
+    a.pieces = a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
 }
 // Bytes that a row needs between the launches, and where they are.
 static size_t bytes_of_row(const Sampling& a) {
-    return (size_t)BINS * 12 + 12 + a.chunks * (sizeof(Peak) + 4 + (a.chunks > 1 ? (size_t)LIST * 8 : 0));
+    return (size_t)BINS * 12 + 12 + a.pieces * sizeof(Peak) + a.chunks * (4 + (a.chunks > 1 ? (size_t)LIST * 8 : 0));
 }
 static void place_rows(Sampling& a, int rows, uint8_t* mem) {
     a.peaks = (Peak*)mem;
-    a.mass = (uint64_t*)(a.peaks + (size_t)rows * a.chunks);
+    a.mass = (uint64_t*)(a.peaks + (size_t)rows * a.pieces);
     a.list = a.mass + (size_t)rows * BINS;
     a.floor_mass = a.list + (a.chunks > 1 ? (size_t)rows * a.chunks * LIST : 0);
     a.count = (uint32_t*)(a.floor_mass + rows);

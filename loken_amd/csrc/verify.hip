@@ -1,18 +1,20 @@
 // Drafted tokens against the target's distribution (lk_verify), and the token that follows those that are accepted.
 //
-// A row's distribution p is what sampling would draw from: weights as integers of 2^-42 of the words that top-k, top-p and min-p keep, over their
-// sum. So the launches are sampling's (peak, steps, and its choice cut short where the kept words' last is known), and one more:
-//   judge   pieces of the row at which a sequence ends. Every workgroup finds that row itself: drafts a lane each, accepted while u q < p. The pieces' sums
-//           of what is left, max(p - q, 0) or p, meet; the sequence's last workgroup finds the piece in which the draw lies and goes through it again.
-// Differences p - q are made in 64 bits and summed as integers of 2^-62, whose sums do not depend on an order.
+// A row's distribution p is what sampling would draw from: weights of the words that top-k, top-p and min-p keep, as numbers of 2^-42, over their
+// sum. Four launches:
+//   pieces  each piece's largest word, and, of rows that no rule cuts, its sum of weights relative to that: one pass over these rows' words.
+//   steps   sampling's histogram, of the other rows alone
+//   kept    where the rules' last word is, as sampling finds it; of rows that nothing cuts the pieces' sums, put to the row's largest word
+//   judge   pieces of the row at which a sequence ends. Every workgroup finds that row itself: drafts a lane each, accepted while u q < p. It sums what is
+//           left, max(p - q, 0) or p, round by round of neighbouring words; the sequence's last workgroup finds the round in which the draw lies and
+//           goes through that again.
+// Differences p - q are made in 64 bits and summed as integers of 2^-51, whose sums do not depend on an order.
 //
-// Bound by the passes over the logits: three of all rows (two where nothing cuts), one and a piece of one row of each sequence, and as much of the draft's row.
+// Bound by the passes over the logits, one of rows that nothing cuts, up to three of others, and by the issue of 30 instructions a weight.
 
 #include "sampling_core.h"
 
 namespace {
-
-constexpr double LEFT_ONE = 4611686018427387904.0;   // 2^62
 
 struct Verify {
     Sampling s;
@@ -24,99 +26,206 @@ struct Verify {
     const float *uniform, *draw;
     int32_t *tokens, *accepted;
     float* probs;
-    uint64_t* left;          // [rows][chunks]: sums of the pieces, of a sequence's at its first row
+    uint64_t* sums;          // [rows][s.pieces]: weights of the pieces of rows that nothing cuts
+    int rounds, per_piece;   // rounds of a row as `judge` goes through it, and those of one of its workgroups
+    uint64_t* left;          // [rows][rounds]: sums of the rounds, of a sequence's at its first row
     uint32_t* met;           // [rows]: pieces that have been summed
 };
 
-// A row's distribution.
-struct Target {
+// Whether a row is sampled from all of its words.
+static __device__ __forceinline__ bool uncut(const Sampling& a, int row) {
+    const int k = a.top_k ? a.top_k[row] : 0;
+    return a.temperature[row] > 0.0f && !(k > 0 && k < a.vocab) && !(a.top_p && a.top_p[row] < 1.0f) && !(a.min_p && a.min_p[row] > 0.0f);
+}
+
+// WORDS a thread.
+template <int WORDS, typename T>
+__global__ __launch_bounds__(SAMPLE_WG) void verify_pieces_kernel(Verify v) {
+    constexpr int VEC = 16 / sizeof(T), RUNS = WORDS / VEC;
+    struct __attribute__((aligned(sizeof(T)))) Run { T v[VEC]; };
+    __shared__ Peak meet[SAMPLE_WAVES];
+    __shared__ uint64_t meet_sums[SAMPLE_WAVES];
+    const Sampling& a = v.s;
+    const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x, wave = t >> 6;
+    const T* words = (const T*)a.logits + row * a.stride;
+    const int begin = c * SAMPLE_WG * WORDS + t * VEC, end = min((c + 1) * SAMPLE_WG * WORDS, a.vocab);
+    float x[WORDS];
+#pragma unroll
+    for (int j = 0; j < RUNS; ++j) {
+        const int i = begin + j * SAMPLE_WG * VEC;
+        if (i + VEC <= end) {
+            const Run r = *(const Run*)(words + i);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[j * VEC + e] = to_f32(r.v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[j * VEC + e] = i + e < end ? to_f32(words[i + e]) : -INFINITY;
+        }
+    }
+    if (t == 0 && c == 0) {
+        a.floor_mass[row] = 0;
+        a.arrived[row] = 0;
+        v.met[row] = 0;
+        v.tokens[row] = -1;
+        if (v.probs) v.probs[row] = 0.0f;
+    }
+    const bool weigh = uncut(a, row);
+    if (!weigh)
+        for (int i = c * SAMPLE_WG + t; i < BINS; i += a.pieces * SAMPLE_WG) {
+            a.mass[(int64_t)row * BINS + i] = 0;
+            a.count[(int64_t)row * BINS + i] = 0;
+        }
+    float best = -INFINITY, lowest = INFINITY;
+    int at = 0;
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) {   // a thread meets the words in rising order
+        const bool more = x[j] > best;
+        best = more ? x[j] : best;
+        at = more ? j : at;
+        lowest = x[j] > -INFINITY ? fminf(lowest, x[j]) : lowest;   // (fminf passes over what is not a number)
+    }
+    at = begin + at / VEC * (SAMPLE_WG * VEC) + at % VEC;
+    Peak p{best > -INFINITY ? (uint64_t)key_of(best) << 32 | (uint32_t)~at : 0, key_of(lowest), 0};
+    wave_peak(p);
+    if ((t & 63) == 0) meet[wave] = p;
+    __syncthreads();
+    p = meet[0];
+#pragma unroll
+    for (int w = 1; w < SAMPLE_WAVES; ++w) {
+        const Peak o = meet[w];
+        p.best = o.best > p.best ? o.best : p.best;
+        p.lowest = o.lowest < p.lowest ? o.lowest : p.lowest;
+    }
+    if (t == 0) a.peaks[(int64_t)row * a.pieces + c] = p;
+    if (!weigh) return;
+    uint64_t sum = 0;
     Scale sc;
-    Kept kept;
-    double by;   // 1 / kept weight
-    __device__ __forceinline__ void init(const Sampling& a, const Kept& k, int row) {
-        kept = k;
-        const Peak peak{k.best, key_of(0.0f), 0};
-        sc.init(peak, kept.kept ? a.temperature[row] : 1.0f, a.min_p ? a.min_p[row] : 0.0f);
-        by = 1.0 / (double)kept.kept;
+    if (sc.init(p, a.temperature[row], 0.0f)) {
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) {
+            const uint64_t w = weight_of(sc.from_top(x[j]), sc.rate);
+            sum += sc.live(sc.below(x[j])) ? w : 0;
+        }
     }
-    __device__ __forceinline__ double share(float v, int i) const {
-        const uint64_t at = (uint64_t)key_of(v) << 32 | (uint32_t)~i;
-        if (kept.kept == 0) return kept.best != 0 && at == kept.best ? 1.0 : 0.0;
-        const bool in = sc.live(sc.below(v)) && at >= kept.last && sc.kept(sc.power(v));
-        return in ? (double)sc.weight(v) * by : 0.0;
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor((unsigned long long)sum, o);
+    if ((t & 63) == 0) meet_sums[wave] = sum;
+    __syncthreads();
+    if (t == 0) {
+        sum = 0;
+        for (int w = 0; w < SAMPLE_WAVES; ++w) sum += meet_sums[w];
+        v.sums[(int64_t)row * a.pieces + c] = sum;
     }
-};
+}
+
+template <typename T>
+__global__ __launch_bounds__(SAMPLE_WG, 4) void verify_steps_kernel(Sampling a) {
+    __shared__ uint64_t mass[BINS];
+    __shared__ uint32_t count[BINS];
+    if (!uncut(a, blockIdx.y)) steps_of_row<T>(a, mass, count);
+}
 
 // Where a row is asked for its distribution alone.
 template <typename T>
 __global__ __launch_bounds__(SAMPLE_WG, 4) void verify_kept_kernel(Verify v, Kept* kept) {
     __shared__ Shared sh;
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        const int row = blockIdx.y;
-        v.met[row] = 0;
-        v.tokens[row] = -1;
-        if (v.probs) v.probs[row] = 0.0f;
+    const int row = blockIdx.y;
+    const Sampling& a = v.s;
+    if (!uncut(a, row)) {
+        choose<true, T>(a, sh, kept);
+        return;
     }
-    choose<true, T>(v.s, sh, kept);
+    if (blockIdx.x || threadIdx.x >= 64) return;
+    const Peak peak = peak_of_row(a, row);
+    Scale sc;
+    double sum = 0.0;
+    if (sc.init(peak, a.temperature[row], 0.0f)) {
+        for (int i = threadIdx.x; i < a.pieces; i += 64) {   // each lane's in the same order always
+            const uint64_t of_piece = a.peaks[(int64_t)row * a.pieces + i].best;
+            const float top = value_of((uint32_t)(of_piece >> 32));
+            if (of_piece && sc.live(sc.below(top))) sum += (double)v.sums[(int64_t)row * a.pieces + i] * power_of(sc.from_top(top), sc.rate);
+        }
+    }
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (threadIdx.x == 0) kept[row] = Kept{peak.best, 0, (uint64_t)(sum + 0.5)};
 }
+
+// A row's distribution.
+struct Target {
+    Scale sc;
+    Kept kept;
+    double by;      // 2^42 / kept weight
+    bool floored;   // whether min-p is asked for
+    __device__ __forceinline__ void init(const Sampling& a, const Kept& k, int row) {
+        kept = k;
+        const Peak peak{k.best, key_of(0.0f), 0};
+        const float least = a.min_p ? a.min_p[row] : 0.0f;
+        sc.init(peak, kept.kept ? a.temperature[row] : 1.0f, least);
+        by = kept.kept ? 4398046511104.0 / (double)kept.kept : 1.0;
+        floored = least > 0.0f;
+    }
+    __device__ __forceinline__ bool in(float v, int i) const {
+        const uint64_t at = (uint64_t)key_of(v) << 32 | (uint32_t)~i;
+        if (kept.kept == 0) return kept.best != 0 && at == kept.best;
+        return sc.live(sc.below(v)) && at >= kept.last && !(floored && !sc.kept(sc.power(v)));
+    }
+    // p of a word that is in it. (Its weight as a number of 2^-42: 1024 more and less.)
+    __device__ __forceinline__ double share(float v) const { return kept.kept == 0 ? 1.0 : ((power_of(sc.from_top(v), sc.rate) + 1024.0) - 1024.0) * by; }
+};
 
 // What is left of a row's words: p, less the draft's share or without the word that was drafted for certain.
 template <typename T, typename Q>
 struct Left {
+    static constexpr int VEC = 16 / sizeof(T), ROUND = SAMPLE_WG * VEC;
+    struct __attribute__((aligned(sizeof(T)))) Words { T v[VEC]; };
+    struct __attribute__((aligned(sizeof(Q)))) Shares { Q v[VEC]; };
     const T* row;
     const Q* draft;    // null: nothing is taken off
     int certain;       // -1: no word
-    // Rounds over neighbouring words begin .. end - 1, VEC of them a thread, that all threads come to; f(first word, what is left of the thread's
-    // words) is false: the last round.
-    template <class F>
-    __device__ __forceinline__ void each_round(const Target& target, int begin, int end, F f) const {
-        constexpr int VEC = 16 / sizeof(T);
-        struct __attribute__((aligned(sizeof(T)))) Words { T v[VEC]; };
-        struct __attribute__((aligned(sizeof(Q)))) Shares { Q v[VEC]; };
-        for (int i0 = begin; i0 < end; i0 += SAMPLE_WG * VEC) {
-            const int i = i0 + (int)threadIdx.x * VEC;
-            float x[VEC], q[VEC];
-            if (i + VEC <= end) {
-                const Words w = *(const Words*)(row + i);
-                Shares s;
-                if (draft) s = *(const Shares*)(draft + i);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    x[e] = to_f32(w.v[e]);
-                    q[e] = draft ? to_f32(s.v[e]) : 0.0f;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    x[e] = i + e < end ? to_f32(row[i + e]) : -INFINITY;
-                    q[e] = draft && i + e < end ? to_f32(draft[i + e]) : 0.0f;
-                }
-            }
-            uint64_t left[VEC];
+    int vocab;
+    // The thread's words of a round, as integers of 2^-51.
+    __device__ __forceinline__ void of_round(const Target& target, int round, uint64_t (&left)[VEC]) const {
+        const int i = round * ROUND + (int)threadIdx.x * VEC;
+        float x[VEC], q[VEC];
+        if (i + VEC <= vocab) {
+            const Words w = *(const Words*)(row + i);
+            Shares s;
+            if (draft) s = *(const Shares*)(draft + i);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const double p = target.share(x[e], i + e) - (double)q[e];
-                left[e] = p > 0.0 && i + e != certain ? (uint64_t)fma(p, LEFT_ONE, 0.5) : 0;
+                x[e] = to_f32(w.v[e]);
+                q[e] = draft ? to_f32(s.v[e]) : 0.0f;
             }
-            if (!f(i, left)) return;
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                x[e] = i + e < vocab ? to_f32(row[i + e]) : -INFINITY;
+                q[e] = draft && i + e < vocab ? to_f32(draft[i + e]) : 0.0f;
+            }
+        }
+        bool in[VEC], any = false;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            left[e] = 0;
+            in[e] = target.in(x[e], i + e) && i + e != certain;
+            any = any || in[e];
+        }
+        if (!__ballot(any)) return;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const double p = target.share(x[e]) - (double)q[e];
+            // (from 2^52 on a number's last place is one)
+            const uint64_t whole = (uint64_t)__double_as_longlong(fma(p, 2251799813685248.0, 4503599627370496.0)) - 0x4330000000000000ull;
+            left[e] = in[e] && p > 0.0 ? whole : 0;
         }
     }
 };
 
-// Sum over the workgroup; meet[..][which] is free again past the barrier after next.
-static __device__ __forceinline__ uint64_t sum_of_all(uint64_t mine, uint64_t (*meet)[2], int which) {
-    for (int o = 32; o; o >>= 1) mine += __shfl_xor((unsigned long long)mine, o);
-    if ((threadIdx.x & 63) == 0) meet[threadIdx.x >> 6][which] = mine;
-    __syncthreads();
-    uint64_t all = 0;
-    for (int w = 0; w < SAMPLE_WAVES; ++w) all += meet[w][which];
-    return all;
-}
-
 template <typename T, typename Q>
 __global__ __launch_bounds__(SAMPLE_WG) void verify_judge_kernel(Verify v) {
+    using L = Left<T, Q>;
     __shared__ uint64_t meet[SAMPLE_WAVES][2];
-    __shared__ int found;
+    __shared__ uint64_t sums[SAMPLE_WG], wanted;
+    __shared__ int found, round_found;
     const Sampling& a = v.s;
     const int seq = blockIdx.y, c = blockIdx.x, t = threadIdx.x, lane = t & 63;
     const int first = min(max(v.starts[seq], 0), v.rows), end = min(max(v.starts[seq + 1], 0), v.rows), drafts = end - first - 1;
@@ -130,7 +239,8 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_judge_kernel(Verify v) {
         if (word < 0 || word >= a.vocab) return 0.0;
         Target target;
         target.init(a, v.kept[row], row);
-        return target.share(to_f32(((const T*)a.logits)[row * a.stride + word]), word);
+        const float x = to_f32(((const T*)a.logits)[row * a.stride + word]);
+        return target.in(x, word) ? target.share(x) : 0.0;
     };
     // The drafts that are accepted: a lane each, each wave for itself.
     int accepted = drafts;
@@ -149,68 +259,69 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_judge_kernel(Verify v) {
     const bool some = accepted < drafts;
     Target target;
     target.init(a, v.kept[row], row);
-    Left<T, Q> words{(const T*)a.logits + row * a.stride, some && v.draft ? (const Q*)v.draft + row * v.draft_stride : nullptr, some && !v.draft ? v.drafted[row] : -1};
-    uint64_t mine = 0;
-    auto add = [&](int, const auto& left) {
-        for (uint64_t l : left) mine += l;
-        return true;
+    L words{(const T*)a.logits + row * a.stride, some && v.draft ? (const Q*)v.draft + row * v.draft_stride : nullptr, some && !v.draft ? v.drafted[row] : -1, a.vocab};
+    // The sums of rounds r0 .. r1 - 1, at `to`; the workgroup's rounds go through LDS.
+    auto sum_rounds = [&](int r0, int r1, uint64_t* to) {
+        sums[t] = 0;
+        __syncthreads();
+        for (int r = r0; r < r1; ++r) {
+            uint64_t left[L::VEC], mine = 0;
+            words.of_round(target, r, left);
+            for (uint64_t l : left) mine += l;
+            for (int o = 32; o; o >>= 1) mine += __shfl_xor((unsigned long long)mine, o);
+            if (lane == 0 && mine) atomicAdd((unsigned long long*)&sums[r - r0], (unsigned long long)mine);
+        }
+        __syncthreads();
+        for (int r = r0 + t; r < r1; r += SAMPLE_WG) __hip_atomic_store(&to[r], sums[r - r0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     };
-    int begin = c * a.chunk, stop = min((c + 1) * a.chunk, a.vocab);
-    words.each_round(target, begin, stop, add);
-    const uint64_t here = sum_of_all(mine, meet, 0);
-    uint64_t* sums = v.left + (int64_t)first * a.chunks;
-    if (t == 0) __hip_atomic_store(&sums[c], here, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // as in sampling: once the store has gone where every XCD reads, the workgroup is counted, and the last one goes on
+    uint64_t* left = v.left + (int64_t)first * v.rounds;
+    sum_rounds(c * v.per_piece, min((c + 1) * v.per_piece, v.rounds), left);
+    // as in sampling: once each wave's stores have gone where every XCD reads, the workgroup is counted, and the last one goes on
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (t == 0) found = atomicAdd(&v.met[first], 1u) == (uint32_t)a.chunks - 1;
+    if (t == 0) found = atomicAdd(&v.met[first], 1u) == gridDim.x - 1;
     __syncthreads();
     if (!found) return;
 
-    uint64_t total = 0;
-    for (int p = 0; p < a.chunks; ++p) total += __hip_atomic_load(&sums[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    uint64_t before = 0, wanted;   // what lies in front of `begin`, and the sum that is looked for
-    if (total == 0) {   // nothing is left: p as it is, all of it by this workgroup
+    // The round in which the draw lies: a round a thread.
+    auto find_round = [&]() {
+        const uint64_t mine = t < v.rounds ? __hip_atomic_load(&left[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        const uint64_t before = sum_before(mine, meet, 0);
+        uint64_t total = 0;
+        for (int w = 0; w < SAMPLE_WAVES; ++w) total += meet[w][0];
+        const uint64_t target_sum = drawn_sum(v.draw[seq], total);
+        if (total && before < target_sum && before + mine >= target_sum) {   // one thread's
+            round_found = t;
+            wanted = target_sum - before;
+        }
+        return total;
+    };
+    if (t == 0) found = -1;
+    uint64_t total = find_round();
+    if (total == 0 && target.kept.best != 0) {   // nothing is left: p as it is, all of it by this workgroup
         words.draft = nullptr;
         words.certain = -1;
-        mine = 0;
-        words.each_round(target, 0, a.vocab, add);
-        total = sum_of_all(mine, meet, 1);
-        wanted = drawn_sum(v.draw[seq], total);
-        begin = 0;
-        stop = a.vocab;
-    } else {
-        wanted = drawn_sum(v.draw[seq], total);
-        int p = 0;
-        for (;; ++p) {
-            const uint64_t of_piece = __hip_atomic_load(&sums[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (before + of_piece >= wanted || p == a.chunks - 1) break;
-            before += of_piece;
-        }
-        begin = p * a.chunk;
-        stop = min((p + 1) * a.chunk, a.vocab);
+        __syncthreads();
+        sum_rounds(0, v.rounds, left);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        total = find_round();
     }
     __syncthreads();
-    if (t == 0) found = -1;
     if (total) {
-        int which = 0;
-        words.each_round(target, begin, stop, [&](int i, const auto& left) {
-            uint64_t held = 0;
-            for (uint64_t l : left) held += l;
-            uint64_t at = before + sum_before(held, meet, which);
-            if (at < wanted && at + held >= wanted) {   // one thread's
-                int e = 0;
-                for (uint64_t l : left) {
-                    at += l;
-                    if (at >= wanted) break;
-                    ++e;
-                }
-                found = i + e;
+        uint64_t of_words[L::VEC], held = 0;
+        words.of_round(target, round_found, of_words);
+        for (uint64_t l : of_words) held += l;
+        uint64_t at = sum_before(held, meet, 1);
+        if (at < wanted && at + held >= wanted) {   // one thread's
+            int e = 0;
+            for (uint64_t l : of_words) {
+                at += l;
+                if (at >= wanted) break;
+                ++e;
             }
-            for (int w = 0; w < SAMPLE_WAVES; ++w) before += meet[w][which];
-            which ^= 1;
-            return before < wanted;
-        });
+            found = round_found * L::ROUND + t * L::VEC + e;
+        }
     }
     __syncthreads();
     const int token = found;
@@ -218,16 +329,17 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_judge_kernel(Verify v) {
         const bool last = j == accepted;
         if (last && token < 0) break;   // a row without words
         v.tokens[first + j] = last ? token : v.drafted[first + j];
-        if (v.probs) v.probs[first + j] = (float)(last ? target.share(to_f32(words.row[token]), token) : share_of_draft(first + j));
+        if (v.probs) v.probs[first + j] = (float)(last ? target.share(to_f32(words.row[token])) : share_of_draft(first + j));
     }
     if (t == 0) v.accepted[seq] = accepted;
 }
 
 template <typename T>
-static void launch(const Verify& v, Kept* kept, int draft_type, hipStream_t s) {
-    const dim3 of_rows(v.s.chunks, v.rows), of_seqs(v.s.chunks, v.seqs), threads(SAMPLE_WG);
-    hipLaunchKernelGGL((sample_peak_kernel<T>), of_rows, threads, 0, s, v.s);
-    hipLaunchKernelGGL((sample_steps_kernel<T>), of_rows, threads, 0, s, v.s);
+static void launch(const Verify& v, Kept* kept, bool wide, int draft_type, hipStream_t s) {
+    const dim3 of_pieces(v.s.pieces, v.rows), of_rows(v.s.chunks, v.rows), of_seqs((v.rounds + v.per_piece - 1) / v.per_piece, v.seqs), threads(SAMPLE_WG);
+    if (wide) hipLaunchKernelGGL((verify_pieces_kernel<16, T>), of_pieces, threads, 0, s, v);
+    else hipLaunchKernelGGL((verify_pieces_kernel<8, T>), of_pieces, threads, 0, s, v);
+    if (v.s.top_k || v.s.top_p || v.s.min_p) hipLaunchKernelGGL((verify_steps_kernel<T>), of_rows, threads, 0, s, v.s);
     hipLaunchKernelGGL((verify_kept_kernel<T>), of_rows, threads, 0, s, v, kept);
     if (draft_type == LK_TYPE_F16) hipLaunchKernelGGL((verify_judge_kernel<T, __half>), of_seqs, threads, 0, s, v);
     else if (draft_type == LK_TYPE_BF16) hipLaunchKernelGGL((verify_judge_kernel<T, __hip_bfloat16>), of_seqs, threads, 0, s, v);
@@ -250,15 +362,25 @@ extern "C" int lk_verify(const void* logits, int type, int64_t stride, int rows,
         ((uintptr_t)draft & (draft_size - 1)))
         return LK_ERR_ARG;
     Verify v{};
-    v.s = Sampling{logits, stride, vocab, 0, 0, nullptr, temperature, top_p, min_p, top_k, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+    v.s = Sampling{logits, stride, vocab, 0, 0, 0, nullptr, temperature, top_p, min_p, top_k, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     cut_rows(v.s, rows, size);
-    const size_t judged = sizeof(Kept) + (size_t)v.s.chunks * 8;
+    // pieces of the first pass: 16 words a thread, 8 where that leaves CUs without two workgroups
+    const int cus = lk_device().cus, most = SAMPLE_WG * 16;
+    const bool wide = (int64_t)rows * ((vocab + most - 1) / most) >= 2 * cus;
+    const int words = wide ? most : most / 2;
+    v.s.pieces = (vocab + words - 1) / words;
+    // rounds of the last one, as many to a workgroup as leave two workgroups to a CU
+    const int round = SAMPLE_WG * 16 / size, of_seq = (2 * cus + seqs - 1) / seqs;
+    v.rounds = (vocab + round - 1) / round;
+    v.per_piece = (v.rounds + of_seq - 1) / of_seq;
+    const size_t judged = sizeof(Kept) + (size_t)(v.s.pieces + v.rounds) * 8;
     LkScratch scratch((hipStream_t)stream);
     uint8_t* mem = (uint8_t*)scratch.get(LK_SCRATCH_SAMPLE, (size_t)rows * (judged + bytes_of_row(v.s) + 4));
     if (!mem) return LK_ERR_NOMEM;
     Kept* kept = (Kept*)mem;
     v.kept = kept;
-    v.left = (uint64_t*)(kept + rows);
+    v.sums = (uint64_t*)(kept + rows);
+    v.left = v.sums + (size_t)rows * v.s.pieces;
     place_rows(v.s, rows, mem + (size_t)rows * judged);
     v.met = v.s.arrived + rows;
     v.drafted = drafted;
@@ -272,8 +394,8 @@ extern "C" int lk_verify(const void* logits, int type, int64_t stride, int rows,
     v.tokens = tokens;
     v.accepted = accepted;
     v.probs = probs;
-    if (type == LK_TYPE_F32) launch<float>(v, kept, draft_type, (hipStream_t)stream);
-    else if (type == LK_TYPE_F16) launch<__half>(v, kept, draft_type, (hipStream_t)stream);
-    else launch<__hip_bfloat16>(v, kept, draft_type, (hipStream_t)stream);
+    if (type == LK_TYPE_F32) launch<float>(v, kept, wide, draft_type, (hipStream_t)stream);
+    else if (type == LK_TYPE_F16) launch<__half>(v, kept, wide, draft_type, (hipStream_t)stream);
+    else launch<__hip_bfloat16>(v, kept, wide, draft_type, (hipStream_t)stream);
     return lk_launch_status();
 }
