@@ -57,7 +57,7 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_steps_kernel(Sampling a) 
 template <typename T>
 __global__ __launch_bounds__(SAMPLE_WG, 4) void sample_choose_kernel(Sampling a) {
     __shared__ Shared sh;
-    choose<false, T>(a, sh, nullptr);
+    choose<false, T>(a, sh, [](const Kept&) {});
 }
 
 template <typename T>

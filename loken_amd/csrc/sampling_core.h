@@ -575,8 +575,8 @@ static __device__ __forceinline__ void steps_of_row(const Sampling& a, uint64_t 
 }
 
 // The choice by one workgroup alone, from the row itself: where the steps in question hold more words than are sorted at once.
-template <bool KEPT, typename T>
-static __device__ __forceinline__ void choose_alone(const Sampling& a, int row, const Scale& sc, Shared& sh, Kept* kept_out, uint64_t best) {
+template <bool KEPT, typename T, class F>
+static __device__ __forceinline__ void choose_alone(const Sampling& a, int row, const Scale& sc, Shared& sh, uint64_t best, F done) {
     const int t = threadIdx.x;
     const T* x = (const T*)a.logits + row * a.stride;
     __syncthreads();
@@ -614,29 +614,50 @@ static __device__ __forceinline__ void choose_alone(const Sampling& a, int row, 
             if (a.probs) a.probs[row] = (float)((double)p.weight / (double)kept);
         }
     }
-    if (KEPT && t == 0) *kept_out = Kept{best, last, min(kept, kept_m)};
+    if (KEPT && t == 0) done(Kept{best, last, min(kept, kept_m)});
 }
 
-// The row's choice; with KEPT what it would be made from, into kept_out[row].
-template <bool KEPT, typename T>
-static __device__ __forceinline__ void choose(const Sampling& a, Shared& sh, Kept* kept_out) {
+// The top 16 bits of the k-th largest of n keys, the rest zeros: found by each wave, bit by bit.
+constexpr int MOST_TOPS = 1024;
+static __device__ __forceinline__ uint32_t bound_of(const uint32_t* keys, int n, int k) {
+    constexpr int PER = MOST_TOPS / 64;
+    const int lane = threadIdx.x & 63;
+    uint32_t mine[PER], bound = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine[i] = i * 64 + lane < n ? keys[i * 64 + lane] : 0;
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t more = bound | 1u << bit;
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (i * 64 < n) reach += __popcll(__ballot(mine[i] >= more));
+        bound = reach >= k ? more : bound;
+    }
+    return bound;
+}
+
+// The row's choice; with KEPT what it would be made from, which one thread hands to `done`. `tops`: keys of the largest words of so many parts of the row
+// (null: none are known): top_k words are then at or above the k-th largest of them, and no histogram is needed to find them.
+template <bool KEPT, typename T, class F>
+static __device__ __forceinline__ void choose(const Sampling& a, Shared& sh, F done, const uint32_t* tops = nullptr, int n_tops = 0) {
     const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     const T* x = (const T*)a.logits + row * a.stride;
     // everything that is read of the row's other launches, at once
     uint64_t mass[PER];
     uint32_t count[PER];
+    if (!KEPT || !tops)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        mass[i] = a.mass[(int64_t)row * BINS + t * PER + i];
-        count[i] = a.count[(int64_t)row * BINS + t * PER + i];
-    }
+        for (int i = 0; i < PER; ++i) {
+            mass[i] = a.mass[(int64_t)row * BINS + t * PER + i];
+            count[i] = a.count[(int64_t)row * BINS + t * PER + i];
+        }
     const uint64_t floor_mass = a.floor_mass[row];
     const Peak peak = peak_of_row(a, row);
     Scale sc;
     if (!sc.init(peak, a.temperature[row], a.min_p ? a.min_p[row] : 0.0f)) {   // no words, or the first of them
         if (c == 0 && t == 0) {
             if (KEPT) {
-                kept_out[row] = Kept{peak.best, 0, 0};
+                done(Kept{peak.best, 0, 0});
             } else {
                 a.tokens[row] = peak.best ? (int)~(uint32_t)peak.best : -1;
                 if (a.probs) a.probs[row] = peak.best ? 1.0f : 0.0f;
@@ -645,24 +666,27 @@ static __device__ __forceinline__ void choose(const Sampling& a, Shared& sh, Kep
         return;
     }
     if (sc.infinite) {   // words beside infinite ones are none: as rare as it is, not worth asking for in the pieces
-        if (c == 0) choose_alone<KEPT, T>(a, row, sc, sh, kept_out + row, peak.best);
+        if (c == 0) choose_alone<KEPT, T>(a, row, sc, sh, peak.best, done);
         return;
     }
     const Wants wants(a, row);
-    scan_held(mass, count, sh.mass, sh.count, sh.meet);   // (what is not counted or weighed is zeros)
+    if (!KEPT || !tops) scan_held(mass, count, sh.mass, sh.count, sh.meet);   // (what is not counted or weighed is zeros)
     const uint64_t one = 1ull << ONE_BITS, kept_m = wants.above ? max(floor_mass, one) : ~0ull;
     const float top_p = a.top_p ? a.top_p[row] : 1.0f, u = KEPT ? 0.0f : a.uniform[row];
     const int k = wants.count ? a.top_k[row] : 0;
-    const bool cut_k = wants.count && (uint32_t)k < sh.count[BINS - 1];
+    const bool cut_k = KEPT && tops ? true : wants.count && (uint32_t)k < sh.count[BINS - 1];
     if (KEPT && wants.mass && !cut_k && !(top_p < 1.0f)) {   // no last word to look for
-        if (c == 0 && t == 0) kept_out[row] = Kept{peak.best, 0, min(sh.mass[BINS - 1], kept_m)};
+        if (c == 0 && t == 0) done(Kept{peak.best, 0, min(sh.mass[BINS - 1], kept_m)});
         return;
     }
     // The steps that are gathered: up to three ranges, [a0, a1] around the end of the top-k words, [b0, b1] around that of top-p's, which
     // is nearer to the top or touches it, [c0, c1] around the draw, nearer still. A range that touches the next one, where there is one
     // (its end is not below 0), is part of it.
     int a0 = BINS, a1 = -1, b0 = BINS, b1 = -1, c0 = BINS, c1 = -1;
-    if (!wants.mass) {   // the top-k words and the rest of their last step
+    if (KEPT && tops) {   // the top-k words and what the bound lets in beside them
+        a0 = 0;
+        a1 = BINS - 1;
+    } else if (!wants.mass) {   // the top-k words and the rest of their last step
         a0 = 0;
         a1 = first_reaching(sh.count, BINS, k);
     } else {
@@ -724,7 +748,14 @@ static __device__ __forceinline__ void choose(const Sampling& a, Shared& sh, Kep
             }
         });
     };
-    if (nb == 0 && nc == 0) take_words(std::integral_constant<int, 1>{});
+    if (KEPT && tops) {
+        const uint32_t bound = bound_of(tops, n_tops, k);
+        each_word<4>(x, c * a.chunk, min((c + 1) * a.chunk, a.vocab), [&](float v, int i) {
+            if (key_of(v) < bound || !sc.live(sc.top - v)) return;
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < LIST) sh.list[at] = (uint64_t)key_of(v) << 32 | (uint32_t)~i;
+        });
+    } else if (nb == 0 && nc == 0) take_words(std::integral_constant<int, 1>{});
     else take_words(std::integral_constant<int, 3>{});
     __syncthreads();
     int n = sh.n;
@@ -745,7 +776,19 @@ static __device__ __forceinline__ void choose(const Sampling& a, Shared& sh, Kep
         // each wave takes pieces in turn; where a piece's words go is what the pieces before it hold
         const int lane = t & 63, wave = t >> 6;
         uint32_t all = 0;
-        for (int p0 = 0; p0 < a.chunks; p0 += 64) {
+        if (KEPT && tops && a.chunks <= 64) {   // a few words of each piece: eight threads to one, all pieces at once
+            const uint32_t mine = lane < a.chunks ? __hip_atomic_load(&listed[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+            uint32_t up_to = mine;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t v = __shfl_up(up_to, o);
+                if (lane >= o) up_to += v;
+            }
+            const int piece = t >> 3;
+            const uint32_t count = __shfl(mine, piece), to = __shfl(up_to, piece) - count;
+            for (uint32_t i = t & 7; i < min(count, (uint32_t)LIST); i += 8)
+                if (to + i < LIST) sh.list[to + i] = __hip_atomic_load(&list[(int64_t)piece * LIST + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            all = __shfl(up_to, 63);
+        } else for (int p0 = 0; p0 < a.chunks; p0 += 64) {
             const uint32_t mine = p0 + lane < a.chunks ? __hip_atomic_load(&listed[p0 + lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
             uint32_t up_to = mine;
             for (int o = 1; o < 64; o <<= 1) {
@@ -762,7 +805,7 @@ static __device__ __forceinline__ void choose(const Sampling& a, Shared& sh, Kep
         n = (int)all;
     }
     if (n > LIST || n == 0) {
-        choose_alone<KEPT, T>(a, row, sc, sh, kept_out + row, peak.best);
+        choose_alone<KEPT, T>(a, row, sc, sh, peak.best, done);
         return;
     }
     __syncthreads();
@@ -801,7 +844,7 @@ static __device__ __forceinline__ void choose(const Sampling& a, Shared& sh, Kep
     }
     kept = min(kept, above);
     if (KEPT) {
-        if (t == 0) kept_out[row] = Kept{peak.best, last, kept};
+        if (t == 0) done(Kept{peak.best, last, kept});
         return;
     }
     const int at = first_reaching(sh.sums, n, drawn_sum(u, kept));

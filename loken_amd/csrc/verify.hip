@@ -4,9 +4,9 @@
 // sum. Four launches:
 //   pieces  each piece's largest word, and, of rows that no rule cuts, its sum of weights relative to that: one pass over these rows' words.
 //   steps   sampling's histogram, of the other rows alone
-//   kept    where the rules' last word is, as sampling finds it; of rows that nothing cuts the pieces' sums, put to the row's largest word
-//   judge   pieces of the row at which a sequence ends. Every workgroup finds that row itself: drafts a lane each, accepted while u q < p. It sums what is
-//           left, max(p - q, 0) or p, round by round of neighbouring words; the sequence's last workgroup finds the round in which the draw lies and
+//   kept    where the rules' last word is, as sampling finds it; of rows that nothing cuts the pieces' sums, put to the row's largest word. Then the
+//           row's draft is looked at: accepted if u q < p.
+//   judge   pieces of the row at which a sequence ends, which every workgroup finds itself. It sums what is left, max(p - q, 0) or p, round by round of neighbouring words; the sequence's last workgroup finds the round in which the draw lies and
 //           goes through that again.
 // Differences p - q are made in 64 bits and summed as integers of 2^-51, whose sums do not depend on an order.
 //
@@ -18,7 +18,8 @@ namespace {
 
 struct Verify {
     Sampling s;
-    const Kept* kept;        // [rows]
+    Kept* kept;              // [rows]
+    double* verdict;         // [rows]: p of the word that was drafted where it is accepted; -1: it is not
     const int32_t *drafted, *starts;
     int seqs, rows;
     const void* draft;
@@ -27,10 +28,33 @@ struct Verify {
     int32_t *tokens, *accepted;
     float* probs;
     uint64_t* sums;          // [rows][s.pieces]: weights of the pieces of rows that nothing cuts
+    uint32_t* tops;          // [rows][s.pieces][waves]: keys of the largest words, of rows of which a few are asked for
     int rounds, per_piece;   // rounds of a row as `judge` goes through it, and those of one of its workgroups
     uint64_t* left;          // [rows][rounds]: sums of the rounds, of a sequence's at its first row
     uint32_t* met;           // [rows]: pieces that have been summed
 };
+
+// Sum and maximum over the wave without the LDS crossbar, whose six exchanges in a row take longer than a round's weights.
+template <int ctrl>
+static __device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+    return (uint64_t)(uint32_t)dpp_i32<ctrl>((int)(v >> 32)) << 32 | (uint32_t)dpp_i32<ctrl>((int)v);
+}
+static __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
+    v += dpp_u64<0xB1>(v);
+    v += dpp_u64<0x4E>(v);
+    v += dpp_u64<0x141>(v);
+    v += dpp_u64<0x140>(v);
+    uint64_t sum = 0;
+#pragma unroll
+    for (int l = 0; l < 64; l += 16)
+        sum += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+    return sum;
+}
+static __device__ __forceinline__ float wave_max(float v) {   // (of no numbers: -infinity)
+    v = group_max32(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 // Whether a row is sampled from all of its words.
 static __device__ __forceinline__ bool uncut(const Sampling& a, int row) {
@@ -38,13 +62,20 @@ static __device__ __forceinline__ bool uncut(const Sampling& a, int row) {
     return a.temperature[row] > 0.0f && !(k > 0 && k < a.vocab) && !(a.top_p && a.top_p[row] < 1.0f) && !(a.min_p && a.min_p[row] > 0.0f);
 }
 
+// Whether a row's top-k words are few beside the waves of the pieces: then those are found by the waves' largest words, without a histogram.
+static __device__ __forceinline__ bool bounded(const Sampling& a, int row) {
+    const int k = a.top_k ? a.top_k[row] : 0, tops = a.pieces * SAMPLE_WAVES;
+    return a.temperature[row] > 0.0f && k > 0 && k < a.vocab && k <= tops / 2 && tops <= MOST_TOPS;
+}
+
 // WORDS a thread.
 template <int WORDS, typename T>
 __global__ __launch_bounds__(SAMPLE_WG) void verify_pieces_kernel(Verify v) {
     constexpr int VEC = 16 / sizeof(T), RUNS = WORDS / VEC;
     struct __attribute__((aligned(sizeof(T)))) Run { T v[VEC]; };
-    __shared__ Peak meet[SAMPLE_WAVES];
-    __shared__ uint64_t meet_sums[SAMPLE_WAVES];
+    __shared__ float most[SAMPLE_WAVES], least[SAMPLE_WAVES];
+    __shared__ uint64_t sums[SAMPLE_WAVES];
+    __shared__ int first;
     const Sampling& a = v.s;
     const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x, wave = t >> 6;
     const T* words = (const T*)a.logits + row * a.stride;
@@ -69,51 +100,55 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_pieces_kernel(Verify v) {
         v.tokens[row] = -1;
         if (v.probs) v.probs[row] = 0.0f;
     }
-    const bool weigh = uncut(a, row);
-    if (!weigh)
+    const bool weigh = uncut(a, row), few = bounded(a, row);
+    if (!weigh && !few)
         for (int i = c * SAMPLE_WG + t; i < BINS; i += a.pieces * SAMPLE_WG) {
             a.mass[(int64_t)row * BINS + i] = 0;
             a.count[(int64_t)row * BINS + i] = 0;
         }
-    float best = -INFINITY, lowest = INFINITY;
-    int at = 0;
+    float top = -INFINITY, bottom = -INFINITY;   // (bottom: of what is turned round)
 #pragma unroll
-    for (int j = 0; j < WORDS; ++j) {   // a thread meets the words in rising order
-        const bool more = x[j] > best;
-        best = more ? x[j] : best;
-        at = more ? j : at;
-        lowest = x[j] > -INFINITY ? fminf(lowest, x[j]) : lowest;   // (fminf passes over what is not a number)
+    for (int j = 0; j < WORDS; ++j) top = fmaxf(top, x[j]);   // (fmaxf passes over what is not a number)
+    if (!weigh) {
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) bottom = fmaxf(bottom, x[j] > -INFINITY ? -x[j] : -INFINITY);
+        bottom = wave_max(bottom);
     }
-    at = begin + at / VEC * (SAMPLE_WG * VEC) + at % VEC;
-    Peak p{best > -INFINITY ? (uint64_t)key_of(best) << 32 | (uint32_t)~at : 0, key_of(lowest), 0};
-    wave_peak(p);
-    if ((t & 63) == 0) meet[wave] = p;
+    top = wave_max(top);
+    if ((t & 63) == 0) {
+        most[wave] = top;
+        least[wave] = bottom;
+        if (few) v.tops[((int64_t)row * a.pieces + c) * SAMPLE_WAVES + wave] = top > -INFINITY ? key_of(top) : 0;
+    }
+    if (t == 0) first = 0x7FFFFFFF;
     __syncthreads();
-    p = meet[0];
 #pragma unroll
-    for (int w = 1; w < SAMPLE_WAVES; ++w) {
-        const Peak o = meet[w];
-        p.best = o.best > p.best ? o.best : p.best;
-        p.lowest = o.lowest < p.lowest ? o.lowest : p.lowest;
+    for (int w = 0; w < SAMPLE_WAVES; ++w) {
+        top = fmaxf(top, most[w]);
+        bottom = fmaxf(bottom, least[w]);
     }
-    if (t == 0) a.peaks[(int64_t)row * a.pieces + c] = p;
-    if (!weigh) return;
+    // the first of the largest words
+    int at = WORDS;
+#pragma unroll
+    for (int j = WORDS - 1; j >= 0; --j) at = x[j] == top ? j : at;
+    if (at < WORDS && top > -INFINITY) atomicMin(&first, begin + at / VEC * (SAMPLE_WG * VEC) + at % VEC);
     uint64_t sum = 0;
     Scale sc;
-    if (sc.init(p, a.temperature[row], 0.0f)) {
-#pragma unroll
+    if (weigh && sc.init(Peak{(uint64_t)key_of(top) << 32 | 1, key_of(0.0f), 0}, top > -INFINITY ? a.temperature[row] : 0.0f, 0.0f)) {
+#pragma unroll 4
         for (int j = 0; j < WORDS; ++j) {
             const uint64_t w = weight_of(sc.from_top(x[j]), sc.rate);
             sum += sc.live(sc.below(x[j])) ? w : 0;
         }
+        sum = wave_sum_u64(sum);
     }
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor((unsigned long long)sum, o);
-    if ((t & 63) == 0) meet_sums[wave] = sum;
+    if ((t & 63) == 0) sums[wave] = sum;
     __syncthreads();
     if (t == 0) {
         sum = 0;
-        for (int w = 0; w < SAMPLE_WAVES; ++w) sum += meet_sums[w];
-        v.sums[(int64_t)row * a.pieces + c] = sum;
+        for (int w = 0; w < SAMPLE_WAVES; ++w) sum += sums[w];
+        if (weigh) v.sums[(int64_t)row * a.pieces + c] = sum;
+        a.peaks[(int64_t)row * a.pieces + c] = Peak{top > -INFINITY ? (uint64_t)key_of(top) << 32 | (uint32_t)~first : 0, key_of(-bottom), 0};
     }
 }
 
@@ -121,32 +156,7 @@ template <typename T>
 __global__ __launch_bounds__(SAMPLE_WG, 4) void verify_steps_kernel(Sampling a) {
     __shared__ uint64_t mass[BINS];
     __shared__ uint32_t count[BINS];
-    if (!uncut(a, blockIdx.y)) steps_of_row<T>(a, mass, count);
-}
-
-// Where a row is asked for its distribution alone.
-template <typename T>
-__global__ __launch_bounds__(SAMPLE_WG, 4) void verify_kept_kernel(Verify v, Kept* kept) {
-    __shared__ Shared sh;
-    const int row = blockIdx.y;
-    const Sampling& a = v.s;
-    if (!uncut(a, row)) {
-        choose<true, T>(a, sh, kept);
-        return;
-    }
-    if (blockIdx.x || threadIdx.x >= 64) return;
-    const Peak peak = peak_of_row(a, row);
-    Scale sc;
-    double sum = 0.0;
-    if (sc.init(peak, a.temperature[row], 0.0f)) {
-        for (int i = threadIdx.x; i < a.pieces; i += 64) {   // each lane's in the same order always
-            const uint64_t of_piece = a.peaks[(int64_t)row * a.pieces + i].best;
-            const float top = value_of((uint32_t)(of_piece >> 32));
-            if (of_piece && sc.live(sc.below(top))) sum += (double)v.sums[(int64_t)row * a.pieces + i] * power_of(sc.from_top(top), sc.rate);
-        }
-    }
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    if (threadIdx.x == 0) kept[row] = Kept{peak.best, 0, (uint64_t)(sum + 0.5)};
+    if (!uncut(a, blockIdx.y) && !bounded(a, blockIdx.y)) steps_of_row<T>(a, mass, count);
 }
 
 // A row's distribution.
@@ -172,6 +182,44 @@ struct Target {
     __device__ __forceinline__ double share(float v) const { return kept.kept == 0 ? 1.0 : ((power_of(sc.from_top(v), sc.rate) + 1024.0) - 1024.0) * by; }
 };
 
+// A row's distribution, and the word that was drafted behind it: how far it is accepted.
+template <typename T, typename Q>
+__global__ __launch_bounds__(SAMPLE_WG, 4) void verify_kept_kernel(Verify v) {
+    __shared__ Shared sh;
+    const int row = blockIdx.y;
+    const Sampling& a = v.s;
+    const bool whole = uncut(a, row);
+    if (whole && (blockIdx.x || threadIdx.x >= 64)) return;
+    const int word = v.drafted[row];
+    const bool is_word = word >= 0 && word < a.vocab;
+    const float x = is_word ? to_f32(((const T*)a.logits)[row * a.stride + word]) : -INFINITY;
+    const double reach = v.draft ? (is_word ? (double)v.uniform[row] * (double)to_f32(((const Q*)v.draft)[row * v.draft_stride + word]) : 0.0) : (double)v.uniform[row];
+    auto done = [&](const Kept& k) {
+        v.kept[row] = k;
+        Target target;
+        target.init(a, k, row);
+        const double p = is_word && target.in(x, word) ? target.share(x) : 0.0;
+        v.verdict[row] = reach < p ? p : -1.0;
+    };
+    if (!whole) {
+        const int tops = a.pieces * SAMPLE_WAVES;
+        choose<true, T>(a, sh, done, bounded(a, row) ? v.tops + (int64_t)row * tops : nullptr, tops);
+        return;
+    }
+    const Peak peak = peak_of_row(a, row);
+    Scale sc;
+    double sum = 0.0;
+    if (sc.init(peak, a.temperature[row], 0.0f)) {
+        for (int i = threadIdx.x; i < a.pieces; i += 64) {   // each lane's in the same order always
+            const uint64_t of_piece = a.peaks[(int64_t)row * a.pieces + i].best;
+            const float top = value_of((uint32_t)(of_piece >> 32));
+            if (of_piece && sc.live(sc.below(top))) sum += (double)v.sums[(int64_t)row * a.pieces + i] * power_of(sc.from_top(top), sc.rate);
+        }
+    }
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (threadIdx.x == 0) done(Kept{peak.best, 0, (uint64_t)(sum + 0.5)});
+}
+
 // What is left of a row's words: p, less the draft's share or without the word that was drafted for certain.
 template <typename T, typename Q>
 struct Left {
@@ -182,10 +230,12 @@ struct Left {
     const Q* draft;    // null: nothing is taken off
     int certain;       // -1: no word
     int vocab;
-    // The thread's words of a round, as integers of 2^-51.
-    __device__ __forceinline__ void of_round(const Target& target, int round, uint64_t (&left)[VEC]) const {
+    struct Read { float x[VEC], q[VEC]; };
+    // The thread's words of a round.
+    __device__ __forceinline__ Read read(int round) const {
         const int i = round * ROUND + (int)threadIdx.x * VEC;
-        float x[VEC], q[VEC];
+        Read r;
+        float (&x)[VEC] = r.x, (&q)[VEC] = r.q;
         if (i + VEC <= vocab) {
             const Words w = *(const Words*)(row + i);
             Shares s;
@@ -202,6 +252,12 @@ struct Left {
                 q[e] = draft && i + e < vocab ? to_f32(draft[i + e]) : 0.0f;
             }
         }
+        return r;
+    }
+    // What is left of them, as integers of 2^-51.
+    __device__ __forceinline__ void of_round(const Target& target, int round, const Read& r, uint64_t (&left)[VEC]) const {
+        const int i = round * ROUND + (int)threadIdx.x * VEC;
+        const float (&x)[VEC] = r.x, (&q)[VEC] = r.q;
         bool in[VEC], any = false;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -233,27 +289,11 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_judge_kernel(Verify v) {
         if (c == 0 && t == 0) v.accepted[seq] = 0;
         return;
     }
-    // p of the word that was drafted behind a row (0: no such word)
-    auto share_of_draft = [&](int row) {
-        const int word = v.drafted[row];
-        if (word < 0 || word >= a.vocab) return 0.0;
-        Target target;
-        target.init(a, v.kept[row], row);
-        const float x = to_f32(((const T*)a.logits)[row * a.stride + word]);
-        return target.in(x, word) ? target.share(x) : 0.0;
-    };
     // The drafts that are accepted: a lane each, each wave for itself.
     int accepted = drafts;
     for (int j0 = 0; j0 < drafts && accepted == drafts; j0 += 64) {
-        bool refused = false;
-        if (j0 + lane < drafts) {
-            const int row = first + j0 + lane;
-            const double p = share_of_draft(row);
-            const double q = p > 0.0 && v.draft ? (double)to_f32(((const Q*)v.draft)[row * v.draft_stride + v.drafted[row]]) : 1.0;
-            refused = !((double)v.uniform[row] * q < p);
-        }
-        const uint64_t all = __ballot(refused);
-        if (all) accepted = j0 + __ffsll((unsigned long long)all) - 1;
+        const uint64_t refused = __ballot(j0 + lane < drafts && v.verdict[first + min(j0 + lane, drafts)] < 0.0);
+        if (refused) accepted = j0 + __ffsll((unsigned long long)refused) - 1;
     }
     const int row = first + accepted;
     const bool some = accepted < drafts;
@@ -264,11 +304,14 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_judge_kernel(Verify v) {
     auto sum_rounds = [&](int r0, int r1, uint64_t* to) {
         sums[t] = 0;
         __syncthreads();
+        auto next = words.read(r0);
         for (int r = r0; r < r1; ++r) {
+            const auto now = next;
+            next = words.read(r + 1 < r1 ? r + 1 : r0);   // (always: what is loaded at times is waited for each time)
             uint64_t left[L::VEC], mine = 0;
-            words.of_round(target, r, left);
+            words.of_round(target, r, now, left);
             for (uint64_t l : left) mine += l;
-            for (int o = 32; o; o >>= 1) mine += __shfl_xor((unsigned long long)mine, o);
+            mine = wave_sum_u64(mine);
             if (lane == 0 && mine) atomicAdd((unsigned long long*)&sums[r - r0], (unsigned long long)mine);
         }
         __syncthreads();
@@ -310,7 +353,7 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_judge_kernel(Verify v) {
     __syncthreads();
     if (total) {
         uint64_t of_words[L::VEC], held = 0;
-        words.of_round(target, round_found, of_words);
+        words.of_round(target, round_found, words.read(round_found), of_words);
         for (uint64_t l : of_words) held += l;
         uint64_t at = sum_before(held, meet, 1);
         if (at < wanted && at + held >= wanted) {   // one thread's
@@ -329,21 +372,25 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_judge_kernel(Verify v) {
         const bool last = j == accepted;
         if (last && token < 0) break;   // a row without words
         v.tokens[first + j] = last ? token : v.drafted[first + j];
-        if (v.probs) v.probs[first + j] = (float)(last ? target.share(to_f32(words.row[token])) : share_of_draft(first + j));
+        if (v.probs) v.probs[first + j] = (float)(last ? target.share(to_f32(words.row[token])) : v.verdict[first + j]);
     }
     if (t == 0) v.accepted[seq] = accepted;
 }
 
-template <typename T>
-static void launch(const Verify& v, Kept* kept, bool wide, int draft_type, hipStream_t s) {
+template <typename T, typename Q>
+static void launch(const Verify& v, bool wide, hipStream_t s) {
     const dim3 of_pieces(v.s.pieces, v.rows), of_rows(v.s.chunks, v.rows), of_seqs((v.rounds + v.per_piece - 1) / v.per_piece, v.seqs), threads(SAMPLE_WG);
     if (wide) hipLaunchKernelGGL((verify_pieces_kernel<16, T>), of_pieces, threads, 0, s, v);
     else hipLaunchKernelGGL((verify_pieces_kernel<8, T>), of_pieces, threads, 0, s, v);
     if (v.s.top_k || v.s.top_p || v.s.min_p) hipLaunchKernelGGL((verify_steps_kernel<T>), of_rows, threads, 0, s, v.s);
-    hipLaunchKernelGGL((verify_kept_kernel<T>), of_rows, threads, 0, s, v, kept);
-    if (draft_type == LK_TYPE_F16) hipLaunchKernelGGL((verify_judge_kernel<T, __half>), of_seqs, threads, 0, s, v);
-    else if (draft_type == LK_TYPE_BF16) hipLaunchKernelGGL((verify_judge_kernel<T, __hip_bfloat16>), of_seqs, threads, 0, s, v);
-    else hipLaunchKernelGGL((verify_judge_kernel<T, float>), of_seqs, threads, 0, s, v);
+    hipLaunchKernelGGL((verify_kept_kernel<T, Q>), of_rows, threads, 0, s, v);
+    hipLaunchKernelGGL((verify_judge_kernel<T, Q>), of_seqs, threads, 0, s, v);
+}
+template <typename T>
+static void launch_draft(const Verify& v, bool wide, int draft_type, hipStream_t s) {
+    if (draft_type == LK_TYPE_F16) launch<T, __half>(v, wide, s);
+    else if (draft_type == LK_TYPE_BF16) launch<T, __hip_bfloat16>(v, wide, s);
+    else launch<T, float>(v, wide, s);
 }
 
 }  // namespace
@@ -369,18 +416,19 @@ extern "C" int lk_verify(const void* logits, int type, int64_t stride, int rows,
     const bool wide = (int64_t)rows * ((vocab + most - 1) / most) >= 2 * cus;
     const int words = wide ? most : most / 2;
     v.s.pieces = (vocab + words - 1) / words;
-    // rounds of the last one, as many to a workgroup as leave two workgroups to a CU
-    const int round = SAMPLE_WG * 16 / size, of_seq = (2 * cus + seqs - 1) / seqs;
+    // rounds of the last one, as many to a workgroup as leave four workgroups to a CU
+    const int round = SAMPLE_WG * 16 / size, of_seq = (4 * cus + seqs - 1) / seqs;
     v.rounds = (vocab + round - 1) / round;
     v.per_piece = (v.rounds + of_seq - 1) / of_seq;
-    const size_t judged = sizeof(Kept) + (size_t)(v.s.pieces + v.rounds) * 8;
+    const size_t judged = sizeof(Kept) + 8 + (size_t)(v.s.pieces * (1 + SAMPLE_WAVES / 2) + v.rounds) * 8;
     LkScratch scratch((hipStream_t)stream);
     uint8_t* mem = (uint8_t*)scratch.get(LK_SCRATCH_SAMPLE, (size_t)rows * (judged + bytes_of_row(v.s) + 4));
     if (!mem) return LK_ERR_NOMEM;
-    Kept* kept = (Kept*)mem;
-    v.kept = kept;
-    v.sums = (uint64_t*)(kept + rows);
+    v.kept = (Kept*)mem;
+    v.verdict = (double*)(v.kept + rows);
+    v.sums = (uint64_t*)(v.verdict + rows);
     v.left = v.sums + (size_t)rows * v.s.pieces;
+    v.tops = (uint32_t*)(v.left + (size_t)rows * v.rounds);
     place_rows(v.s, rows, mem + (size_t)rows * judged);
     v.met = v.s.arrived + rows;
     v.drafted = drafted;
@@ -394,8 +442,8 @@ extern "C" int lk_verify(const void* logits, int type, int64_t stride, int rows,
     v.tokens = tokens;
     v.accepted = accepted;
     v.probs = probs;
-    if (type == LK_TYPE_F32) launch<float>(v, kept, wide, draft_type, (hipStream_t)stream);
-    else if (type == LK_TYPE_F16) launch<__half>(v, kept, wide, draft_type, (hipStream_t)stream);
-    else launch<__hip_bfloat16>(v, kept, wide, draft_type, (hipStream_t)stream);
+    if (type == LK_TYPE_F32) launch_draft<float>(v, wide, draft_type, (hipStream_t)stream);
+    else if (type == LK_TYPE_F16) launch_draft<__half>(v, wide, draft_type, (hipStream_t)stream);
+    else launch_draft<__hip_bfloat16>(v, wide, draft_type, (hipStream_t)stream);
     return lk_launch_status();
 }
