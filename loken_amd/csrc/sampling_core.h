@@ -116,11 +116,7 @@ static __device__ __forceinline__ double fma_by(double a, double b, double c) {
 // 2^x, x = below * rate, -43 <= x <= 0. x = n + r, |r| <= 1/2; 2^r = 1 + r f(r), f the polynomial of degree 8
 // through (2^r - 1) / r at the nine Chebyshev points of [-1/2, 1/2]: off by 2.8e-14. Its terms from r^5 on, which are below 2.4e-6 of
 // the result, are made in 32 bits: off by 2e-13.
-static __device__ __forceinline__ double power_of(double below, double rate) {
-    const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
-    const double y = fma(below, rate, magic);
-    const int n = (int)(uint32_t)__double_as_longlong(y);
-    const double r = fma(below, rate, magic - y);
+static __device__ __forceinline__ double power_at(double r, int n) {
     const float s = (float)r;
     const float high = fmaf(s, fmaf(s, fmaf(s, 1.0203121e-07f, 1.3255225e-06f), 1.5252687e-05f), 0.00015403455f);
     double p = fma_by(r, (double)high, 0.0013333558179043112);
@@ -131,6 +127,11 @@ static __device__ __forceinline__ double power_of(double below, double rate) {
     p = fma(r, p, 1.0);
     // times 2^n in the exponent
     return __longlong_as_double((long long)((uint64_t)__double_as_longlong(p) + ((uint64_t)(uint32_t)(n << 20) << 32)));
+}
+static __device__ __forceinline__ double power_of(double below, double rate) {
+    const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
+    const double y = fma(below, rate, magic);
+    return power_at(fma(below, rate, magic - y), (int)(uint32_t)__double_as_longlong(y));
 }
 // The same as an integer of 2^-42: 1024 more, and the last place is 2^-42: what the sum rounds to is the integer.
 static __device__ __forceinline__ uint64_t weight_of(double below, double rate) {

@@ -27,7 +27,7 @@ struct Verify {
     const float *uniform, *draw;
     int32_t *tokens, *accepted;
     float* probs;
-    uint64_t* sums;          // [rows][s.pieces]: weights of the pieces of rows that nothing cuts
+    double* sums;            // [rows][s.pieces]: weights of the pieces of rows that nothing cuts, relative to a piece's largest word
     uint32_t* tops;          // [rows][s.pieces][waves]: keys of the largest words, of rows of which a few are asked for
     int rounds, per_piece;   // rounds of a row as `judge` goes through it, and those of one of its workgroups
     uint64_t* left;          // [rows][rounds]: sums of the rounds, of a sequence's at its first row
@@ -50,10 +50,31 @@ static __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
         sum += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, l);
     return sum;
 }
+static __device__ __forceinline__ double wave_sum_f64(double v) {
+    auto step = [&](auto ctrl) { return __longlong_as_double((long long)dpp_u64<decltype(ctrl)::value>((uint64_t)__double_as_longlong(v))); };
+    v += step(std::integral_constant<int, 0xB1>{});
+    v += step(std::integral_constant<int, 0x4E>{});
+    v += step(std::integral_constant<int, 0x141>{});
+    v += step(std::integral_constant<int, 0x140>{});
+    double sum = 0.0;
+#pragma unroll
+    for (int l = 0; l < 64; l += 16) {
+        const uint64_t b = (uint64_t)__double_as_longlong(v);
+        sum += __longlong_as_double((long long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)b, l)));
+    }
+    return sum;
+}
 static __device__ __forceinline__ float wave_max(float v) {   // (of no numbers: -infinity)
     v = group_max32(v);
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// 2^x for any x <= 0 (and 0 for what is no number), to 2e-13 of it; nothing is left of it below 2^-900.
+static __device__ __forceinline__ double power_of_any(double below, double rate) {
+    const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the nearest whole number
+    const double x = fmax(below * rate, -900.0), y = x + magic;
+    return power_at(x - (y - magic), (int)(uint32_t)__double_as_longlong(y));
 }
 
 // Whether a row is sampled from all of its words.
@@ -74,7 +95,7 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_pieces_kernel(Verify v) {
     constexpr int VEC = 16 / sizeof(T), RUNS = WORDS / VEC;
     struct __attribute__((aligned(sizeof(T)))) Run { T v[VEC]; };
     __shared__ float most[SAMPLE_WAVES], least[SAMPLE_WAVES];
-    __shared__ uint64_t sums[SAMPLE_WAVES];
+    __shared__ double sums[SAMPLE_WAVES];
     __shared__ int first;
     const Sampling& a = v.s;
     const int row = blockIdx.y, c = blockIdx.x, t = threadIdx.x, wave = t >> 6;
@@ -127,25 +148,24 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_pieces_kernel(Verify v) {
         top = fmaxf(top, most[w]);
         bottom = fmaxf(bottom, least[w]);
     }
-    // the first of the largest words
-    int at = WORDS;
+    if (most[wave] == top && top > -INFINITY) {   // the first of the largest words
+        int at = WORDS;
 #pragma unroll
-    for (int j = WORDS - 1; j >= 0; --j) at = x[j] == top ? j : at;
-    if (at < WORDS && top > -INFINITY) atomicMin(&first, begin + at / VEC * (SAMPLE_WG * VEC) + at % VEC);
-    uint64_t sum = 0;
+        for (int j = WORDS - 1; j >= 0; --j) at = x[j] == top ? j : at;
+        if (at < WORDS) atomicMin(&first, begin + at / VEC * (SAMPLE_WG * VEC) + at % VEC);
+    }
+    // Weights relative to the piece's largest word, summed in an order that is always the same.
+    double sum = 0.0;
     Scale sc;
     if (weigh && sc.init(Peak{(uint64_t)key_of(top) << 32 | 1, key_of(0.0f), 0}, top > -INFINITY ? a.temperature[row] : 0.0f, 0.0f)) {
-#pragma unroll 4
-        for (int j = 0; j < WORDS; ++j) {
-            const uint64_t w = weight_of(sc.from_top(x[j]), sc.rate);
-            sum += sc.live(sc.below(x[j])) ? w : 0;
-        }
-        sum = wave_sum_u64(sum);
+#pragma unroll 8
+        for (int j = 0; j < WORDS; ++j) sum += sc.infinite ? (x[j] == INFINITY ? 1.0 : 0.0) : power_of_any((double)x[j] - (double)top, sc.rate);
+        sum = wave_sum_f64(sum);
     }
     if ((t & 63) == 0) sums[wave] = sum;
     __syncthreads();
     if (t == 0) {
-        sum = 0;
+        sum = 0.0;
         for (int w = 0; w < SAMPLE_WAVES; ++w) sum += sums[w];
         if (weigh) v.sums[(int64_t)row * a.pieces + c] = sum;
         a.peaks[(int64_t)row * a.pieces + c] = Peak{top > -INFINITY ? (uint64_t)key_of(top) << 32 | (uint32_t)~first : 0, key_of(-bottom), 0};
@@ -165,6 +185,7 @@ struct Target {
     Kept kept;
     double by;      // 2^42 / kept weight
     bool floored;   // whether min-p is asked for
+    bool plain;     // whether every word is in it, and the largest is a number
     __device__ __forceinline__ void init(const Sampling& a, const Kept& k, int row) {
         kept = k;
         const Peak peak{k.best, key_of(0.0f), 0};
@@ -172,6 +193,7 @@ struct Target {
         sc.init(peak, kept.kept ? a.temperature[row] : 1.0f, least);
         by = kept.kept ? 4398046511104.0 / (double)kept.kept : 1.0;
         floored = least > 0.0f;
+        plain = kept.kept != 0 && kept.last == 0 && !floored && !sc.infinite;
     }
     __device__ __forceinline__ bool in(float v, int i) const {
         const uint64_t at = (uint64_t)key_of(v) << 32 | (uint32_t)~i;
@@ -213,11 +235,11 @@ __global__ __launch_bounds__(SAMPLE_WG, 4) void verify_kept_kernel(Verify v) {
         for (int i = threadIdx.x; i < a.pieces; i += 64) {   // each lane's in the same order always
             const uint64_t of_piece = a.peaks[(int64_t)row * a.pieces + i].best;
             const float top = value_of((uint32_t)(of_piece >> 32));
-            if (of_piece && sc.live(sc.below(top))) sum += (double)v.sums[(int64_t)row * a.pieces + i] * power_of(sc.from_top(top), sc.rate);
+            if (of_piece && sc.live(sc.below(top))) sum += v.sums[(int64_t)row * a.pieces + i] * power_of(sc.from_top(top), sc.rate);
         }
     }
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    if (threadIdx.x == 0) done(Kept{peak.best, 0, (uint64_t)(sum + 0.5)});
+    if (threadIdx.x == 0) done(Kept{peak.best, 0, (uint64_t)(sum * 4398046511104.0 + 0.5)});
 }
 
 // What is left of a row's words: p, less the draft's share or without the word that was drafted for certain.
@@ -258,21 +280,26 @@ struct Left {
     __device__ __forceinline__ void of_round(const Target& target, int round, const Read& r, uint64_t (&left)[VEC]) const {
         const int i = round * ROUND + (int)threadIdx.x * VEC;
         const float (&x)[VEC] = r.x, (&q)[VEC] = r.q;
-        bool in[VEC], any = false;
+        // (from 2^52 on a number's last place is one)
+        auto whole = [](double p) { return (uint64_t)__double_as_longlong(fma(fmax(p, 0.0), 2251799813685248.0, 4503599627370496.0)) - 0x4330000000000000ull; };
+        if (target.plain) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            left[e] = 0;
-            in[e] = target.in(x[e], i + e) && i + e != certain;
-            any = any || in[e];
-        }
-        if (!__ballot(any)) return;
+            for (int e = 0; e < VEC; ++e) left[e] = whole(fma(power_of_any((double)x[e] - (double)target.sc.top, target.sc.rate), target.by, -(double)q[e]));
+        } else {
+            bool in[VEC], any = false;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const double p = target.share(x[e]) - (double)q[e];
-            // (from 2^52 on a number's last place is one)
-            const uint64_t whole = (uint64_t)__double_as_longlong(fma(p, 2251799813685248.0, 4503599627370496.0)) - 0x4330000000000000ull;
-            left[e] = in[e] && p > 0.0 ? whole : 0;
+            for (int e = 0; e < VEC; ++e) {
+                left[e] = 0;
+                in[e] = target.in(x[e], i + e);
+                any = any || in[e];
+            }
+            if (!__ballot(any)) return;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) left[e] = in[e] ? whole(target.share(x[e]) - (double)q[e]) : 0;
         }
+        if (certain >= i && certain < i + VEC)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) left[e] = i + e == certain ? 0 : left[e];
     }
 };
 
@@ -426,8 +453,8 @@ extern "C" int lk_verify(const void* logits, int type, int64_t stride, int rows,
     if (!mem) return LK_ERR_NOMEM;
     v.kept = (Kept*)mem;
     v.verdict = (double*)(v.kept + rows);
-    v.sums = (uint64_t*)(v.verdict + rows);
-    v.left = v.sums + (size_t)rows * v.s.pieces;
+    v.sums = v.verdict + rows;
+    v.left = (uint64_t*)(v.sums + (size_t)rows * v.s.pieces);
     v.tops = (uint32_t*)(v.left + (size_t)rows * v.rounds);
     place_rows(v.s, rows, mem + (size_t)rows * judged);
     v.met = v.s.arrived + rows;
