@@ -148,7 +148,8 @@ class KvCacheMxfp4:
 
     def _at(self):
         """Where the tensors are now: a program may have given one other memory since."""
-        return tuple(t.data_ptr() for t in self._tensors)
+        k, v, k_powers, v_powers = self._tensors
+        return k.data_ptr(), v.data_ptr(), k_powers.data_ptr(), v_powers.data_ptr()
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page_tokens: int = 16, device="cuda") -> "KvCacheMxfp4":

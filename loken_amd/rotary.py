@@ -29,7 +29,7 @@ class Rotary:
                 raise ValueError("rotary: its tensors are on several devices")
         if not math.isfinite(factor):
             raise ValueError("rotary: the factor is a number")
-        self._tensors, self.neighbours, self.factor = (frequencies, axis), bool(neighbours), float(factor)
+        self._tensors, self.neighbours, self.factor = (frequencies, axis), int(bool(neighbours)), float(factor)
 
     frequencies = property(lambda self: self._tensors[0])
     axis = property(lambda self: self._tensors[1])
@@ -44,32 +44,43 @@ def _arguments(what, q, k, positions, rotary, q_weight, k_weight, eps):
     of_k, kv_heads, ks = _rows(what, "k", k, None, dim)
     if of_k != rows or k.dtype is not q.dtype or heads == 0 or kv_heads == 0:
         raise ValueError(f"{what}: queries and keys are of one type and number of rows")
-    frequencies, axis = rotary.frequencies, rotary.axis
-    if 2 * frequencies.numel() > dim:
+    frequencies, axis = rotary._tensors
+    pairs = frequencies.numel()
+    if 2 * pairs > dim:
         raise ValueError(f"{what}: more pairs than a head has")
-    if positions.dtype is not torch.int32 or positions.dim() not in (1, 2) or positions.shape[-1] != rows:
+    shape = positions.shape
+    axes = 1 if len(shape) == 1 else shape[0] if len(shape) == 2 else 0
+    if positions.dtype is not torch.int32 or axes == 0 or shape[-1] != rows:
         raise ValueError(f"{what}: positions are int32 [rows] or [axes, rows]")
-    axes = positions.shape[0] if positions.dim() == 2 else 1
-    if not 1 <= axes <= MAX_AXES or (rows > 1 and positions.stride(-1) != 1):
-        raise ValueError(f"{what}: positions are int32 [rows] or [axes, rows], an axis together, up to {MAX_AXES} axes")
-    across = positions.stride(0) if axes > 1 else rows
-    if across < rows:
-        raise ValueError(f"{what}: axes of positions overlap")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            _vector(what, name, w, torch.float32, dim)
+    across = rows
+    if not positions.is_contiguous():
+        if rows > 1 and positions.stride(-1) != 1:
+            raise ValueError(f"{what}: an axis of positions stands together")
+        across = positions.stride(0) if axes > 1 else rows
+    if axes > MAX_AXES or across < rows:
+        raise ValueError(f"{what}: up to {MAX_AXES} axes of positions, which do not overlap")
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"{what}: eps is a number from zero on")
-    on = [t for t in (q, k, positions, frequencies, axis, q_weight, k_weight) if t is not None]
-    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    tail = (at(q_weight), at(k_weight), eps, positions.data_ptr(), across, axes, frequencies.data_ptr(), at(axis), frequencies.numel(),
-            int(rotary.neighbours), rotary.factor)
+    on = [q, k, positions, frequencies]
+    qw = kw = of_axis = None
+    if q_weight is not None:
+        _vector(what, "q_weight", q_weight, torch.float32, dim)
+        qw = q_weight.data_ptr()
+        on.append(q_weight)
+    if k_weight is not None:
+        _vector(what, "k_weight", k_weight, torch.float32, dim)
+        kw = k_weight.data_ptr()
+        on.append(k_weight)
+    if axis is not None:
+        of_axis = axis.data_ptr()
+        on.append(axis)
+    tail = (qw, kw, eps, positions.data_ptr(), across, axes, frequencies.data_ptr(), of_axis, pairs, rotary.neighbours, rotary.factor)
     return dim, rows, heads, kv_heads, qs, ks, on, tail
 
 
 def _output(what, name, out, like, rows, heads, dim):
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=like.dtype, device=like.device)
+        return like.new_empty((rows, heads, dim)), heads * dim
     of_out, _, stride = _rows(what, name, out, heads, dim)
     if out.dtype is not like.dtype or of_out != rows:
         raise ValueError(f"{what}: {name} has the type and shape of {name[0]}")

@@ -1,0 +1,148 @@
+"""A served step with drafted tokens over the 4-bit cache, operator after operator as a decode loop uses them between its quantized linears:
+eagerly against the definitions, and recorded."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import mxfp4_reference as ref
+import serving_reference as served
+from loken_amd import kv, lib, ops, rotary, sampling, synth
+from test_gpu_graph_scratch import record
+from test_gpu_kv_attention import i32
+from test_gpu_mxfp4_cache import check_cache, dev
+
+pytestmark = pytest.mark.gpu
+
+HEADS, KV_HEADS, DIM, PAGE, PAGES, VOCAB, SEQS, MOST, DRAFTS, CAP = 4, 2, 64, 16, 60, 1003, 3, 128, 3, 30.0
+HIDDEN = HEADS * DIM
+
+
+def linear(weights, x, ns):
+    """The mat-vec launch takes up to eight rows."""
+    parts = [ops.mmvq_fused(lib.TYPE_Q8_0, weights, x[i:i + 8], ns) for i in range(0, len(x), 8)]
+    return [torch.cat(of_one) for of_one in zip(*parts)]
+
+
+class Loop:
+    """Sequences of a small layer with quantized linears: x -> q, k, v -> norms, rotation, cache -> attention -> logits -> the check of the
+    drafts, whose number of accepted ones says how far each sequence has come."""
+
+    def __init__(self, seed):
+        g = np.random.default_rng(seed)
+        sizes = (HIDDEN, KV_HEADS * DIM, KV_HEADS * DIM, VOCAB)
+        self.weights = [dev(synth.weight(lib.TYPE_Q8_0, n, HIDDEN, seed=seed, stream=i)) for i, n in enumerate(sizes)]
+        self.words = dev(g.normal(size=(VOCAB, HIDDEN)).astype(np.float32))
+        self.cache = kv.KvCacheMxfp4.empty(PAGES, KV_HEADS, DIM, PAGE)
+        self.frequencies = (10000.0 ** (-np.arange(DIM // 2) / (DIM // 2))).astype(np.float32)
+        self.rotary = rotary.Rotary(dev(self.frequencies))
+        self.norm = g.uniform(0.5, 1.5, (2, DIM)).astype(np.float32)
+        self.q_weight, self.k_weight = dev(self.norm[0]), dev(self.norm[1])
+        self.free = g.permutation(PAGES).astype(np.int32)
+        self.free_pages, self.table, self.past, self.taken = i32(self.free), i32(np.full((SEQS, MOST // PAGE), -1)), i32([0] * SEQS), i32([0])
+        self.draws, self.u = g.random((40, SEQS)).astype(np.float32), g.random((40, SEQS * (DRAFTS + 1))).astype(np.float32)
+        self.draw, self.uniform = torch.empty(SEQS, device="cuda"), torch.empty(SEQS * (DRAFTS + 1), device="cuda")
+        rows = SEQS * (DRAFTS + 1)
+        self.rules = [np.full(rows, 0.9, np.float32), np.tile([0, 40, 7, 0], SEQS).astype(np.int32), np.full(rows, 0.95, np.float32)]
+        self.rules_there = [dev(r) for r in self.rules]
+
+    def step(self, x, drafted, share, fresh, plan):
+        kv.kv_plan(self.past, fresh, self.table, self.free_pages, PAGE, plan, self.taken)
+        q, k, v = linear(self.weights[:3], x, [HIDDEN, KV_HEADS * DIM, KV_HEADS * DIM])
+        q, k, v = q.view(-1, HEADS, DIM), k.unflatten(1, (KV_HEADS, DIM)), v.unflatten(1, (KV_HEADS, DIM))
+        turned = rotary.rotate_into(self.cache, q, k, v, plan.positions, plan.slots, self.rotary, q_weight=self.q_weight, k_weight=self.k_weight)
+        out = kv.kv_attention(turned, self.cache, self.table, plan.lens, plan.starts, max_fresh=DRAFTS + 1, max_len=MOST, softcap=CAP)
+        logits = linear(self.weights[3:], out.view(-1, HIDDEN), [VOCAB])[0]
+        tokens, accepted, probs = sampling.verify(logits, drafted, plan.starts, self.uniform, self.draw, *self.rules_there, draft=share)
+        return q, k, v, turned, out, logits, tokens, accepted, probs
+
+    def after(self, plan, accepted):
+        """What was drafted behind the accepted tokens is forgotten: the next step writes over it."""
+        self.past.add_(accepted + 1)
+        self.taken.copy_(plan.taken)
+
+
+def bring_drafts(loop, words, x, drafted, share, fresh, plan):
+    """Drafts from the layer itself, at a higher temperature, one after the other: a step over what is there so far gives the next one's
+    distribution, and the steps after it write over its rows. Its largest word, or in every third sequence another, is drafted."""
+    first = torch.arange(SEQS, device="cuda") * (DRAFTS + 1)
+    drafted.zero_()
+    share.fill_(1.0 / VOCAB)
+    x.copy_(loop.words[words.repeat_interleave(DRAFTS + 1).long()])
+    for j in range(DRAFTS):
+        logits = loop.step(x, drafted, share, fresh, plan)[5][first + j]
+        share[first + j] = torch.softmax(logits / 1.5, -1)
+        word = logits.argmax(-1)
+        word[j % SEQS] = (word[j % SEQS] + 1) % VOCAB
+        drafted[first + j] = word.int()
+        x[first + j + 1] = loop.words[word]
+
+
+def test_a_loop_of_drafted_steps():
+    loop, g = Loop(3), np.random.default_rng(4)
+    want, table = ref.Cache(PAGES, KV_HEADS, PAGE, DIM), np.full((SEQS, MOST // PAGE), -1, np.int32)
+    past, taken, rows = np.zeros(SEQS, np.int32), 0, SEQS * (DRAFTS + 1)
+    words, fresh, some = dev(np.array([5, 77, 900])), i32([DRAFTS + 1] * SEQS), 0
+    x, drafted, share = torch.empty((rows, HIDDEN), device="cuda"), i32([0] * rows), torch.empty((rows, VOCAB), device="cuda")
+    for n in range(12):
+        plan = kv.KvPlan(SEQS, rows)
+        bring_drafts(loop, words, x, drafted, share, fresh, plan)
+        loop.draw.copy_(dev(loop.draws[n]))
+        loop.uniform.copy_(dev(loop.u[n]))
+        q, k, v, turned, out, logits, tokens, accepted, probs = loop.step(x, drafted, share, fresh, plan)
+        table, lens, starts, slots, positions, taken = served.plan(past, [DRAFTS + 1] * SEQS, table, loop.free, PAGE, rows, taken)
+        for got, w in zip((loop.table, plan.lens, plan.starts, plan.slots, plan.positions, plan.taken), (table, lens, starts, slots, positions, [taken])):
+            assert np.array_equal(got.cpu().numpy(), w), n
+        kn, vn = k.double().cpu().numpy(), v.double().cpu().numpy()
+        want.write(ref.rope(kn, positions, loop.frequencies, None, loop.norm[1]), vn, slots)
+        check_cache(loop.cache, want)
+        exact_q = ref.rope(q.double().cpu().numpy(), positions, loop.frequencies, None, loop.norm[0])
+        size = np.sqrt((exact_q ** 2).max(-1, keepdims=True)) * np.sqrt(2)
+        assert (np.abs(turned.double().cpu().numpy() - exact_q) <= 16 * 2.0 ** -24 * size).all(), n      # as for any rows
+        exact, reach, most = ref.attention(turned.cpu().numpy(), want, table, lens, starts, DIM ** -0.5, 0, CAP, np.zeros(out.shape))
+        score = (3 * DIM + 6) * 2.0 ** -24 * reach + CAP * 2.0 ** -22
+        bound = most * (2 * score + 4 * 2.0 ** -22 + 2 * lens.max() * 2.0 ** -24 + 2.0 ** -24)
+        assert (np.abs(out.double().cpu().numpy() - exact) <= bound[..., None] + 2.0 ** -24 * np.abs(exact)).all(), n
+        chosen, how_many, p = ref.verify(logits.double().cpu().numpy(), drafted.cpu().numpy(), starts, loop.u[n], loop.draws[n], *loop.rules,
+                                         draft=share.double().cpu().numpy())
+        assert np.array_equal(tokens.cpu().numpy(), chosen) and np.array_equal(accepted.cpu().numpy(), how_many)
+        assert np.allclose(probs.double().cpu().numpy(), p, rtol=2.0 ** -24 + 1e-9, atol=1e-11)
+        loop.after(plan, accepted)
+        past = past + how_many.astype(np.int32) + 1
+        some += int(how_many.sum())
+        words = dev(chosen[starts[:-1] + how_many])
+    assert past.max() > PAGE and 0 < some < 12 * SEQS * DRAFTS and np.array_equal(loop.past.cpu().numpy(), past)
+
+
+def test_a_recorded_step_is_the_eager_one():
+    """Replays with the loop's own eager work (lengths, the next rows and drafts) and a synchronization between them."""
+    eager, other = Loop(5), Loop(5)
+    rows = SEQS * (DRAFTS + 1)
+    fresh, plans = i32([DRAFTS + 1] * SEQS), [kv.KvPlan(SEQS, rows) for _ in "ab"]
+    x, drafted, share = torch.empty((rows, HIDDEN), device="cuda"), i32([0] * rows), torch.empty((rows, VOCAB), device="cuda")
+    words, first = dev(np.array([5, 77, 900])), torch.arange(SEQS, device="cuda") * (DRAFTS + 1)
+
+    def bring(n):
+        bring_drafts(eager, words, x, drafted, share, fresh, plans[0])
+        for loop in (eager, other):
+            loop.draw.copy_(dev(loop.draws[n]))
+            loop.uniform.copy_(dev(loop.u[n]))
+
+    bring(0)
+    for loop, plan in zip((eager, other), plans):
+        accepted = loop.step(x, drafted, share, fresh, plan)[7]
+        loop.after(plan, accepted)
+    torch.cuda.synchronize()
+    graph, got = record(lambda: other.step(x, drafted, share, fresh, plans[1]), torch.cuda.Stream())
+    for n in range(1, 9):
+        bring(n)
+        want = eager.step(x, drafted, share, fresh, plans[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert torch.equal(a, b), n
+        for a, b in zip((*eager.cache._tensors, eager.table), (*other.cache._tensors, other.table)):
+            assert torch.equal(a, b), n
+        words = want[6][first + want[7]]
+        eager.after(plans[0], want[7])
+        other.after(plans[1], got[7])
