@@ -113,6 +113,12 @@ def parse_args():
     ap.add_argument("--context", type=int, default=0,
                     help="--workload decode-1p7b: every row is a sequence of so many tokens in a paged 8-bit cache, and the step has its "
                          "plan of pages, cache writes, attention and the choice of the next token as well (0: linears only)")
+    ap.add_argument("--kv-cache", default="q8", choices=["q8", "mxfp4"],
+                    help="--workload decode-1p7b with --context: the cache in 8 bits, or in 4 with the head norms and the rotation in the launch that "
+                         "writes it")
+    ap.add_argument("--drafts", type=int, default=0,
+                    help="--workload decode-1p7b with --kv-cache mxfp4: drafted tokens of a sequence, checked at the step's end; the batch's rows are "
+                         "each sequence's drafts and one more")
     ap.add_argument("--launches", type=int, default=200, help="timed launches of the per-launch workloads")
     return ap.parse_args()
 

@@ -12,7 +12,10 @@
   decode-1p7b every quantized linear of a Qwen3-1.7B-shaped decode step at `--batch` rows:
               mat-vec launches at one row, the rows kernels or the tiled matmul above; with
               `--context` also what stands between them: the plan of pages, each layer's cache
-              write and attention over so many tokens a row, and the choice of the next token
+              write and attention over so many tokens a row, and the choice of the next token; with
+              `--kv-cache mxfp4` the head norms and the rotation too, in one launch with the write
+              into a cache of 4 bits, and with `--drafts` a sequence's rows are its drafted tokens
+              and one more, whose check is the step's end
 
 Timing: 20 warm-up launches, then `--launches` (default 200) launches each bracketed by its own
 pair of events on the launch stream; median, p10, p90, min and max are reported (the protocol of
@@ -511,6 +514,71 @@ class Between:
             top_p.data_ptr(), None, self.tokens.data_ptr(), self.probs.data_ptr(), s))
 
 
+class BetweenMxfp4(Between):
+    """The same over a cache in 4 bits, with the head norms and the rotation that stand in front of it. With ``drafts`` a sequence has that many
+    drafted tokens and one more in the batch of ``rows``, and the step ends in their check."""
+
+    def __init__(self, rows, context, heads, kv_heads, mk, drafts=0):
+        fresh = drafts + 1
+        if rows % fresh:
+            raise SystemExit("--drafts: the batch holds whole sequences, of their drafts and one row more")
+        super().__init__(rows // fresh, context + drafts, heads, kv_heads, mk)   # pages for all of them
+        self.rows, self.context, self.drafts = rows, context, drafts
+        self.past.fill_(context)
+        self.fresh.fill_(fresh)
+        held = -(-context // PAGE_TOKENS)
+        self.table[:, held:] = -1
+        self.free = torch.randperm(self.pages, device=mk.dev, generator=mk.gen).to(torch.int32)
+        # (pages of other sequences: what they hold does not matter to a measured step)
+        self.plan = kv.KvPlan(self.seqs, rows, mk.dev)
+        f32 = lambda *shape: torch.rand(shape, device=mk.dev, generator=mk.gen)  # noqa: E731
+        self.norms = [f32(HEAD_DIM) + 0.5 for _ in "qk"]
+        self.frequencies = (1e6 ** (-torch.arange(HEAD_DIM // 2, dtype=torch.float64) / (HEAD_DIM // 2))).float().to(mk.dev)
+        self.turned = torch.empty((rows, heads, HEAD_DIM), device=mk.dev)
+        if drafts:
+            self.rules = [r.repeat_interleave(fresh) for r in self.rules]
+            self.draw, self.accepted = f32(self.seqs), torch.empty(self.seqs, dtype=torch.int32, device=mk.dev)
+            self.tokens, self.probs = torch.empty(rows, dtype=torch.int32, device=mk.dev), torch.empty(rows, device=mk.dev)
+
+    def bytes_read(self):
+        """Codes and powers of the keys and values that a layer's attention reads."""
+        return 2 * self.seqs * (self.context + self.drafts + 1) * self.kv_heads * HEAD_DIM * 17 // 32
+
+    def plan_item(self, s):
+        kind, fn, a = super().plan_item(s)
+        return kind, fn, (*a[:-3], self.rows, *a[-2:])
+
+    def attention_items(self, q, k, v, out, s):
+        L, f32, p, t = lib.load(), lib.TYPE_F32, self.plan, self.table
+        c = kv.KvCacheMxfp4.empty(self.pages, self.kv_heads, HEAD_DIM, PAGE_TOKENS, self.mk.dev)
+        for codes, powers in ((c.k, c.k_powers), (c.v, c.v_powers)):
+            codes.random_(0, 256, generator=self.mk.gen)
+            powers.random_(124, 127, generator=self.mk.gen)
+        self.caches.append(c)
+        q_weight, k_weight = self.norms
+        return [("status", L.lk_qk_norm_rope_kv_mxfp4, (
+                    q.data_ptr(), k.data_ptr(), v.data_ptr(), f32, q.stride(0), k.stride(0), v.stride(0), self.turned.data_ptr(), self.turned.stride(0),
+                    p.slots.data_ptr(), self.rows, self.heads, self.kv_heads, HEAD_DIM, q_weight.data_ptr(), k_weight.data_ptr(), 1e-6,
+                    p.positions.data_ptr(), self.rows, 1, self.frequencies.data_ptr(), None, HEAD_DIM // 2, 0, 1.0, PAGE_TOKENS, self.pages,
+                    *c._at(), s)),
+                ("status", L.lk_kv_attention_mxfp4, (
+                    self.turned.data_ptr(), f32, self.turned.stride(0), out.data_ptr(), out.stride(0), *c._at(), self.pages, PAGE_TOKENS,
+                    t.data_ptr(), t.stride(0), t.shape[1], p.lens.data_ptr(), p.starts.data_ptr(), self.seqs, self.rows, self.drafts + 1,
+                    self.context + self.drafts + 1, self.heads, self.kv_heads, HEAD_DIM, HEAD_DIM ** -0.5, 0, 0.0, s))]
+
+    def sample_item(self, logits, vocab, s):
+        if not self.drafts:
+            return super().sample_item(logits, vocab, s)
+        u, temperature, top_k, top_p = self.rules
+        rows = self.rows
+        self.share = torch.softmax(torch.randn((rows, vocab), device=self.mk.dev, generator=self.mk.gen) * 3.0, -1)
+        self.drafted = torch.multinomial(self.share, 1, generator=self.mk.gen)[:, 0].int()
+        return ("status", lib.load().lk_verify, (
+            logits.data_ptr(), lib.TYPE_F32, logits.stride(0), rows, vocab, self.drafted.data_ptr(), self.plan.starts.data_ptr(), self.seqs,
+            self.share.data_ptr(), lib.TYPE_F32, self.share.stride(0), u.data_ptr(), self.draw.data_ptr(), temperature.data_ptr(), top_k.data_ptr(),
+            top_p.data_ptr(), None, self.tokens.data_ptr(), self.accepted.data_ptr(), self.probs.data_ptr(), s))
+
+
 # ---------------------------------------------------------------------------- decode-1p7b
 def decode_1p7b(args, dev):
     L = lib.load()
@@ -716,7 +784,11 @@ def decode_1p7b(args, dev):
 
     if args.context < 0:
         raise SystemExit("--context: tokens of a sequence, 0 or more")
-    between = Between(b, args.context, hidden // HEAD_DIM, kv // HEAD_DIM, mk) if args.context else None
+    drafts, in_4_bits = getattr(args, "drafts", 0), getattr(args, "kv_cache", "q8") == "mxfp4"
+    if drafts < 0 or (drafts or in_4_bits) and not args.context or drafts and not in_4_bits:
+        raise SystemExit("--kv-cache mxfp4 goes with a --context, --drafts (0 or more) with both")
+    heads = (hidden // HEAD_DIM, kv // HEAD_DIM)
+    between = (BetweenMxfp4(b, args.context, *heads, mk, drafts) if in_4_bits else Between(b, args.context, *heads, mk)) if args.context else None
     if between:
         plan.append(between.plan_item(s))
     for _ in range(layers):
@@ -759,7 +831,9 @@ def decode_1p7b(args, dev):
     return line(args, value, "GB/s", ms, "int8",
                 {"workload": f"qwen3-1.7b decode-step quantized linears (Q4_K attention and gate/up, Q6_K down and "
                              f"lm_head), batch {b}, 28 layers" + (f"; the plan of pages, cache write and attention of a layer over {args.context} "
-                             f"tokens a sequence, and the choice of the next token (value: weight and cache bytes)" if between else ""),
+                             f"tokens a sequence, and the choice of the next token (value: weight and cache bytes)" if between else "")
+                             + ("; a cache in 4 bits, head norms and rotation in the launch that writes it" if in_4_bits else "")
+                             + (f"; {drafts} drafted tokens and one more of each of {b // (drafts + 1)} sequences, and their check" if drafts else ""),
                  "path": "mat-vec (fused: q + k + v, o from f32 rows; gate + up as the pair launch that writes down's Q8_1 rows)" if paired
                          else "mat-vec (fused; own quantizer launch for rows over 8192 values)" if matvec
                          else "16-row tiles on the matrix unit: q + k + v in one launch, o, gate + up with SiLU in one launch that writes "

@@ -1,5 +1,8 @@
 """A served step with drafted tokens over the 4-bit cache, operator after operator as a decode loop uses them between its quantized linears:
 eagerly against the definitions, and recorded."""
+import json
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 
@@ -7,7 +10,7 @@ torch = pytest.importorskip("torch")
 
 import mxfp4_reference as ref
 import serving_reference as served
-from loken_amd import kv, lib, ops, rotary, sampling, synth
+from loken_amd import kv, lib, ops, rotary, sampling, synth, workloads
 from test_gpu_graph_scratch import record
 from test_gpu_kv_attention import i32
 from test_gpu_mxfp4_cache import check_cache, dev
@@ -146,3 +149,43 @@ def test_a_recorded_step_is_the_eager_one():
         words = want[6][first + want[7]]
         eager.after(plans[0], want[7])
         other.after(plans[1], got[7])
+
+
+@pytest.mark.parametrize("batch,context,drafts", [(1, 64, 0), (6, 100, 2)])
+def test_the_measured_step_over_the_4_bit_cache(batch, context, drafts, capsys):
+    """bench.py's step: its line, and a layer's attention and the check at its end over what it left."""
+    made = []
+
+    class Kept(workloads.BetweenMxfp4):
+        def __init__(self, *a):
+            super().__init__(*a)
+            made.append(self)
+
+        def attention_items(self, q, k, v, out, s):
+            wide = self.kv_heads * workloads.HEAD_DIM   # (of rows as wide as the queries')
+            self.rows_of = (q, k[:, :wide], v[:, :wide], out.view(self.rows, self.heads, workloads.HEAD_DIM))
+            return super().attention_items(q, k, v, out, s)
+
+    args = SimpleNamespace(batch=batch, context=context, kv_cache="mxfp4", drafts=drafts, mid_rows="auto", acts="f32", steps=1, warmup=1, gpus=1)
+    before, workloads.BetweenMxfp4 = workloads.BetweenMxfp4, Kept
+    try:
+        assert workloads.decode_1p7b(args, torch.device("cuda", 0)) == 0
+    finally:
+        workloads.BetweenMxfp4 = before
+    line = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    between = made[0]
+    assert "4 bits" in line["config"]["workload"] and line["config"]["cache_bytes_per_step"] == 28 * between.bytes_read()
+    q, k, v, out = between.rows_of
+    heads = lambda x: x.unflatten(1, (-1, workloads.HEAD_DIM))  # noqa: E731
+    p, turning = between.plan, rotary.Rotary(between.frequencies)
+    turned, turned_k = rotary.rotate(heads(q), heads(k), p.positions, turning, q_weight=between.norms[0], k_weight=between.norms[1])
+    there = kv.kv_read(between.caches[-1], p.slots)
+    for got, rows in zip(there, (turned_k, heads(v))):      # (a key's code may be the border's other one: 64 bits there, 32 here)
+        want = torch.tensor(ref.values(*ref.quantize(rows.double().cpu().numpy())))
+        assert (got.double().cpu() != want).double().mean() < 1e-3
+    exact = kv.kv_attention(turned, between.caches[-1], between.table, p.lens, p.starts, max_fresh=drafts + 1, max_len=context + drafts + 1)
+    assert torch.allclose(out, exact, rtol=1e-4, atol=1e-4)
+    if drafts:
+        assert ((between.accepted >= 0) & (between.accepted <= drafts)).all()
+        first = p.starts[:-1].long() + between.accepted
+        assert (between.tokens[first] >= 0).all() and (between.probs[first] > 0).all()
