@@ -54,6 +54,44 @@ static __device__ __forceinline__ float mx_tanh(float x) {
     return fabsf(x) < 0.25f ? near : far;
 }
 
+// The maximum over the four lanes l, l + 16, l + 32, l + 48.
+static __device__ __forceinline__ float mx_max_over_groups(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int WORDS>
+struct __attribute__((aligned(WORDS >= 4 ? 16 : 8))) MxWords { uint32_t w[WORDS]; };
+
+// The row tile of that number among those of all sequences, from the last one on; false: there are fewer. Found by each wave.
+static __device__ __forceinline__ bool mx_tile_at(const Attend& a, int rows_of_tile, int number, int& seq, int& tile) {
+    const int lane = threadIdx.x & 63;
+    auto tiles_of = [&](int i) {
+        if (i >= a.seqs) return 0;
+        const unsigned rows = (unsigned)KvSeq(a, i).tokens() * (unsigned)a.group;
+        return (int)rows <= a.few_rows ? 0 : (int)((rows + rows_of_tile - 1) / rows_of_tile);
+    };
+    for (int base = (a.seqs - 1) & ~63; base >= 0; base -= 64) {
+        const int mine = tiles_of(base + lane);
+        int behind = mine;   // of this sequence and those behind it
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_down(behind, o);
+            if (lane + o < 64) behind += v;
+        }
+        const uint64_t over = __ballot(behind > number);
+        if (over) {
+            const int l = 63 - __clzll((long long)over);
+            seq = base + l;
+            tile = __builtin_amdgcn_readlane(behind, l) - 1 - number;
+            return true;
+        }
+        number -= __builtin_amdgcn_readfirstlane(behind);
+    }
+    return false;
+}
+
 // Sequences of up to so many rows (token, head of a group) are the few-rows kernel's, and rows of its workgroups: with slots for the pieces while
 // these fit (in one operand, or f32 in two), else sixteen.
 constexpr int MX_FEW_ROWS = 16;

@@ -19,16 +19,7 @@ namespace {
 
 constexpr int WAVES = 4;
 
-static __device__ __forceinline__ float max_over_groups(float v) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
 static __device__ __forceinline__ float sum_over_groups(float v) { return swap_add32(swap_add16(v)); }
-
-template <int WORDS>
-struct __attribute__((aligned(WORDS >= 4 ? 16 : 8))) Words { uint32_t w[WORDS]; };
 
 template <typename T, int D, int NT, int SLOTS>
 struct Few {
@@ -117,46 +108,46 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
 
         // (as memory that nobody writes, which scalar loads read: what a wave's vector loads wait for stays theirs)
         const auto* entries = (const __attribute__((address_space(4))) int32_t*)(uint64_t)(a.table + seq * a.table_stride);
-        // the page of a step's tile; -1: absent, or behind the last position
-        auto page_of = [&](int t, int b) {
-            const int p0 = lo + t * KV_TILE + 16 * b;
-            const int page = t < t_end && p0 < hi ? entries[p0 >> shift] : -1;
-            return (unsigned)page < (unsigned)a.mx.pages ? page : -1;
-        };
+        // A step's tile, from its first position; past the end the last one again, which is in the cache (a load that is left out at times
+        // would be waited for at the next use of any).
+        const int last_tile = (min(hi, lo + t_end * KV_TILE) - 1) & ~15;
+        auto at_tile = [&](int t, int b) { return min(lo + t * KV_TILE + 16 * b, last_tile); };
+        auto page_of = [&](int t, int b) { return entries[at_tile(t, b) >> shift]; };
         // (a page's address is the wave's own, a lane's place in a tile always the same)
         const uint32_t key_at = i * (D / 2) + g * (D / 8), key_power_at = i * F::PART + (D == 256 ? 2 * g : D == 64 ? g >> 1 : g);
         const uint32_t value_at = (g * 16 + i) * (D / 8), value_power_at = ((i * F::PART / 16) << shift) + 4 * g;
         // A step's codes and powers. Two of them: the next step's are loaded while this one's are at work.
         struct Loaded {
-            Words<F::W> k[4], v[4];
+            MxWords<F::W> k[4], v[4];
             uint32_t kp[4], vp[4];   // powers: of the lane's block or two of a key; of four tokens' values
         } loaded[2];
+        const uint8_t *keys = a.mx.k + key_at, *key_powers = a.mx.k_powers + key_power_at, *values = a.mx.v + value_at, *value_powers = a.mx.v_powers + value_power_at;
         auto load = [&](Loaded& into, int t, const int (&pages)[4]) {
+            int64_t page[4], tok[4];   // a page's tokens among all, and a tile's: rows of either side are as long
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const int64_t page = ((int64_t)max(pages[b], 0) * a.mx.heads + kv) << shift;
-                const int at = (lo + t * KV_TILE + 16 * b) & ((1 << shift) - 1);
-                const uint8_t *codes = a.mx.k + (page + at) * (D / 2), *powers = a.mx.k_powers + (page + at) * F::PART;
-                into.k[b] = *(const Words<F::W>*)(codes + key_at);
-                if (D == 256) into.kp[b] = *(const uint16_t*)(powers + key_power_at);
-                else into.kp[b] = powers[key_power_at];
+                const int p = (unsigned)pages[b] < (unsigned)a.mx.pages ? pages[b] : 0;
+                page[b] = ((int64_t)p * a.mx.heads + kv) << shift;
+                tok[b] = page[b] + (at_tile(t, b) & ((1 << shift) - 1));
+                into.k[b] = *(const MxWords<F::W>*)(keys + tok[b] * (D / 2));
+                if (D == 256) into.kp[b] = *(const uint16_t*)(key_powers + tok[b] * F::PART);
+                else into.kp[b] = key_powers[tok[b] * F::PART];
             }
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const int64_t page = ((int64_t)max(pages[b], 0) * a.mx.heads + kv) << shift;
-                const int at = (lo + t * KV_TILE + 16 * b) & ((1 << shift) - 1);
-                const uint8_t *codes = a.mx.v + (page + at) * (D / 2), *powers = a.mx.v_powers + page * F::PART + at;
-                into.v[b] = *(const Words<F::W>*)(codes + value_at);
-                into.vp[b] = *(const uint32_t*)(powers + value_power_at);
+                into.v[b] = *(const MxWords<F::W>*)(values + tok[b] * (D / 2));
+                into.vp[b] = *(const uint32_t*)(value_powers + page[b] * (F::PART - 1) + tok[b]);
             }
         };
         int t = t_begin + wave;
-        int pages[4], next[4];   // of this step and of the wave's next one
+        int pages[4] = {}, next[4] = {};   // of this step and of the wave's next one
+        if (t < t_end) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) pages[b] = page_of(t, b);
+            for (int b = 0; b < 4; ++b) pages[b] = page_of(t, b);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) next[b] = page_of(t + WAVES, b);
-        if (t < t_end) load(loaded[0], t, pages);
+            for (int b = 0; b < 4; ++b) next[b] = page_of(t + WAVES, b);
+            load(loaded[0], t, pages);
+        }
 
         const float capped = CAP ? a.scale / a.cap : 0.f;   // what a product is under the tanh
         // the rows' pieces, and what a product, or its tanh, is in powers of two
@@ -221,19 +212,15 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
 
         auto step = [&](Loaded& now, Loaded& then) {
             const int p0 = lo + t * KV_TILE;
-            // (Behind the last step this one's are loaded again, out of the cache: a load that is left out at times would be waited for at the
-            // next use of any.)
-            const bool more = t + WAVES < t_end;
-            int from[4], behind[4];
+            int behind[4], absent = 0;
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                from[b] = more ? next[b] : pages[b];
                 behind[b] = page_of(t + 2 * WAVES, b);
+                absent |= (unsigned)pages[b] < (unsigned)a.mx.pages ? 0 : 1 << b;
             }
-            load(then, t + WAVES, from);
+            load(then, t + WAVES, next);
             // whether every row sees every position of the step
-            const bool here = pages[0] >= 0 && pages[1] >= 0 && pages[2] >= 0 && pages[3] >= 0;
-            const bool whole = p0 + KV_TILE - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && here;
+            const bool whole = p0 + KV_TILE - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && absent == 0;
             v4f sc[NT][4];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -252,10 +239,6 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
 #pragma unroll
                 for (int n = 0; n < NT; ++n) sc[n][b] = c[n];
             }
-            int absent = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) absent |= (pages[b] < 0) << b;
-
             uint32_t share[NT][F::SP][4][2];   // weights: of a tile's four positions
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -277,7 +260,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
-                top = max_over_groups(top);
+                top = mx_max_over_groups(top);
                 if (__ballot(top > m[n])) {
                     const float most = fmaxf(m[n], top), to = most == -INFINITY ? 0.f : most * unit[n];
                     const float keep = m[n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base[n] - to);

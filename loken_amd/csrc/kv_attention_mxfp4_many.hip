@@ -15,16 +15,6 @@ namespace {
 constexpr int WAVES = 2, STEP = 32, TILES = STEP / 16;
 constexpr float SLACK = 8.f;   // a power of two
 
-static __device__ __forceinline__ float max_over_groups(float v) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-template <int WORDS>
-struct __attribute__((aligned(WORDS >= 4 ? 16 : 8))) Words { uint32_t w[WORDS]; };
-
 template <typename T, int D>
 struct Many {
     static constexpr bool FINE = sizeof(T) == 4;
@@ -32,33 +22,6 @@ struct Many {
     static constexpr int SP = QP;                                                  // and of a weight: 8 bits beside bf16, 16, 24
     static constexpr int ROWS = mx_many_rows(FINE, D), NT = ROWS / 16, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
 };
-
-// The row tile of that number among those of all sequences, from the last one on; false: there are fewer. Found by each wave.
-static __device__ __forceinline__ bool tile_at(const Attend& a, int rows_of_tile, int number, int& seq, int& tile) {
-    const int lane = threadIdx.x & 63;
-    auto tiles_of = [&](int i) {
-        if (i >= a.seqs) return 0;
-        const unsigned rows = (unsigned)KvSeq(a, i).tokens() * (unsigned)a.group;
-        return (int)rows <= a.few_rows ? 0 : (int)((rows + rows_of_tile - 1) / rows_of_tile);
-    };
-    for (int base = (a.seqs - 1) & ~63; base >= 0; base -= 64) {
-        const int mine = tiles_of(base + lane);
-        int behind = mine;   // of this sequence and those behind it
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_down(behind, o);
-            if (lane + o < 64) behind += v;
-        }
-        const uint64_t over = __ballot(behind > number);
-        if (over) {
-            const int l = 63 - __clzll((long long)over);
-            seq = base + l;
-            tile = __builtin_amdgcn_readlane(behind, l) - 1 - number;
-            return true;
-        }
-        number -= __builtin_amdgcn_readfirstlane(behind);
-    }
-    return false;
-}
 
 // CAP: whether scores are capped (as a branch at run time the compiler takes the tanh always, and the result where it is asked for)
 template <typename T, int D, bool CAP>
@@ -73,7 +36,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
     block /= a.mx.heads;
     const int part = block % a.splits;
     int seq = 0, tile = 0;
-    if (!tile_at(a, M::ROWS, block / a.splits, seq, tile)) return;
+    if (!mx_tile_at(a, M::ROWS, block / a.splits, seq, tile)) return;
     seq = __builtin_amdgcn_readfirstlane(seq);
     tile = __builtin_amdgcn_readfirstlane(tile);
     const KvSeq s(a, seq);
@@ -88,45 +51,46 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
 
     // (as memory that nobody writes, which scalar loads read: what a wave's vector loads wait for stays theirs)
     const auto* entries = (const __attribute__((address_space(4))) int32_t*)(uint64_t)(a.table + seq * a.table_stride);
-    auto page_of = [&](int t, int b) {
-        const int p0 = lo + t * STEP + 16 * b;
-        const int page = t < t_end && p0 < hi ? entries[p0 >> shift] : -1;
-        return (unsigned)page < (unsigned)a.mx.pages ? page : -1;
-    };
+    // A step's tile, from its first position; past the end the last one again, which is in the cache (a load that is left out at times
+    // would be waited for at the next use of any).
+    const int last_tile = (min(hi, lo + t_end * STEP) - 1) & ~15;
+    auto at_tile = [&](int t, int b) { return min(lo + t * STEP + 16 * b, last_tile); };
+    auto page_of = [&](int t, int b) { return entries[at_tile(t, b) >> shift]; };
     // (a page's address is the wave's own, a lane's place in a tile always the same)
     const uint32_t key_at = i * (D / 2) + g * (D / 8), key_power_at = i * M::PART + (D == 256 ? 2 * g : D == 64 ? g >> 1 : g);
     const uint32_t value_at = (g * 16 + i) * (D / 8), value_power_at = ((i * M::PART / 16) << shift) + 4 * g;
     // A step's codes and powers. Two of them: the next step's are loaded while this one's are at work.
     struct Loaded {
-        Words<M::W> k[TILES], v[TILES];
+        MxWords<M::W> k[TILES], v[TILES];
         uint32_t kp[TILES], vp[TILES];   // powers: of the lane's block or two of a key; of four tokens' values
     } loaded[2];
+    const uint8_t *keys = a.mx.k + key_at, *key_powers = a.mx.k_powers + key_power_at, *values = a.mx.v + value_at, *value_powers = a.mx.v_powers + value_power_at;
     auto load = [&](Loaded& into, int t, const int (&pages)[TILES]) {
+        int64_t page[TILES], tok[TILES];   // a page's tokens among all, and a tile's: rows of either side are as long
 #pragma unroll
         for (int b = 0; b < TILES; ++b) {
-            const int64_t page = ((int64_t)max(pages[b], 0) * a.mx.heads + kv) << shift;
-            const int at = (lo + t * STEP + 16 * b) & ((1 << shift) - 1);
-            const uint8_t *codes = a.mx.k + (page + at) * (D / 2), *powers = a.mx.k_powers + (page + at) * M::PART;
-            into.k[b] = *(const Words<M::W>*)(codes + key_at);
-            if (D == 256) into.kp[b] = *(const uint16_t*)(powers + key_power_at);
-            else into.kp[b] = powers[key_power_at];
+            const int p = (unsigned)pages[b] < (unsigned)a.mx.pages ? pages[b] : 0;
+            page[b] = ((int64_t)p * a.mx.heads + kv) << shift;
+            tok[b] = page[b] + (at_tile(t, b) & ((1 << shift) - 1));
+            into.k[b] = *(const MxWords<M::W>*)(keys + tok[b] * (D / 2));
+            if (D == 256) into.kp[b] = *(const uint16_t*)(key_powers + tok[b] * M::PART);
+            else into.kp[b] = key_powers[tok[b] * M::PART];
         }
 #pragma unroll
         for (int b = 0; b < TILES; ++b) {
-            const int64_t page = ((int64_t)max(pages[b], 0) * a.mx.heads + kv) << shift;
-            const int at = (lo + t * STEP + 16 * b) & ((1 << shift) - 1);
-            const uint8_t *codes = a.mx.v + (page + at) * (D / 2), *powers = a.mx.v_powers + page * M::PART + at;
-            into.v[b] = *(const Words<M::W>*)(codes + value_at);
-            into.vp[b] = *(const uint32_t*)(powers + value_power_at);
+            into.v[b] = *(const MxWords<M::W>*)(values + tok[b] * (D / 2));
+            into.vp[b] = *(const uint32_t*)(value_powers + page[b] * (M::PART - 1) + tok[b]);
         }
     };
-    int pages[TILES], next[TILES];   // of this step and of the wave's next one
+    int pages[TILES] = {}, next[TILES] = {};   // of this step and of the wave's next one
+    if (t < t_end) {
 #pragma unroll
-    for (int b = 0; b < TILES; ++b) {
-        pages[b] = page_of(t, b);
-        next[b] = page_of(t + WAVES, b);
+        for (int b = 0; b < TILES; ++b) {
+            pages[b] = page_of(t, b);
+            next[b] = page_of(t + WAVES, b);
+        }
+        load(loaded[0], t, pages);
     }
-    if (t < t_end) load(loaded[0], t, pages);
 
     const float capped = CAP ? a.scale / a.cap : 0.f;   // what a product is under the tanh
     // the rows' pieces, and what a product, or its tanh, is in powers of two
@@ -177,20 +141,17 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
 
     auto step = [&](Loaded& now, Loaded& then) {
         const int p0 = lo + t * STEP;
-        // (Behind the last step this one's are loaded again, out of the cache: a load that is left out at times would be waited for at the
-        // next use of any.)
-        const bool more = t + WAVES < t_end;
-        int from[TILES], behind[TILES], absent = 0;
+        int behind[TILES], absent = 0;
 #pragma unroll
         for (int b = 0; b < TILES; ++b) {
-            from[b] = more ? next[b] : pages[b];
             behind[b] = page_of(t + 2 * WAVES, b);
-            absent |= (pages[b] < 0) << b;
+            absent |= (unsigned)pages[b] < (unsigned)a.mx.pages ? 0 : 1 << b;
         }
-        load(then, t + WAVES, from);
+        load(then, t + WAVES, next);
         // whether every row sees every position of the step
         const bool whole = p0 + STEP - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && absent == 0;
         v4f sc[M::NT][TILES];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int b = 0; b < TILES; ++b) {
 #pragma unroll
@@ -205,6 +166,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
                     for (int p = 0; p < M::QP; ++p) sc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, q[n][ks][p], sc[n][b], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         mx_b8 share[M::NT][M::SP];
 #pragma unroll
         for (int n = 0; n < M::NT; ++n) {
@@ -227,7 +189,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
 #pragma unroll
             for (int e = 0; e < 4 * TILES; ++e) most = fmaxf(most, x[e]);
             if (__ballot(most > top[n])) {
-                most = max_over_groups(most);
+                most = mx_max_over_groups(most);
                 const bool first = top[n] == -INFINITY, up = most > top[n];
                 const float to = up ? most * unit[n] : base[n], keep = first ? 1.f : __builtin_amdgcn_exp2f(base[n] - to);
                 l[n] *= keep;
