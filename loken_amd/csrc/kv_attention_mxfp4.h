@@ -104,7 +104,9 @@ constexpr int mx_few_on_simd(bool f32, int head_dim, int rows) { return head_dim
 
 // Rows of a workgroup of the many-rows kernel, and its waves on a SIMD.
 constexpr int mx_many_rows(bool f32, int head_dim) { return head_dim == 256 && f32 ? 16 : 32; }
-constexpr int mx_many_on_simd(bool f32, bool f16, int head_dim) { return head_dim == 256 || (head_dim == 128 && (f32 || f16)) ? 1 : 2; }
+constexpr int mx_many_on_simd(bool f32, bool f16, int head_dim) {
+    return head_dim == 64 ? (f32 || f16 ? 3 : 4) : head_dim == 128 ? (f32 || f16 ? 2 : 3) : 1;
+}
 
 int kv_attention_mxfp4_few(const AttendMx& a, int type, int head_dim, int max_rows, hipStream_t stream);
 int kv_attention_mxfp4_many(const AttendMx& a, int type, int head_dim, hipStream_t stream);

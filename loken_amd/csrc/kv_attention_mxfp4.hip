@@ -16,17 +16,20 @@ static void cut(Attend& a, int64_t groups, int tiles, int want, int least) {
     a.least_tiles = tiles > a.splits ? (tiles + a.splits - 1) / a.splits : 1;
 }
 
-// Parts of the many-rows kernel's contexts, of `tiles` steps for `groups` row tiles and heads, `slots` workgroups at once: those that take the least
-// time where a workgroup takes 5 us to start and 0.8 us a step, and each row and head's part 0.35 ns to be stored and joined, 4 us in all beside.
-static void cut_many(Attend& a, int64_t groups, int tiles, int64_t slots) {
+// Parts of the many-rows kernel's contexts, of `tiles` steps for `groups` row tiles and heads, `layer` workgroups being one wave for every SIMD and
+// `on_simd` of them there at once: those that take the least time where a workgroup takes 5 us to start and `step` us a step, waves that fill a SIMD
+// that much each and those that do not 0.7 of a step more, and each row and head's part 0.35 ns to be stored and joined, 4 us in all beside.
+static void cut_many(Attend& a, int64_t groups, int tiles, int64_t layer, int on_simd, double step) {
     const double rows = (double)a.rows * a.heads;
     double least = 1e30;
     for (int parts = 1, of = 0; parts <= 64 && parts <= tiles / 2 + 1; ++parts) {
         const int per = (tiles + parts - 1) / parts;
         if (per == of) continue;
         of = per;
-        const int64_t rounds = (groups * parts + slots - 1) / slots;
-        const double time = (double)rounds * (per * 0.8 + 5.0) + (parts > 1 ? 4.0 + rows * parts * 0.35e-3 : 0.0);
+        const int64_t full = groups * parts / (layer * on_simd), rest = (groups * parts - full * layer * on_simd + layer - 1) / layer;
+        const double most = on_simd > 1 ? on_simd : 1.5, last = rest ? rest + 0.7 : 0.0;
+        const double waves = full * most + (last < most ? last : most);
+        const double time = waves * per * step + 5.0 * (full + (rest > 0)) + (parts > 1 ? 4.0 + rows * parts * 0.35e-3 : 0.0);
         if (time < least) {
             least = time;
             a.splits = parts;
@@ -95,8 +98,9 @@ extern "C" int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, 
     if (many) {
         am.few_rows = few ? few_max : 0;
         // as many sequences as fill the batch with the most rows that one has
-        const int64_t long_seqs = min((int64_t)seqs, (rows + (int64_t)tokens / 2) / tokens);
-        cut_many(am, long_seqs * ((max_rows - 1) / many_rows + 1) * kv_heads, tiles, 2 * cus * mx_many_on_simd(f32, f16, head_dim));
+        const int64_t filled = (rows + (int64_t)tokens / 2) / tokens, long_seqs = filled < seqs ? filled : seqs;
+        cut_many(am, long_seqs * ((max_rows - 1) / many_rows + 1) * kv_heads, tiles, 2 * cus, mx_many_on_simd(f32, f16, head_dim),
+                 (f32 ? 1.1 : f16 ? 0.8 : 0.6) * head_dim / 128);
         if (am.splits > 1) part_rows_m = (int64_t)rows * heads * am.splits;
     }
     LkScratch scratch(s);

@@ -20,14 +20,16 @@ struct Many {
     static constexpr bool FINE = sizeof(T) == 4;
     static constexpr int QP = FINE ? 3 : std::is_same<T, __half>::value ? 2 : 1;   // pieces of a query value
     static constexpr int SP = QP;                                                  // and of a weight: 8 bits beside bf16, 16, 24
-    static constexpr int ROWS = mx_many_rows(FINE, D), NT = ROWS / 16, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
+    static constexpr int ROWS = mx_many_rows(FINE, D), NT = ROWS / 16, PITCH = D + 4, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
+    static constexpr int QUERIES = NT * KS * QP * 64 * 16, HANDED = NT * 16 * PITCH * 4, LDS = QUERIES > HANDED ? QUERIES : HANDED;
 };
 
 // CAP: whether scores are capped (as a branch at run time the compiler takes the tanh always, and the result where it is asked for)
 template <typename T, int D, bool CAP>
 __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof(T) == 2 && std::is_same<T, __half>::value, D))) void mx_many_kernel(AttendMx a) {
     using M = Many<T, D>;
-    __shared__ __attribute__((aligned(16))) float handed[M::NT][16][D + 4];
+    __shared__ uint4 lds[M::LDS / 16];   // the rows' operands, in the end half of the sums on their way to the other wave
+    __shared__ float units[M::ROWS];
     __shared__ float tops[WAVES][M::ROWS], weights[WAVES][M::ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4, shift = a.mx.page_shift;
@@ -59,27 +61,26 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
     // (a page's address is the wave's own, a lane's place in a tile always the same)
     const uint32_t key_at = i * (D / 2) + g * (D / 8), key_power_at = i * M::PART + (D == 256 ? 2 * g : D == 64 ? g >> 1 : g);
     const uint32_t value_at = (g * 16 + i) * (D / 8), value_power_at = ((i * M::PART / 16) << shift) + 4 * g;
-    // A step's codes and powers. Two of them: the next step's are loaded while this one's are at work.
-    struct Loaded {
-        MxWords<M::W> k[TILES], v[TILES];
-        uint32_t kp[TILES], vp[TILES];   // powers: of the lane's block or two of a key; of four tokens' values
-    } loaded[2];
+    MxWords<M::W> k[TILES], v[TILES];
+    uint32_t kp[TILES], vp[TILES];   // powers: of the lane's block or two of a key; of four tokens' values
     const uint8_t *keys = a.mx.k + key_at, *key_powers = a.mx.k_powers + key_power_at, *values = a.mx.v + value_at, *value_powers = a.mx.v_powers + value_power_at;
-    auto load = [&](Loaded& into, int t, const int (&pages)[TILES]) {
-        int64_t page[TILES], tok[TILES];   // a page's tokens among all, and a tile's: rows of either side are as long
+    // a page's tokens among all: rows of either side are as long
+    auto tokens_before = [&](int page) { return ((int64_t)((unsigned)page < (unsigned)a.mx.pages ? page : 0) * a.mx.heads + kv) << shift; };
+    auto load_keys = [&](int t, const int (&pages)[TILES]) {
 #pragma unroll
         for (int b = 0; b < TILES; ++b) {
-            const int p = (unsigned)pages[b] < (unsigned)a.mx.pages ? pages[b] : 0;
-            page[b] = ((int64_t)p * a.mx.heads + kv) << shift;
-            tok[b] = page[b] + (at_tile(t, b) & ((1 << shift) - 1));
-            into.k[b] = *(const MxWords<M::W>*)(keys + tok[b] * (D / 2));
-            if (D == 256) into.kp[b] = *(const uint16_t*)(key_powers + tok[b] * M::PART);
-            else into.kp[b] = key_powers[tok[b] * M::PART];
+            const int64_t tok = tokens_before(pages[b]) + (at_tile(t, b) & ((1 << shift) - 1));
+            k[b] = *(const MxWords<M::W>*)(keys + tok * (D / 2));
+            if (D == 256) kp[b] = *(const uint16_t*)(key_powers + tok * M::PART);
+            else kp[b] = key_powers[tok * M::PART];
         }
+    };
+    auto load_values = [&](int t, const int (&pages)[TILES]) {
 #pragma unroll
         for (int b = 0; b < TILES; ++b) {
-            into.v[b] = *(const MxWords<M::W>*)(values + tok[b] * (D / 2));
-            into.vp[b] = *(const uint32_t*)(value_powers + page[b] * (M::PART - 1) + tok[b]);
+            const int64_t page = tokens_before(pages[b]), tok = page + (at_tile(t, b) & ((1 << shift) - 1));
+            v[b] = *(const MxWords<M::W>*)(values + tok * (D / 2));
+            vp[b] = *(const uint32_t*)(value_powers + page * (M::PART - 1) + tok);
         }
     };
     int pages[TILES] = {}, next[TILES] = {};   // of this step and of the wave's next one
@@ -89,12 +90,13 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             pages[b] = page_of(t, b);
             next[b] = page_of(t + WAVES, b);
         }
-        load(loaded[0], t, pages);
+        load_keys(t, pages);
+        load_values(t, pages);
     }
 
     const float capped = CAP ? a.scale / a.cap : 0.f;   // what a product is under the tanh
-    // the rows' pieces, and what a product, or its tanh, is in powers of two
-    mx_b8 q[M::NT][M::KS][M::QP];
+    // The rows' pieces as operands, in LDS, each wave half of them; and what a product, or its tanh, is in powers of two.
+    uint4* const queries = lds;
     float unit[M::NT];
     int pos[M::NT];
 #pragma unroll
@@ -102,6 +104,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
         const unsigned r = r0 + 16 * n + i;
         const int of_seq = a.token_of(min(r, r1)), tok = s.first + of_seq, head = kv * a.group + (int)(min(r, r1) - (unsigned)of_seq * a.group);
         pos[n] = r <= r1 ? (int)max(s.pos_of_0 + tok, (int64_t)-1) : -1;
+        if ((n & 1) != wave) continue;
         const T* row = (const T*)a.q + tok * a.q_stride + (int64_t)head * D + g * (D / 4);
         bool finite = true;
 #pragma unroll
@@ -118,12 +121,14 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
                 for (int p = 0; p < M::QP; ++p) w[p][e] = both[p];
             }
 #pragma unroll
-            for (int p = 0; p < M::QP; ++p) q[n][ks][p] = __builtin_bit_cast(mx_b8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
+            for (int p = 0; p < M::QP; ++p) queries[((n * M::KS + ks) * M::QP + p) * 64 + lane] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
         }
         const uint64_t odd = __ballot(!finite);
-        finite = (odd >> i & 0x0001000100010001ull) == 0;
-        unit[n] = finite ? (CAP ? a.cap : a.scale) * 1.4426950408889634f : NAN;
+        if (g == 0) units[16 * n + i] = (odd >> i & 0x0001000100010001ull) == 0 ? (CAP ? a.cap : a.scale) * 1.4426950408889634f : NAN;
     }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < M::NT; ++n) unit[n] = units[16 * n + i];
     // positions that all rows see (of a window: behind the last one's first)
     const int pos_least = (int)max(s.pos_of_0 + s.first + a.token_of(r0), (int64_t)-1), pos_most = (int)max(s.pos_of_0 + s.first + a.token_of(r1), (int64_t)-1);
 
@@ -139,7 +144,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
     }
     const mx_b8 ones = __builtin_bit_cast(mx_b8, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
 
-    auto step = [&](Loaded& now, Loaded& then) {
+    for (; t < t_end; t += WAVES) {
         const int p0 = lo + t * STEP;
         int behind[TILES], absent = 0;
 #pragma unroll
@@ -147,7 +152,6 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             behind[b] = page_of(t + 2 * WAVES, b);
             absent |= (unsigned)pages[b] < (unsigned)a.mx.pages ? 0 : 1 << b;
         }
-        load(then, t + WAVES, next);
         // whether every row sees every position of the step
         const bool whole = p0 + STEP - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && absent == 0;
         v4f sc[M::NT][TILES];
@@ -158,15 +162,17 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             for (int n = 0; n < M::NT; ++n) sc[n][b] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < M::KS; ++ks) {
-                const float power = D == 256 && ks >= M::KS / 2 ? mx_power_of<1>(now.kp[b]) : mx_power_of<0>(now.kp[b]);
-                const mx_b8 op = mx_eight(now.k[b].w[ks], power);
+                const float power = D == 256 && ks >= M::KS / 2 ? mx_power_of<1>(kp[b]) : mx_power_of<0>(kp[b]);
+                const mx_b8 op = mx_eight(k[b].w[ks], power);
 #pragma unroll
                 for (int n = 0; n < M::NT; ++n)
 #pragma unroll
-                    for (int p = 0; p < M::QP; ++p) sc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, q[n][ks][p], sc[n][b], 0, 0, 0);
+                    for (int p = 0; p < M::QP; ++p)
+                        sc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, __builtin_bit_cast(mx_b8, queries[((n * M::KS + ks) * M::QP + p) * 64 + lane]), sc[n][b], 0, 0, 0);
             }
         }
         __builtin_amdgcn_s_setprio(0);
+        load_keys(t + WAVES, next);
         mx_b8 share[M::NT][M::SP];
 #pragma unroll
         for (int n = 0; n < M::NT; ++n) {
@@ -219,16 +225,16 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
                     const int at = p0 + 16 * b + 4 * g + j;
                     if (at >= seen_from && at < hi && !(absent >> b & 1)) seen |= 0xFFu << (8 * j);
                 }
-                now.vp[b] &= seen;
+                vp[b] &= seen;
             }
         }
         float power[4 * TILES];
 #pragma unroll
         for (int b = 0; b < TILES; ++b) {
-            power[4 * b] = mx_power_of<0>(now.vp[b]);
-            power[4 * b + 1] = mx_power_of<1>(now.vp[b]);
-            power[4 * b + 2] = mx_power_of<2>(now.vp[b]);
-            power[4 * b + 3] = mx_power_of<3>(now.vp[b]);
+            power[4 * b] = mx_power_of<0>(vp[b]);
+            power[4 * b + 1] = mx_power_of<1>(vp[b]);
+            power[4 * b + 2] = mx_power_of<2>(vp[b]);
+            power[4 * b + 3] = mx_power_of<3>(vp[b]);
         }
 #pragma unroll
         for (int n = 0; n < M::NT; ++n)
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int at = (j & 3) * M::PART + byte;
-                const uint32_t word = now.v[j >> 2].w[at >> 2];
+                const uint32_t word = v[j >> 2].w[at >> 2];
                 const int sel = at & 3;
                 c[j] = sel == 0 ? mx_two<0>(word, power[j]) : sel == 1 ? mx_two<1>(word, power[j]) : sel == 2 ? mx_two<2>(word, power[j]) : mx_two<3>(word, power[j]);
             }
@@ -260,16 +266,12 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
                     acc[n][2 * byte + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op1, share[n][j], acc[n][2 * byte + 1], 0, 0, 0);
                 }
         }
+        load_values(t + WAVES, next);
 #pragma unroll
         for (int b = 0; b < TILES; ++b) {
             pages[b] = next[b];
             next[b] = behind[b];
         }
-        t += WAVES;
-    };
-    while (t < t_end) {
-        step(loaded[0], loaded[1]);
-        if (t < t_end) step(loaded[1], loaded[0]);
     }
 
     // The two waves' sums relative to their common maximum: each wave hands the other the half of the rows that it does not finish.
@@ -279,6 +281,8 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             tops[wave][16 * n + i] = top[n] == -INFINITY ? -INFINITY : base[n];
             weights[wave][16 * n + i] = l[n][0];
         }
+    __syncthreads();   // the last queries have been read
+    float* const handed = (float*)lds;
 #pragma unroll
     for (int n = 0; n < M::NT; ++n)
         if (n != wave) {
@@ -286,7 +290,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int b = 0; b < M::NB; b += 4)
-                    *(float4*)&handed[n][i][(4 * g + e) * (D / 16) + b] = make_float4(acc[n][b][e], acc[n][b + 1][e], acc[n][b + 2][e], acc[n][b + 3][e]);
+                    *(float4*)&handed[(n * 16 + i) * M::PITCH + (4 * g + e) * (D / 16) + b] = make_float4(acc[n][b][e], acc[n][b + 1][e], acc[n][b + 2][e], acc[n][b + 3][e]);
         }
     __syncthreads();
 #pragma unroll
@@ -307,7 +311,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             const int d0 = (4 * g + e) * (D / 16);
             float x[M::NB];
 #pragma unroll
-            for (int b = 0; b < M::NB; ++b) x[b] = fmaf(handed[n][i][d0 + b], others, acc[n][b][e] * mine) * by;
+            for (int b = 0; b < M::NB; ++b) x[b] = fmaf(handed[(n * 16 + i) * M::PITCH + d0 + b], others, acc[n][b][e] * mine) * by;
             if (span.parts > 1) {
 #pragma unroll
                 for (int b = 0; b < M::NB; ++b) a.part_o[place * D + d0 + b] = x[b];
