@@ -6,7 +6,7 @@
 // LDS, in 64 bits (a far position's angle in 32 bits is off by position * 2^-24), and its waves take heads in turn.
 //
 // A lane holds four neighbouring pairs of a head (a, b apart by `pairs`, or side by side), so a pair never leaves its lane; what is not rotated
-// counts as pairs whose angle is 0. Queries are computed in 32 bits and rounded once. Keys that go to the cache are computed in 64: a value next
+// goes the same way, by pairs that stay as they are. Queries are computed in 32 bits and rounded once. Keys that go to the cache are computed in 64: a value next
 // to the border of two codes would else come out as the other one. They pass through LDS, where a block's 32 values come together.
 //
 // Bound by the rows' bytes; a few tokens by the chain position, angle, rows.
@@ -52,9 +52,10 @@ struct Runs {
     }
 };
 
-// A lane's four pairs, normed and turned. `angle`: their cosines and sines.
+// A lane's four pairs, normed, and turned if they are of the rotation.
 template <typename F, typename T, int D, bool NEIGHBOURS>
-static __device__ __forceinline__ void turn(const T* x, const float* weight, float eps, const Runs& at, const F (&cosine)[VEC], const F (&sine)[VEC], F (&y)[2 * VEC]) {
+static __device__ __forceinline__ void turn(const T* x, const float* weight, float eps, const Runs& at, bool turned, const F (&cosine)[VEC], const F (&sine)[VEC],
+                                            F (&y)[2 * VEC]) {
     const Four<T> lo = *(const Four<T>*)(x + at.lo), hi = *(const Four<T>*)(x + at.hi);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
@@ -75,6 +76,7 @@ static __device__ __forceinline__ void turn(const T* x, const float* weight, flo
             y[VEC + j] = y[VEC + j] * by * (F)wh.v[j];
         }
     }
+    if (!turned) return;   // (not by an angle of 0: beside an infinity that would leave no number)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const int a = NEIGHBOURS ? 2 * j : j, b = NEIGHBOURS ? 2 * j + 1 : VEC + j;
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(WG) void rotate_kernel(Rotate r, int tokens) {
     float cq[VEC], sq[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        const Angle a = u0 < r.pairs ? angles[tok * r.pairs + u0 + j] : Angle{1, 0};
+        const Angle a = u0 < r.pairs ? angles[tok * r.pairs + u0 + j] : Angle{0, 0};
         ck[j] = a.c;
         sk[j] = a.s;
         cq[j] = (float)a.c;
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(WG) void rotate_kernel(Rotate r, int tokens) {
         if (item < of_q) {
             const int head = item * AT_ONCE + sub, from = min(head, r.heads - 1);   // (a whole wave comes to the lane exchanges)
             float y[2 * VEC];
-            turn<float, T, D, NEIGHBOURS>((const T*)r.q + row * r.q_stride + from * D, r.q_weight, r.eps, at, cq, sq, y);
+            turn<float, T, D, NEIGHBOURS>((const T*)r.q + row * r.q_stride + from * D, r.q_weight, r.eps, at, u0 < r.pairs, cq, sq, y);
             if (head < r.heads) {
                 Four<T> lo, hi;
 #pragma unroll
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(WG) void rotate_kernel(Rotate r, int tokens) {
         } else if (item < of_q + of_k) {
             const int head = (item - of_q) * AT_ONCE + sub, from = min(head, r.kv_heads - 1);
             K y[2 * VEC];
-            turn<K, T, D, NEIGHBOURS>((const T*)r.k + row * r.k_stride + from * D, r.k_weight, r.eps, at, ck, sk, y);
+            turn<K, T, D, NEIGHBOURS>((const T*)r.k + row * r.k_stride + from * D, r.k_weight, r.eps, at, u0 < r.pairs, ck, sk, y);
             if constexpr (CACHE) {
                 K* mine = meet[wave] + sub * D;
                 __builtin_amdgcn_wave_barrier();

@@ -149,6 +149,30 @@ def test_far_positions():
 
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("dim,neighbours", [(64, False), (128, True), (256, False)])
+def test_what_is_not_rotated_passes_as_it_is(dim, neighbours, dtype):
+    """Infinities, no numbers and zeros of either sign behind the rotated pairs: each leaves what is beside it alone."""
+    g = np.random.default_rng(dim)
+    x = rows_of(dtype, g, 3, 2, dim)
+    past = x[:, :, dim // 2:]
+    past[:, :, ::7], past[:, :, 1::11], past[:, :, 2::13], past[:, :, 3::17] = float("inf"), float("-inf"), float("nan"), -0.0
+    r = rotary.Rotary(dev(np.linspace(0.1, 1, dim // 4).astype(np.float32)), neighbours=neighbours)
+    d, pos = x.cuda(), dev(np.array([3, 0, 9], np.int32))
+    for got in rotary.rotate(d, d, pos, r):
+        bits = torch.int32 if dtype == "f32" else torch.int16
+        number = ~past.isnan()
+        assert torch.equal(got[:, :, dim // 2:].cpu().view(bits)[number], past.contiguous().view(bits)[number])
+        assert got[:, :, dim // 2:].isnan().cpu().equal(~number)
+    want = ref.Cache(2, 2, 16, dim, seed=1)
+    cache, slots = handle(want), np.array([0, 17, 5])
+    rotary.rotate_into(cache, d, d, d, pos, dev(slots), r)
+    xn = x.double().numpy()
+    keys = np.concatenate([ref.rope(xn[:, :, :dim // 2], pos.cpu().numpy()[None], np.linspace(0.1, 1, dim // 4).astype(np.float32), neighbours=neighbours), xn[:, :, dim // 2:]], -1)
+    want.write(keys, xn, slots)
+    check_cache(cache, want)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("norm", [True, False])
 @pytest.mark.parametrize("rows,heads,kv_heads,dim,pairs,axes,neighbours", CASES)
 def test_rotation_into_the_cache(rows, heads, kv_heads, dim, pairs, axes, neighbours, norm, dtype):
