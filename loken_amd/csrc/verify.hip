@@ -366,7 +366,10 @@ __global__ __launch_bounds__(SAMPLE_WG) void verify_judge_kernel(Verify v) {
         }
         return total;
     };
-    if (t == 0) found = -1;
+    if (t == 0) {
+        found = -1;
+        round_found = 0;   // (shares of a draft that are far below 0 leave sums that wrap, and may leave no round)
+    }
     uint64_t total = find_round();
     if (total == 0 && target.kept.best != 0) {   // nothing is left: p as it is, all of it by this workgroup
         words.draft = nullptr;

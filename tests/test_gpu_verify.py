@@ -132,6 +132,18 @@ def test_rows_with_few_words_or_none():
     assert got[0][:3].tolist() == [-1, -1, -1] and got[1][0] == 0
 
 
+@pytest.mark.parametrize("share", [-1.0, -1e30, float("-inf"), float("inf"), float("nan")])
+def test_shares_that_are_none_leave_the_calls_rows_in_bounds(share):
+    """What a draft that is no distribution gives is not defined, but it is a word or none, and other sequences' are theirs."""
+    d = Drafts([3, 4, 2], 5003, "f32", "f32", [(1.0, 0, 1.0, 0.0), (1.0, 9, 1.0, 0.0)], seed=6)
+    d.uniform[3:6] = 1.0 - 2.0 ** -24
+    want = d.call()
+    d.draft[3:6, 1::2] = share
+    tokens, accepted, _ = d.call()
+    assert 0 <= int(accepted[1]) <= 3 and (tokens >= -1).all() and (tokens < 5003).all()
+    assert torch.equal(tokens[[0, 1, 2, 7, 8]], want[0][[0, 1, 2, 7, 8]]) and torch.equal(accepted[[0, 2]], want[1][[0, 2]])
+
+
 def test_words_outside_the_vocabulary_are_refused():
     for draft in ("f32", None):
         d = Drafts([3, 3, 3], 1000, "f32", draft, seed=8)
