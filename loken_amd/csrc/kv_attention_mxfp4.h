@@ -100,7 +100,7 @@ constexpr int mx_few_rows(bool f32, int head_dim, int max_rows) {
     return f32 && max_rows <= 8 && head_dim < 256 ? 8 : 16;
 }
 // Its waves on a SIMD, for that many rows: two where the registers hold them.
-constexpr int mx_few_on_simd(bool f32, int head_dim, int rows) { return head_dim == 256 || (head_dim == 128 && f32 && rows == 8) ? 1 : 2; }
+constexpr int mx_few_on_simd(bool f32, bool f16, int head_dim, int rows) { return head_dim == 256 && rows == 16 && (f32 || f16) ? 1 : 2; }
 
 // Rows of a workgroup of the many-rows kernel, and its waves on a SIMD.
 constexpr int mx_many_rows(bool f32, int head_dim) { return head_dim == 256 && f32 ? 16 : 32; }

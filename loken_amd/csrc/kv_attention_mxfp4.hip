@@ -82,7 +82,7 @@ extern "C" int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, 
     if (few) {
         af.few_rows = many ? few_max : 0x7FFFFFFF;
         const int64_t groups = (int64_t)seqs * kv_heads * ((few_max - 1) / per + 1);
-        const int slots = cus * mx_few_on_simd(f32, head_dim, per);   // workgroups that run at once
+        const int slots = cus * mx_few_on_simd(f32, f16, head_dim, per);   // workgroups that run at once
         const int64_t most_steps = (int64_t)seqs * ((table_tokens + KV_TILE - 1) / KV_TILE + 1);
         if (seqs > 1 && few_max <= per && groups <= 4 * cus && groups * tiles > 16 * cus && most_steps < 0x7FFFFFFF) {
             af.chunks = (slots + kv_heads - 1) / kv_heads;

@@ -27,7 +27,8 @@ struct Few {
     static constexpr int SHARES = sizeof(T) == 4 ? 3 : 2;                                         // of a weight
     static constexpr int QP = SLOTS == 1 ? PIECES : 1, SP = SLOTS == 1 ? SHARES : 1;              // operands of them
     static constexpr int RPT = 16 / SLOTS, ROWS = RPT * NT, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
-    static constexpr int ON_SIMD = mx_few_on_simd(sizeof(T) == 4, D, ROWS);
+    static constexpr int ON_SIMD = mx_few_on_simd(sizeof(T) == 4, std::is_same<T, __half>::value, D, ROWS);
+    static constexpr bool ONE = ON_SIMD > 1 && (D == 256 || (D == 128 && sizeof(T) == 4 && ROWS > 4));   // buffer of codes
 };
 
 // What the slots of a row have together.
@@ -116,27 +117,30 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
         // (a page's address is the wave's own, a lane's place in a tile always the same)
         const uint32_t key_at = i * (D / 2) + g * (D / 8), key_power_at = i * F::PART + (D == 256 ? 2 * g : D == 64 ? g >> 1 : g);
         const uint32_t value_at = (g * 16 + i) * (D / 8), value_power_at = ((i * F::PART / 16) << shift) + 4 * g;
-        // A step's codes and powers. Two of them: the next step's are loaded while this one's are at work.
+        // A step's codes and powers. Where registers hold two of them the next step's are loaded while this one's are at work, else its keys once this
+        // one's scores are there and its values behind this one's products.
         struct Loaded {
             MxWords<F::W> k[4], v[4];
             uint32_t kp[4], vp[4];   // powers: of the lane's block or two of a key; of four tokens' values
-        } loaded[2];
+        } loaded[F::ONE ? 1 : 2];
         const uint8_t *keys = a.mx.k + key_at, *key_powers = a.mx.k_powers + key_power_at, *values = a.mx.v + value_at, *value_powers = a.mx.v_powers + value_power_at;
-        auto load = [&](Loaded& into, int t, const int (&pages)[4]) {
-            int64_t page[4], tok[4];   // a page's tokens among all, and a tile's: rows of either side are as long
+        // a page's tokens among all: rows of either side are as long
+        auto tokens_before = [&](int page) { return ((int64_t)((unsigned)page < (unsigned)a.mx.pages ? page : 0) * a.mx.heads + kv) << shift; };
+        auto load_keys = [&](Loaded& into, int t, const int (&pages)[4]) {
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const int p = (unsigned)pages[b] < (unsigned)a.mx.pages ? pages[b] : 0;
-                page[b] = ((int64_t)p * a.mx.heads + kv) << shift;
-                tok[b] = page[b] + (at_tile(t, b) & ((1 << shift) - 1));
-                into.k[b] = *(const MxWords<F::W>*)(keys + tok[b] * (D / 2));
-                if (D == 256) into.kp[b] = *(const uint16_t*)(key_powers + tok[b] * F::PART);
-                else into.kp[b] = key_powers[tok[b] * F::PART];
+                const int64_t tok = tokens_before(pages[b]) + (at_tile(t, b) & ((1 << shift) - 1));
+                into.k[b] = *(const MxWords<F::W>*)(keys + tok * (D / 2));
+                if (D == 256) into.kp[b] = *(const uint16_t*)(key_powers + tok * F::PART);
+                else into.kp[b] = key_powers[tok * F::PART];
             }
+        };
+        auto load_values = [&](Loaded& into, int t, const int (&pages)[4]) {
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                into.v[b] = *(const MxWords<F::W>*)(values + tok[b] * (D / 2));
-                into.vp[b] = *(const uint32_t*)(value_powers + page[b] * (F::PART - 1) + tok[b]);
+                const int64_t page = tokens_before(pages[b]), tok = page + (at_tile(t, b) & ((1 << shift) - 1));
+                into.v[b] = *(const MxWords<F::W>*)(values + tok * (D / 2));
+                into.vp[b] = *(const uint32_t*)(value_powers + page * (F::PART - 1) + tok);
             }
         };
         int t = t_begin + wave;
@@ -146,7 +150,8 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             for (int b = 0; b < 4; ++b) pages[b] = page_of(t, b);
 #pragma unroll
             for (int b = 0; b < 4; ++b) next[b] = page_of(t + WAVES, b);
-            load(loaded[0], t, pages);
+            load_keys(loaded[0], t, pages);
+            load_values(loaded[0], t, pages);
         }
 
         const float capped = CAP ? a.scale / a.cap : 0.f;   // what a product is under the tanh
@@ -218,7 +223,10 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
                 behind[b] = page_of(t + 2 * WAVES, b);
                 absent |= (unsigned)pages[b] < (unsigned)a.mx.pages ? 0 : 1 << b;
             }
-            load(then, t + WAVES, next);
+            if (!F::ONE) {
+                load_keys(then, t + WAVES, next);
+                load_values(then, t + WAVES, next);
+            }
             // whether every row sees every position of the step
             const bool whole = p0 + KV_TILE - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && absent == 0;
             v4f sc[NT][4];
@@ -239,6 +247,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
 #pragma unroll
                 for (int n = 0; n < NT; ++n) sc[n][b] = c[n];
             }
+            if (F::ONE) load_keys(then, t + WAVES, next);
             uint32_t share[NT][F::SP][4][2];   // weights: of a tile's four positions
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -358,6 +367,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
                         }
                 }
             }
+            if (F::ONE) load_values(then, t + WAVES, next);
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 pages[b] = next[b];
@@ -366,8 +376,8 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             t += WAVES;
         };
         while (t < t_end) {
-            step(loaded[0], loaded[1]);
-            if (t < t_end) step(loaded[1], loaded[0]);
+            step(loaded[0], loaded[F::ONE ? 0 : 1]);
+            if (!F::ONE && t < t_end) step(loaded[F::ONE ? 0 : 1], loaded[0]);
         }
 
         // the slots' sums, and the four waves' relative to their common maximum, an operand's rows at a time
