@@ -99,10 +99,12 @@ constexpr int mx_few_rows(bool f32, int head_dim, int max_rows) {
     if (max_rows <= (f32 ? 4 : 8)) return f32 ? 4 : 8;
     return f32 && max_rows <= 8 && head_dim < 256 ? 8 : 16;
 }
-// Its waves on a SIMD, for that many rows: two where the registers hold them.
-constexpr int mx_few_on_simd(bool f32, bool f16, int head_dim, int rows) { return head_dim == 256 && rows == 16 && (f32 || f16) ? 1 : 2; }
+// Its waves on a SIMD, for that many rows: as many as the registers hold. Heads of 128 in three with one buffer of codes, for two with two: 64 sequences of up
+// to 2000 tokens in pieces, bf16, 49 to 40 us, 131072 tokens of one the same; f32 of more than four rows two for one, 64 x 2 rows 90 to 73 us.
+constexpr int mx_few_on_simd(bool f32, bool f16, int head_dim, int rows) { return head_dim == 256 && rows == 16 && (f32 || f16) ? 1 : head_dim == 128 && rows < 16 && !(f32 && rows > 4) ? 3 : 2; }
 
-// Rows of a workgroup of the many-rows kernel, and its waves on a SIMD.
+// Rows of a workgroup of the many-rows kernel, and its waves on a SIMD, as the registers hold them. (Heads of 256 in two spill: 300 rows of two sequences
+// behind 1000 42 us for 37.)
 constexpr int mx_many_rows(bool f32, int head_dim) { return head_dim == 256 && f32 ? 16 : 32; }
 constexpr int mx_many_on_simd(bool f32, bool f16, int head_dim) {
     return head_dim == 64 ? (f32 || f16 ? 3 : 4) : head_dim == 128 ? (f32 || f16 ? 2 : 3) : 1;

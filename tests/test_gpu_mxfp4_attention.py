@@ -124,6 +124,15 @@ def test_long_contexts(lens, fresh, dtype):
 
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("heads,kv_heads,dim,fresh,window", [(8, 4, 128, [1] * 8, 0), (4, 4, 256, [1, 1, 3, 0, 1, 2, 1, 1], 0), (16, 4, 64, [1, 1, 2, 1, 0, 1, 2, 1], 1500), (4, 4, 64, [1, 1, 1, 60, 1, 1, 1, 1], 0)])
+def test_pieces_of_a_batch(heads, kv_heads, dim, fresh, window, dtype):
+    """A table that is wide enough for long contexts, by which the batch is cut into pieces of equal lengths, and sequences that begin and end in them."""
+    b = Batch([4000, 1, 2700, 900, 9, 700, 4100, 130], fresh, heads, kv_heads, dim, 16, dtype, seed=7, pad=2)
+    b.table = np.concatenate([b.table, np.full((8, 4000 - b.table.shape[1]), -1, np.int32)], 1)
+    b.check(max_len=64000, window=window)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("fresh", [1, 3, 70])
 def test_absent_pages(fresh, dtype):
     b = Batch([200, 100, 700], [fresh] * 3, 4, 2, 128, 16, dtype, seed=fresh)
