@@ -9,7 +9,8 @@
 // goes the same way, by pairs that stay as they are. Queries are computed in 32 bits and rounded once. Keys that go to the cache are computed in 64: a value next
 // to the border of two codes would else come out as the other one. They pass through LDS, where a block's 32 values come together.
 //
-// Bound by the rows' bytes; a few tokens by the chain position, angle, rows.
+// Bound by the rows' bytes: 4096 tokens of 32 + 8 heads of 128, bf16, three axes of positions 16.9 us, 5.0 TB/s in and out. Into the cache by the 64-bit norms and
+// rotations too: 2048 tokens of 32 + 8 + 8 heads, bf16, 14.5 us; a few tokens by the chain position, angle, rows: one token 3.1 us.
 
 #include <type_traits>
 
@@ -86,13 +87,14 @@ static __device__ __forceinline__ void turn(const T* x, const float* weight, flo
     }
 }
 
-// `tokens` (1 or WAVES) to a workgroup: one whose heads the waves share, or one a wave.
+// `tokens` to a workgroup: one whose heads the waves share, or, into the cache, WAVES of them, one a wave.
 template <typename T, int D, bool NEIGHBOURS, bool CACHE>
-__global__ __launch_bounds__(WG) void rotate_kernel(Rotate r, int tokens) {
+__global__ __launch_bounds__(WG) void rotate_kernel(Rotate r, int tokens_of) {
+    const int tokens = CACHE ? tokens_of : 1;
     constexpr int LANES = D / 2 / VEC, AT_ONCE = 64 / LANES;   // lanes of a head, heads of a wave
     using K = typename std::conditional<CACHE, double, float>::type;
     struct Angle { K c, s; };
-    __shared__ Angle angles[WAVES * D / 2];
+    __shared__ Angle angles[(CACHE ? WAVES : 1) * D / 2];
     __shared__ K meet[CACHE ? WAVES : 1][CACHE ? AT_ONCE * D : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row0 = blockIdx.x * tokens;
@@ -177,8 +179,10 @@ __global__ __launch_bounds__(WG) void rotate_kernel(Rotate r, int tokens) {
 
 template <typename T, int D, bool CACHE>
 static int launch_of(const Rotate& r, bool neighbours, hipStream_t s) {
-    // A token's heads over four waves while that leaves CUs with fewer than four workgroups, else a token a wave, whose angles are made side by side
-    const int tokens = r.rows > 4 * lk_device().cus ? WAVES : 1;
+    // A token's heads over four waves, but into the cache, whose angles in 64 bits take long, a token a wave once each CU has more than eight tokens: their
+    // angles are made side by side. 32 + 8 heads of 128, bf16: 4096 tokens into the cache 30.0 us in fours of waves, 27.1 a token a wave, 2048 17.6 and 18.8;
+    // without the cache 4096 16.7 and 17.5, 1024 7.6 and 11.5.
+    const int tokens = CACHE && r.rows > 8 * lk_device().cus ? WAVES : 1;
     const dim3 grid((unsigned)((r.rows + tokens - 1) / tokens)), threads(WG);
     if (neighbours) hipLaunchKernelGGL((rotate_kernel<T, D, true, CACHE>), grid, threads, 0, s, r, tokens);
     else hipLaunchKernelGGL((rotate_kernel<T, D, false, CACHE>), grid, threads, 0, s, r, tokens);

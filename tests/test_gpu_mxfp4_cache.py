@@ -199,6 +199,12 @@ def test_rotation_into_the_cache(rows, heads, kv_heads, dim, pairs, axes, neighb
     check_cache(cache, want)
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,pairs,axes,neighbours", [(2051, 3, 1, 64, 32, 1, False), (4097, 1, 1, 128, 32, 3, True), (2222, 2, 3, 256, 128, 2, False)])
+def test_many_rows_into_the_cache(rows, heads, kv_heads, dim, pairs, axes, neighbours, dtype):
+    test_rotation_into_the_cache(rows, heads, kv_heads, dim, pairs, axes, neighbours, True, dtype)
+
+
 def test_recorded_rows_go_where_the_slots_say():
     """Replays with other rows, positions and slots, and eager work between them."""
     g = np.random.default_rng(8)
