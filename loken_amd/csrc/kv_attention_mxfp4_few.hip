@@ -388,9 +388,9 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
         // the slots' sums, and the four waves' relative to their common maximum, an operand's rows at a time
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float lw = sum_over_groups(l[n]);
+            l[n] = sum_over_groups(l[n]);
             m[n] = m[n] == -INFINITY ? m[n] : base[n];
-            if (g == 0 && slot == 0) { tops[wave][n * F::RPT + i / SLOTS] = m[n]; weights[wave][n * F::RPT + i / SLOTS] = lw; }
+            if (g == 0 && slot == 0) tops[wave][n * F::RPT + i / SLOTS] = m[n];
             if (SLOTS > 1) {
 #pragma unroll
                 for (int b = 0; b < F::NB; ++b)
@@ -407,6 +407,8 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             const float f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
             // column of the sums: the lane's rows 4 g + e of the operand are sixteenths of the head
             if (slot == 0) {
+                // (a part whose scores are no numbers has a sum that is none, and may have no maximum)
+                if (g == 0) weights[wave][r] = m[n] == -INFINITY ? l[n] : l[n] * f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -415,13 +417,11 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             __syncthreads();
             for (int at = threadIdx.x; at < min(r1 - r0 + 1 - n * F::RPT, F::RPT) * D; at += 64 * WAVES) {
                 const int rr = at / D, d = at % D, row_of = n * F::RPT + rr;
-                const float most = fmaxf(fmaxf(tops[0][row_of], tops[1][row_of]), fmaxf(tops[2][row_of], tops[3][row_of]));
                 float total = 0.f, lw = 0.f;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) {
                     total += sums[w][rr][d];
-                    // (a part whose scores are no numbers has a sum that is none, and may have no maximum)
-                    lw += tops[w][row_of] == -INFINITY ? weights[w][row_of] : weights[w][row_of] * __builtin_amdgcn_exp2f(tops[w][row_of] - most);
+                    lw += weights[w][row_of];
                 }
                 const int of_seq = a.token_of(r0 + row_of), head = kv * a.group + r0 + row_of - of_seq * a.group;
                 const int64_t row = s.first + of_seq;
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
                 } else {
                     const int64_t place = a.chunks ? to + row_of : (a.part_row(seq, s, (int)row) * a.heads + head) * a.splits + part;
                     a.part_o[place * D + d] = total;
-                    if (d == 0) a.part_ml[place] = make_float2(most, lw);
+                    if (d == 0) a.part_ml[place] = make_float2(fmaxf(fmaxf(tops[0][row_of], tops[1][row_of]), fmaxf(tops[2][row_of], tops[3][row_of])), lw);
                 }
             }
         }
