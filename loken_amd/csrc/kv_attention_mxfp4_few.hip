@@ -159,7 +159,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             load_values(loaded[0], t, pages);
         }
 
-        const float capped = CAP ? a.scale / a.cap : 0.f;   // what a product is under the tanh
+        const float under = CAP ? mx_under<sizeof(T) == 4>(a.scale, a.cap) : 0.f;
         // the rows' pieces, and what a product, or its tanh, is in powers of two
         mx_b8 q[NT][F::KS][F::QP];
         float unit[NT];
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             }
             const uint64_t odd = __ballot(!finite);
             finite = (odd >> i & 0x0001000100010001ull) == 0;
-            unit[n] = finite ? (CAP ? a.cap : a.scale) * 1.4426950408889634f : NAN;
+            unit[n] = finite ? (CAP ? mx_unit<sizeof(T) == 4>(a.cap) : a.scale) * 1.4426950408889634f : NAN;
         }
         int pos_least = 0x7FFFFFFF, pos_most = -1;
 #pragma unroll
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
                 for (int e = 0; e < 16; ++e) x[e] = sum_of_slots<SLOTS>(sc[n][e >> 2][e & 3]);
                 if (CAP) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = mx_tanh<sizeof(T) == 4>(x[e] * capped);
+                    for (int e = 0; e < 16; ++e) x[e] = mx_tanh<sizeof(T) == 4>(x[e], under);
                 }
                 if (!whole) {
                     asm volatile("");   // (stays a branch: the looks at sixteen positions would else be made in every step)

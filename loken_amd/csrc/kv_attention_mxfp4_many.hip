@@ -102,7 +102,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
         load_values(t, pages);
     }
 
-    const float capped = CAP ? a.scale / a.cap : 0.f;   // what a product is under the tanh
+    const float under = CAP ? mx_under<M::FINE>(a.scale, a.cap) : 0.f;
     // The rows' pieces as operands, in LDS, each wave half of them; and what a product, or its tanh, is in powers of two.
     uint4* const queries = lds;
     float unit[M::NT];
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             for (int p = 0; p < M::QP; ++p) queries[((n * M::KS + ks) * M::QP + p) * 64 + lane] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
         }
         const uint64_t odd = __ballot(!finite);
-        if (g == 0) units[16 * n + i] = (odd >> i & 0x0001000100010001ull) == 0 ? (CAP ? a.cap : a.scale) * 1.4426950408889634f : NAN;
+        if (g == 0) units[16 * n + i] = (odd >> i & 0x0001000100010001ull) == 0 ? (CAP ? mx_unit<M::FINE>(a.cap) : a.scale) * 1.4426950408889634f : NAN;
     }
     __syncthreads();
 #pragma unroll
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             for (int e = 0; e < 4 * TILES; ++e) x[e] = sc[n][e >> 2][e & 3];
             if (CAP) {
 #pragma unroll
-                for (int e = 0; e < 4 * TILES; ++e) x[e] = mx_tanh<M::FINE>(x[e] * capped);
+                for (int e = 0; e < 4 * TILES; ++e) x[e] = mx_tanh<M::FINE>(x[e], under);
             }
             if (!whole) {
                 asm volatile("");   // (stays a branch: the looks at eight positions would else be made in every step)
