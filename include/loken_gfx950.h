@@ -897,7 +897,7 @@ int lk_qk_norm_rope_kv_mxfp4(const void* q, const void* k, const void* v, int ty
                              int page_tokens, int pages, void* k_codes, void* v_codes, void* k_powers, void* v_powers, void* stream);
 
 /* Attention of the batch's rows over the 4-bit cache: lk_kv_attention_q8's arguments, rows, masks, absent pages and limits, and
- *   cap > 0: scores are cap * tanh(scale * q . k / cap) before the softmax   (0: as they are)
+ *   cap > 0: scores are cap * tanh(scale * q . k / cap) before the softmax   (0: as they are; else 2^-64 .. 2^64)
  * Powers below 31 and above 252, which nothing here writes, are not defined at positions that some row sees. Products are exact but for the softmax weights, which
  * are held to 24 bits in f32 and 16 in f16 and bf16 (8 where bf16 comes in many rows of a sequence); sums are f32. A query value keeps all its bits down to 2^-126. A product of a
  * row and a key, and a sum of weights times values, have to be numbers of f32. Scratch as for lk_kv_attention_q8. */

@@ -44,18 +44,20 @@ static __device__ __forceinline__ void mx_pieces(float a, float b, uint32_t (&ou
     }
 }
 
-// What a capped score is made of, from a product and what it is under the tanh, mx_under: tanh x = 1 - 2 / (e^2x + 1). A softmax does not see the 1: but for f32
-// it is -1 / (e^2x + 1), whose unit, mx_unit, is twice the cap. f32: the tanh, off by 1.2e-7; below a quarter by its series: to a few last places of x.
-template <bool FINE>
-static __device__ __forceinline__ float mx_under(float scale, float cap) { return scale / cap * (FINE ? 1.f : 2.8853900817779268f); }
-template <bool FINE>
-static __device__ __forceinline__ float mx_unit(float cap) { return FINE ? cap : 2.f * cap; }
-template <bool FINE>
+// What a capped score is made of, from a product and what it is under the tanh, mx_under: tanh x = 1 - 2 / (e^2x + 1). A softmax does not see the 1: MX_NEAR leaves it
+// off, -1 / (e^2x + 1), whose unit, mx_unit, is twice the cap. A score is then off by cap * 2^-23: for f16 and bf16 with caps up to 64, where that is below what their
+// weights are held to. MX_FAR: the tanh, off by 1.2e-7; below a quarter by its series, to a few last places of x.
+enum MxCap { MX_NONE, MX_NEAR, MX_FAR };
+static inline int mx_cap_of(float cap, bool f32) { return !(cap > 0.f) ? MX_NONE : f32 || cap > 64.f ? MX_FAR : MX_NEAR; }
+template <int CAP>
+static __device__ __forceinline__ float mx_under(float scale, float cap) { return CAP == MX_NONE ? 0.f : scale / cap * (CAP == MX_NEAR ? 2.8853900817779268f : 1.f); }
+template <int CAP>
+static __device__ __forceinline__ float mx_unit(float scale, float cap) { return (CAP == MX_NONE ? scale : CAP == MX_NEAR ? 2.f * cap : cap) * 1.4426950408889634f; }
+template <int CAP>
 static __device__ __forceinline__ float mx_tanh(float product, float under) {
     const float x = product * under;
-    if (!FINE) return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x));
-    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.8853900817779268f) + 1.f);
-    const float s = x * x;
+    if (CAP == MX_NEAR) return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x));
+    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.8853900817779268f) + 1.f), s = x * x;
     const float near = fmaf(x * s, fmaf(s, fmaf(s, fmaf(s, 0.021869488f, -0.053968254f), 0.13333334f), -0.33333334f), x);
     return fabsf(x) < 0.25f ? near : far;
 }

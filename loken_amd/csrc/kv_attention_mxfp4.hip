@@ -49,7 +49,7 @@ extern "C" int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, 
     if (!size) return LK_ERR_TYPE;
     if (!mx_pool_ok(k_codes, v_codes, k_powers, v_powers, pages, kv_heads, head_dim, page_tokens)) return LK_ERR_ARG;
     if (seqs < 0 || rows < 0 || max_fresh < 0 || max_len < 0 || table_cols < 0 || table_stride < table_cols || window < 0 ||
-        !(scale > 0.0f && scale <= 3.402823466e38f) || !(cap >= 0.0f && cap <= 3.402823466e38f) || heads <= 0 || heads > 65535 || heads % kv_heads != 0)
+        !(scale > 0.0f && scale <= 3.402823466e38f) || !(cap == 0.0f || (cap >= 5.421010862e-20f && cap <= 1.8446744074e19f)) || heads <= 0 || heads > 65535 || heads % kv_heads != 0)
         return LK_ERR_ARG;
     if (seqs == 0 || rows == 0) return LK_OK;
     const int64_t row = (int64_t)heads * head_dim;

@@ -44,8 +44,8 @@ static __device__ __forceinline__ float sum_of_slots(float v) {
     return v;
 }
 
-// CAP: whether scores are capped (as a branch at run time the compiler takes the tanh always, and the result where it is asked for)
-template <typename T, int D, int NT, int SLOTS, bool CAP>
+// CAP: whether and how scores are capped (as a branch at run time the compiler takes the tanh always, and the result where it is asked for)
+template <typename T, int D, int NT, int SLOTS, int CAP>
 __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void mx_few_kernel(AttendMx a, int row_tiles) {
     using F = Few<T, D, NT, SLOTS>;
     __shared__ float sums[WAVES][F::RPT][D + 4];
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             load_values(loaded[0], t, pages);
         }
 
-        const float under = CAP ? mx_under<sizeof(T) == 4>(a.scale, a.cap) : 0.f;
+        const float under = mx_under<CAP>(a.scale, a.cap);
         // the rows' pieces, and what a product, or its tanh, is in powers of two
         mx_b8 q[NT][F::KS][F::QP];
         float unit[NT];
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             }
             const uint64_t odd = __ballot(!finite);
             finite = (odd >> i & 0x0001000100010001ull) == 0;
-            unit[n] = finite ? (CAP ? mx_unit<sizeof(T) == 4>(a.cap) : a.scale) * 1.4426950408889634f : NAN;
+            unit[n] = finite ? mx_unit<CAP>(a.scale, a.cap) : NAN;
         }
         int pos_least = 0x7FFFFFFF, pos_most = -1;
 #pragma unroll
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
                 for (int e = 0; e < 16; ++e) x[e] = sum_of_slots<SLOTS>(sc[n][e >> 2][e & 3]);
                 if (CAP) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = mx_tanh<sizeof(T) == 4>(x[e], under);
+                    for (int e = 0; e < 16; ++e) x[e] = mx_tanh<CAP>(x[e], under);
                 }
                 if (!whole) {
                     asm volatile("");   // (stays a branch: the looks at sixteen positions would else be made in every step)
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
     }
 }
 
-template <typename T, int D, bool CAP>
+template <typename T, int D, int CAP>
 static int launch(const AttendMx& a, int max_rows, hipStream_t s) {
     constexpr int SLOTS = sizeof(T) == 4 ? 4 : 2;
     const int per = mx_few_rows(sizeof(T) == 4, D, max_rows), row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / per + 1;
@@ -458,7 +458,10 @@ static int launch(const AttendMx& a, int max_rows, hipStream_t s) {
 
 template <typename T, int D>
 static int by_cap(const AttendMx& a, int max_rows, hipStream_t s) {
-    return a.cap > 0.f ? launch<T, D, true>(a, max_rows, s) : launch<T, D, false>(a, max_rows, s);
+    const int cap = mx_cap_of(a.cap, sizeof(T) == 4);
+    if constexpr (sizeof(T) == 2)
+        if (cap == MX_NEAR) return launch<T, D, MX_NEAR>(a, max_rows, s);
+    return cap == MX_FAR ? launch<T, D, MX_FAR>(a, max_rows, s) : launch<T, D, MX_NONE>(a, max_rows, s);
 }
 
 template <typename T>

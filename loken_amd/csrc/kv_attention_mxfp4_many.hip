@@ -32,8 +32,8 @@ struct Many {
     static constexpr int QUERIES = NT * KS * QP * 64 * 16, HANDED = NT * 16 * PITCH * 4, LDS = QUERIES > HANDED ? QUERIES : HANDED;
 };
 
-// CAP: whether scores are capped (as a branch at run time the compiler takes the tanh always, and the result where it is asked for)
-template <typename T, int D, bool CAP>
+// CAP: whether and how scores are capped (as a branch at run time the compiler takes the tanh always, and the result where it is asked for)
+template <typename T, int D, int CAP>
 __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof(T) == 2 && std::is_same<T, __half>::value, D))) void mx_many_kernel(AttendMx a) {
     using M = Many<T, D>;
     __shared__ uint4 lds[M::LDS / 16];   // the rows' operands, in the end half of the sums on their way to the other wave
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
         load_values(t, pages);
     }
 
-    const float under = CAP ? mx_under<M::FINE>(a.scale, a.cap) : 0.f;
+    const float under = mx_under<CAP>(a.scale, a.cap);
     // The rows' pieces as operands, in LDS, each wave half of them; and what a product, or its tanh, is in powers of two.
     uint4* const queries = lds;
     float unit[M::NT];
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             for (int p = 0; p < M::QP; ++p) queries[((n * M::KS + ks) * M::QP + p) * 64 + lane] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
         }
         const uint64_t odd = __ballot(!finite);
-        if (g == 0) units[16 * n + i] = (odd >> i & 0x0001000100010001ull) == 0 ? (CAP ? mx_unit<M::FINE>(a.cap) : a.scale) * 1.4426950408889634f : NAN;
+        if (g == 0) units[16 * n + i] = (odd >> i & 0x0001000100010001ull) == 0 ? mx_unit<CAP>(a.scale, a.cap) : NAN;
     }
     __syncthreads();
 #pragma unroll
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
             for (int e = 0; e < 4 * TILES; ++e) x[e] = sc[n][e >> 2][e & 3];
             if (CAP) {
 #pragma unroll
-                for (int e = 0; e < 4 * TILES; ++e) x[e] = mx_tanh<M::FINE>(x[e], under);
+                for (int e = 0; e < 4 * TILES; ++e) x[e] = mx_tanh<CAP>(x[e], under);
             }
             if (!whole) {
                 asm volatile("");   // (stays a branch: the looks at eight positions would else be made in every step)
@@ -338,8 +338,15 @@ template <typename T, int D>
 static int launch(const AttendMx& a, hipStream_t s) {
     const int64_t tiles = ((int64_t)a.rows * a.group + Many<T, D>::ROWS - 1) / Many<T, D>::ROWS + a.seqs, blocks = tiles * a.mx.heads * a.splits;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
-    if (a.cap > 0.f) hipLaunchKernelGGL((mx_many_kernel<T, D, true>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a);
-    else hipLaunchKernelGGL((mx_many_kernel<T, D, false>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, a);
+    const dim3 grid((unsigned)blocks), threads(64 * WAVES);
+    const int cap = mx_cap_of(a.cap, sizeof(T) == 4);
+    if constexpr (sizeof(T) == 2)
+        if (cap == MX_NEAR) {
+            hipLaunchKernelGGL((mx_many_kernel<T, D, MX_NEAR>), grid, threads, 0, s, a);
+            return lk_launch_status();
+        }
+    if (cap == MX_FAR) hipLaunchKernelGGL((mx_many_kernel<T, D, MX_FAR>), grid, threads, 0, s, a);
+    else hipLaunchKernelGGL((mx_many_kernel<T, D, MX_NONE>), grid, threads, 0, s, a);
     return lk_launch_status();
 }
 

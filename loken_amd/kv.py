@@ -236,7 +236,7 @@ def kv_attention(q: torch.Tensor, cache: KvCacheQ8 | KvCacheMxfp4, table: torch.
                  out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the rows ``q`` ``[rows, heads, head_dim]`` over the cache, causal, each sequence's rows being its last positions;
     ``window`` > 0: that many positions, the row's own among them. Rows behind the last sequence stay as they are in ``out``
-    (without one: zeros). ``softcap`` > 0 (the 4-bit cache alone): scores are softcap * tanh(score / softcap). ``max_fresh``, ``max_len``: the most rows and tokens of a sequence as far as the caller knows them."""
+    (without one: zeros). ``softcap`` > 0 (the 4-bit cache alone, 2^-64 to 2^64): scores are softcap * tanh(score / softcap). ``max_fresh``, ``max_len``: the most rows and tokens of a sequence as far as the caller knows them."""
     seqs = lens.numel()
     rows, heads, stride = _rows("kv_attention", "q", q, None, cache.head_dim)
     if heads == 0 or heads % cache.kv_heads:
@@ -250,8 +250,8 @@ def kv_attention(q: torch.Tensor, cache: KvCacheQ8 | KvCacheMxfp4, table: torch.
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError("kv_attention: the scale is a number above zero")
     in_4_bits = isinstance(cache, KvCacheMxfp4)
-    if not (softcap >= 0.0 and math.isfinite(softcap)) or (softcap and not in_4_bits):
-        raise ValueError("kv_attention: softcap is a number from zero on, and zero over the 8-bit cache")
+    if softcap and (not in_4_bits or not 2.0 ** -64 <= softcap <= 2.0 ** 64):
+        raise ValueError("kv_attention: softcap is zero, or 2^-64 to 2^64 over the 4-bit cache")
     if out is None:
         out = torch.zeros((rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
     of_out, _, out_stride = _rows("kv_attention", "out", out, heads, cache.head_dim)

@@ -103,6 +103,28 @@ def test_capped_scores(cap, scale, dtype):
     Batch([1, 70, 500, 260], [1, 4, 3, 90], 4, 2, 128, 16, dtype, seed=int(cap) & 255).check(cap=cap, scale=scale)
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("fresh", [1, 40])
+@pytest.mark.parametrize("cap", [1e4, 1e9])
+def test_a_cap_far_above_the_scores(cap, fresh, dtype):
+    """cap tanh(s / cap) is s but for s^3 / (3 cap^2): what is asked of the scores as they are, of scores up to 30."""
+    b = Batch([300, 77], [fresh, fresh], 4, 2, 64, 16, dtype, seed=11)
+    plain = b.check().double()
+    at = b.q.cuda(), b.cache(), i32(b.table), i32(b.lens), i32(b.starts)
+    got = kv.kv_attention(*at, max_fresh=fresh, max_len=300, softcap=cap).double()
+    want, reach, most = ref.attention(b.q.double().numpy(), b.want, b.table, b.lens, b.starts, 0.125, 0, 0.0, np.zeros(b.q.shape))
+    assert reach.max() < 600
+    # the bound of the scores as they are for either, and 8 half steps of a score more for the cap's product, series and product; s^3 / (3 cap^2) of a
+    # score of 30 is below 1e-4 at 1e4
+    fine, length = dtype == "f32", 300
+    score = (3 * 64 + 6 + 8) * 2.0 ** -24 * reach + 30.0 ** 3 / (3 * cap ** 2)
+    bound = most * (2 * score + 4 * 2.0 ** -22 + 2 * length * 2.0 ** -24 + (2.0 ** -24 if fine else 2.0 ** -9 if dtype == "bf16" else 2.0 ** -17))
+    step = 2.0 ** -24 if fine else torch.finfo(TYPES[dtype]).eps / 2
+    for out in (plain, got):
+        off = np.abs(out.cpu().numpy() - want) - step * np.abs(want) - bound[..., None]
+        assert (off <= 0).all(), off.max()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("hint", [(0, 0), (1, 1), (1, 100000), (5000, 1), (5000, 100000)])
 def test_sizes_given_are_hints(hint, dtype):

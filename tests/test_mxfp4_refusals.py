@@ -76,6 +76,14 @@ def test_attention(change, status):
     assert call("lk_kv_attention_mxfp4", ATTEND, change) == status
 
 
+@pytest.mark.parametrize("cap", [2.0 ** -65, 2.0 ** 65, 1e-40, 3e38])
+def test_caps_that_leave_no_scores(cap):
+    assert call("lk_kv_attention_mxfp4", ATTEND, dict(cap=cap)) == ARG
+    with pytest.raises(ValueError, match="softcap"):
+        kv.kv_attention(torch.zeros((2, 6, 64)), cache(), torch.zeros((1, 4), dtype=torch.int32), torch.tensor([5], dtype=torch.int32), torch.tensor([0, 2], dtype=torch.int32),
+                        max_fresh=2, max_len=5, softcap=cap)
+
+
 JUDGE = dict(logits=P, type=0, stride=1000, rows=5, vocab=1000, drafted=P, starts=P, seqs=2, draft=P, draft_type=0, draft_stride=1000, uniform=P, draw=P,
              temperature=P, top_k=None, top_p=None, min_p=None, tokens=P, accepted=P, probs=P, stream=None)
 
