@@ -91,6 +91,25 @@ def test_a_few_tokens_a_sequence(n, dtype):
     Batch([n, 100, 64 + n], [n, n, n], 4, 2, 128, 16, dtype, seed=n).check()
 
 
+@pytest.mark.parametrize("fresh", [1, 20])
+def test_pages_behind_32_bit_offsets(fresh):
+    """The same pages of a small cache and of one whose codes pass 2^32 bytes: the same rows, bit for bit."""
+    b = Batch([700, 300], [fresh, fresh], 4, 2, 256, 256, "bf16", seed=3)
+    small = b.cache()
+    at = b.q.cuda(), i32(b.lens), i32(b.starts)
+    want = kv.kv_attention(at[0], small, i32(b.table), *at[1:], max_fresh=fresh, max_len=700)
+    pages = (1 << 32) // (2 * 256 * 128) + small.pages
+    large = kv.KvCacheMxfp4.empty(pages, 2, 256, 256)
+    to = torch.arange(pages - small.pages, pages, device="cuda")
+    to[0] = 1
+    for into, of in zip((large.k, large.v, large.k_powers, large.v_powers), (small.k, small.v, small.k_powers, small.v_powers)):
+        into[to] = of
+    assert large.k[int(to[1]):].data_ptr() - large.k.data_ptr() >= 1 << 32
+    table = np.where(b.table >= 0, to.cpu().numpy()[np.maximum(b.table, 0)], -1).astype(np.int32)
+    got = kv.kv_attention(at[0], large, i32(table), *at[1:], max_fresh=fresh, max_len=700)
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("window", [1, 2, 16, 17, 63, 64, 100, 1000, 0x7FFFFFFF])
 def test_windows(window, dtype):

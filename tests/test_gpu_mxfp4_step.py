@@ -189,3 +189,30 @@ def test_the_measured_step_over_the_4_bit_cache(batch, context, drafts, capsys):
         assert ((between.accepted >= 0) & (between.accepted <= drafts)).all()
         first = p.starts[:-1].long() + between.accepted
         assert (between.tokens[first] >= 0).all() and (between.probs[first] > 0).all()
+
+
+def test_two_streams_at_once():
+    """Cut contexts, prompts and checks of drafts whose workspaces are their stream's, in turn on two streams."""
+    from test_gpu_mxfp4_attention import Batch
+    from test_gpu_verify import Drafts
+    calls = []
+    for seed, lens, fresh, heads in ((1, [9000, 40], [1, 1], (8, 2)), (2, [600, 900, 70], [90, 300, 2], (4, 4)), (3, [5000], [4], (4, 1))):
+        b = Batch(lens, fresh, *heads, 128, 16, "bf16", seed=seed)
+        at = b.q.cuda(), b.cache(), i32(b.table), i32(b.lens), i32(b.starts)
+        calls.append(lambda at=at, fresh=fresh, lens=lens: kv.kv_attention(*at, max_fresh=max(fresh), max_len=max(lens)))
+        d = Drafts([5, 1, 3], 20011, seed=seed)
+        given = dict(logits=d.logits.cuda(), drafted=dev(d.drafted), starts=dev(d.starts), uniform=dev(d.uniform), draw=dev(d.draw), temperature=dev(d.temperature),
+                     top_k=dev(d.top_k), top_p=dev(d.top_p), min_p=dev(d.min_p), draft=d.draft.cuda())
+        calls.append(lambda given=given: torch.cat([t.double() for t in sampling.verify(**given)]))
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    sides, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for turn in range(3):
+        for i in range(len(calls)):
+            for j, side in enumerate(sides):
+                with torch.cuda.stream(side):
+                    at = (i + j * (turn + 1)) % len(calls)
+                    got.append((at, calls[at]()))
+    torch.cuda.synchronize()
+    for at, out in got:
+        assert torch.equal(out, want[at])
