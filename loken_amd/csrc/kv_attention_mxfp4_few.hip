@@ -15,7 +15,7 @@
 // are cut into parts, which a second launch joins.
 //
 // Bound by the cache's bytes where they are many: 64 sequences of up to 8192 tokens, 8 heads of 128, 287 MB in 71 us, 4.0 TB/s of the 4.9 that a copy
-// reaches; 131072 tokens of one sequence 29 us, 4.9 TB/s. Else by the chain table, codes, scores, sums, join: 517 tokens 10.7 us with its launches.
+// reaches; 131072 tokens of one sequence 30.5 us, 4.7 TB/s. Else by the chain table, codes, scores, sums, join: 517 tokens 10.7 us with its launches.
 
 #include "kv_attention_mxfp4.h"
 

@@ -9,8 +9,8 @@
 // goes the same way, by pairs that stay as they are. Queries are computed in 32 bits and rounded once. Keys that go to the cache are computed in 64: a value next
 // to the border of two codes would else come out as the other one. They pass through LDS, where a block's 32 values come together.
 //
-// Bound by the rows' bytes: 4096 tokens of 32 + 8 heads of 128, bf16, three axes of positions 16.9 us, 5.0 TB/s in and out. Into the cache by the 64-bit norms and
-// rotations too: 2048 tokens of 32 + 8 + 8 heads, bf16, 14.5 us; a few tokens by the chain position, angle, rows: one token 3.1 us.
+// Bound by the rows' bytes: 4096 tokens of 32 + 8 heads of 128, bf16, three axes of positions 17.2 us, 4.9 TB/s in and out. Into the cache by the 64-bit norms and
+// rotations too: 2048 tokens of 32 + 8 + 8 heads, bf16, 14.1 us; a few tokens by the chain position, angle, rows: one token 3.1 us.
 
 #include <type_traits>
 
