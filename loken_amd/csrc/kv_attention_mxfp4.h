@@ -100,16 +100,14 @@ static __device__ __forceinline__ bool mx_tile_at(const Attend& a, int rows_of_t
     return false;
 }
 
-// Sequences of up to so many rows (token, head of a group) are the few-rows kernel's, and rows of its workgroups: with slots for the pieces while
-// these fit (in one operand, or f32 in two), else sixteen.
+// Sequences of up to so many rows (token, head of a group) are the few-rows kernel's, and rows of its workgroups: those whose pieces fit one operand, else
+// sixteen. (A piece an operand for four rows: 64 sequences of up to 8192 tokens in f32 77 us, in slots 68; two operands of slots for eight f32 rows 63 us, 64 x 2 behind
+// up to 4096, sixteen columns 52.)
 constexpr int MX_FEW_ROWS = 16;
-constexpr int mx_few_rows(bool f32, int head_dim, int max_rows) {
-    if (max_rows <= (f32 ? 4 : 8)) return f32 ? 4 : 8;
-    return f32 && max_rows <= 8 && head_dim < 256 ? 8 : 16;
-}
+constexpr int mx_few_rows(bool f32, int max_rows) { return max_rows > (f32 ? 4 : 8) ? 16 : f32 ? 4 : 8; }
 // Its waves on a SIMD, for that many rows: as many as the registers hold. Heads of 128 in three with one buffer of codes, for two with two: 64 sequences of up
-// to 2000 tokens in pieces, bf16, 49 to 40 us, 131072 tokens of one the same; f32 of more than four rows two for one, 64 x 2 rows 90 to 73 us.
-constexpr int mx_few_on_simd(bool f32, bool f16, int head_dim, int rows) { return head_dim == 256 && rows == 16 && (f32 || f16) ? 1 : head_dim == 128 && rows < 16 && !(f32 && rows > 4) ? 3 : 2; }
+// to 2000 tokens in pieces, bf16, 49 to 40 us, 131072 tokens of one the same.
+constexpr int mx_few_on_simd(bool f32, bool f16, int head_dim, int rows) { return head_dim == 256 && rows == 16 && (f32 || f16) ? 1 : head_dim == 128 && rows < 16 ? 3 : 2; }
 
 // Rows of a workgroup of the many-rows kernel, and its waves on a SIMD, as the registers hold them. (Heads of 256 in two spill: 300 rows of two sequences
 // behind 1000 42 us for 37.)

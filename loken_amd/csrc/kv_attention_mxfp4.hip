@@ -77,7 +77,7 @@ extern "C" int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, 
     const int tiles = (int)((min(seen, table_tokens) + KV_TILE - 1) / KV_TILE), cus = lk_device().cus;
     AttendMx af = a, am = a;
     // Beside a sequence of many rows the few-rows kernel takes what one of its workgroups holds for a token's rows.
-    const int few_max = many ? mx_few_rows(f32, head_dim, group) : max_rows, per = mx_few_rows(f32, head_dim, few_max);
+    const int few_max = many ? mx_few_rows(f32, group) : max_rows, per = mx_few_rows(f32, few_max);
     const int few_tokens = many ? few_max / group : tokens;
     if (few) {
         af.few_rows = many ? few_max : 0x7FFFFFFF;

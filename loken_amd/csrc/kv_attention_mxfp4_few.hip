@@ -25,15 +25,15 @@ constexpr int WAVES = 4;
 
 static __device__ __forceinline__ float sum_over_groups(float v) { return swap_add32(swap_add16(v)); }
 
-template <typename T, int D, int NT, int SLOTS>
+template <typename T, int D, int SLOTS>
 struct Few {
     static constexpr int PIECES = sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1;   // of a query value
     static constexpr int SHARES = sizeof(T) == 4 ? 3 : 2;                                         // of a weight
     static constexpr int QP = SLOTS == 1 ? PIECES : 1, SP = SLOTS == 1 ? SHARES : 1;              // operands of them
-    static constexpr int RPT = 16 / SLOTS, ROWS = RPT * NT, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
+    static constexpr int ROWS = 16 / SLOTS, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;
     static constexpr int ON_SIMD = mx_few_on_simd(sizeof(T) == 4, std::is_same<T, __half>::value, D, ROWS);
     // One buffer of codes, where that puts one more wave on a SIMD.
-    static constexpr bool ONE = ON_SIMD > (D == 128 && (sizeof(T) != 4 || ROWS <= 4) ? 2 : 1) && D > 64;
+    static constexpr bool ONE = ON_SIMD > (D == 128 && SLOTS > 1 ? 2 : 1) && D > 64;
 };
 
 // What the slots of a row have together.
@@ -45,10 +45,10 @@ static __device__ __forceinline__ float sum_of_slots(float v) {
 }
 
 // CAP: whether and how scores are capped (as a branch at run time the compiler takes the tanh always, and the result where it is asked for)
-template <typename T, int D, int NT, int SLOTS, int CAP>
-__global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void mx_few_kernel(AttendMx a, int row_tiles) {
-    using F = Few<T, D, NT, SLOTS>;
-    __shared__ float sums[WAVES][F::RPT][D + 4];
+template <typename T, int D, int SLOTS, int CAP>
+__global__ __launch_bounds__(64 * WAVES, (Few<T, D, SLOTS>::ON_SIMD)) void mx_few_kernel(AttendMx a, int row_tiles) {
+    using F = Few<T, D, SLOTS>;
+    __shared__ float sums[WAVES][F::ROWS][D + 4];
     __shared__ float tops[WAVES][F::ROWS], weights[WAVES][F::ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
@@ -161,64 +161,50 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
 
         const float under = mx_under<CAP>(a.scale, a.cap);
         // the rows' pieces, and what a product, or its tanh, is in powers of two
-        mx_b8 q[NT][F::KS][F::QP];
-        float unit[NT];
-        int pos[NT];
+        mx_b8 q[F::KS][F::QP];
+        const int r = r0 + i / SLOTS;
+        const int of_seq = a.token_of(min(r, r1)), tok = s.first + of_seq, head = kv * a.group + min(r, r1) - of_seq * a.group;
+        const int pos = r <= r1 ? (int)max(s.pos_of_0 + tok, (int64_t)-1) : -1;
+        const T* row = (const T*)a.q + tok * a.q_stride + (int64_t)head * D + g * (D / 4);
+        bool finite = true;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int r = r0 + n * F::RPT + i / SLOTS;
-            const int of_seq = a.token_of(min(r, r1)), tok = s.first + of_seq, head = kv * a.group + min(r, r1) - of_seq * a.group;
-            pos[n] = r <= r1 ? (int)max(s.pos_of_0 + tok, (int64_t)-1) : -1;
-            const T* row = (const T*)a.q + tok * a.q_stride + (int64_t)head * D + g * (D / 4);
-            bool finite = true;
+        for (int ks = 0; ks < F::KS; ++ks) {
+            const MxEight<T> raw = *(const MxEight<T>*)(row + 8 * ks);
+            uint32_t w[F::PIECES][4];
 #pragma unroll
-            for (int ks = 0; ks < F::KS; ++ks) {
-                const MxEight<T> raw = *(const MxEight<T>*)(row + 8 * ks);
-                uint32_t w[F::PIECES][4];
+            for (int e = 0; e < 4; ++e) {
+                const float x = to_f32(raw.v[2 * e]), y = to_f32(raw.v[2 * e + 1]);
+                finite = finite && fabsf(x) < INFINITY && fabsf(y) < INFINITY;
+                uint32_t both[F::PIECES];
+                mx_pieces<F::PIECES>(x, y, both);
+#pragma unroll
+                for (int p = 0; p < F::PIECES; ++p) w[p][e] = both[p];
+            }
+            if (SLOTS > 1) {   // the slot's piece alone
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float x = to_f32(raw.v[2 * e]), y = to_f32(raw.v[2 * e + 1]);
-                    finite = finite && fabsf(x) < INFINITY && fabsf(y) < INFINITY;
-                    uint32_t both[F::PIECES];
-                    mx_pieces<F::PIECES>(x, y, both);
+                    uint32_t mine = slot == 0 ? w[0][e] : 0;
 #pragma unroll
-                    for (int p = 0; p < F::PIECES; ++p) w[p][e] = both[p];
+                    for (int p = 1; p < F::PIECES; ++p) mine = slot == p ? w[p][e] : mine;
+                    w[0][e] = mine;
                 }
-                if (SLOTS > 1) {   // the slot's piece alone
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t mine = slot == 0 ? w[0][e] : 0;
-#pragma unroll
-                        for (int p = 1; p < F::PIECES; ++p) mine = slot == p ? w[p][e] : mine;
-                        w[0][e] = mine;
-                    }
-                }
-#pragma unroll
-                for (int p = 0; p < F::QP; ++p) q[n][ks][p] = __builtin_bit_cast(mx_b8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
             }
-            const uint64_t odd = __ballot(!finite);
-            finite = (odd >> i & 0x0001000100010001ull) == 0;
-            unit[n] = finite ? mx_unit<CAP>(a.scale, a.cap) : NAN;
-        }
-        int pos_least = 0x7FFFFFFF, pos_most = -1;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (r0 + n * F::RPT + i / SLOTS <= r1) { pos_least = min(pos_least, pos[n]); pos_most = max(pos_most, pos[n]); }
+            for (int p = 0; p < F::QP; ++p) q[ks][p] = __builtin_bit_cast(mx_b8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
         }
+        const uint64_t odd = __ballot(!finite);
+        finite = (odd >> i & 0x0001000100010001ull) == 0;
+        const float unit = finite ? mx_unit<CAP>(a.scale, a.cap) : NAN;
+        int pos_least = r <= r1 ? pos : 0x7FFFFFFF, pos_most = pos;
         for (int o = 1; o < 16; o <<= 1) {
             pos_least = min(pos_least, __shfl_xor(pos_least, o));
             pos_most = max(pos_most, __shfl_xor(pos_most, o));
         }
 
-        float m[NT], base[NT], l[NT];   // the largest product or tanh, that as a score, and the sum of weights relative to it
-        v4f acc[NT][F::NB];
+        float m = -INFINITY, base = 0.f, l = 0.f;   // the largest product or tanh, that as a score, and the sum of weights relative to it
+        v4f acc[F::NB];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            m[n] = -INFINITY;
-            base[n] = l[n] = 0.f;
-#pragma unroll
-            for (int b = 0; b < F::NB; ++b) acc[n][b] = (v4f){0.f, 0.f, 0.f, 0.f};
-        }
+        for (int b = 0; b < F::NB; ++b) acc[b] = (v4f){0.f, 0.f, 0.f, 0.f};
 
         auto step = [&](Loaded& now, Loaded& then) {
             const int p0 = lo + t * KV_TILE;
@@ -234,84 +220,75 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
             }
             // whether every row sees every position of the step
             const bool whole = p0 + KV_TILE - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && absent == 0;
-            v4f sc[NT][4];
+            v4f sc[4];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                v4f c[NT];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) c[n] = (v4f){0.f, 0.f, 0.f, 0.f};
+                sc[b] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int ks = 0; ks < F::KS; ++ks) {
                     const float power = D == 256 && ks >= F::KS / 2 ? mx_power_of<1>(now.kp[b]) : mx_power_of<0>(now.kp[b]);
                     const mx_b8 op = mx_eight(now.k[b].w[ks], power);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int p = 0; p < F::QP; ++p) c[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, q[n][ks][p], c[n], 0, 0, 0);
+                    for (int p = 0; p < F::QP; ++p) sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, q[ks][p], sc[b], 0, 0, 0);
                 }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) sc[n][b] = c[n];
             }
             if (F::ONE) load_keys(then, t + WAVES, next);
-            uint32_t share[NT][F::SP][4][2];   // weights: of a tile's four positions
+            uint32_t share[F::SP][4][2];   // weights: of a tile's four positions
+            float x[16], top = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float x[16], top = -INFINITY;
+            for (int e = 0; e < 16; ++e) x[e] = sum_of_slots<SLOTS>(sc[e >> 2][e & 3]);
+            if (CAP) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = sum_of_slots<SLOTS>(sc[n][e >> 2][e & 3]);
-                if (CAP) {
+                for (int e = 0; e < 16; ++e) x[e] = mx_tanh<CAP>(x[e], under);
+            }
+            if (!whole) {
+                asm volatile("");   // (stays a branch: the looks at sixteen positions would else be made in every step)
+                const int last = pos - p0 - 4 * g, first = a.window > 0 ? last - a.window : -0x40000000;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = mx_tanh<CAP>(x[e], under);
+                for (int e = 0; e < 16; ++e) {
+                    const int at = 16 * (e >> 2) + (e & 3);
+                    if (at > last || at <= first || (absent >> (e >> 2) & 1)) x[e] = -INFINITY;
                 }
-                if (!whole) {
-                    asm volatile("");   // (stays a branch: the looks at sixteen positions would else be made in every step)
-                    const int last = pos[n] - p0 - 4 * g, first = a.window > 0 ? last - a.window : -0x40000000;
+            }
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int at = 16 * (e >> 2) + (e & 3);
-                        if (at > last || at <= first || (absent >> (e >> 2) & 1)) x[e] = -INFINITY;
-                    }
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
+            top = mx_max_over_groups(top);
+            if (__ballot(top > m)) {
+                const float most = fmaxf(m, top), to = most == -INFINITY ? 0.f : most * unit;
+                const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base - to);
+                l *= keep;
+#pragma unroll
+                for (int b = 0; b < F::NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[b][e] *= keep;
+                m = most;
+                base = to;
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(x[4 * b + e], unit, -base));
+                    l += p[e];
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
-                top = mx_max_over_groups(top);
-                if (__ballot(top > m[n])) {
-                    const float most = fmaxf(m[n], top), to = most == -INFINITY ? 0.f : most * unit[n];
-                    const float keep = m[n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base[n] - to);
-                    l[n] *= keep;
+                for (int h = 0; h < 2; ++h) {
+                    if (SLOTS > 1) {
+                        uint32_t piece = mx_pack(p[2 * h], p[2 * h + 1]);
 #pragma unroll
-                    for (int b = 0; b < F::NB; ++b)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[n][b][e] *= keep;
-                    m[n] = most;
-                    base[n] = to;
-                }
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    float p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        p[e] = __builtin_amdgcn_exp2f(fmaf(x[4 * b + e], unit[n], -base[n]));
-                        l[n] += p[e];
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (SLOTS > 1) {
-                            uint32_t piece = mx_pack(p[2 * h], p[2 * h + 1]);
-#pragma unroll
-                            for (int j = 1; j < F::SHARES; ++j) {
-                                const float less = j == 1 ? second : third;
-                                p[2 * h] = fmaf(__uint_as_float(piece << 16), -less, p[2 * h]);
-                                p[2 * h + 1] = fmaf(__uint_as_float(piece & 0xFFFF0000u), -less, p[2 * h + 1]);
-                                piece = mx_pack(p[2 * h], p[2 * h + 1]);
-                            }
-                            share[n][0][b][h] = piece;
-                        } else {
-                            uint32_t both[F::SHARES];
-                            mx_pieces<F::SHARES>(p[2 * h], p[2 * h + 1], both);
-#pragma unroll
-                            for (int j = 0; j < F::SP; ++j) share[n][j][b][h] = both[j];
+                        for (int j = 1; j < F::SHARES; ++j) {
+                            const float less = j == 1 ? second : third;
+                            p[2 * h] = fmaf(__uint_as_float(piece << 16), -less, p[2 * h]);
+                            p[2 * h + 1] = fmaf(__uint_as_float(piece & 0xFFFF0000u), -less, p[2 * h + 1]);
+                            piece = mx_pack(p[2 * h], p[2 * h + 1]);
                         }
+                        share[0][b][h] = piece;
+                    } else {
+                        uint32_t both[F::SHARES];
+                        mx_pieces<F::SHARES>(p[2 * h], p[2 * h + 1], both);
+#pragma unroll
+                        for (int j = 0; j < F::SP; ++j) share[j][b][h] = both[j];
                     }
                 }
             }
@@ -339,12 +316,10 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
                     power[4 * b + 2] = mx_power_of<2>(now.vp[b0 + b]);
                     power[4 * b + 3] = mx_power_of<3>(now.vp[b0 + b]);
                 }
-                mx_b8 w[NT][F::SP];
+                mx_b8 w[F::SP];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < F::SP; ++j)
-                        w[n][j] = __builtin_bit_cast(mx_b8, make_uint4(share[n][j][b0][0], share[n][j][b0][1], share[n][j][b0 + 1][0], share[n][j][b0 + 1][1]));
+                for (int j = 0; j < F::SP; ++j)
+                    w[j] = __builtin_bit_cast(mx_b8, make_uint4(share[j][b0][0], share[j][b0][1], share[j][b0 + 1][0], share[j][b0 + 1][1]));
 #pragma unroll
                 for (int byte = 0; byte < F::PART; ++byte) {   // columns 2 byte and 2 byte + 1 of the lane's sixteenth
                     uint32_t c[8];
@@ -364,12 +339,10 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
                     const mx_b8 op0 = __builtin_bit_cast(mx_b8, make_uint4(even[0], even[1], even[2], even[3]));
                     const mx_b8 op1 = __builtin_bit_cast(mx_b8, make_uint4(odd[0], odd[1], odd[2], odd[3]));
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int j = 0; j < F::SP; ++j) {
-                            acc[n][2 * byte] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op0, w[n][j], acc[n][2 * byte], 0, 0, 0);
-                            acc[n][2 * byte + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op1, w[n][j], acc[n][2 * byte + 1], 0, 0, 0);
-                        }
+                    for (int j = 0; j < F::SP; ++j) {
+                        acc[2 * byte] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op0, w[j], acc[2 * byte], 0, 0, 0);
+                        acc[2 * byte + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op1, w[j], acc[2 * byte + 1], 0, 0, 0);
+                    }
                 }
             }
             if (F::ONE) load_values(then, t + WAVES, next);
@@ -386,52 +359,45 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
         }
 
         // the slots' sums, and the four waves' relative to their common maximum, an operand's rows at a time
+        l = sum_over_groups(l);
+        m = m == -INFINITY ? m : base;
+        if (g == 0 && slot == 0) tops[wave][i / SLOTS] = m;
+        if (SLOTS > 1) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            l[n] = sum_over_groups(l[n]);
-            m[n] = m[n] == -INFINITY ? m[n] : base[n];
-            if (g == 0 && slot == 0) tops[wave][n * F::RPT + i / SLOTS] = m[n];
-            if (SLOTS > 1) {
+            for (int b = 0; b < F::NB; ++b)
 #pragma unroll
-                for (int b = 0; b < F::NB; ++b)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[n][b][e] = sum_of_slots<SLOTS>(slot < F::SHARES ? acc[n][b][e] : 0.f);
-            }
+                for (int e = 0; e < 4; ++e) acc[b][e] = sum_of_slots<SLOTS>(slot < F::SHARES ? acc[b][e] : 0.f);
         }
         __syncthreads();
+        const int column = i / SLOTS;
+        const float top = fmaxf(fmaxf(tops[0][column], tops[1][column]), fmaxf(tops[2][column], tops[3][column]));
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        // column of the sums: the lane's rows 4 g + e of the operand are sixteenths of the head
+        if (slot == 0) {
+            // (a part whose scores are no numbers has a sum that is none, and may have no maximum)
+            if (g == 0) weights[wave][column] = m == -INFINITY ? l : l * f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (n) __syncthreads();
-            const int r = n * F::RPT + i / SLOTS;
-            const float top = fmaxf(fmaxf(tops[0][r], tops[1][r]), fmaxf(tops[2][r], tops[3][r]));
-            const float f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
-            // column of the sums: the lane's rows 4 g + e of the operand are sixteenths of the head
-            if (slot == 0) {
-                // (a part whose scores are no numbers has a sum that is none, and may have no maximum)
-                if (g == 0) weights[wave][r] = m[n] == -INFINITY ? l[n] : l[n] * f;
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int b = 0; b < F::NB; ++b) sums[wave][column][(4 * g + e) * (D / 16) + b] = acc[b][e] * f;
+        }
+        __syncthreads();
+        for (int at = threadIdx.x; at < min(r1 - r0 + 1, F::ROWS) * D; at += 64 * WAVES) {
+            const int rr = at / D, d = at % D;
+            float total = 0.f, lw = 0.f;
 #pragma unroll
-                    for (int b = 0; b < F::NB; ++b) sums[wave][i / SLOTS][(4 * g + e) * (D / 16) + b] = acc[n][b][e] * f;
+            for (int w = 0; w < WAVES; ++w) {
+                total += sums[w][rr][d];
+                lw += weights[w][rr];
             }
-            __syncthreads();
-            for (int at = threadIdx.x; at < min(r1 - r0 + 1 - n * F::RPT, F::RPT) * D; at += 64 * WAVES) {
-                const int rr = at / D, d = at % D, row_of = n * F::RPT + rr;
-                float total = 0.f, lw = 0.f;
-#pragma unroll
-                for (int w = 0; w < WAVES; ++w) {
-                    total += sums[w][rr][d];
-                    lw += weights[w][row_of];
-                }
-                const int of_seq = a.token_of(r0 + row_of), head = kv * a.group + r0 + row_of - of_seq * a.group;
-                const int64_t row = s.first + of_seq;
-                if (to < 0) {
-                    ((T*)a.out)[row * a.out_stride + (int64_t)head * D + d] = from_f32<T>(lw == 0.f ? 0.f : total / lw);
-                } else {
-                    const int64_t place = a.chunks ? to + row_of : (a.part_row(seq, s, (int)row) * a.heads + head) * a.splits + part;
-                    a.part_o[place * D + d] = total;
-                    if (d == 0) a.part_ml[place] = make_float2(fmaxf(fmaxf(tops[0][row_of], tops[1][row_of]), fmaxf(tops[2][row_of], tops[3][row_of])), lw);
-                }
+            const int of_seq = a.token_of(r0 + rr), head = kv * a.group + r0 + rr - of_seq * a.group;
+            const int64_t row = s.first + of_seq;
+            if (to < 0) {
+                ((T*)a.out)[row * a.out_stride + (int64_t)head * D + d] = from_f32<T>(lw == 0.f ? 0.f : total / lw);
+            } else {
+                const int64_t place = a.chunks ? to + rr : (a.part_row(seq, s, (int)row) * a.heads + head) * a.splits + part;
+                a.part_o[place * D + d] = total;
+                if (d == 0) a.part_ml[place] = make_float2(fmaxf(fmaxf(tops[0][rr], tops[1][rr]), fmaxf(tops[2][rr], tops[3][rr])), lw);
             }
         }
         __syncthreads();
@@ -442,17 +408,12 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, NT, SLOTS>::ON_SIMD)) void m
 template <typename T, int D, int CAP>
 static int launch(const AttendMx& a, int max_rows, hipStream_t s) {
     constexpr int SLOTS = sizeof(T) == 4 ? 4 : 2;
-    const int per = mx_few_rows(sizeof(T) == 4, D, max_rows), row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / per + 1;
+    const int per = mx_few_rows(sizeof(T) == 4, max_rows), row_tiles = max_rows < 1 ? 1 : (max_rows - 1) / per + 1;
     const int64_t blocks = a.chunks ? (int64_t)a.chunks * a.mx.heads : (int64_t)a.seqs * a.mx.heads * row_tiles * a.splits;
     if (blocks > 0x7FFFFFFF) return LK_ERR_SIZE;
     const dim3 grid((unsigned)blocks), threads(64 * WAVES);
-    if constexpr (sizeof(T) == 4 && D < 256)
-        if (per == 8) {
-            hipLaunchKernelGGL((mx_few_kernel<T, D, 2, SLOTS, CAP>), grid, threads, 0, s, a, row_tiles);
-            return lk_launch_status();
-        }
-    if (per == 16 / SLOTS) hipLaunchKernelGGL((mx_few_kernel<T, D, 1, SLOTS, CAP>), grid, threads, 0, s, a, row_tiles);
-    else hipLaunchKernelGGL((mx_few_kernel<T, D, 1, 1, CAP>), grid, threads, 0, s, a, row_tiles);
+    if (per == 16 / SLOTS) hipLaunchKernelGGL((mx_few_kernel<T, D, SLOTS, CAP>), grid, threads, 0, s, a, row_tiles);
+    else hipLaunchKernelGGL((mx_few_kernel<T, D, 1, CAP>), grid, threads, 0, s, a, row_tiles);
     return lk_launch_status();
 }
 
