@@ -212,7 +212,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, SLOTS>::ON_SIMD)) void mx_fe
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 behind[b] = page_of(t + 2 * WAVES, b);
-                absent |= (unsigned)pages[b] < (unsigned)a.mx.pages ? 0 : 1 << b;
+                absent |= (unsigned)pages[b] < (unsigned)a.mx.pages && p0 + 16 * b < hi ? 0 : 1 << b;   // (behind the table's end: the last tile again)
             }
             if (!F::ONE) {
                 load_keys(then, t + WAVES, next);

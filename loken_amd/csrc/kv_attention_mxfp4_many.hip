@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
 #pragma unroll
         for (int b = 0; b < TILES; ++b) {
             behind[b] = page_of(t + 2 * WAVES, b);
-            absent |= (unsigned)pages[b] < (unsigned)a.mx.pages ? 0 : 1 << b;
+            absent |= (unsigned)pages[b] < (unsigned)a.mx.pages && p0 + 16 * b < hi ? 0 : 1 << b;   // (behind the table's end: the last tile again)
         }
         // whether every row sees every position of the step
         const bool whole = p0 + STEP - 1 <= pos_least && (a.window == 0 || p0 > pos_most - a.window) && absent == 0;

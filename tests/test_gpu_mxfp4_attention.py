@@ -1,4 +1,6 @@
 """Attention over the paged 4-bit cache against its definition in 64 bits over the same codes."""
+import math
+
 import numpy as np
 import pytest
 
@@ -272,3 +274,28 @@ def test_recorded_attention_beside_other_calls(what):
         return lambda: kv.kv_attention(*at, max_fresh=max(fresh), max_len=max(lens), softcap=30.0)
 
     check_replays([call(seed) for seed in (1, 2, 3)], torch.cuda.Stream())
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("fresh", [1, 5, 50])
+@pytest.mark.parametrize("page,cols", [(16, 1), (16, 9), (16, 7), (16, 18), (32, 3), (32, 5)])
+def test_lengths_past_the_end_of_the_table(page, cols, fresh, dtype):
+    """Positions whose column the table does not have are absent: of a sequence that ends inside the step in which the table does, of one that ends far
+    behind it, and of one that ends before."""
+    limit = page * cols
+    lens = [max(limit - 3, fresh), max(limit + 1, fresh), max(limit | 63, fresh), limit + 300]
+    b = Batch(lens, [fresh] * 4, 4, 2, 64, page, dtype, seed=cols)
+    b.table = np.ascontiguousarray(b.table[:, :cols])
+    b.check()
+    b.check(window=90)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("heads,kv_heads,dim,fresh", [(8, 4, 128, 1), (4, 4, 256, 2), (16, 4, 64, 9)])
+def test_long_lengths_past_the_end_of_the_table(heads, kv_heads, dim, fresh, dtype):
+    """The same of contexts in parts and of a batch in pieces."""
+    for lens in ([4000, 300, 2700, 900, 1500, 700, 4100, 130], [9000]):
+        b = Batch(lens, [fresh] * len(lens), heads, kv_heads, dim, 16, dtype, seed=dim)
+        b.table = np.ascontiguousarray(b.table[:, :157])
+        b.check()
+        b.check(max_len=64000)
