@@ -199,8 +199,8 @@ struct Target {
     }
     __device__ __forceinline__ bool in(float v, int i) const {
         const uint64_t at = (uint64_t)key_of(v) << 32 | (uint32_t)~i;
-        if (kept.kept == 0) return kept.best != 0 && at == kept.best;
-        return sc.live(sc.below(v)) && at >= kept.last && !(floored && !sc.kept(sc.power(v)));
+        if (at == kept.best && kept.best != 0) return true;   // (also where min-p, of more than 1, keeps nothing)
+        return kept.kept != 0 && sc.live(sc.below(v)) && at >= kept.last && !(floored && !sc.kept(sc.power(v)));
     }
     // p of a word that is in it. (Its weight as a number of 2^-42: 1024 more and less.)
     __device__ __forceinline__ double share(float v) const { return kept.kept == 0 ? 1.0 : ((power_of(sc.from_top(v), sc.rate) + 1024.0) - 1024.0) * by; }

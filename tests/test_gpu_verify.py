@@ -215,3 +215,18 @@ def test_recorded_beside_other_calls(draft):
         return lambda: torch.cat([t.double() for t in sampling.verify(**at)])
 
     check_replays([call(seed) for seed in (1, 2, 3)], torch.cuda.Stream())
+
+
+FLOORS = [(1.0, 0, 1.0, 1.0), (1.0, 0, 1.0, 2.0), (0.7, 0, 0.9, 2.0), (0.9, 20, 1.0, 1.5), (1.1, 20, 0.95, 1.0), (1.0, 3000, 0.99, 3.0), (0.0, 0, 1.0, 2.0)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("draft", ["f32", None])
+@pytest.mark.parametrize("rule", FLOORS)
+def test_the_first_word_always_stays(rule, draft, dtype):
+    """min_p of 1 and above leaves the first word (of 1: and those that are equal to it), which is then all of the distribution."""
+    d = Drafts([4, 1, 3, 5], 30011, dtype, draft, [rule], seed=21)
+    d.logits[5, [7, 20000, 30010]] = 40.0     # equal ones
+    got = d.check()
+    first = d.starts[:-1] + got[1].cpu().numpy()
+    assert (got[0].cpu().numpy()[first] >= 0).all() and (got[2].cpu().numpy()[first] > 0).all()
