@@ -230,3 +230,27 @@ def test_the_first_word_always_stays(rule, draft, dtype):
     got = d.check()
     first = d.starts[:-1] + got[1].cpu().numpy()
     assert (got[0].cpu().numpy()[first] >= 0).all() and (got[2].cpu().numpy()[first] > 0).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("draft", ["f32", None])
+def test_many_rows_in_several_pieces(draft, dtype):
+    """Rows enough for pieces of sixteen words a thread, the last of them a part of one, every rule, and largest words that are equal across pieces."""
+    lengths = np.random.default_rng(30).integers(1, 6, 100)
+    d = Drafts(list(lengths), 16411, dtype, draft, RULES + FLOORS, seed=31)
+    assert d.rows * 3 >= 512
+    d.logits[::3, [17, 4100, 8200, 16410]] = 30.0
+    d.logits[1::9, 16408:] = 31.0
+    d.check()
+
+
+@pytest.mark.parametrize("vocab", [1 << 20, (1 << 20) - 3, 300007])
+@pytest.mark.parametrize("draft", ["bf16", None])
+@pytest.mark.parametrize("rule", [(1.0, 0, 1.0, 0.0), (0.8, 50, 1.0, 0.0), (0.8, 20, 0.9, 0.0), (1.0, 0, 0.95, 0.0)])
+def test_the_largest_vocabularies(rule, draft, vocab):
+    for lengths in ([1], [2, 1]):
+        d = Drafts(lengths, vocab, "f32", draft, [rule], seed=33)
+        d.uniform[0] = 0.9999
+        for draw in (1e-6, 0.5, 1 - 1e-6):
+            d.draw[:] = draw
+            d.check()
