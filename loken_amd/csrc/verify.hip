@@ -286,7 +286,10 @@ struct Left {
         auto whole = [](double p) { return (uint64_t)__double_as_longlong(fma(fmax(p, 0.0), 2251799813685248.0, 4503599627370496.0)) - 0x4330000000000000ull; };
         if (target.plain) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) left[e] = whole(fma(power_of_any((double)x[e] - (double)target.sc.top, target.sc.rate), target.by, -(double)q[e]));
+            for (int e = 0; e < VEC; ++e) {
+                const float v = target.sc.live(target.sc.top - x[e]) ? x[e] : -INFINITY;   // (else its weight is none)
+                left[e] = whole(fma(power_of_any((double)v - (double)target.sc.top, target.sc.rate), target.by, -(double)q[e]));
+            }
         } else {
             bool in[VEC], any = false;
 #pragma unroll

@@ -254,3 +254,16 @@ def test_the_largest_vocabularies(rule, draft, vocab):
         for draw in (1e-6, 0.5, 1 - 1e-6):
             d.draw[:] = draw
             d.check()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_words_whose_weight_rounds_to_none_are_not_drawn(dtype):
+    """As in sampling: 2^-44.7 of the largest word's weight is none, also where no rule cuts and the draw is 0."""
+    d = Drafts([1, 1, 2, 2], 5003, dtype, None, [(1.0, 0, 1.0, 0.0)], seed=40)
+    d.logits[:] = -100.0
+    d.logits[:, 0], d.logits[:, 4900] = -31.0, 0.0
+    d.draw[:], d.uniform[:] = 0.0, 0.5
+    d.drafted[:] = 0                       # refused: its weight is none
+    tokens, accepted, probs = d.call()
+    first = torch.tensor(d.starts[:-1], device="cuda").long()
+    assert accepted.tolist() == [0, 0, 0, 0] and (tokens[first] == 4900).all() and (probs[first] == 1).all()
