@@ -44,6 +44,17 @@ static __device__ __forceinline__ void mx_pieces(float a, float b, uint32_t (&ou
     }
 }
 
+// Query values likewise, all of their bits: cut, not rounded, so that those beside f32's end have no infinity among their pieces.
+template <int PIECES>
+static __device__ __forceinline__ void mx_cut(float a, float b, uint32_t (&out)[PIECES]) {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        out[p] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+        a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+        b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+    }
+}
+
 // What a capped score is made of, from a product and what it is under the tanh, mx_under: tanh x = 1 - 2 / (e^2x + 1). A softmax does not see the 1: MX_NEAR leaves it
 // off, -1 / (e^2x + 1), whose unit, mx_unit, is twice the cap. A score is then off by cap * 2^-23: for f16 and bf16 with caps up to 64, where that is below what their
 // weights are held to. MX_FAR: the tanh, off by 1.2e-7; below a quarter by its series, to a few last places of x.

@@ -176,7 +176,7 @@ __global__ __launch_bounds__(64 * WAVES, (Few<T, D, SLOTS>::ON_SIMD)) void mx_fe
                 const float x = to_f32(raw.v[2 * e]), y = to_f32(raw.v[2 * e + 1]);
                 finite = finite && fabsf(x) < INFINITY && fabsf(y) < INFINITY;
                 uint32_t both[F::PIECES];
-                mx_pieces<F::PIECES>(x, y, both);
+                mx_cut<F::PIECES>(x, y, both);
 #pragma unroll
                 for (int p = 0; p < F::PIECES; ++p) w[p][e] = both[p];
             }

@@ -124,7 +124,7 @@ __global__ __launch_bounds__(64 * WAVES, (mx_many_on_simd(sizeof(T) == 4, sizeof
                 const float x = to_f32(raw.v[2 * e]), y = to_f32(raw.v[2 * e + 1]);
                 finite = finite && fabsf(x) < INFINITY && fabsf(y) < INFINITY;
                 uint32_t both[M::QP];
-                mx_pieces<M::QP>(x, y, both);
+                mx_cut<M::QP>(x, y, both);
 #pragma unroll
                 for (int p = 0; p < M::QP; ++p) w[p][e] = both[p];
             }

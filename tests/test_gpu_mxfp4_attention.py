@@ -1,6 +1,4 @@
 """Attention over the paged 4-bit cache against its definition in 64 bits over the same codes."""
-import math
-
 import numpy as np
 import pytest
 
@@ -299,3 +297,13 @@ def test_long_lengths_past_the_end_of_the_table(heads, kv_heads, dim, fresh, dty
         b.table = np.ascontiguousarray(b.table[:, :157])
         b.check()
         b.check(max_len=64000)
+
+
+@pytest.mark.parametrize("fresh", [1, 6, 40])
+def test_the_largest_f32_queries(fresh):
+    """Values within a bf16's half step of f32's end, which round to infinity as one."""
+    b = Batch([200], [fresh], 4, 2, 64, 16, "f32", seed=31, powers=(31, 32))
+    b.want.powers["v"][:] = 127
+    most = float(np.finfo(np.float32).max)
+    b.q[..., 5], b.q[..., 9] = most, -most * (1 - 2.0 ** -10)
+    b.check(scale=2.0 ** -33)
