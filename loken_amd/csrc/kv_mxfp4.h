@@ -87,7 +87,7 @@ static __device__ __forceinline__ void mx_store_eight(const MxPool& p, bool valu
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const F m = x[e] < 0 ? -x[e] : x[e];
-        most = m <= (F)3.402823466e38 && m > most ? m : most;   // (past f32, infinite or no number: does not count)
+        most = m <= (F)3.4028234663852886e38 && m > most ? m : most;   // (past f32's end, infinite or no number: does not count)
     }
     F other = __shfl_xor(most, 1);
     most = other > most ? other : most;

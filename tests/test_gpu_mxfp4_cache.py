@@ -253,3 +253,23 @@ def test_rows_behind_32_bit_offsets():
     codes = ref.quantize(x.double().numpy())
     for got, part in zip(kv.kv_read(cache, dev(slots)), (slice(0, kv_heads), slice(kv_heads, None))):
         assert np.array_equal(got.cpu().numpy(), ref.values(codes[0][:, part], codes[1][:, part]).astype(np.float32))
+
+
+@pytest.mark.parametrize("pairs", [0, 16])
+def test_the_largest_numbers_of_f32_are_numbers(pairs):
+    """They count for a block's power, as rows that are there already and as keys on their way from the norms."""
+    most = np.finfo(np.float32).max
+    x = np.zeros((3, 3, 64), np.float32)
+    x[0, :, 40], x[1, :, 41], x[2, :, 63] = most, -most, np.nextafter(most, np.float32(0))
+    x[:, :, 32] = 1e30
+    r = rotary.Rotary(dev(np.ones(pairs, np.float32)))
+    slots, d = np.array([3, 17, 30]), dev(x)
+    want = ref.Cache(2, 1, 16, 64)
+    want.write(x[:, 1:2], x[:, 2:], slots)
+    for into in ("write", "rotate"):
+        cache = kv.KvCacheMxfp4.empty(2, 1, 64)
+        if into == "write":
+            kv.kv_write(cache, d[:, 1:2], d[:, 2:], dev(slots))
+        else:
+            rotary.rotate_into(cache, d[:, :1], d[:, 1:2], d[:, 2:], dev(np.array([1, 2, 3], np.int32)), dev(slots), r)
+        check_cache(cache, want)
