@@ -299,6 +299,55 @@ def test_long_lengths_past_the_end_of_the_table(heads, kv_heads, dim, fresh, dty
         b.check(max_len=64000)
 
 
+def test_starts_past_the_batch_are_cut():
+    """A plan of more rows than the batch holds: those that it holds are computed, nothing is written behind it."""
+    b = Batch([40, 60], [10, 20], 2, 1, 64, 16, "f32", seed=12)
+    guard = torch.full((40, 2, 64), 9.0, device="cuda")
+    kv.kv_attention(b.q[:17].cuda().contiguous(), b.cache(), i32(b.table), i32(b.lens), i32(b.starts), max_fresh=20, max_len=60, out=guard[:17])
+    assert (guard[17:] == 9).all()
+    b.q, b.rows = b.q[:17], 17
+    assert torch.equal(b.check(max_fresh=20, max_len=60), guard[:17])
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("hint", [1, 40])
+def test_first_rows_far_outside_the_batch(hint, dtype):
+    """Rows that a sequence claims are those of the batch at most, whatever `starts` holds."""
+    b = Batch([300, 200, 100], [0, 0, 0], 4, 2, 64, 16, dtype, pad=40)
+    out = torch.full((b.rows, b.heads, b.dim), 7.0, dtype=TYPES[dtype], device="cuda")
+    for starts, want in (([2000000000, -2000000000, -2147483648, -2147483648], 7.0), ([2147483647, -2147483648, 2147483647, -2147483648], 0.0),
+                         ([2147483647, -5, -2147483648, 0], 7.0)):
+        out.fill_(7.0)
+        kv.kv_attention(b.q.cuda(), b.cache(), i32(b.table), i32(b.lens), i32(starts), max_fresh=hint, max_len=300, out=out)
+        assert (out == want).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("fresh", [1, 40])
+def test_rows_that_see_nothing_are_zeros(fresh, dtype):
+    """Pages that are absent, a sequence without tokens that brings rows, and more rows than tokens."""
+    b = Batch([90, 200, 64, 5], [fresh] * 4, 4, 1, 128, 16, dtype, seed=8)
+    b.table[0] = -1
+    b.table[1, 3:6] = [-1, 10 ** 6, -(1 << 31)]
+    b.lens[2] = 0
+    out = b.check()
+    assert (out[:fresh] == 0).all() and (out[2 * fresh:3 * fresh] == 0).all()
+    if fresh > 5:
+        assert (out[3 * fresh:4 * fresh - 5] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fresh", [1, 30])
+def test_queries_whose_scale_alone_would_overflow(fresh, dtype):
+    """Scores of ordinary size from queries at the end of the type's range and the smallest keys."""
+    b = Batch([200], [fresh], 4, 2, 64, 16, dtype, seed=31, powers=(31, 34))
+    b.want.powers["v"][:] = 127
+    b.q = (b.q.float() * 7e37).clamp(-3e38, 3e38)
+    b.q[..., 5] = 3e38
+    b.q = b.q.to(TYPES[dtype])
+    b.check(scale=2.0 ** -33)
+
+
 @pytest.mark.parametrize("fresh", [1, 6, 40])
 def test_the_largest_f32_queries(fresh):
     """Values within a bf16's half step of f32's end, which round to infinity as one."""
@@ -307,3 +356,59 @@ def test_the_largest_f32_queries(fresh):
     most = float(np.finfo(np.float32).max)
     b.q[..., 5], b.q[..., 9] = most, -most * (1 - 2.0 ** -10)
     b.check(scale=2.0 ** -33)
+
+
+def two_positions(fresh, heads, dtype, seed):
+    """Sequences whose rows see a position 0 of score 0 and value 1, a position 1 of score -d (a row and head's own) and value -1, and others of
+    weight 0: an output is tanh(d / 2), the difference of two weights that are nearly equal."""
+    g = np.random.default_rng(seed)
+    c = ref.Cache(6, 1, 16, 64)
+    c.powers["k"][:], c.powers["v"][:] = 127, 127
+    c.codes["k"][:, 0, :, 1], c.powers["k"][..., 0] = 15, 136   # -6 * 2^9
+    c.codes["k"][0, 0, 0], c.codes["k"][0, 0, 1] = 0, 0
+    c.codes["k"][0, 0, 1, 0], c.powers["k"][0, 0, 1] = 10, 127   # -1
+    c.codes["v"][:] = 7
+    c.codes["v"][0, 0, 0], c.codes["v"][0, 0, 1] = 2, 10
+    q = torch.zeros((fresh, heads, 64), dtype=TYPES[dtype])
+    q[:, :, 0] = torch.tensor(2.0 ** g.uniform(-9, -6, (fresh, heads))).to(TYPES[dtype])
+    q[:, :, 1] = 1
+    return c, q
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("fresh,heads", [(1, 1), (1, 4), (3, 1), (2, 4), (6, 1), (5, 3), (4, 4), (40, 1), (30, 5)])
+def test_the_weights_bits(fresh, heads, dtype):
+    """Weights are held to 24 bits in f32, to 16 in f16 and in bf16 of few rows: what is left of a difference of two says so."""
+    for seed in range(4):
+        c, q = two_positions(fresh, heads, dtype, seed)
+        length = 2 + fresh
+        out = kv.kv_attention(q.cuda(), handle(c), i32([range(6)]), i32([length]), i32([0, fresh]), max_fresh=fresh, max_len=length, scale=1.0)
+        want = np.tanh(q[:, :, :1].double().numpy() / 2)
+        # The weights 1 and w = e^-d: w's power of two and its argument are off by 2^-22, the weight as it goes into the product by half a step of its pieces,
+        # 2^-24 (three), 2^-16 (two) or 2^-8 (one), each halved by 1 / (1 + w). Sums, quotient: 2^-22 of the result. Then the result's rounding.
+        pieces = 3 if dtype == "f32" else 1 if dtype == "bf16" and fresh * heads > 16 else 2
+        step = 2.0 ** -24 if dtype == "f32" else torch.finfo(TYPES[dtype]).eps / 2
+        bound = 0.5 * (2.0 ** -22 + 2.0 ** (-8 * pieces)) + (step + 2.0 ** -22) * np.abs(want)
+        off = np.abs(out.double().cpu().numpy() - want)
+        assert (off <= bound).all(), (off.max(), bound.max())
+
+
+@pytest.mark.parametrize("fresh,heads", [(1, 1), (2, 2), (6, 1), (4, 4), (40, 1)])
+@pytest.mark.parametrize("dtype,bit", [("f32", 23), ("f16", 10), ("bf16", 7)])
+def test_every_bit_of_a_query_counts(dtype, bit, fresh, heads):
+    """Two scores that differ by the last bit of a query's value, at a scale that makes it one half either way; others of weight 0."""
+    c = ref.Cache(4, 1, 16, 64)
+    c.powers["k"][:], c.powers["v"][:] = 127, 127
+    c.codes["k"][:, 0, :, 2] = 15
+    c.codes["k"][0, 0, :2, 2] = 0
+    c.codes["k"][0, 0, 0, :2], c.codes["k"][0, 0, 1, :2] = [2, 10], [10, 2]      # (1, -1) and (-1, 1)
+    c.codes["v"][0, 0, 0], c.codes["v"][0, 0, 1] = 2, 10
+    q = torch.zeros((fresh, heads, 64))
+    q[..., 0], q[..., 1], q[..., 2] = 1 + 2.0 ** -bit, 1, 1
+    out = kv.kv_attention(q.to(TYPES[dtype]).cuda(), handle(c), i32([range(4)]), i32([2 + fresh]), i32([0, fresh]), max_fresh=fresh, max_len=2 + fresh,
+                          scale=2.0 ** (bit - 1))
+    want, one = np.tanh(0.5), dtype == "bf16" and fresh * heads > 16     # weights e^(1/2) and e^(-1/2)
+    # (a weight of e^-1 in two pieces is off by 2^-16 of itself, in one by 2^-8, which the quotient makes 2 / (1 + e^-1)^2 = 1.07 of; the result's rounding)
+    step = 2.0 ** -21 if dtype == "f32" else 2.0 ** -16 + (2.0 ** -9 if one else 0) + torch.finfo(TYPES[dtype]).eps / 2 * want
+    assert np.abs(out.double().cpu().numpy() - want).max() <= step
+    assert out.shape == (fresh, heads, 64)
