@@ -7,6 +7,13 @@ namespace {
 
 constexpr int MOST_PARTS = 1024;
 
+// Whether what a product is multiplied by, mx_unit or mx_under, is a normal number: an infinite one makes none of a product of 0, a subnormal one has lost bits.
+static bool factor_ok(float scale, float cap) {
+    if (!(scale >= 0x1p-126f && scale <= 0x1p127f) || !(cap == 0.0f || (cap >= 0x1p-64f && cap <= 0x1p64f))) return false;
+    const double of_cap = cap > 0.0f ? (double)scale / cap : 1.0;
+    return of_cap >= 0x1p-124 && of_cap <= 0x1p125;
+}
+
 // Parts of a context of `tiles` steps for `groups` workgroups of one part each: until there are `want` workgroups, of at
 // least `least` steps.
 static void cut(Attend& a, int64_t groups, int tiles, int want, int least) {
@@ -49,7 +56,7 @@ extern "C" int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, 
     if (!size) return LK_ERR_TYPE;
     if (!mx_pool_ok(k_codes, v_codes, k_powers, v_powers, pages, kv_heads, head_dim, page_tokens)) return LK_ERR_ARG;
     if (seqs < 0 || rows < 0 || max_fresh < 0 || max_len < 0 || table_cols < 0 || table_stride < table_cols || window < 0 ||
-        !(scale > 0.0f && scale <= 3.402823466e38f) || !(cap == 0.0f || (cap >= 5.421010862e-20f && cap <= 1.8446744074e19f)) || heads <= 0 || heads > 65535 || heads % kv_heads != 0)
+        !factor_ok(scale, cap) || heads <= 0 || heads > 65535 || heads % kv_heads != 0)
         return LK_ERR_ARG;
     if (seqs == 0 || rows == 0) return LK_OK;
     const int64_t row = (int64_t)heads * head_dim;

@@ -252,6 +252,8 @@ def kv_attention(q: torch.Tensor, cache: KvCacheQ8 | KvCacheMxfp4, table: torch.
     in_4_bits = isinstance(cache, KvCacheMxfp4)
     if softcap and (not in_4_bits or not 2.0 ** -64 <= softcap <= 2.0 ** 64):
         raise ValueError("kv_attention: softcap is zero, or 2^-64 to 2^64 over the 4-bit cache")
+    if in_4_bits and not (2.0 ** -126 <= scale <= 2.0 ** 127 and (not softcap or 2.0 ** -124 <= scale / softcap <= 2.0 ** 125)):
+        raise ValueError("kv_attention: over the 4-bit cache the scale is 2^-126 to 2^127, and 2^-124 to 2^125 of a softcap")
     if out is None:
         out = torch.zeros((rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
     of_out, _, out_stride = _rows("kv_attention", "out", out, heads, cache.head_dim)

@@ -412,3 +412,13 @@ def test_every_bit_of_a_query_counts(dtype, bit, fresh, heads):
     step = 2.0 ** -21 if dtype == "f32" else 2.0 ** -16 + (2.0 ** -9 if one else 0) + torch.finfo(TYPES[dtype]).eps / 2 * want
     assert np.abs(out.double().cpu().numpy() - want).max() <= step
     assert out.shape == (fresh, heads, 64)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fresh", [1, 6, 40])
+@pytest.mark.parametrize("scale", [0.125, 4.0])
+def test_values_near_the_end_of_f32(scale, fresh, dtype):
+    """130 positions of up to 6 * 2^110, in scores of any order: 2^8 times all of them is a number still."""
+    b = Batch([130, 70], [fresh] * 2, 4, 2, 64, 16, dtype, seed=60)
+    b.want.powers["v"][:] = 110 + 127
+    b.check(scale=scale)

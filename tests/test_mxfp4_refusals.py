@@ -168,3 +168,18 @@ def test_verification_arguments():
                 dict(draft=torch.zeros((3, 50), dtype=torch.int32)), dict(draft=torch.zeros((50, 3)).T), {}):
         with pytest.raises(ValueError):
             sampling.verify(**{**good, **bad})
+
+
+@pytest.mark.parametrize("change", [dict(scale=3e38), dict(scale=1e-40), dict(scale=2.0 ** 127 * 1.01), dict(scale=2.0 ** 70, cap=2.0 ** -64),
+                                    dict(scale=2.0 ** -70, cap=2.0 ** 64), dict(scale=1e-37, cap=1e3)])
+def test_scales_past_what_a_factor_of_f32_holds(change):
+    """A score's factor, scale * log2 e or scale / cap, has to be a normal number: an infinite one leaves no number of a product of 0."""
+    assert call("lk_kv_attention_mxfp4", ATTEND, change) == ARG
+    with pytest.raises(ValueError, match="scale"):
+        kv.kv_attention(torch.zeros((2, 6, 64)), cache(), torch.zeros((1, 4), dtype=torch.int32), torch.tensor([5], dtype=torch.int32),
+                        torch.tensor([0, 2], dtype=torch.int32), max_fresh=2, max_len=5, scale=change["scale"], softcap=change.get("cap", 0.0))
+
+
+@pytest.mark.parametrize("change", [dict(scale=2.0 ** 127), dict(scale=2.0 ** -126), dict(scale=2.0 ** 60, cap=2.0 ** -64), dict(scale=2.0 ** -60, cap=2.0 ** 64)])
+def test_scales_at_both_ends(change):
+    assert call("lk_kv_attention_mxfp4", ATTEND, dict(change, rows=0)) == OK
