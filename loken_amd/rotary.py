@@ -52,6 +52,8 @@ def _arguments(what, q, k, positions, rotary, q_weight, k_weight, eps):
     axes = 1 if len(shape) == 1 else shape[0] if len(shape) == 2 else 0
     if positions.dtype is not torch.int32 or axes == 0 or shape[-1] != rows:
         raise ValueError(f"{what}: positions are int32 [rows] or [axes, rows]")
+    if axes > 1 and axis is None:
+        raise ValueError(f"{what}: positions of several axes go with a rotation whose axis says which of them turns a pair")
     across = rows
     if not positions.is_contiguous():
         if rows > 1 and positions.stride(-1) != 1:
@@ -90,7 +92,7 @@ def _output(what, name, out, like, rows, heads, dim):
 def rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary: Rotary, *, q_weight: torch.Tensor | None = None,
            k_weight: torch.Tensor | None = None, eps: float = 1e-6, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
     """``q`` [rows, heads, head_dim] and ``k`` [rows, kv_heads, head_dim] (f32, f16 or bf16; rows may be parts of wider ones), normed head by
-    head where there is a weight (f32 [head_dim]) and turned by ``positions`` (int32 [rows] or [axes, rows]); into ``q_out`` and ``k_out``
+    head where there is a weight (f32 [head_dim]) and turned by ``positions`` (int32 [rows], or [axes, rows] for a rotation with ``axis``); into ``q_out`` and ``k_out``
     (new ones without; ``q`` and ``k`` themselves may be given)."""
     dim, rows, heads, kv_heads, qs, ks, on, tail = _arguments("rotate", q, k, positions, rotary, q_weight, k_weight, eps)
     q_out, qo = _output("rotate", "q_out", q_out, q, rows, heads, dim)

@@ -170,6 +170,20 @@ def test_verification_arguments():
             sampling.verify(**{**good, **bad})
 
 
+def test_rotation_by_several_axes_needs_to_know_which():
+    """Positions of several axes and a rotation that does not say which of them turns a pair: all would go by the first."""
+    several = torch.zeros((3, 4), dtype=torch.int32)
+    good = dict(q=torch.zeros((4, 6, 64)), k=torch.zeros((4, 3, 64)), positions=several, rotary=rotary.Rotary(torch.ones(32)))
+    into = dict(good, cache=cache(), v=torch.zeros((4, 3, 64)), slots=torch.zeros(4, dtype=torch.int64))
+    for call_of, given in ((rotary.rotate, good), (rotary.rotate_into, into)):
+        with pytest.raises(ValueError, match="axis"):
+            call_of(**given)
+        with pytest.raises(ValueError, match="device"):     # one axis, or a rotation that says
+            call_of(**dict(given, positions=several[:1]))
+        with pytest.raises(ValueError, match="device"):
+            call_of(**dict(given, rotary=rotary.Rotary(torch.ones(32), axis=torch.zeros(32, dtype=torch.uint8))))
+
+
 @pytest.mark.parametrize("change", [dict(scale=3e38), dict(scale=1e-40), dict(scale=2.0 ** 127 * 1.01), dict(scale=2.0 ** 70, cap=2.0 ** -64),
                                     dict(scale=2.0 ** -70, cap=2.0 ** 64), dict(scale=1e-37, cap=1e3)])
 def test_scales_past_what_a_factor_of_f32_holds(change):
