@@ -527,9 +527,9 @@ class BetweenMxfp4(Between):
         self.past.fill_(context)
         self.fresh.fill_(fresh)
         held = -(-context // PAGE_TOKENS)
-        self.table[:, held:] = -1
-        self.free = torch.randperm(self.pages, device=mk.dev, generator=mk.gen).to(torch.int32)
-        # (pages of other sequences: what they hold does not matter to a measured step)
+        more = self.table[:, held:]
+        self.free = torch.cat([more[more >= 0], self.free])   # what the drafts and the rows behind the context need
+        more.fill_(-1)
         self.plan = kv.KvPlan(self.seqs, rows, mk.dev)
         f32 = lambda *shape: torch.rand(shape, device=mk.dev, generator=mk.gen)  # noqa: E731
         self.norms = [f32(HEAD_DIM) + 0.5 for _ in "qk"]
