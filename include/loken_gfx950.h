@@ -900,7 +900,7 @@ int lk_qk_norm_rope_kv_mxfp4(const void* q, const void* k, const void* v, int ty
  *   cap > 0: scores are cap * tanh(scale * q . k / cap) before the softmax   (0: as they are; else 2^-64 .. 2^64)
  * scale: 2^-126 .. 2^127, scale / cap 2^-124 .. 2^125, else LK_ERR_ARG.
  * Powers below 31 and above 252, which nothing here writes, are not defined at positions that some row sees. Products are exact but for the softmax weights, which
- * are held to 24 bits in f32 and 16 in f16 and bf16 (8 where bf16 comes in many rows of a sequence); sums are f32. A query value keeps all its bits down to 2^-126. A product of a
+ * are held to 24 bits in f32 and 16 in f16 and bf16; sums are f32. A query value keeps all its bits down to 2^-126. A product of a
  * row and a key has to be a number of f32, and so has 2^8 times the positions that a row sees times their largest value (weights of a part of them are
  * relative to a score of that part, up to 2^8 below its largest). Scratch as for lk_kv_attention_q8. */
 int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, void* out, int64_t out_stride, const void* k_codes, const void* v_codes,

@@ -378,15 +378,15 @@ def two_positions(fresh, heads, dtype, seed):
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("fresh,heads", [(1, 1), (1, 4), (3, 1), (2, 4), (6, 1), (5, 3), (4, 4), (40, 1), (30, 5)])
 def test_the_weights_bits(fresh, heads, dtype):
-    """Weights are held to 24 bits in f32, to 16 in f16 and in bf16 of few rows: what is left of a difference of two says so."""
+    """Weights are held to 24 bits in f32, to 16 in f16 and bf16: what is left of a difference of two says so."""
     for seed in range(4):
         c, q = two_positions(fresh, heads, dtype, seed)
         length = 2 + fresh
         out = kv.kv_attention(q.cuda(), handle(c), i32([range(6)]), i32([length]), i32([0, fresh]), max_fresh=fresh, max_len=length, scale=1.0)
         want = np.tanh(q[:, :, :1].double().numpy() / 2)
         # The weights 1 and w = e^-d: w's power of two and its argument are off by 2^-22, the weight as it goes into the product by half a step of its pieces,
-        # 2^-24 (three), 2^-16 (two) or 2^-8 (one), each halved by 1 / (1 + w). Sums, quotient: 2^-22 of the result. Then the result's rounding.
-        pieces = 3 if dtype == "f32" else 1 if dtype == "bf16" and fresh * heads > 16 else 2
+        # 2^-24 (three) or 2^-16 (two), each halved by 1 / (1 + w). Sums, quotient: 2^-22 of the result. Then the result's rounding.
+        pieces = 3 if dtype == "f32" else 2
         step = 2.0 ** -24 if dtype == "f32" else torch.finfo(TYPES[dtype]).eps / 2
         bound = 0.5 * (2.0 ** -22 + 2.0 ** (-8 * pieces)) + (step + 2.0 ** -22) * np.abs(want)
         off = np.abs(out.double().cpu().numpy() - want)
@@ -407,9 +407,9 @@ def test_every_bit_of_a_query_counts(dtype, bit, fresh, heads):
     q[..., 0], q[..., 1], q[..., 2] = 1 + 2.0 ** -bit, 1, 1
     out = kv.kv_attention(q.to(TYPES[dtype]).cuda(), handle(c), i32([range(4)]), i32([2 + fresh]), i32([0, fresh]), max_fresh=fresh, max_len=2 + fresh,
                           scale=2.0 ** (bit - 1))
-    want, one = np.tanh(0.5), dtype == "bf16" and fresh * heads > 16     # weights e^(1/2) and e^(-1/2)
-    # (a weight of e^-1 in two pieces is off by 2^-16 of itself, in one by 2^-8, which the quotient makes 2 / (1 + e^-1)^2 = 1.07 of; the result's rounding)
-    step = 2.0 ** -21 if dtype == "f32" else 2.0 ** -16 + (2.0 ** -9 if one else 0) + torch.finfo(TYPES[dtype]).eps / 2 * want
+    want = np.tanh(0.5)     # weights e^(1/2) and e^(-1/2)
+    # (a weight of e^-1 in two pieces is off by 2^-16 of itself, which the quotient makes 2 / (1 + e^-1)^2 = 1.07 of; the result's rounding)
+    step = 2.0 ** -21 if dtype == "f32" else 2.0 ** -16 + torch.finfo(TYPES[dtype]).eps / 2 * want
     assert np.abs(out.double().cpu().numpy() - want).max() <= step
     assert out.shape == (fresh, heads, 64)
 
