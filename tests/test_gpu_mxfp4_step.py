@@ -216,3 +216,57 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for at, out in got:
         assert torch.equal(out, want[at])
+
+
+def test_pages_of_refused_drafts_go_back_to_the_list():
+    """A recorded step and what follows its check, recorded too and without a look at the device: the pages that refused drafts alone had are the
+    next ones to be given, so that a loop in a cache of as many pages as its tokens need comes through."""
+    loop = Loop(6)
+    rows, pages = SEQS * (DRAFTS + 1), SEQS * (MOST // PAGE)
+    free = torch.cat([loop.free_pages[:pages], i32([-1])])      # one place behind the list, for what is not given back
+    loop.free_pages = free[:pages]
+    fresh, plan = i32([DRAFTS + 1] * SEQS), kv.KvPlan(SEQS, rows)
+    x, drafted, share = torch.empty((rows, HIDDEN), device="cuda"), i32([0] * rows), torch.empty((rows, VOCAB), device="cuda")
+    cols, words = torch.arange(MOST // PAGE, device="cuda"), dev(np.array([5, 77, 900]))
+    first = torch.arange(SEQS, device="cuda") * (DRAFTS + 1)
+
+    def give_back(accepted):
+        loop.past.add_(accepted + 1)
+        back = (cols >= ((loop.past + PAGE - 1) // PAGE)[:, None]) & (cols < ((plan.lens + PAGE - 1) // PAGE)[:, None])
+        up_to = back.flatten().long().cumsum(0)
+        loop.taken.copy_(plan.taken - up_to[-1])
+        place = torch.where(back.flatten(), loop.taken + up_to - 1, pages)
+        free.scatter_(0, place, loop.table.flatten())
+
+    def step():
+        out = loop.step(x, drafted, share, fresh, plan)
+        give_back(out[7])
+        return out
+
+    def bring(n):
+        x.copy_(loop.words[words.repeat_interleave(DRAFTS + 1).long()])
+        share.fill_(1.0 / VOCAB)
+        drafted.copy_(dev(np.random.default_rng(n).integers(0, VOCAB, rows).astype(np.int32)))
+        loop.draw.copy_(dev(loop.draws[n]))
+        loop.uniform.copy_(dev(loop.u[n]))
+
+    bring(0)
+    step()
+    torch.cuda.synchronize()
+    graph, got = record(step, torch.cuda.Stream())
+    refused = 0
+    for n in range(1, 40):
+        past, table, list_before, taken = (t.cpu().numpy().copy() for t in (loop.past, loop.table, free, loop.taken))
+        bring(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, lens, *_ , after = served.plan(past, [DRAFTS + 1] * SEQS, table, list_before[:pages], PAGE, rows, int(taken[0]))
+        assert np.array_equal(loop.table.cpu().numpy(), want), n
+        past = past + got[7].cpu().numpy() + 1
+        assert np.array_equal(loop.past.cpu().numpy(), past), n
+        held = [int(e) for i in range(SEQS) for e in want[i, :-(-int(past[i]) // PAGE)]]
+        left = free[int(loop.taken):pages].tolist()
+        assert sorted(held + left) == sorted(loop.free[:pages].tolist()), n      # each page once
+        refused += after - int(loop.taken)
+        words = got[6][first + got[7]]
+    assert refused > 3 and past.max() > PAGE
