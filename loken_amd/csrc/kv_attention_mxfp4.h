@@ -112,16 +112,16 @@ static __device__ __forceinline__ bool mx_tile_at(const Attend& a, int rows_of_t
 }
 
 // Sequences of up to so many rows (token, head of a group) are the few-rows kernel's, and rows of its workgroups: those whose pieces fit one operand, else
-// sixteen. (A piece an operand for four rows: 64 sequences of up to 8192 tokens in f32 77 us, in slots 68; two operands of slots for eight f32 rows 63 us, 64 x 2 behind
-// up to 4096, sixteen columns 52.)
+// sixteen. (Sixteen columns, an operand a piece, for the one to four rows of 64 sequences of up to 8192 tokens in f32 83 us, in slots 73, kernel trace; for eight f32
+// rows two operands of slots took 63 us, 64 x 2 behind up to 4096, where sixteen columns took 52, calls.)
 constexpr int MX_FEW_ROWS = 16;
 constexpr int mx_few_rows(bool f32, int max_rows) { return max_rows > (f32 ? 4 : 8) ? 16 : f32 ? 4 : 8; }
 // Its waves on a SIMD, for that many rows: as many as the registers hold. Heads of 128 in three with one buffer of codes, for two with two: 64 sequences of up
-// to 2000 tokens in pieces, bf16, 49 to 40 us, 131072 tokens of one the same.
+// to 2000 tokens in pieces, bf16, 49 to 40 us (calls), 131072 tokens of one the same.
 constexpr int mx_few_on_simd(bool f32, bool f16, int head_dim, int rows) { return head_dim == 256 && rows == 16 && (f32 || f16) ? 1 : head_dim == 128 && rows < 16 ? 3 : 2; }
 
 // Rows of a workgroup of the many-rows kernel, and its waves on a SIMD, as the registers hold them. (Heads of 256 in two spill: 300 rows of two sequences
-// behind 1000 42 us for 37.)
+// behind 1000, weights of one piece, 42 us for 37, calls.)
 constexpr int mx_many_rows(bool f32, int head_dim) { return head_dim == 256 && f32 ? 16 : 32; }
 constexpr int mx_many_on_simd(bool f32, bool f16, int head_dim) {
     return head_dim == 64 ? (f32 || f16 ? 3 : 4) : head_dim == 128 ? (f32 || f16 ? 2 : 3) : 1;

@@ -93,13 +93,13 @@ extern "C" int lk_kv_attention_mxfp4(const void* q, int type, int64_t q_stride, 
         const int64_t most_steps = (int64_t)seqs * ((table_tokens + KV_TILE - 1) / KV_TILE + 1);
         // Pieces of equal lengths, across sequences, where those are long: a piece has to find its sequence and begins anew at each, some 10 us in all,
         // which ragged lengths win back from 96 steps a CU on, or 224 where sequences are many beside their steps. 8 sequences up to 32768 tokens, 8 heads of
-        // 128, bf16: 45 us by sequence, 38 in pieces; 64 up to 8192 71, 65; 32 up to 8192 45, 51; 64 up to 2000 28, 40.
+        // 128, bf16: 45 us by sequence, 38 in pieces; 64 up to 8192 71, 65; 32 up to 8192 45, 51; 64 up to 2000 28, 40 (calls).
         const bool long_ones = tiles > seqs && groups * tiles >= (int64_t)(tiles >= 8 * (int64_t)seqs ? 96 : 224) * cus;
         if (seqs > 1 && few_max <= per && groups <= 4 * cus && long_ones && most_steps < 0x7FFFFFFF) {
             af.chunks = (slots + kv_heads - 1) / kv_heads;
             af.least_tiles = 4;
         } else {
-            cut(af, groups, tiles, slots < 2 * cus ? slots : 2 * cus, tiles <= 16 ? 16 : 4);   // (three to a CU: 37 us for 35 of 131072 tokens, more to join)
+            cut(af, groups, tiles, slots < 2 * cus ? slots : 2 * cus, tiles <= 16 ? 16 : 4);   // (three to a CU: 131072 tokens 2 us longer, more to join)
             af.part_seq = few_tokens;
         }
     }

@@ -3,10 +3,10 @@
 // Both products run on v_mfma_f32_16x16x32_bf16: a code times its block's power of two is a bf16 exactly, two codes an instruction, and so are
 // queries and softmax weights as sums of bf16 pieces (bf16 queries one, f16 two, f32 three; weights two, f32 three). Products are then exact but for
 // weights of 16 bits, sums are f32. Up to four rows (f32; eight else) leave room for the pieces in the operand of sixteen columns: a slot of a row takes
-// one piece, and a product is one instruction; more rows take a column each and an instruction a piece.
+// one piece, and a product is one instruction; a row's slots, two or four neighbouring lanes, add up what they have. More rows take a column each and an instruction a piece.
 //
 // One wave takes a step: 64 positions as four tiles of sixteen. Scores come as (16 positions) x (16 columns): a lane holds column l % 16 and four positions
-// of each tile, which are, two tiles together, what the second product wants of the weights in that lane: nothing crosses lanes but maxima.
+// of each tile, which are, two tiles together, what the second product wants of the weights in that lane: nothing crosses lanes but maxima and the slots' sums.
 // The values' operand is (16 columns) x (32 positions): the cache has the values of four tokens that a lane takes in one piece; codes of one token
 // become bf16 by its block's power, and halves of words change places to bring a column's positions together.
 // Sums come as (16 columns) x (16 rows): a lane's row again, so maxima and corrections are the lane's own.
@@ -14,8 +14,8 @@
 // The next step's loads are in flight through a step, the pages of the one behind it too. Four waves take steps in turn and meet in LDS; long contexts
 // are cut into parts, which a second launch joins.
 //
-// Bound by the cache's bytes where they are many: 64 sequences of up to 8192 tokens, 8 heads of 128, 287 MB in 71 us, 4.0 TB/s of the 4.9 that a copy
-// reaches; 131072 tokens of one sequence 30.5 us, 4.7 TB/s. Else by the chain table, codes, scores, sums, join: 517 tokens 10.7 us with its launches.
+// Bound by the cache's bytes where they are many: 64 sequences of up to 8192 tokens, 8 heads of 128, 287 MB in 73 to 75 us, 3.9 TB/s of the 4.9 that a copy
+// reaches; 131072 tokens of one sequence 30.9 us, 4.6 TB/s. Else by the chain table, codes, scores, sums: 517 tokens 11.4 us. (Kernel trace.)
 
 #include "kv_attention_mxfp4.h"
 

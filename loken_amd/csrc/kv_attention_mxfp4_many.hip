@@ -5,16 +5,16 @@
 // LDS at the end. Nothing is shared before: no barrier, and each wave converts the codes for itself.
 //
 // The rows' pieces stay in LDS and the next step's keys are loaded when this one's scores are there, its values behind this one's products: bf16 heads of 128 then
-// take 168 registers, three waves a SIMD. (In registers with two buffers two waves: 2048 rows 57 us for 53, 700 rows behind 1000 52 for 35.)
+// take 168 registers, three waves a SIMD. (In registers with two buffers two waves, weights of one piece: 2048 rows 57 us for 53, 700 rows behind 1000 52 for 35, calls.)
 //
 // A row's weights are taken relative to a maximum that is put up only where a score lies 2^SLACK above it: bf16 has f32's range, so that costs no
 // bits, and a step without such a score needs no exchange between lanes and no correction. The sum of weights is a product with ones, of
 // the weights as they went into the sums of values: their roundings cancel.
 //
-// Bound by the issue of vector and matrix instructions, which take turns on a SIMD: of a step of 32 rows x 32 positions, heads of 128, 34 matrix
-// instructions of 16 cycles and 190 vector ones, 64 of them from codes to bf16. 2048 rows behind 14336 positions, 32 heads of 128, bf16: 617 us, 835 TFLOP/s of the
-// 1222 that a plain product reaches; 2048 rows alone 53 us. Not kept: 64 rows a wave (one wave a SIMD, 662 us for 642), 128 rows that share the
-// values' operands through LDS (598 for 616, and slower at every shorter size).
+// Bound by the issue of vector and matrix instructions, which take turns on a SIMD: of a step of 32 rows x 32 positions, heads of 128, 52 matrix
+// instructions of 16 cycles and 230 vector ones, 64 of them from codes to bf16. 2048 rows behind 14336 positions, 32 heads of 128, bf16: 770 us (calls), 669 TFLOP/s of the
+// 1222 that a plain product reaches; 2048 rows alone 74.7 us (kernel trace). Not kept, with weights of one piece: 64 rows a wave (one wave a SIMD, 662 us for 642), 128
+// rows that share the values' operands through LDS (598 for 616, and slower at every shorter size).
 
 #include "kv_attention_mxfp4.h"
 
@@ -27,7 +27,7 @@ template <typename T, int D>
 struct Many {
     static constexpr bool FINE = sizeof(T) == 4;
     static constexpr int QP = FINE ? 3 : std::is_same<T, __half>::value ? 2 : 1;   // pieces of a query value
-    // Pieces of a weight: 16 bits, 24 beside f32. (One, 8 bits, in bf16: 2048 rows alone 61 us for 74, behind 14336 625 for 770, and outputs
+    // Pieces of a weight: 16 bits, 24 beside f32. (One, 8 bits, in bf16: 2048 rows alone 61 us for 74, behind 14336 625 for 770, calls, and outputs
     // off by 0.0020 of their size, root mean square, where 16 bits leave the output's own rounding, 0.0016.)
     static constexpr int SP = FINE ? 3 : 2;
     static constexpr int ROWS = mx_many_rows(FINE, D), NT = ROWS / 16, PITCH = D + 4, KS = D / 32, NB = D / 16, W = D / 32, PART = D / 32;

@@ -9,8 +9,8 @@
 // goes the same way, by pairs that stay as they are. Queries are computed in 32 bits and rounded once. Keys that go to the cache are computed in 64: a value next
 // to the border of two codes would else come out as the other one. They pass through LDS, where a block's 32 values come together.
 //
-// Bound by the rows' bytes: 4096 tokens of 32 + 8 heads of 128, bf16, three axes of positions 17.2 us, 4.9 TB/s in and out. Into the cache by the 64-bit norms and
-// rotations too: 2048 tokens of 32 + 8 + 8 heads, bf16, 14.1 us; a few tokens by the chain position, angle, rows: one token 3.1 us.
+// Bound by the rows' bytes: 4096 tokens of 32 + 8 heads of 128, bf16, three axes of positions 17.4 us, 4.8 TB/s in and out. Into the cache by the 64-bit norms and
+// rotations too: 2048 tokens of 32 + 8 + 8 heads, bf16, 14.6 us without norms, 18.3 with them; a few tokens by the chain position, angle, rows: one token 3.1 us. (Kernel trace.)
 
 #include <type_traits>
 
@@ -180,8 +180,8 @@ __global__ __launch_bounds__(WG) void rotate_kernel(Rotate r, int tokens_of) {
 template <typename T, int D, bool CACHE>
 static int launch_of(const Rotate& r, bool neighbours, hipStream_t s) {
     // A token's heads over four waves, but into the cache, whose angles in 64 bits take long, a token a wave once each CU has more than eight tokens: their
-    // angles are made side by side. 32 + 8 heads of 128, bf16: 4096 tokens into the cache 30.0 us in fours of waves, 27.1 a token a wave, 2048 17.6 and 18.8;
-    // without the cache 4096 16.7 and 17.5, 1024 7.6 and 11.5.
+    // angles are made side by side. 32 + 8 heads of 128 with norms, bf16, kernel trace: 4096 tokens into the cache 30.6 us in fours of waves, 26.9 a token a wave, 2048
+    // 18.8 and 19.6, 1024 11.0 and 17.0; without the cache (calls) 4096 16.7 and 17.5, 1024 7.6 and 11.5.
     const int tokens = CACHE && r.rows > 8 * lk_device().cus ? WAVES : 1;
     const dim3 grid((unsigned)((r.rows + tokens - 1) / tokens)), threads(WG);
     if (neighbours) hipLaunchKernelGGL((rotate_kernel<T, D, true, CACHE>), grid, threads, 0, s, r, tokens);

@@ -11,8 +11,8 @@
 // Differences p - q are made in 64 bits and summed as integers of 2^-51, whose sums do not depend on an order.
 //
 // Bound by the passes over the logits, one of rows that nothing cuts, up to three of others, and by the issue of 30 instructions a weight. 158 rows of 151936
-// bf16 words that nothing cuts: pieces 29 us (1.6 TB/s; the vector unit's), kept 8, judge 17; 320 rows of 128256 f32 words with every rule: 35 (4.7 TB/s, the copy
-// rate), steps 38, kept 38, judge 26; five rows of 151936 with top-k: 31 in all, the chains of four launches.
+// bf16 words that nothing cuts: pieces 29 us (1.6 TB/s; the vector unit's), kept 8, judge 18; 320 rows of 128256 f32 words with every rule: 35 (4.7 TB/s, the copy
+// rate), steps 39, kept 37, judge 27; five rows of 151936 with top-k: 32 in all, the chains of four launches. (Kernel trace.)
 
 #include "sampling_core.h"
 
@@ -447,7 +447,7 @@ extern "C" int lk_verify(const void* logits, int type, int64_t stride, int rows,
     v.s = Sampling{logits, stride, vocab, 0, 0, 0, nullptr, temperature, top_p, min_p, top_k, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     cut_rows(v.s, rows, size);
     // pieces of the first pass: 16 words a thread (half as many sums and largest words to bring together), 8 where that leaves CUs without two workgroups:
-    // 320 bf16 rows of 151936 words 82 us (93 with 8), 40 rows 27.6 (29.1), 5 rows 24.1 (22.9)
+    // 320 bf16 rows of 151936 words 82 us (93 with 8), 40 rows 27.6 (29.1), 5 rows 24.1 (22.9), calls
     const int cus = lk_device().cus, most = SAMPLE_WG * 16;
     const bool wide = (int64_t)rows * ((vocab + most - 1) / most) >= 2 * cus;
     const int words = wide ? most : most / 2;
