@@ -422,3 +422,46 @@ def test_values_near_the_end_of_f32(scale, fresh, dtype):
     b = Batch([130, 70], [fresh] * 2, 4, 2, 64, 16, dtype, seed=60)
     b.want.powers["v"][:] = 110 + 127
     b.check(scale=scale)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("seqs,longest", [(70, 150), (130, 40), (200, 300)])
+def test_long_and_short_sequences_of_a_batch(seqs, longest, dtype):
+    """Row tiles of a few sequences among many that have none, in more than one look's worth of sequences; hints too small as well."""
+    g = np.random.default_rng(seqs)
+    fresh = [int(g.integers(0, longest)) if i % 9 == 4 else int(g.integers(0, 3)) for i in range(seqs)]
+    fresh[-1] = longest
+    b = Batch([f + int(g.integers(0, 30)) for f in fresh], fresh, 4, 2, 64, 16, dtype, seed=seqs, pad=3)
+    assert (b.check()[-3:] == 7).all()
+    b.check(max_fresh=17, max_len=5)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("what", ["ragged", "one long", "window", "more rows than said", "beside a prompt"])
+def test_many_contexts_are_cut_into_equal_pieces(what, dtype):
+    """Enough sequences for pieces that hold several of them, ends of them, and sequences without rows or tokens."""
+    g = np.random.default_rng(40)
+    lens = [0, 1, 64, 65, 0] + [int(v) for v in g.integers(1, 5000, 36)] + [0, 3]
+    fresh = [0] + [1] * 42
+    fresh[4], fresh[11], fresh[20], fresh[42] = 1, 0, 2, 0
+    if what == "one long":
+        lens = [100] * 42 + [40000]
+    if what == "more rows than said":
+        fresh[7], fresh[30] = 9, 40
+    if what == "beside a prompt":
+        fresh[9] = 70
+    b = Batch(lens, fresh, 16, 16, 64, 16, dtype, seed=41, pad=3)
+    b.table = np.concatenate([b.table, np.full((43, 4100 - b.table.shape[1]), -1, np.int32)], 1)     # (room for contexts that are worth pieces)
+    out = b.check(window=700 if what == "window" else 0, max_fresh=2 if what != "beside a prompt" else 70, max_len=64000)
+    assert (out[-3:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_a_row_does_not_depend_on_its_companions(dtype):
+    """The same sequence alone and in a batch, and the same call again: the same bits, but for contexts that are cut elsewhere."""
+    b = Batch([500, 60, 900], [1, 1, 1], 8, 2, 128, 16, dtype, seed=31)
+    whole = b.check(max_len=900)
+    for i in range(3):
+        one = kv.kv_attention(b.q[i:i + 1].cuda(), b.cache(), i32(b.table[i:i + 1]), i32(b.lens[i:i + 1]), i32([0, 1]), max_fresh=1, max_len=900)
+        assert (one[0].float() - whole[i].float()).abs().max() <= (2e-5 if dtype == "f32" else 2 * torch.finfo(TYPES[dtype]).eps) * whole[i].float().abs().max()
+    assert torch.equal(whole, b.check(max_len=900))
